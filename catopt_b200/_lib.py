@@ -140,6 +140,21 @@ SIGNATURES: dict[str, tuple] = {
 }
 
 
+_P, _I, _L, _F = C.c_void_p, C.c_int, C.c_longlong, C.c_float
+SIGNATURES.update({
+    "cb2_paged_append": (
+        _I, [_P, _L, _L] * 3 + [_P] * 3 + [_L] * 2 + [_P] * 7 + [_F] + [_P] * 2 + [_I] * 12 + [_P] * 2,
+    ),
+    "cb2_om_paged_scratch_bytes": (C.c_size_t, [_I] * 9),
+    "cb2_om_paged_fwd": (
+        _I, [_P, _L, _L, _P, _P, _L, _L] + [_P] * 5 + [_I] * 10 + [_F, _I, _I, _P, C.c_size_t, _P, _P],
+    ),
+    "cb2_paged_evict": (
+        _I, [_P, _P, _L, _L] + [_P] * 6 + [_I] * 12 + [_P] * 2,
+    ),
+})
+
+
 class B200Error(RuntimeError):
     """The native library is missing or an entry point reported an error."""
 

@@ -34,6 +34,9 @@ SOURCES = [
     "om_causal.cu",
     "om_causal_tc.cu",
     "device_wait.cu",
+    "om_paged.cu",
+    "paged_append.cu",
+    "paged_evict.cu",
 ]
 
 NVCC_FLAGS = [

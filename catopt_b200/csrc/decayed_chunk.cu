@@ -104,6 +104,7 @@ extern "C" const char* cb2_status_str(int status) {
     case CB2_WAIT_TIMEOUT: return "device wait timed out";
     case CB2_NULL_PTR: return "null pointer";
     case CB2_SCRATCH_TOO_SMALL: return "scratch too small";
+    case CB2_BAD_INDEX: return "index tensor value out of range";
     default: return "unknown status";
   }
 }

@@ -1,0 +1,292 @@
+// Attention of a ragged batch of new tokens over a paged key/value cache: what its kernels share.
+//
+// Pools   k_pages, v_pages: [n_pages, Hkv, page_size, d] (a page of one kv head is contiguous; the
+//         distance between pages is free), page_size a power of two.  Request r owns the pages
+//         table[r][0..]; key slot j of it sits in page table[r][j / page_size], row j % page_size.
+// Rows    The G = Hq / Hkv query heads of a kv head share its keys, so the rows of a unit of work are
+//         the packed pairs (token, head of the group): row = token * G + g, n_r * G rows per
+//         (request, kv head), cut into tiles of RT rows.
+// Work    One unit = (request, kv head, row tile); its cost is the number of KB-key blocks some row of
+//         the tile can see.  All blocks of all units form one line, which is cut into equal shares, one
+//         per CTA: ragged lengths, causal tiles and single long requests balance by themselves, from
+//         lengths that only the device knows (a captured graph stays right when they change).  A unit
+//         that lies in one share is finished there; one that crosses shares leaves a partial carrier
+//         (m, l, a) per share, which paged_combine_kernel joins in share order (no atomics: the same
+//         inputs give the same bits).
+#pragma once
+#include "common.cuh"
+
+namespace cb2 {
+
+// The index tensors of a ragged batch.  Values out of range are clamped where they are read and
+// reported as CB2_BAD_INDEX, so that no index tensor can lead to an access out of bounds.
+struct PagedBatch {
+  const int* table;   // [R, max_pages]
+  const int* lens;    // [R] cached keys, the new tokens included
+  const int* cu;      // [R+1] first row of each request in q
+  int R, max_pages, n_pages, page_log2, n_tokens, max_k;
+  int* status;
+};
+
+struct PagedPools {
+  const void* k;
+  const void* v;
+  long long k_page_stride, v_page_stride;   // elements
+  int Hkv, d;
+};
+
+struct PagedReq {
+  int t0, n, len;     // first row in q, new tokens, cached keys
+};
+
+__device__ __forceinline__ void paged_flag(const PagedBatch& b) {
+  if (b.status) atomicExch(b.status, CB2_BAD_INDEX);
+}
+
+__device__ __forceinline__ PagedReq paged_request(const PagedBatch& b, int r) {
+  const int c0 = __ldg(b.cu + r), c1 = __ldg(b.cu + r + 1), l = __ldg(b.lens + r);
+  PagedReq q;
+  q.t0 = min(max(c0, 0), b.n_tokens);
+  q.n = max(min(c1, b.n_tokens) - q.t0, 0);
+  q.len = min(max(l, 0), b.max_k);
+  if (q.t0 != c0 || q.t0 + q.n != c1 || q.len != l) paged_flag(b);
+  return q;
+}
+
+// Pool page of table entry i of request r; page 0 (always there) for an id out of range.
+__device__ __forceinline__ int paged_page(const PagedBatch& b, int r, int i) {
+  const int p = __ldg(b.table + (long long)r * b.max_pages + i);
+  if (unsigned(p) < unsigned(b.n_pages)) return p;
+  paged_flag(b);
+  return 0;
+}
+
+// sum of floor((a i + b) / m) over i < n, for 0 <= a, b and a n + b < 2^31: the lattice points under
+// a line, counted by exchanging the axes as in Euclid's algorithm.
+__device__ inline long long lattice_sum(unsigned n, unsigned m, unsigned a, unsigned b) {
+  long long sum = 0;
+  bool add = true;    // the exchanged problem counts the complement
+  while (n > 0) {
+    long long part = 0;
+    if (a >= m) {
+      part += (long long)(a / m) * ((long long)n * (n - 1) / 2);
+      a %= m;
+    }
+    if (b >= m) {
+      part += (long long)(b / m) * n;
+      b %= m;
+    }
+    sum += add ? part : -part;
+    // with a, b < m: sum_i floor((a i + b)/m) = n h - #{(i, y): 0 < y <= h, a i + b < m y}, h = the
+    // largest term; the y-th row holds ceil((m y - b)/a) = floor((m y - b + a - 1)/a) of these points
+    const unsigned h = a == 0 ? 0 : (a * (n - 1) + b) / m;
+    if (h == 0) break;
+    sum += add ? (long long)n * h : -(long long)n * h;
+    add = !add;
+    // rows y = 1..h  ->  i' = y - 1: floor((m i' + m - b + a - 1) / a)
+    const unsigned nb = m - b + a - 1, na = m, nm = a;
+    n = h;
+    a = na;
+    b = nb;
+    m = nm;
+  }
+  return sum;
+}
+
+// The requests that a kernel takes: all of them, those with at most `few` packed rows, or the others.
+enum { kPagedAll = 0, kPagedFew = 1, kPagedChunk = 2 };
+
+template <int RT, int KB>
+struct PagedCost {
+  int G, Hkv, causal, which, few;
+  __device__ __forceinline__ bool takes(const PagedReq& q) const {
+    if (q.n == 0) return false;
+    return which == kPagedAll || (which == kPagedFew) == (q.n * G <= few);
+  }
+  __device__ __forceinline__ int tiles(const PagedReq& q) const { return (q.n * G + RT - 1) / RT; }
+  __device__ __forceinline__ int all_blocks(const PagedReq& q) const { return max(1, (q.len + KB - 1) / KB); }
+  // blocks that tile i visits: up to the last token of the tile
+  __device__ __forceinline__ int blocks(const PagedReq& q, int i) const {
+    const int base = q.len - q.n;
+    if (!causal || base < 0 || i == tiles(q) - 1) return all_blocks(q);
+    return int((unsigned(i) * RT + RT - 1 + unsigned(G) * (base + KB)) / (unsigned(G) * KB));
+  }
+  // blocks of the first `k` tiles of one kv head
+  __device__ __forceinline__ long long before(const PagedReq& q, int k) const {
+    const int base = q.len - q.n, nt = tiles(q);
+    if (!causal || base < 0) return (long long)k * all_blocks(q);
+    const int m = min(k, nt - 1);
+    long long s = lattice_sum(m, unsigned(G) * KB, RT, RT - 1 + unsigned(G) * (base + KB));
+    if (k == nt) s += all_blocks(q);
+    return s;
+  }
+  __device__ __forceinline__ long long of_request(const PagedReq& q) const {
+    if (!takes(q)) return 0;
+    return before(q, tiles(q)) * Hkv;
+  }
+};
+
+struct PagedFindSmem {
+  long long warp_sum[32];
+  long long carry;
+  long long off;
+  int r;
+};
+
+// Start of this CTA's share [lo, hi) of the line: request and offset in it.  All T threads call it.
+struct PagedShare {
+  long long total, lo, hi;
+  int r;            // request that holds lo
+  long long off;    // lo - start of that request
+};
+
+__device__ __forceinline__ long long paged_cut(long long total, int c, int n) { return total * c / n; }
+
+template <int T, class Cost>
+__device__ PagedShare paged_find_share(const PagedBatch& b, const Cost& cost, int cta, int n_cta, PagedFindSmem* s) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  PagedShare out;
+  const int passes = (b.R + T - 1) / T;
+  // inclusive prefix of the costs of requests [pass * T, pass * T + T), on top of `carry`
+  auto scan = [&](int pass, long long& mine, long long carry, long long& block_total) -> long long {
+    const int r = pass * T + tid;
+    mine = r < b.R ? cost.of_request(paged_request(b, r)) : 0;
+    long long x = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) s->warp_sum[warp] = x;
+    __syncthreads();
+    long long pre = carry;
+    for (int w = 0; w < warp; ++w) pre += s->warp_sum[w];
+    block_total = 0;
+    for (int w = 0; w < T / 32; ++w) block_total += s->warp_sum[w];
+    __syncthreads();
+    return x + pre;
+  };
+  long long mine, block_total, incl = 0, total = 0;
+  for (int p = 0; p < passes; ++p) {
+    incl = scan(p, mine, total, block_total);
+    total += block_total;
+  }
+  out.total = total;
+  out.lo = paged_cut(total, cta, n_cta);
+  out.hi = paged_cut(total, cta + 1, n_cta);
+  if (tid == 0) {
+    s->r = 0;
+    s->off = 0;
+  }
+  __syncthreads();
+  long long carry = 0;
+  for (int p = 0; p < passes; ++p) {
+    if (passes > 1) {
+      incl = scan(p, mine, carry, block_total);
+      carry += block_total;
+    }
+    if (mine > 0 && out.lo >= incl - mine && out.lo < incl) {
+      s->r = p * T + tid;
+      s->off = out.lo - (incl - mine);
+    }
+  }
+  __syncthreads();
+  out.r = s->r;
+  out.off = s->off;
+  return out;
+}
+
+// Walks the pieces of a share: piece = blocks [b0, b1) of the nb blocks of unit (r, h, tile).
+// Every thread of a warp keeps the same walk.
+template <class Cost>
+struct PagedWalk {
+  const PagedBatch& batch;
+  const Cost& cost;
+  long long cur, hi, per_head;
+  PagedReq q;
+  int r, h, tile, nb, b0, b1;
+
+  __device__ PagedWalk(const PagedBatch& b, const Cost& c, const PagedShare& s) : batch(b), cost(c), cur(s.lo), hi(s.hi), r(s.r) {
+    if (cur >= hi) return;
+    q = paged_request(b, r);
+    per_head = cost.before(q, cost.tiles(q));
+    h = int(s.off / per_head);
+    const long long rest = s.off - h * per_head;
+    // last tile whose start is <= rest: 32 candidates a round, one per lane
+    int lo = 0, n = cost.tiles(q);
+    const int lane = threadIdx.x & 31;
+    while (n > 1) {
+      const int step = (n + 31) / 32;
+      const int cand = lo + lane * step;
+      const bool le = lane * step < n && cost.before(q, cand) <= rest;
+      const int k = 31 - __clz(__ballot_sync(0xffffffffu, le));
+      n = min(step, n - k * step);
+      lo += k * step;
+    }
+    tile = lo;
+    nb = cost.blocks(q, tile);
+    b0 = int(rest - cost.before(q, tile));
+  }
+  __device__ bool valid() const { return cur < hi; }
+  __device__ void clip() { b1 = int(min((long long)nb, b0 + (hi - cur))); }
+  __device__ void next() {
+    cur += b1 - b0;
+    b0 = 0;
+    if (cur >= hi) return;
+    if (++tile == cost.tiles(q)) {
+      tile = 0;
+      if (++h == cost.Hkv) {
+        h = 0;
+        do {
+          ++r;
+          q = paged_request(batch, r);
+        } while (!cost.takes(q));
+      }
+    }
+    nb = cost.blocks(q, tile);
+  }
+};
+
+// A unit that starts in share c and goes on in the next ones: written by CTA c for the combine kernel.
+struct PagedJoin {
+  int r, h, tile, last;     // r < 0: none; last = share that holds the unit's last block
+};
+// Partial carriers: share c owns slot 2c (a piece that does not start its unit) and 2c + 1 (a piece
+// that starts a unit and does not finish it).  Slot: m[RT], l[RT], a[RT][d], fp32, m in log2 units.
+__host__ __device__ __forceinline__ size_t paged_slot_floats(int rt, int d) { return size_t(rt) * (d + 2); }
+
+__device__ __forceinline__ float ex2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <class Walk>
+__device__ __forceinline__ void paged_write_join(const Walk& w, const PagedShare& s, int cta, int n_cta, PagedJoin* joins) {
+  // called for a piece with b0 == 0 and b1 < nb: the unit's last block sits at cur + nb - 1
+  PagedJoin j;
+  j.r = w.r;
+  j.h = w.h;
+  j.tile = w.tile;
+  j.last = int(((w.cur + w.nb) * n_cta - 1) / s.total);
+  joins[cta] = j;
+}
+
+// Scratch of one attention kernel of n_cta shares: the line's length, the joins, the partial carriers.
+struct PagedScratch {
+  long long* total;
+  PagedJoin* joins;
+  float* parts;
+};
+__host__ __device__ inline size_t paged_scratch_bytes(int n_cta, int rt, int d) {
+  return 16 + size_t(n_cta) * sizeof(PagedJoin) + size_t(n_cta) * 2 * paged_slot_floats(rt, d) * 4;
+}
+inline PagedScratch paged_scratch(void* base, int n_cta) {
+  PagedScratch s;
+  s.total = static_cast<long long*>(base);
+  s.joins = reinterpret_cast<PagedJoin*>(static_cast<char*>(base) + 16);
+  s.parts = reinterpret_cast<float*>(static_cast<char*>(base) + 16 + size_t(n_cta) * sizeof(PagedJoin));
+  return s;
+}
+
+}  // namespace cb2

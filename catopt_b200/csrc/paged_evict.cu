@@ -1,0 +1,228 @@
+// Eviction from a paged key/value cache by accumulated attention weight.
+//
+// A request longer than the budget keeps, for every kv head by itself, its first and last slots and, of the
+// slots between, those of the largest weight (ties to the lowest slot; NaN counts as the smallest), in slot
+// order; they are copied to the pages of another table, keys, values and weights alike.  A shorter request is
+// copied whole.  The old pages stay as they are, so shared prefixes are no hazard and the copy needs no order.
+//
+// Two launches.  paged_select_kernel: one CTA per (request, kv head) finds the budget-th weight by radix
+// selection on the weights' order-preserving bit patterns and writes the kept slots in ascending order.
+// paged_move_kernel: copies rows, bound by memory (kept rows read once and written once).
+#include "om_paged.cuh"
+
+namespace cb2 {
+namespace {
+
+constexpr int kSelThreads = 512, kMoveThreads = 256, kMoveRows = 64;
+
+// Unsigned key of the same order as the float: NaN lowest, -0 and +0 the same.
+__device__ __forceinline__ uint32_t weight_key(float w) {
+  if (w != w) return 0u;
+  const uint32_t u = __float_as_uint(w + 0.f);
+  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+
+struct EvictArgs {
+  const float* weights;
+  int Hkv, budget, first, last;
+  int* kept;        // [R, Hkv, budget]
+  int* new_lens;    // [R]
+};
+
+struct WeightReader {
+  const PagedBatch& b;
+  const float* w;
+  int r, h, Hkv;
+  __device__ __forceinline__ uint32_t operator()(int j) const {
+    const int page = paged_page(b, r, j >> b.page_log2), ps = 1 << b.page_log2;
+    return weight_key(w[((long long)page * Hkv + h) * ps + (j & (ps - 1))]);
+  }
+};
+
+__global__ void __launch_bounds__(kSelThreads)
+paged_select_kernel(const EvictArgs a, const PagedBatch batch) {
+  __shared__ int hist[256];
+  __shared__ int warp_keep[kSelThreads / 32], warp_tie[kSelThreads / 32];
+  __shared__ uint32_t s_prefix;
+  __shared__ int s_need;
+  const int h = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int l0 = __ldg(batch.lens + r), len = min(max(l0, 0), batch.max_k);
+  if (len != l0) paged_flag(batch);
+  int* kept = a.kept + ((long long)r * a.Hkv + h) * a.budget;
+  if (h == 0 && tid == 0) a.new_lens[r] = min(len, a.budget);
+  if (len <= a.budget) {
+    for (int i = tid; i < a.budget; i += kSelThreads) kept[i] = i < len ? i : -1;
+    return;
+  }
+  const WeightReader key{batch, a.weights, r, h, a.Hkv};
+  const int lo = a.first, hi = len - a.last;             // first + last <= budget < len
+  // the (budget - first - last)-th largest key of [lo, hi), byte by byte
+  if (tid == 0) {
+    s_prefix = 0;
+    s_need = a.budget - a.first - a.last;
+  }
+  __syncthreads();
+  const bool any = a.budget - a.first - a.last > 0;
+  for (int shift = 24; any && shift >= 0; shift -= 8) {
+    for (int i = tid; i < 256; i += kSelThreads) hist[i] = 0;
+    __syncthreads();
+    const uint32_t prefix = s_prefix, mask = shift == 24 ? 0u : ~0u << (shift + 8);
+    for (int j = lo + tid; j < hi; j += kSelThreads) {
+      const uint32_t k = key(j);
+      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255u], 1);
+    }
+    __syncthreads();
+    if (warp == 0) {
+      // bins from the top, eight a lane: the bin in which the need runs out
+      int c[8], sum = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        c[i] = hist[255 - (lane * 8 + i)];
+        sum += c[i];
+      }
+      int incl = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
+      }
+      int before = incl - sum;
+      const int need = s_need;
+      __syncwarp();
+      if (before < need && incl >= need) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (before < need && before + c[i] >= need) {
+            s_prefix = prefix | (uint32_t(255 - (lane * 8 + i)) << shift);
+            s_need = need - before;
+          }
+          before += c[i];
+        }
+      }
+    }
+    __syncthreads();
+  }
+  const uint32_t cut = s_prefix;
+  const int ties = any ? s_need : 0;       // how many keys equal to the cut are kept, the lowest slots first
+  int base_keep = 0, base_tie = 0;
+  for (int j0 = 0; j0 < len; j0 += kSelThreads) {
+    const int j = j0 + tid;
+    bool keep = false, tie = false;
+    if (j < len) {
+      if (j < lo || j >= hi) {
+        keep = true;
+      } else if (any) {
+        const uint32_t k = key(j);
+        keep = k > cut;
+        tie = k == cut;
+      }
+    }
+    const unsigned below = (1u << lane) - 1;
+    const unsigned bt = __ballot_sync(0xffffffffu, tie);
+    if (lane == 0) warp_tie[warp] = __popc(bt);
+    __syncthreads();
+    int tb = base_tie, tt = 0;
+    for (int w = 0; w < kSelThreads / 32; ++w) {
+      if (w < warp) tb += warp_tie[w];
+      tt += warp_tie[w];
+    }
+    if (tie && tb + __popc(bt & below) < ties) keep = true;
+    const unsigned bk = __ballot_sync(0xffffffffu, keep);
+    if (lane == 0) warp_keep[warp] = __popc(bk);
+    __syncthreads();
+    int kb = base_keep, kt = 0;
+    for (int w = 0; w < kSelThreads / 32; ++w) {
+      if (w < warp) kb += warp_keep[w];
+      kt += warp_keep[w];
+    }
+    if (keep) kept[kb + __popc(bk & below)] = j;
+    base_keep += kt;
+    base_tie += tt;
+  }
+}
+
+struct MoveArgs {
+  char *k, *v;
+  long long k_page_bytes, v_page_bytes;
+  float* weights;
+  const int* kept;
+  const int* to_table;
+  int to_pages, Hkv, budget, row_bytes;
+};
+
+__global__ void __launch_bounds__(kMoveThreads)
+paged_move_kernel(const MoveArgs a, const PagedBatch batch) {
+  __shared__ long long src[kMoveRows], dst[kMoveRows];    // (page * 2^32 + slot), -1: nothing
+  const int r = blockIdx.z, h = blockIdx.y, i0 = blockIdx.x * kMoveRows, tid = threadIdx.x;
+  const int ps = 1 << batch.page_log2;
+  if (tid < kMoveRows) {
+    const int i = i0 + tid;
+    long long s = -1, t = -1;
+    if (i < a.budget) {
+      const int j = a.kept[((long long)r * a.Hkv + h) * a.budget + i];
+      if (j >= 0) {
+        const int from = __ldg(batch.table + (long long)r * batch.max_pages + (j >> batch.page_log2));
+        const int to = __ldg(a.to_table + (long long)r * a.to_pages + (i >> batch.page_log2));
+        if (unsigned(from) < unsigned(batch.n_pages) && unsigned(to) < unsigned(batch.n_pages)) {
+          s = ((long long)from << 32) | (j & (ps - 1));
+          t = ((long long)to << 32) | (i & (ps - 1));
+        } else {
+          paged_flag(batch);
+        }
+      }
+    }
+    src[tid] = s;
+    dst[tid] = t;
+    if (s >= 0)
+      a.weights[((t >> 32) * a.Hkv + h) * ps + int(t & 0xffffffff)] = a.weights[((s >> 32) * a.Hkv + h) * ps + int(s & 0xffffffff)];
+  }
+  __syncthreads();
+  const int nv = a.row_bytes / 16;
+  const int total = kMoveRows * nv;
+  for (int e = tid; e < total; e += kMoveThreads) {
+    const int row = e / nv, c = (e % nv) * 16;
+    const long long s = src[row], t = dst[row];
+    if (s < 0) continue;
+    const long long so = (long long)(h * ps + int(s & 0xffffffff)) * a.row_bytes + c;
+    const long long to = (long long)(h * ps + int(t & 0xffffffff)) * a.row_bytes + c;
+    const uint4 kk = *reinterpret_cast<const uint4*>(a.k + (s >> 32) * a.k_page_bytes + so);
+    const uint4 vv = *reinterpret_cast<const uint4*>(a.v + (s >> 32) * a.v_page_bytes + so);
+    *reinterpret_cast<uint4*>(a.k + (t >> 32) * a.k_page_bytes + to) = kk;
+    *reinterpret_cast<uint4*>(a.v + (t >> 32) * a.v_page_bytes + to) = vv;
+  }
+}
+
+}  // namespace
+}  // namespace cb2
+
+extern "C" int cb2_paged_evict(void* k_pages, void* v_pages, long long k_page_stride, long long v_page_stride, float* weights,
+                               const int* block_table, const int* seq_lens, const int* new_table, int* kept, int* new_lens,
+                               int R, int Hkv, int d, int page_size, int n_pages, int max_pages, int new_pages, int max_k,
+                               int budget, int keep_first, int keep_last, int dtype, int* dev_status, void* stream) {
+  using namespace cb2;
+  if (!k_pages || !v_pages || !weights || !block_table || !seq_lens || !new_table || !kept || !new_lens) return CB2_NULL_PTR;
+  if (R < 1 || R > 65535 || Hkv < 1 || Hkv > 65535 || d < 8 || d > 128 || d % 8 || n_pages < 1 || max_pages < 1 || new_pages < 1)
+    return CB2_BAD_SHAPE;
+  if (page_size < 8 || page_size > 1024 || (page_size & (page_size - 1)) || max_k < 1 || max_k > (1 << 30) ||
+      int64_t(max_pages) * page_size < max_k)
+    return CB2_BAD_SHAPE;
+  if (budget < 1 || keep_first < 0 || keep_last < 0 || int64_t(keep_first) + keep_last > budget || int64_t(new_pages) * page_size < budget)
+    return CB2_BAD_SHAPE;
+  const long long page = (long long)Hkv * page_size * d;
+  if (k_page_stride < page || v_page_stride < page) return CB2_BAD_SHAPE;
+  if (dtype != CB2_BF16 && dtype != CB2_F32) return CB2_UNSUPPORTED_DTYPE;
+  const int esz = dtype == CB2_BF16 ? 2 : 4;
+  if (!aligned16(k_pages) || !aligned16(v_pages) || k_page_stride * esz % 16 || v_page_stride * esz % 16) return CB2_BAD_ALIGN;
+  int page_log2 = 0;
+  while ((1 << page_log2) < page_size) ++page_log2;
+  const PagedBatch batch{block_table, seq_lens, nullptr, R, max_pages, n_pages, page_log2, 0, max_k, dev_status};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const EvictArgs e{weights, Hkv, budget, keep_first, keep_last, kept, new_lens};
+  paged_select_kernel<<<dim3(Hkv, R), kSelThreads, 0, st>>>(e, batch);
+  CB2_LAUNCH_CHECK();
+  const MoveArgs m{static_cast<char*>(k_pages), static_cast<char*>(v_pages), k_page_stride * esz, v_page_stride * esz, weights,
+                   kept, new_table, new_pages, Hkv, budget, d * esz};
+  paged_move_kernel<<<dim3((budget + kMoveRows - 1) / kMoveRows, Hkv, R), kMoveThreads, 0, st>>>(m, batch);
+  CB2_LAUNCH_CHECK();
+  return CB2_OK;
+}

@@ -675,3 +675,201 @@ def gated_contract(s: torch.Tensor, g: torch.Tensor, v: torch.Tensor) -> torch.T
                                             T, K, dv, rule[0], rule[1], code, status.data_ptr(), stream_ptr())
     check(rc, "cb2_gated_contract_fwd")
     return out
+
+
+# --------------------------------------------------------------------------- paged cache
+def _no_grad_asked(what: str, *tensors: torch.Tensor | None) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise B200Error(f"{what} serves a cache and has no gradient: call it under torch.no_grad()")
+
+
+def _pools(what: str, k_pages: torch.Tensor, v_pages: torch.Tensor) -> tuple[int, int]:
+    """Page strides (elements) of two pools ``[n_pages, Hkv, page_size, d]`` that are dense inside a page."""
+    require_device(k_pages, v_pages)
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype or 0 in k_pages.shape:
+        raise B200Error(f"{what}: k_pages and v_pages are [n_pages, Hkv, page_size, d] of one shape and dtype")
+    n, hkv, ps, d = k_pages.shape
+    page = hkv * ps * d
+    strides = []
+    for pool in (k_pages, v_pages):
+        if not pool[0].is_contiguous() or (n > 1 and pool.stride(0) < page):
+            raise B200Error(f"{what}: a page [Hkv, page_size, d] must be contiguous")
+        strides.append(pool.stride(0) if n > 1 else page)
+    return strides[0], strides[1]
+
+
+def _page_weights(what: str, weights: torch.Tensor, k_pages: torch.Tensor) -> None:
+    require_cuda(weights)
+    if weights.dtype != torch.float32 or weights.shape != k_pages.shape[:3]:
+        raise B200Error(f"{what}: weights are float32 [n_pages, Hkv, page_size]")
+
+
+def _index(what: str, name: str, t: torch.Tensor, shape: tuple) -> None:
+    require_cuda(t)
+    if t.dtype != torch.int32 or tuple(t.shape) != shape:
+        raise B200Error(f"{what}: {name} is int32 {list(shape)}, got {t.dtype} {list(t.shape)}")
+
+
+def _ragged_batch(what: str, block_table: torch.Tensor, seq_lens: torch.Tensor, cu_q: torch.Tensor) -> tuple[int, int]:
+    if block_table.dim() != 2 or 0 in block_table.shape:
+        raise B200Error(f"{what}: block_table is int32 [R, max_pages]")
+    R, max_pages = block_table.shape
+    _index(what, "block_table", block_table, (R, max_pages))
+    _index(what, "seq_lens", seq_lens, (R,))
+    _index(what, "cu_q", cu_q, (R + 1,))
+    return R, max_pages
+
+
+def _token_rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` ``[n_tokens, heads, d]`` as the kernels read it: 16-byte steps between heads and tokens (a view
+    that has them is read in place)."""
+    unit = 16 // t.element_size()
+    if t.numel() and (t.stride(2) != 1 or t.stride(0) % unit or t.stride(1) % unit or t.data_ptr() % 16):
+        return t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _dense_out(what: str, out: torch.Tensor | None, q: torch.Tensor) -> torch.Tensor:
+    if out is None:
+        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    require_cuda(out)
+    if out.shape != q.shape or out.dtype != q.dtype:
+        raise B200Error(f"{what}: out must have the shape and dtype of q")
+    return out
+
+
+def paged_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                 block_table: torch.Tensor, seq_lens: torch.Tensor, cu_q: torch.Tensor, *,
+                 q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 1e-6,
+                 cos: torch.Tensor | None = None, sin: torch.Tensor | None = None, positions: torch.Tensor | None = None,
+                 interleaved: bool = False, weights: torch.Tensor | None = None,
+                 out: torch.Tensor | None = None) -> torch.Tensor | None:
+    """New tokens enter a paged cache: norms of ``q`` and ``k`` per head, position rotation, and the write of
+    ``k`` and ``v`` into their pages, in one pass (``cb2_paged_append``).
+
+    ``q [n, Hq, d]`` (or ``None``), ``k``, ``v [n, Hkv, d]``, any strides; request r's new tokens are rows
+    ``cu_q[r]:cu_q[r+1]`` and take its slots ``seq_lens[r] - n_r ..`` (``seq_lens`` counts them already), slot j
+    being row ``j % page_size`` of page ``block_table[r, j // page_size]`` of the pools ``[n_pages, Hkv, page_size,
+    d]``.  ``q_weight``/``k_weight [d]``: root-mean-square norm of each head; ``cos``/``sin`` float32 ``[rows,
+    rotary/2]`` with ``positions`` int32 ``[n]``: rotation of the first ``rotary`` columns in pairs ``(i, i +
+    rotary/2)``, or ``(2i, 2i+1)`` if ``interleaved``.  ``weights`` (float32 ``[n_pages, Hkv, page_size]``) is
+    zeroed at the new slots.  Returns the normed and rotated ``q`` (rows behind ``cu_q[R]`` are not written)."""
+    what = "paged_append"
+    require_device(q, k, v)
+    ks, vs = _pools(what, k_pages, v_pages)
+    R, max_pages = _ragged_batch(what, block_table, seq_lens, cu_q)
+    n_pages, hkv, ps, d = k_pages.shape
+    if k.dim() != 3 or tuple(k.shape[1:]) != (hkv, d) or v.shape != k.shape or not (k.dtype == v.dtype == k_pages.dtype):
+        raise B200Error(f"{what}: k and v are [n_tokens, {hkv}, {d}] of the pools' dtype")
+    n = k.shape[0]
+    if q is not None and (q.dim() != 3 or q.shape[0] != n or q.shape[2] != d or q.dtype != k.dtype):
+        raise B200Error(f"{what}: q is [n_tokens, Hq, {d}] of the dtype of k")
+    for w in (q_weight, k_weight):
+        if w is not None:
+            require_cuda(w)
+            if tuple(w.shape) != (d,) or w.dtype != k.dtype:
+                raise B200Error(f"{what}: norm weights are [{d}] of the dtype of k")
+    rotary = rows = 0
+    if cos is not None or sin is not None or positions is not None:
+        if cos is None or sin is None or positions is None:
+            raise B200Error(f"{what}: rotation takes cos, sin and positions")
+        require_cuda(cos, sin)
+        if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32 or \
+                0 in cos.shape or 2 * cos.shape[1] > d:
+            raise B200Error(f"{what}: cos and sin are float32 [rows, rotary/2], rotary <= {d}")
+        _index(what, "positions", positions, (n,))
+        rows, rotary = cos.shape[0], 2 * cos.shape[1]
+    if weights is not None:
+        _page_weights(what, weights, k_pages)
+    _no_grad_asked(what, q, k, v, q_weight, k_weight, cos, sin)
+    k, v = _token_rows(k), _token_rows(v)
+    if q is not None:
+        res = _dense_out(what, out, q)
+        q = _token_rows(q)
+        qa = (q.data_ptr(), q.stride(0), q.stride(1))
+    else:
+        res, qa = None, (None, 0, 0)
+    rc = _lib.load().cb2_paged_append(
+        *qa, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), _ptr(res), k_pages.data_ptr(),
+        v_pages.data_ptr(), ks, vs, _ptr(weights), block_table.data_ptr(), seq_lens.data_ptr(), cu_q.data_ptr(),
+        _ptr(positions), _ptr(q_weight), _ptr(k_weight), float(eps), _ptr(cos), _ptr(sin), rows, rotary,
+        1 if interleaved else 0, n, R, 0 if q is None else q.shape[1], hkv, d, ps, n_pages, max_pages, dtype_code(k.dtype),
+        device_status(k.device).data_ptr(), stream_ptr())
+    check(rc, "cb2_paged_append")
+    return res
+
+
+def om_paged_fwd(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
+                 seq_lens: torch.Tensor, cu_q: torch.Tensor, max_q: int, *, max_k: int | None = None,
+                 scale: float | None = None, causal: bool = True, weights: torch.Tensor | None = None,
+                 out: torch.Tensor | None = None) -> torch.Tensor:
+    """Softmax attention of a ragged batch of new tokens over a paged cache (``cb2_om_paged_fwd``): single
+    tokens, chunks of prompts, or both in one batch.
+
+    ``q [n, Hq, d]`` (any strides), request r's rows ``cu_q[r]:cu_q[r+1]``; its ``seq_lens[r]`` cached keys, the
+    new tokens' included, lie in pages ``block_table[r]`` of the pools ``[n_pages, Hkv, page_size, d]``; query
+    head h reads kv head ``h // (Hq // Hkv)``.  Row i of n_r sees the slots up to ``seq_lens[r] - n_r + i``
+    (all of them without ``causal``); a row that sees none gives 0.  ``max_q``, ``max_k``: bounds of the requests'
+    new tokens and cached keys (``max_k`` defaults to what the table holds); the scratch grows with them.
+    ``weights`` (float32 ``[n_pages, Hkv, page_size]``): the softmax probability that every cached key gets, summed
+    over rows and the heads of its group, is added to it.  ``scale`` defaults to ``1/sqrt(d)``."""
+    what = "om_paged_fwd"
+    require_device(q)
+    ks, vs = _pools(what, k_pages, v_pages)
+    R, max_pages = _ragged_batch(what, block_table, seq_lens, cu_q)
+    n_pages, hkv, ps, d = k_pages.shape
+    if q.dim() != 3 or q.shape[2] != d or q.dtype != k_pages.dtype or q.shape[1] == 0 or q.shape[1] % hkv:
+        raise B200Error(f"{what}: q is [n_tokens, Hq, {d}] of the pools' dtype, Hq a multiple of {hkv}")
+    if weights is not None:
+        _page_weights(what, weights, k_pages)
+    _no_grad_asked(what, q, k_pages, v_pages)
+    res = _dense_out(what, out, q)
+    q = _token_rows(q)
+    n, hq = q.shape[0], q.shape[1]
+    max_k = max_pages * ps if max_k is None else int(max_k)
+    code, w = dtype_code(q.dtype), 0 if weights is None else 1
+    lib = _lib.load()
+    need = lib.cb2_om_paged_scratch_bytes(n, R, hq, hkv, d, max_q, max_k, w, code)
+    # a buffer of its own for every call: two captured graphs, or two streams, never share one
+    scratch = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)
+    rc = lib.cb2_om_paged_fwd(q.data_ptr(), q.stride(0), q.stride(1), k_pages.data_ptr(), v_pages.data_ptr(), ks, vs,
+                              res.data_ptr(), _ptr(weights), block_table.data_ptr(), seq_lens.data_ptr(), cu_q.data_ptr(),
+                              n, R, hq, hkv, d, ps, n_pages, max_pages, int(max_q), max_k,
+                              1.0 / float(d) ** 0.5 if scale is None else float(scale), 1 if causal else 0, code,
+                              scratch.data_ptr(), need, device_status(q.device).data_ptr(), stream_ptr())
+    check(rc, "cb2_om_paged_fwd")
+    return res
+
+
+def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, weights: torch.Tensor, block_table: torch.Tensor,
+                seq_lens: torch.Tensor, new_table: torch.Tensor, budget: int, *, keep_first: int = 0, keep_last: int = 0,
+                max_k: int | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Cut every request of a paged cache to ``budget`` keys by accumulated attention weight (``cb2_paged_evict``).
+
+    Each kv head of a longer request keeps its first ``keep_first`` and last ``keep_last`` slots and the heaviest of
+    those between (ties to the lowest slot), in slot order; a shorter request keeps all.  Keys, values and
+    ``weights`` are copied to the pages ``new_table`` (int32 ``[R, >= ceil(budget / page_size)]``) of the same pools,
+    none of which may belong to a request of this call; the old pages stay as they are.  Returns ``(kept, new_lens)``:
+    int32 ``[R, Hkv, budget]``, the old slot of every new one and -1 behind the last, and int32 ``[R]``."""
+    what = "paged_evict"
+    ks, vs = _pools(what, k_pages, v_pages)
+    if block_table.dim() != 2 or 0 in block_table.shape or new_table.dim() != 2 or 0 in new_table.shape:
+        raise B200Error(f"{what}: block_table and new_table are int32 [R, pages]")
+    R, max_pages = block_table.shape
+    _index(what, "block_table", block_table, (R, max_pages))
+    _index(what, "seq_lens", seq_lens, (R,))
+    _index(what, "new_table", new_table, (R, new_table.shape[1]))
+    _page_weights(what, weights, k_pages)
+    n_pages, hkv, ps, d = k_pages.shape
+    max_k = max_pages * ps if max_k is None else int(max_k)
+    if budget < 1 or new_table.shape[1] * ps < budget:
+        raise B200Error(f"{what}: a budget of {budget} keys does not fit {new_table.shape[1]} pages of {ps}")
+    kept = torch.empty(R, hkv, budget, dtype=torch.int32, device=k_pages.device)
+    new_lens = torch.empty(R, dtype=torch.int32, device=k_pages.device)
+    rc = _lib.load().cb2_paged_evict(k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, weights.data_ptr(),
+                                     block_table.data_ptr(), seq_lens.data_ptr(), new_table.data_ptr(), kept.data_ptr(),
+                                     new_lens.data_ptr(), R, hkv, d, ps, n_pages, max_pages, new_table.shape[1], max_k,
+                                     int(budget), int(keep_first), int(keep_last), dtype_code(k_pages.dtype),
+                                     device_status(k_pages.device).data_ptr(), stream_ptr())
+    check(rc, "cb2_paged_evict")
+    return kept, new_lens

@@ -42,7 +42,9 @@ enum {
   CB2_LAUNCH_FAIL = 4,       /* the CUDA runtime refused the launch                 */
   CB2_WAIT_TIMEOUT = 5,      /* written to *dev_status by a kernel, never returned  */
   CB2_NULL_PTR = 6,          /* a required pointer is NULL                          */
-  CB2_SCRATCH_TOO_SMALL = 7  /* scratch_bytes below the *_scratch_bytes() answer    */
+  CB2_SCRATCH_TOO_SMALL = 7, /* scratch_bytes below the *_scratch_bytes() answer    */
+  CB2_BAD_INDEX = 8          /* written to *dev_status by a kernel that met a length, offset, position or
+                              * page id out of range in an index tensor; never returned */
 };
 
 /* ---- element types ------------------------------------------------------ */
@@ -397,6 +399,83 @@ int cb2_om_bias_step(const void* q, const void* k, const void* v, const float* b
                      int B, int H, int Tq, int Tk, int dk, int dv, float scale,
                      int causal, int key_offset, int dtype, void* scratch,
                      size_t scratch_bytes, int* dev_status, void* stream);
+
+/* -------------------------------------------------------------------------
+ * (b'') a paged key/value cache: what writes it, the attention that reads it, and what
+ * shrinks it.  The serving side of the streaming carrier above (`StreamingOMModule`,
+ * om_lower.py:996-1040, folds dense blocks and keeps no cache); no counterpart in the
+ * reference.
+ *
+ * Pools k_pages, v_pages: n_pages pages of [Hkv, page_size, d], dense inside a page, the
+ * distance between two pages (elements) free; page_size a power of two from 8 to 1024, d a
+ * multiple of 8 up to 128.  weights (may be NULL where the comment says so): float
+ * [n_pages, Hkv, page_size], the attention weight that each cached key has received.
+ * A ragged batch of R requests: request r has its new tokens in rows [cu_q[r], cu_q[r+1])
+ * of q / k / v (int32 [R+1], ascending), seq_lens[r] cached keys WITH the new tokens (int32
+ * [R]) and the pages block_table[r][0 .. ceil(seq_lens[r] / page_size)) (int32
+ * [R, max_pages]; later entries are not read).  Key slot j is row j % page_size of page
+ * block_table[r][j / page_size]; new token i takes slot seq_lens[r] - n_r + i.  A request
+ * without new tokens takes no part in append and attention.  Rows of q behind cu_q[R] are
+ * not read and the rows of the outputs there not written.
+ * All index tensors are device memory and are read by the kernels, so a captured graph
+ * follows them.  A length, offset, position or page id out of range leads to no access out
+ * of bounds: it is clamped or skipped, the outputs of that request are then unspecified, and
+ * CB2_BAD_INDEX is left in *dev_status.
+ * ------------------------------------------------------------------------- */
+
+/* New tokens enter the cache: norms of q and k per head, position rotation, and the write of
+ * k and v into their pages, in one pass.
+ *     x' = x / sqrt(mean(x^2) + eps) * w          q and k, each where its weight [d] is given
+ *     (a, b) -> (a cos - b sin, b cos + a sin)    pairs (i, i + rotary/2) of the first `rotary`
+ *                                                 columns, or (2i, 2i+1) when interleaved
+ * with cos, sin: float [table_rows, rotary/2], row positions[t] (int32 [n_tokens]) for token t.
+ * q: [n_tokens, Hq, d] (Hq may be 0, q NULL), k, v: [n_tokens, Hkv, d], each with its token and
+ * head strides in elements, so views of a fused projection need no copy; q_out: [n_tokens, Hq,
+ * d] dense, apart from q.  Norm weights have the tensors' element type.  Everything is computed
+ * in fp32 and rounded once.  weights (may be NULL): set to 0 at the new slots.  No scratch.
+ * Pointers 16-byte aligned, strides multiples of 16 bytes. */
+int cb2_paged_append(const void* q, long long q_token_stride, long long q_head_stride, const void* k,
+                     long long k_token_stride, long long k_head_stride, const void* v, long long v_token_stride,
+                     long long v_head_stride, void* q_out, void* k_pages, void* v_pages, long long k_page_stride,
+                     long long v_page_stride, float* weights, const int* block_table, const int* seq_lens,
+                     const int* cu_q, const int* positions, const void* q_weight, const void* k_weight, float eps,
+                     const float* cos, const float* sin, int table_rows, int rotary, int interleaved, int n_tokens,
+                     int R, int Hq, int Hkv, int d, int page_size, int n_pages, int max_pages, int dtype,
+                     int* dev_status, void* stream);
+
+/* Attention of the new tokens over the cache, from one token per request to whole prompts:
+ *     o[t, head] = sum_j softmax_j(scale q.k_j) v_j,   kv head = head / (Hq / Hkv),
+ * over the slots j <= seq_lens[r] - n_r + i that row i of request r sees (causal != 0), or all
+ * of its slots.  A row that sees no key (seq_lens[r] = 0, or less than n_r) is 0.  What the
+ * slots behind seq_lens[r] hold, NaN included, has no effect.
+ * q: [n_tokens, Hq, d] with token and head strides in elements; o: [n_tokens, Hq, d] dense,
+ * apart from q.  max_q: no request has more new tokens; max_k: none more cached keys.
+ * weights (may be NULL): weights[key] += sum over the rows that see it, and the heads of its
+ * group, of the softmax probability.  Results do not depend on the order in which CTAs run.
+ * Products of bf16 tensors accumulate in fp32 and probabilities are rounded to bf16 for the
+ * product with v; sums, maxima and accumulators are fp32 throughout.  scale > 0, (n_tokens +
+ * max_k + 256) * Hq / Hkv < 2^30.
+ * scratch: cb2_om_paged_scratch_bytes() bytes, 16-byte aligned. */
+size_t cb2_om_paged_scratch_bytes(int n_tokens, int R, int Hq, int Hkv, int d, int max_q, int max_k, int weights,
+                                  int dtype);
+int cb2_om_paged_fwd(const void* q, long long q_token_stride, long long q_head_stride, const void* k_pages,
+                     const void* v_pages, long long k_page_stride, long long v_page_stride, void* o, float* weights,
+                     const int* block_table, const int* seq_lens, const int* cu_q, int n_tokens, int R, int Hq, int Hkv,
+                     int d, int page_size, int n_pages, int max_pages, int max_q, int max_k, float scale, int causal,
+                     int dtype, void* scratch, size_t scratch_bytes, int* dev_status, void* stream);
+
+/* Eviction by accumulated attention weight: of a request with more than `budget` cached keys every
+ * kv head keeps its slots [0, keep_first), its last keep_last slots and the heaviest of those
+ * between (ties to the lowest slot; NaN counts as the smallest), `budget` in all, in slot order;
+ * a shorter request keeps all.  Kept keys, values and weights are copied to the pages
+ * new_table[r][..] (int32 [R, new_pages]) of the same pools; none of them may be among the pages of
+ * a request of this call.  The old pages stay as they are, so requests may share them.
+ * kept: int32 [R, Hkv, budget], the old slot of every new one, -1 behind the last; new_lens: int32
+ * [R] = min(seq_lens, budget).  max_k: no request has more cached keys.  No scratch. */
+int cb2_paged_evict(void* k_pages, void* v_pages, long long k_page_stride, long long v_page_stride, float* weights,
+                    const int* block_table, const int* seq_lens, const int* new_table, int* kept, int* new_lens, int R,
+                    int Hkv, int d, int page_size, int n_pages, int max_pages, int new_pages, int max_k, int budget,
+                    int keep_first, int keep_last, int dtype, int* dev_status, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,269 @@
+"""Paged-cache operators on the GPU against plain 64-bit forms (paged_reference), whose error bounds count
+the roundings a kernel makes.  Needs a B200: run with ``-m gpu``."""
+import pytest
+import torch
+
+import paged_reference as ref
+
+pytestmark = pytest.mark.gpu
+BF, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.fixture(scope="module")
+def dev():
+    from catopt_b200 import build
+
+    build.build()
+    torch.cuda.set_device(0)
+    return torch.device("cuda", 0)
+
+
+def close(got, want, tol, what):
+    bad = ~((got.double() - want).abs() <= tol)
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} off, worst {((got.double() - want).abs() / tol).max().item():.3g} of the bound"
+
+
+def run_attend(dev, new, lens, kv, group, d, page, dtype, causal=True, weights=False, seed=0, strided=False, scale=None, **cache_kw):
+    from catopt_b200 import ops
+
+    c = ref.make_cache(lens, kv, page, d, dtype, dev, seed, **cache_kw)
+    g = torch.Generator(device=dev).manual_seed(seed + 1)
+    n, hq = sum(new), kv * group
+    wide = (1.5 * torch.randn(n, hq + 3, d + 8, generator=g, device=dev)).to(dtype)
+    q = wide[:, 1:hq + 1, 8:] if strided else wide[:, 1:hq + 1, 8:].contiguous()
+    w0 = torch.rand(c["k"].shape[:3], generator=g, device=dev) if weights else None
+    w = None if w0 is None else w0.clone()
+    cu = ref.offsets(new, dev)
+    o = ops.om_paged_fwd(q, c["k"], c["v"], c["table"], c["lens"], cu, max(new), max_k=max(max(lens), 1), causal=causal,
+                         weights=w, scale=scale)
+    ops.check_device_status(dev)
+    want, tol, ww, wtol = ref.attend(q, c, new, lens, d ** -0.5 if scale is None else scale, causal)
+    close(o, want, tol, "o")
+    if weights:
+        close(w, w0.double() + ww, wtol + 2 * ref.U32 * (w0 + ww), "weights")
+    return c, q, o, w
+
+
+RAGGED = [
+    ([1], [1]), ([1, 1, 0, 1], [7, 130, 0, 513]), ([5, 1, 17], [5, 64, 400]), ([3, 0, 1, 2], [0, 0, 1, 1]),
+    ([40, 1, 129], [170, 259, 129]), ([300], [1000]),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("new,lens", RAGGED, ids=lambda x: "-".join(map(str, x)))
+@pytest.mark.parametrize("kv,group,d,page", [(2, 4, 64, 16), (1, 3, 80, 8), (3, 1, 128, 32), (1, 16, 40, 256), (2, 8, 128, 64)])
+def test_attention(dev, dtype, new, lens, kv, group, d, page):
+    run_attend(dev, new, lens, kv, group, d, page, dtype, weights=True, seed=len(new) + d)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("group", [1, 5])
+def test_attention_all_keys_visible(dev, dtype, group):
+    # queries against another sequence's states: more rows than keys, too
+    run_attend(dev, [33, 1, 70, 9], [20, 300, 129, 0], 2, group, 64, 16, dtype, causal=False, weights=True)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+def test_attention_strided_rows_and_spaced_pages(dev, dtype):
+    run_attend(dev, [9, 1, 140], [60, 200, 333], 2, 4, 64, 16, dtype, strided=True, page_gap=64, weights=True, scale=0.3)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("new,lens,kv,group", [([1], [20000], 1, 2), ([1] * 37, [(97 * i) % 700 + 1 for i in range(37)], 2, 4),
+                                               ([2], [9001], 2, 7), ([64], [6000], 1, 4), ([1] * 300, [3 + i % 50 for i in range(300)], 1, 1)],
+                         ids=["long", "many", "two", "chunk", "r300"])
+def test_attention_work_cut_over_keys(dev, dtype, new, lens, kv, group):
+    run_attend(dev, new, lens, kv, group, 128 if kv == 2 else 64, 16, dtype, weights=True, fill=float("inf"))
+
+
+def test_large_scores_and_ties(dev):
+    # a few keys dominate; the running maximum moves late, then by a lot
+    from catopt_b200 import ops
+
+    d, n = 64, 700
+    c = ref.make_cache([n], 1, 16, d, F32, dev, 3)
+    for pool in ("k", "v"):
+        c[pool] = c[pool].to(BF)
+    c["k"][c["table"][0, 600 // 16].long(), 0, 600 % 16] = 6.0
+    q = torch.full((1, 2, d), 2.0, dtype=BF, device=dev)
+    q[0, 1] = -2.0
+    o = ops.om_paged_fwd(q, c["k"], c["v"], c["table"], c["lens"], ref.offsets([1], dev), 1, max_k=n, scale=1.0)
+    want, tol, _, _ = ref.attend(q, c, [1], [n], 1.0, True)
+    close(o, want, tol, "o")
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+def test_attention_same_bits_and_untouched_rows(dev, dtype):
+    from catopt_b200 import ops
+
+    new, lens = [1, 60, 1, 16], [900, 500, 40, 2000]
+    c, q, o, _ = run_attend(dev, new, lens, 2, 4, 64, 16, dtype)
+    cu = ref.offsets(new, dev)
+    more = torch.cat([q, torch.full((5, *q.shape[1:]), float("nan"), dtype=dtype, device=dev)])
+    out = torch.full_like(more, 7.0)
+    again = ops.om_paged_fwd(more, c["k"], c["v"], c["table"], c["lens"], cu, 60, max_k=2000, out=out)
+    assert again is out
+    assert torch.equal(out[:q.shape[0]], o) and (out[q.shape[0]:] == 7.0).all()
+
+
+def test_attention_graph_follows_lengths(dev):
+    """A captured call reads lengths, offsets and table when it is replayed; two graphs share nothing."""
+    from catopt_b200 import ops
+
+    lens = [300, 90]
+    c = ref.make_cache(lens, 2, 16, 64, BF, dev, 5)
+    q = torch.randn(6, 8, 64, device=dev).to(BF)
+    cu = ref.offsets([1, 5], dev)
+    w = torch.zeros(c["k"].shape[:3], device=dev)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    outs, graphs = [], []
+    with torch.cuda.stream(stream):
+        for _ in range(2):
+            ops.om_paged_fwd(q, c["k"], c["v"], c["table"], c["lens"], cu, 5, max_k=300, weights=w)
+        for _ in range(2):
+            gph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(gph, stream=stream):
+                outs.append(ops.om_paged_fwd(q, c["k"], c["v"], c["table"], c["lens"], cu, 5, max_k=300, weights=w))
+            graphs.append(gph)
+    torch.cuda.synchronize()
+    for new, lens in (([1, 5], [300, 90]), ([4, 2], [77, 10]), ([6, 0], [250, 0])):
+        c["lens"].copy_(torch.tensor(lens, dtype=torch.int32))
+        cu.copy_(ref.offsets(new, dev))
+        w.zero_()
+        for gph in graphs:
+            gph.replay()
+        torch.cuda.synchronize()
+        ops.check_device_status(dev)
+        want, tol, ww, wtol = ref.attend(q, c, new, lens, 0.125, True)
+        for o in outs:
+            close(o, want, tol, "o")
+        close(w, 2 * ww, 2 * wtol + 4 * ref.U32 * ww, "weights")
+
+
+def test_bad_indices_are_reported(dev):
+    from catopt_b200 import B200Error, ops
+
+    for dtype in (BF, F32):
+        c = ref.make_cache([40, 70], 2, 16, 64, dtype, dev, 6, fill=0.0)
+        q = torch.randn(3, 4, 64, device=dev).to(dtype)
+        cu = ref.offsets([1, 2], dev)
+        good = ops.om_paged_fwd(q, c["k"], c["v"], c["table"], c["lens"], cu, 2)
+        ops.check_device_status(dev)
+
+        def bad(table=None, lens=None, cu_q=None):
+            o = ops.om_paged_fwd(q, c["k"], c["v"], c["table"] if table is None else table, c["lens"] if lens is None else lens,
+                                 cu if cu_q is None else cu_q, 2)
+            with pytest.raises(B200Error, match="index"):
+                ops.check_device_status(dev)
+            return o
+
+        t = c["table"].clone()
+        t[0, 0] = 1 << 30
+        assert torch.equal(bad(table=t)[1:], good[1:])       # the other request is not touched by it
+        t[0, 0] = -5
+        bad(table=t)
+        bad(lens=torch.tensor([40, 1 << 30], dtype=torch.int32, device=dev))
+        bad(lens=torch.tensor([-3, 70], dtype=torch.int32, device=dev))
+        bad(cu_q=torch.tensor([0, 1, 900], dtype=torch.int32, device=dev))
+        bad(cu_q=torch.tensor([-7, 1, 3], dtype=torch.int32, device=dev))
+        k = torch.randn(3, 2, 64, device=dev).to(dtype)
+        t = c["table"].clone()
+        t[1, 4] = c["k"].shape[0]
+        before = c["k"].clone()
+        ops.paged_append(None, k, k, c["k"], c["v"], t, c["lens"], cu)
+        with pytest.raises(B200Error, match="index"):
+            ops.check_device_status(dev)
+        changed = (c["k"] != before).any(-1).any(1).sum().item()
+        assert changed == 1                                    # request 0's token; request 1's have no page
+
+
+# --------------------------------------------------------------------------- append
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("new,start", [([1], [0]), ([3, 0, 1, 20], [5, 0, 16, 30]), ([700, 1, 2500], [0, 31, 8])],
+                         ids=["one", "ragged", "many"])
+@pytest.mark.parametrize("d,rot,interleaved,norm", [(128, 128, False, True), (80, 40, True, False), (64, 0, False, True),
+                                                    (40, 20, False, True), (128, 96, True, True)])
+@pytest.mark.parametrize("strided", [False, True], ids=["dense", "fused"])
+def test_append(dev, dtype, new, start, d, rot, interleaved, norm, strided):
+    from catopt_b200 import ops
+
+    kv, hq, page = 2, 6, 16
+    lens = [a + b if a else 0 for a, b in zip(new, start)]
+    c = ref.make_cache(lens, kv, page, d, dtype, dev, 11, fill=3.0)
+    g = torch.Generator(device=dev).manual_seed(d)
+    n = sum(new)
+    extra = 4                                    # rows behind the last sequence
+    x = torch.randn(n + extra, hq + 2 * kv, d, generator=g, device=dev).to(dtype)
+    q, k, v = x[:, :hq], x[:, hq:hq + kv], x[:, hq + kv:]
+    if not strided:
+        q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+    qw = kw = cos = sin = pos = None
+    if norm:
+        qw, kw = (1 + 0.2 * torch.randn(d, generator=g, device=dev).to(dtype) for _ in range(2))
+    if rot:
+        ang = torch.rand(5000, rot // 2, generator=g, device=dev) * 6.3
+        cos, sin = ang.cos(), ang.sin()
+        pos = torch.randint(0, 5000, (n + extra,), generator=g, device=dev, dtype=torch.int32)
+    w = torch.rand(c["k"].shape[:3], generator=g, device=dev)
+    before = [t.clone() for t in (c["k"], c["v"], w)]
+    out = torch.full((n + extra, hq, d), 9.0, dtype=dtype, device=dev)
+    cu = ref.offsets(new, dev)
+    got = ops.paged_append(q, k, v, c["k"], c["v"], c["table"], c["lens"], cu, q_weight=qw, k_weight=kw, eps=1e-5, cos=cos, sin=sin,
+                           positions=pos, interleaved=interleaved, weights=w, out=out)
+    ops.check_device_status(dev)
+    wq, tq = ref.turned(q[:n], qw, 1e-5, cos, sin, None if pos is None else pos[:n], interleaved)
+    wk, tk = ref.turned(k[:n], kw, 1e-5, cos, sin, None if pos is None else pos[:n], interleaved)
+    assert got is out
+    close(out[:n], wq, tq, "q")
+    assert (out[n:] == 9.0).all()
+    want_k, want_v, want_w = before
+    tol_k = torch.zeros(want_k.shape, dtype=torch.float64, device=dev)
+    want_k = want_k.double()
+    t = 0
+    for r, x in enumerate(new):
+        for j in range(lens[r] - x, lens[r]):
+            p, s = int(c["table"][r, j // page]), j % page
+            want_k[p, :, s], tol_k[p, :, s], want_v[p, :, s] = wk[t], tk[t], v[t]
+            want_w[p, :, s] = 0
+            t += 1
+    close(c["k"], want_k, tol_k, "k pages")
+    assert torch.equal(c["v"], want_v) and torch.equal(w, want_w)
+
+
+# --------------------------------------------------------------------------- evict
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("lens,budget,first,last", [
+    ([5, 1, 40, 0], 8, 2, 3), ([300, 17, 16, 33], 16, 0, 0), ([700], 200, 4, 64), ([64, 65], 64, 32, 32), ([2500, 1300], 1111, 1, 0),
+    ([9000], 4096, 16, 100), ([20], 1, 0, 1)])
+@pytest.mark.parametrize("kv,d,page", [(2, 64, 16), (3, 40, 8), (1, 128, 128)])
+def test_evict(dev, dtype, lens, budget, first, last, kv, d, page):
+    from catopt_b200 import ops
+
+    need = (budget + page - 1) // page
+    c = ref.make_cache(lens, kv, page, d, dtype, dev, 21, fill=float("nan"), spare=need * len(lens) + 2)
+    g = torch.Generator(device=dev).manual_seed(sum(lens))
+    w = torch.randn(c["k"].shape[:3], generator=g, device=dev)
+    w = torch.where(torch.rand(w.shape, generator=g, device=dev) < 0.3, (w * 2).round() / 2, w)     # ties, and both zeros
+    w[torch.rand(w.shape, generator=g, device=dev) < 0.02] = float("nan")
+    w[torch.rand(w.shape, generator=g, device=dev) < 0.02] = float("inf")
+    to = torch.tensor(c["free"][:need * len(lens)], dtype=torch.int32, device=dev).view(len(lens), need)
+    want = [t.clone() for t in (c["k"], c["v"], w)]
+    kept_want = torch.full((len(lens), kv, budget), -1, dtype=torch.int32)
+    for r, n in enumerate(lens):
+        for h in range(kv):
+            ids = c["table"][r, :(n + page - 1) // page].long()
+            kept = ref.keep(w[ids, h].reshape(-1).cpu(), n, budget, first, last)
+            kept_want[r, h, :len(kept)] = torch.tensor(kept, dtype=torch.int32)
+            j = torch.tensor(kept, device=dev, dtype=torch.long)
+            i = torch.arange(len(kept), device=dev)
+            for t in want:
+                t[to[r].long()[i // page], h, i % page] = t[ids[j // page], h, j % page]
+    kept, new_lens = ops.paged_evict(c["k"], c["v"], w, c["table"], c["lens"], to, budget, keep_first=first, keep_last=last)
+    ops.check_device_status(dev)
+    assert torch.equal(kept.cpu(), kept_want)
+    assert new_lens.tolist() == [min(n, budget) for n in lens]
+    bits = {2: torch.int16, 4: torch.int32}
+    for got, exp in zip((c["k"], c["v"], w), want):
+        assert torch.equal(got.view(bits[got.element_size()]), exp.view(bits[exp.element_size()]))

@@ -1,0 +1,77 @@
+"""Paged-cache operators without a GPU: what the entry points refuse."""
+import ctypes as C
+
+import pytest
+import torch
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from catopt_b200 import _lib, build
+
+    build.build()
+    return _lib.load()
+
+
+P = 4096        # a non-null, aligned address; never read, every call here is refused before a launch
+
+ATTEND = dict(q=P, qt=256, qh=64, k=P, v=P, ks=2 * 16 * 64, vs=2 * 16 * 64, o=P, w=None, table=P, lens=P, cu=P, n=8, R=2, Hq=4,
+              Hkv=2, d=64, page=16, n_pages=4, max_pages=2, max_q=4, max_k=32, scale=0.125, causal=1, dtype=1, scratch=P,
+              bytes=1 << 30, status=None, stream=None)
+APPEND = dict(q=P, qt=256, qh=64, k=P, kt=128, kh=64, v=P, vt=128, vh=64, out=P, kp=P, vp=P, ks=2048, vs=2048, w=None, table=P,
+              lens=P, cu=P, pos=P, qw=None, kw=None, eps=1e-6, cos=P, sin=P, rows=8, rot=64, inter=0, n=8, R=2, Hq=4, Hkv=2, d=64,
+              page=16, n_pages=4, max_pages=2, dtype=1, status=None, stream=None)
+EVICT = dict(k=P, v=P, ks=2048, vs=2048, w=P, table=P, lens=P, to=P, kept=P, new=P, R=2, Hkv=2, d=64, page=16, n_pages=4,
+             max_pages=2, new_pages=1, max_k=32, budget=8, first=2, last=2, dtype=1, status=None, stream=None)
+NULL, SHAPE, ALIGN, DTYPE, SCRATCH = 6, 1, 2, 3, 7
+
+
+@pytest.mark.parametrize("change,want", [
+    (dict(k=None), NULL), (dict(table=None), NULL), (dict(q=None), NULL), (dict(scratch=None), NULL), (dict(n=-1), SHAPE),
+    (dict(R=0), SHAPE), (dict(Hq=3), SHAPE), (dict(Hkv=0), SHAPE), (dict(d=60), SHAPE), (dict(d=136), SHAPE), (dict(page=12), SHAPE),
+    (dict(page=4), SHAPE), (dict(page=2048), SHAPE), (dict(max_k=33), SHAPE), (dict(max_k=0), SHAPE), (dict(max_q=-1), SHAPE),
+    (dict(n_pages=0), SHAPE), (dict(scale=0.0), SHAPE), (dict(scale=float("nan")), SHAPE), (dict(scale=float("inf")), SHAPE),
+    (dict(ks=2040), SHAPE), (dict(n=1 << 30), SHAPE), (dict(dtype=7), DTYPE), (dict(q=P + 2), ALIGN), (dict(qt=252), ALIGN),
+    (dict(v=P + 8), ALIGN), (dict(bytes=16), SCRATCH),
+], ids=str)
+def test_attention_refusals(lib, change, want):
+    assert lib.cb2_om_paged_fwd(*{**ATTEND, **change}.values()) == want
+
+
+@pytest.mark.parametrize("change,want", [
+    (dict(k=None), NULL), (dict(out=None), NULL), (dict(cos=None), NULL), (dict(pos=None), NULL), (dict(cu=None), NULL),
+    (dict(rot=66), SHAPE), (dict(rot=3), SHAPE), (dict(rows=0), SHAPE), (dict(d=4), SHAPE), (dict(page=17), SHAPE),
+    (dict(eps=-1.0), SHAPE), (dict(eps=float("nan")), SHAPE), (dict(vs=8), SHAPE), (dict(n=-4), SHAPE), (dict(kt=-128), SHAPE),
+    (dict(dtype=2), DTYPE), (dict(kt=130), ALIGN), (dict(vp=P + 4), ALIGN), (dict(qw=P + 2), ALIGN),
+], ids=str)
+def test_append_refusals(lib, change, want):
+    assert lib.cb2_paged_append(*{**APPEND, **change}.values()) == want
+
+
+@pytest.mark.parametrize("change,want", [
+    (dict(w=None), NULL), (dict(kept=None), NULL), (dict(budget=0), SHAPE), (dict(budget=17), SHAPE), (dict(first=-1), SHAPE),
+    (dict(first=5, last=4), SHAPE), (dict(max_k=40), SHAPE), (dict(R=65536), SHAPE), (dict(page=0), SHAPE), (dict(dtype=5), DTYPE),
+    (dict(k=P + 2), ALIGN), (dict(vs=2052), ALIGN),
+], ids=str)
+def test_evict_refusals(lib, change, want):
+    assert lib.cb2_paged_evict(*{**EVICT, **change}.values()) == want
+
+
+def test_no_tokens_is_no_launch(lib):
+    assert lib.cb2_om_paged_fwd(*{**ATTEND, "n": 0, "q": None, "o": None, "scratch": None, "bytes": 0}.values()) == 0
+    assert lib.cb2_paged_append(*{**APPEND, "n": 0, "q": None, "k": None, "v": None}.values()) == 0
+    assert lib.cb2_om_paged_scratch_bytes(0, 2, 4, 2, 64, 1, 32, 0, 1) == 0
+    assert "index" in lib.cb2_status_str(C.c_int(8)).decode()
+
+
+def test_host_tensors_are_refused():
+    from catopt_b200 import B200Error, ops
+
+    pool = torch.zeros(2, 2, 16, 64)
+    i = torch.zeros(1, 1, dtype=torch.int32)
+    with pytest.raises(B200Error):
+        ops.om_paged_fwd(torch.zeros(1, 4, 64), pool, pool, i, i[0], torch.zeros(2, dtype=torch.int32), 1)
+    with pytest.raises(B200Error):
+        ops.paged_append(None, torch.zeros(1, 2, 64), torch.zeros(1, 2, 64), pool, pool, i, i[0], torch.zeros(2, dtype=torch.int32))
+    with pytest.raises(B200Error):
+        ops.paged_evict(pool, pool, pool[..., 0], i, i[0], i, 4)
