@@ -35,6 +35,7 @@ SOURCES = [
     "om_causal_tc.cu",
     "device_wait.cu",
     "om_paged.cu",
+    "om_paged_tc.cu",
     "paged_append.cu",
     "paged_evict.cu",
 ]

@@ -27,13 +27,6 @@ __device__ __forceinline__ void store4(__nv_bfloat16* p, float4 v) {
   *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
 }
 
-struct PagedRows {
-  const void* q;
-  long long q_token, q_head;   // strides in elements
-  int G, Hkv;
-  float scale_log2e;
-};
-
 // Rows [row0, row0 + kRT) of (request, kv head) as fp32 in shared memory, zeros past the last.
 template <class T>
 __device__ __forceinline__ void load_rows(float* Qs, int ld, const PagedRows& rows, const PagedReq& q, int h, int row0, int d) {
@@ -95,7 +88,7 @@ __device__ __forceinline__ int last_slot(const PagedReq& q, int row, int G, int 
 
 template <class T>
 __global__ void __launch_bounds__(kThreads)
-paged_fma_kernel(PagedRows rows, PagedPools pools, PagedBatch batch, PagedCost<kRT, kKB> cost, T* __restrict__ o,
+paged_fma_kernel(const PagedRows rows, const PagedPools pools, const PagedBatch batch, const PagedCost<kRT, kKB> cost, T* __restrict__ o,
                  float* __restrict__ lse2, PagedScratch scratch) {
   extern __shared__ __align__(16) float sm[];
   __shared__ PagedFindSmem find;
@@ -207,7 +200,7 @@ paged_fma_kernel(PagedRows rows, PagedPools pools, PagedBatch batch, PagedCost<k
         if (lse2 && lane == 0) lse2[at] = lr > 0.f ? ml[rr] + log2f(lr) : INFINITY;
       }
     } else {
-      if (tid == 0 && w.b0 == 0) paged_write_join(w, share, cta, n_cta, scratch.joins);
+      if (tid == 0 && w.b0 == 0) paged_write_join(w, share.total, cta, n_cta, scratch.joins);
       float* slot = scratch.parts + paged_slot_floats(kRT, d) * (2 * cta + (w.b0 == 0));
       if (tid < kRT) {
         slot[tid] = ml[tid];
@@ -320,43 +313,65 @@ paged_weights_fma_kernel(PagedRows rows, PagedPools pools, PagedBatch batch, Pag
 constexpr int kFmaCtas = kNumSMs * 3;
 
 struct Plan {
-  bool weights;
-  size_t fma, lse, total;
+  size_t lse, parts, total;
 };
 
 size_t up16(size_t n) { return (n + 15) & ~size_t(15); }
 
-Plan plan(int n_tokens, int Hq, int d, bool weights) {
+Plan plan(int n_tokens, int Hq, int d, bool weights, int dtype) {
   Plan p;
-  p.weights = weights;
   p.lse = weights ? up16(size_t(n_tokens) * Hq * 4) : 0;
-  p.fma = up16(paged_scratch_bytes(kFmaCtas, kRT, d));
-  p.total = p.lse + p.fma;
+  p.parts = up16(dtype == CB2_BF16 ? paged_tc_scratch_bytes(d) : paged_scratch_bytes(kFmaCtas, kRT, d));
+  p.total = p.lse + p.parts;
   return p;
 }
 
 template <class T>
-int run(const PagedRows& rows, const PagedPools& pools, const PagedBatch& batch, const PagedCost<kRT, kKB>& cost, T* o,
-        float* weights, char* scratch, const Plan& p, int max_q, cudaStream_t st) {
+int join(int rt, int n_cta, const PagedScratch& ws, T* o, float* lse2, const PagedBatch& batch, const PagedRows& rows, int d,
+         cudaStream_t st) {
+  paged_combine_kernel<T><<<dim3(n_cta, rt / 16), 512, 0, st>>>(rt, ws, o, lse2, batch, rows.G, rows.Hkv, d);
+  CB2_LAUNCH_CHECK();
+  return CB2_OK;
+}
+
+template <class T>
+int fma_weights(const PagedRows& rows, const PagedPools& pools, const PagedBatch& batch, const PagedCost<kRT, kKB>& cost,
+                const float* lse2, float* weights, cudaStream_t st) {
+  const int ld = pools.d + 4, smem = (kRT * ld + kKB * ld + 8 * kKB) * 4;
+  if (cudaFuncSetAttribute(paged_weights_fma_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return CB2_LAUNCH_FAIL;
+  const dim3 grid((batch.max_k + kKB - 1) / kKB, rows.Hkv, batch.R < 256 ? batch.R : 256);
+  paged_weights_fma_kernel<T><<<grid, kThreads, smem, st>>>(rows, pools, batch, cost, lse2, weights);
+  CB2_LAUNCH_CHECK();
+  return CB2_OK;
+}
+
+int run_f32(const PagedRows& rows, const PagedPools& pools, const PagedBatch& batch, int causal, float* o, float* weights,
+            char* scratch, const Plan& p, cudaStream_t st) {
+  const PagedCost<kRT, kKB> cost{rows.G, rows.Hkv, causal, kPagedAll, 0};
   float* lse2 = weights ? reinterpret_cast<float*>(scratch) : nullptr;
   const PagedScratch ws = paged_scratch(scratch + p.lse, kFmaCtas);
   const int d = pools.d, ld = d + 4;
   const int smem = (kRT * ld + kKB * ld + kKB * d + kRT * (kKB + 4) + kRT) * 4;
-  if (cudaFuncSetAttribute(paged_fma_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+  if (cudaFuncSetAttribute(paged_fma_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return CB2_LAUNCH_FAIL;
-  paged_fma_kernel<T><<<kFmaCtas, kThreads, smem, st>>>(rows, pools, batch, cost, o, lse2, ws);
+  paged_fma_kernel<float><<<kFmaCtas, kThreads, smem, st>>>(rows, pools, batch, cost, o, lse2, ws);
   CB2_LAUNCH_CHECK();
-  paged_combine_kernel<T><<<dim3(kFmaCtas, kRT / 16), 512, 0, st>>>(kRT, ws, o, lse2, batch, rows.G, rows.Hkv, d);
-  CB2_LAUNCH_CHECK();
-  if (weights) {
-    const int wsmem = (kRT * ld + kKB * ld + 8 * kKB) * 4;
-    if (cudaFuncSetAttribute(paged_weights_fma_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, wsmem) != cudaSuccess)
-      return CB2_LAUNCH_FAIL;
-    const dim3 grid((batch.max_k + kKB - 1) / kKB, rows.Hkv, batch.R < 256 ? batch.R : 256);
-    paged_weights_fma_kernel<T><<<grid, kThreads, wsmem, st>>>(rows, pools, batch, cost, lse2, weights);
-    CB2_LAUNCH_CHECK();
-  }
-  return CB2_OK;
+  int rc = join(kRT, kFmaCtas, ws, o, lse2, batch, rows, d, st);
+  if (rc == CB2_OK && weights) rc = fma_weights<float>(rows, pools, batch, cost, lse2, weights, st);
+  return rc;
+}
+
+int run_bf16(const PagedRows& rows, const PagedPools& pools, const PagedBatch& batch, int causal, __nv_bfloat16* o, float* weights,
+             char* scratch, const Plan& p, cudaStream_t st) {
+  float* lse2 = weights ? reinterpret_cast<float*>(scratch) : nullptr;
+  PagedScratch ws;
+  int n_cta, rt;
+  int rc = paged_tc_run(rows, pools, batch, causal, 0, o, lse2, scratch + p.lse, &ws, &n_cta, &rt, st);
+  if (rc == CB2_OK) rc = join(rt, n_cta, ws, o, lse2, batch, rows, pools.d, st);
+  const PagedCost<kRT, kKB> cost{rows.G, rows.Hkv, causal, kPagedAll, 0};
+  if (rc == CB2_OK && weights) rc = fma_weights<__nv_bfloat16>(rows, pools, batch, cost, lse2, weights, st);
+  return rc;
 }
 
 bool sizes_ok(int n_tokens, int R, int Hq, int Hkv, int d, int max_q, int max_k) {
@@ -373,7 +388,7 @@ extern "C" size_t cb2_om_paged_scratch_bytes(int n_tokens, int R, int Hq, int Hk
   using namespace cb2;
   if (!sizes_ok(n_tokens, R, Hq, Hkv, d, max_q, max_k) || n_tokens == 0) return 0;
   if (dtype != CB2_F32 && dtype != CB2_BF16) return 0;
-  return plan(n_tokens, Hq, d, weights != 0).total;
+  return plan(n_tokens, Hq, d, weights != 0, dtype).total;
 }
 
 extern "C" int cb2_om_paged_fwd(const void* q, long long q_token_stride, long long q_head_stride, const void* k_pages,
@@ -396,17 +411,15 @@ extern "C" int cb2_om_paged_fwd(const void* q, long long q_token_stride, long lo
   if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(o) || !aligned16(scratch) ||
       q_token_stride % vec || q_head_stride % vec || k_page_stride % vec || v_page_stride % vec)
     return CB2_BAD_ALIGN;
-  const Plan p = plan(n_tokens, Hq, d, weights != nullptr);
+  const Plan p = plan(n_tokens, Hq, d, weights != nullptr, dtype);
   if (scratch_bytes < p.total) return CB2_SCRATCH_TOO_SMALL;
   int page_log2 = 0;
   while ((1 << page_log2) < page_size) ++page_log2;
   const PagedBatch batch{block_table, seq_lens, cu_q, R, max_pages, n_pages, page_log2, n_tokens, max_k, dev_status};
   const PagedPools pools{k_pages, v_pages, k_page_stride, v_page_stride, Hkv, d};
   const PagedRows rows{q, q_token_stride, q_head_stride, Hq / Hkv, Hkv, scale * 1.4426950408889634f};
-  const PagedCost<kRT, kKB> cost{Hq / Hkv, Hkv, causal != 0, kPagedAll, 0};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   char* ws = static_cast<char*>(scratch);
-  if (dtype == CB2_BF16)
-    return run(rows, pools, batch, cost, static_cast<__nv_bfloat16*>(o), weights, ws, p, max_q, st);
-  return run(rows, pools, batch, cost, static_cast<float*>(o), weights, ws, p, max_q, st);
+  if (dtype == CB2_BF16) return run_bf16(rows, pools, batch, causal != 0, static_cast<__nv_bfloat16*>(o), weights, ws, p, st);
+  return run_f32(rows, pools, batch, causal != 0, static_cast<float*>(o), weights, ws, p, st);
 }

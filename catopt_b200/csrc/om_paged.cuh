@@ -35,6 +35,13 @@ struct PagedPools {
   int Hkv, d;
 };
 
+struct PagedRows {
+  const void* q;
+  long long q_token, q_head;   // strides in elements
+  int G, Hkv;
+  float scale_log2e;
+};
+
 struct PagedReq {
   int t0, n, len;     // first row in q, new tokens, cached keys
 };
@@ -197,19 +204,28 @@ __device__ PagedShare paged_find_share(const PagedBatch& b, const Cost& cost, in
 }
 
 // Walks the pieces of a share: piece = blocks [b0, b1) of the nb blocks of unit (r, h, tile).
-// Every thread of a warp keeps the same walk.
-template <class Cost>
-struct PagedWalk {
-  const PagedBatch& batch;
-  const Cost& cost;
-  long long cur, hi, per_head;
+// Every thread of a warp keeps the same walk; the state may rest in shared memory between uses.
+struct PagedWalkState {
+  long long cur, hi;
   PagedReq q;
   int r, h, tile, nb, b0, b1;
+};
 
-  __device__ PagedWalk(const PagedBatch& b, const Cost& c, const PagedShare& s) : batch(b), cost(c), cur(s.lo), hi(s.hi), r(s.r) {
+template <class Cost>
+struct PagedWalk : PagedWalkState {
+  const PagedBatch& batch;
+  const Cost& cost;
+
+  __device__ PagedWalk(const PagedBatch& b, const Cost& c, const PagedWalkState& s) : PagedWalkState(s), batch(b), cost(c) {}
+  __device__ PagedWalk(const PagedBatch& b, const Cost& c, const PagedShare& s) : batch(b), cost(c) {
+    cur = s.lo;
+    hi = s.hi;
+    r = s.r;
+    h = tile = nb = b0 = b1 = 0;
+    q = PagedReq{0, 0, 0};
     if (cur >= hi) return;
     q = paged_request(b, r);
-    per_head = cost.before(q, cost.tiles(q));
+    const long long per_head = cost.before(q, cost.tiles(q));
     h = int(s.off / per_head);
     const long long rest = s.off - h * per_head;
     // last tile whose start is <= rest: 32 candidates a round, one per lane
@@ -217,8 +233,7 @@ struct PagedWalk {
     const int lane = threadIdx.x & 31;
     while (n > 1) {
       const int step = (n + 31) / 32;
-      const int cand = lo + lane * step;
-      const bool le = lane * step < n && cost.before(q, cand) <= rest;
+      const bool le = lane * step < n && cost.before(q, lo + lane * step) <= rest;
       const int k = 31 - __clz(__ballot_sync(0xffffffffu, le));
       n = min(step, n - k * step);
       lo += k * step;
@@ -261,14 +276,13 @@ __device__ __forceinline__ float ex2_approx(float x) {
   return y;
 }
 
-template <class Walk>
-__device__ __forceinline__ void paged_write_join(const Walk& w, const PagedShare& s, int cta, int n_cta, PagedJoin* joins) {
+__device__ __forceinline__ void paged_write_join(const PagedWalkState& w, long long total, int cta, int n_cta, PagedJoin* joins) {
   // called for a piece with b0 == 0 and b1 < nb: the unit's last block sits at cur + nb - 1
   PagedJoin j;
   j.r = w.r;
   j.h = w.h;
   j.tile = w.tile;
-  j.last = int(((w.cur + w.nb) * n_cta - 1) / s.total);
+  j.last = int(((w.cur + w.nb) * n_cta - 1) / total);
   joins[cta] = j;
 }
 
@@ -288,5 +302,11 @@ inline PagedScratch paged_scratch(void* base, int n_cta) {
   s.parts = reinterpret_cast<float*>(static_cast<char*>(base) + 16 + size_t(n_cta) * sizeof(PagedJoin));
   return s;
 }
+
+// om_paged_tc.cu: requests of more than `few` packed rows (bf16), on the tensor cores.  What it leaves for
+// the join: row tiles of *rt rows, *n_cta shares.
+size_t paged_tc_scratch_bytes(int d);
+int paged_tc_run(const PagedRows& rows, const PagedPools& pools, const PagedBatch& batch, int causal, int few, void* o,
+                 float* lse2, void* scratch, PagedScratch* parts, int* n_cta, int* rt, cudaStream_t st);
 
 }  // namespace cb2

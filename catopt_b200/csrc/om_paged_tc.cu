@@ -1,0 +1,436 @@
+// Attention over a paged key/value cache on the tensor cores (bf16), for requests with many packed rows
+// (chunks of prompts): the work line of om_paged.cuh with tiles of 128 packed rows and 128-key blocks.
+//
+// A CTA keeps two to an SM (half of the tensor memory and of the shared memory each), so one's softmax runs
+// while the other's products are on the tensor core, and walks its share of the line:
+//   MMA1  S = Q K_j^T -> TMEM;   P = 2^(S scale - m) as bf16 over S, l and the running m in registers (thread
+//   = row = TMEM lane);   MMA2  O += P V_j with P read from TMEM.
+// The reference point m follows the maximum lazily (when it moved by more than 2^8), so O is rarely rescaled.
+// Only a block that some row of the tile may not see whole is masked, per element.  Of the last block of a
+// request the value rows behind its length are zeroed in shared memory, since 0 x NaN is NaN.
+//
+// Roles: warp 0 = loads (pages by TMA: one box per page and 64 columns, each lane its own page; the packed
+// query rows by 16-byte asynchronous copies, since a tile may start inside a token's group), warp 1 = MMA issue
+// and TMEM owner, warps 2..5 = softmax.  The pieces of a share are listed in shared memory in batches, so that
+// the softmax threads spend no registers on the walk.  Every wait is bounded.
+#include "om_paged.cuh"
+#include "umma.cuh"
+
+namespace cb2 {
+namespace {
+
+constexpr int kRT = 128, kKB = 128;
+constexpr int kThreads = 192;
+constexpr int kBatch = 32;                // pieces listed at a time
+constexpr uint32_t kTile = umma::kTileBytes;
+constexpr uint32_t kOffQ = 0, kOffK = kTile, kOffV = 2 * kTile;
+constexpr uint32_t kOffBars = 3 * kTile;
+constexpr int kNumBars = 10;
+constexpr uint32_t kColS = 0, kColO = 128, kTmemCols = 256;
+
+struct Piece {
+  int r, h, row0, t0, n, len, b0, b1;
+  int whole;      // the unit's blocks all lie in this share
+};
+
+struct Smem {
+  uint32_t tmem;
+  int abort;
+  int count;      // pieces listed; more follow if count == kBatch
+  int loads_k, loads_v;     // issued so far
+  PagedWalkState walk;
+  long long total;
+  Piece pieces[kBatch];
+  PagedFindSmem find;
+};
+constexpr uint32_t kOffMisc = kOffBars + kNumBars * 8;
+constexpr uint32_t kSmemBytes = kOffMisc + uint32_t(sizeof(Smem)) + 1024;
+static_assert(2 * kSmemBytes <= 227 * 1024, "two CTAs per SM");
+
+struct TcArgs {
+  const __nv_bfloat16* q;
+  long long q_token, q_head;
+  __nv_bfloat16* o;
+  float* lse2;
+  float scale_log2e;
+  int G, Hkv, d;
+};
+
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* m, int x, int y, int z, int w, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+          smem_u32(dst)),
+      "l"(m), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+      : "memory");
+}
+// 16-byte asynchronous copy that writes zeros when `there` is false.
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+
+__global__ void __launch_bounds__(kThreads, 2)
+paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const TcArgs a,
+                const PagedBatch batch, const PagedCost<kRT, kKB> cost, const PagedScratch scratch) {
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kOffBars);
+  uint64_t *k_full = bars, *k_empty = bars + 1, *v_full = bars + 2, *v_empty = bars + 3, *q_full = bars + 4, *q_empty = bars + 5,
+           *s_ready = bars + 6, *p_ready = bars + 7, *o_done = bars + 8;
+  Smem* sh = reinterpret_cast<Smem*>(smem + kOffMisc);
+  volatile int* s_abort = &sh->abort;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int cta = blockIdx.x, n_cta = gridDim.x;
+
+  if (tid == 0) {
+    mbar_init(k_full, 1);
+    mbar_init(k_empty, 1);
+    mbar_init(v_full, 1);
+    mbar_init(v_empty, 1);
+    mbar_init(q_full, 32);
+    mbar_init(q_empty, 1);
+    mbar_init(s_ready, 1);
+    mbar_init(p_ready, 128);
+    mbar_init(o_done, 1);
+    sh->abort = sh->loads_k = sh->loads_v = 0;
+    scratch.joins[cta].r = -1;
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    __syncwarp();
+    umma::tmem_alloc(&sh->tmem, kTmemCols);
+  }
+  {
+    const PagedShare share = paged_find_share<kThreads>(batch, cost, cta, n_cta, &sh->find);
+    if (cta == 0 && tid == 0) *scratch.total = share.total;
+    if (warp == 0) {
+      const PagedWalk<PagedCost<kRT, kKB>> walk(batch, cost, share);
+      if (lane == 0) {
+        sh->walk = walk;
+        sh->total = share.total;
+      }
+    }
+  }
+  umma::fence_before_sync();
+  __syncthreads();
+  umma::fence_after_sync();
+  const uint32_t tmem = sh->tmem;
+  const uint32_t q_addr = smem_u32(smem + kOffQ), k_addr = smem_u32(smem + kOffK), v_addr = smem_u32(smem + kOffV);
+  const int d = a.d, halves = (d + 63) >> 6;
+
+  uint32_t n_blk = 0, n_piece = 0;        // blocks and pieces this role has gone through: the barriers' phases
+  for (;;) {
+    if (warp == 0) {
+      PagedWalk<PagedCost<kRT, kKB>> walk(batch, cost, sh->walk);
+      __syncwarp();
+      int count = 0;
+      for (; count < kBatch && walk.valid(); ++count, walk.next()) {
+        walk.clip();
+        if (lane == 0) {
+          const bool whole = walk.b0 == 0 && walk.b1 == walk.nb;
+          sh->pieces[count] = Piece{walk.r, walk.h, walk.tile * kRT, walk.q.t0, walk.q.n, walk.q.len, walk.b0, walk.b1, whole};
+          if (walk.b0 == 0 && !whole) paged_write_join(walk, sh->total, cta, n_cta, scratch.joins);
+        }
+      }
+      if (lane == 0) {
+        sh->count = count;
+        sh->walk = walk;
+      }
+    }
+    __syncthreads();
+    const int count = sh->count;
+
+    if (warp == 0) {
+      const int ps_log2 = batch.page_log2, box_log2 = min(ps_log2, 7), boxes = kKB >> box_log2;
+      for (int p = 0; p < count; ++p, ++n_piece) {
+        const Piece pc = sh->pieces[p];
+        const int blocks = pc.b1 - pc.b0;
+        auto load_block = [&](int j, const CUtensorMap* map, unsigned char* dst, uint64_t* full, uint64_t* empty) -> bool {
+          const int k0 = (pc.b0 + j) * kKB;
+          const bool mine = lane < boxes && k0 + (lane << box_log2) < pc.len;
+          int page = 0;
+          if (mine) page = paged_page(batch, pc.r, (k0 + (lane << box_log2)) >> ps_log2);
+          const unsigned have = __ballot_sync(0xffffffffu, mine);
+          bool ok = true;
+          if (n_blk + j > 0) ok = mbar_wait_abortable(empty, (n_blk + j - 1) & 1, s_abort);
+          if (!__all_sync(0xffffffffu, ok)) return false;
+          const uint32_t box_bytes = 128u << box_log2;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(full, __popc(have) * halves * box_bytes);
+            ++*(full == k_full ? &sh->loads_k : &sh->loads_v);
+          }
+          __syncwarp();
+          if (mine) {
+            const int y = k0 & ((1 << ps_log2) - 1);       // inside the page when pages are longer than a block
+            for (int hf = 0; hf < halves; ++hf)
+              tma_load_4d(dst + hf * umma::kSubTileBytes + lane * box_bytes, map, hf * 64, ps_log2 > 7 ? y : 0, pc.h, page, full);
+          }
+          return true;
+        };
+        if (!load_block(0, &map_k, smem + kOffK, k_full, k_empty)) break;
+        // the packed rows of the tile
+        bool ok = n_piece == 0 || mbar_wait_abortable(q_empty, (n_piece - 1) & 1, s_abort);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        const int chunks = halves * 8, rows = pc.n * a.G - pc.row0;
+        for (int e = lane; e < kRT * chunks; e += 32) {
+          const int rr = e / chunks, col = (e % chunks) * 8;
+          const bool there = rr < rows && col < d;
+          const int row = pc.row0 + (there ? rr : 0);
+          const __nv_bfloat16* src = a.q + (pc.t0 + row / a.G) * a.q_token + (pc.h * a.G + row % a.G) * a.q_head + (there ? col : 0);
+          cp_async16_or_zero(q_addr + umma::tile_chunk_offset(rr, col), src, there);
+        }
+        cp_async_commit();
+        cp_async_wait_all();
+        fence_proxy_async_smem();
+        mbar_arrive(q_full);
+        if (!load_block(0, &map_v, smem + kOffV, v_full, v_empty)) break;
+        bool fine = true;
+        for (int j = 1; fine && j < blocks; ++j)
+          fine = load_block(j, &map_k, smem + kOffK, k_full, k_empty) && load_block(j, &map_v, smem + kOffV, v_full, v_empty);
+        if (!fine) break;
+        n_blk += blocks;
+      }
+    } else if (warp == 1) {
+      if (lane == 0) {
+        const int ksteps = (d + 15) >> 4;
+        constexpr uint32_t idesc_kk = umma::instr_desc_bf16(128, 128, false, false);
+        const uint32_t idesc_kn = umma::instr_desc_bf16(128, uint32_t(d + 15) & ~15u, false, true);
+        for (int p = 0; p < count; ++p, ++n_piece) {
+          const int blocks = sh->pieces[p].b1 - sh->pieces[p].b0;
+          auto issue_scores = [&](int j) -> bool {
+            if (!mbar_wait_abortable(k_full, (n_blk + j) & 1, s_abort)) return false;
+            umma::fence_after_sync();
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks)
+              if (ks < ksteps)
+                umma::mma_bf16(tmem + kColS, umma::desc_kmajor(q_addr, ks), umma::desc_kmajor(k_addr, ks), idesc_kk, ks > 0);
+            umma::mma_commit(s_ready);
+            umma::mma_commit(k_empty);
+            if (j == blocks - 1) umma::mma_commit(q_empty);
+            return true;
+          };
+          bool ok = mbar_wait_abortable(q_full, n_piece & 1, s_abort) && issue_scores(0);
+          for (int j = 0; ok && j < blocks; ++j) {
+            ok = mbar_wait_abortable(p_ready, (n_blk + j) & 1, s_abort) && mbar_wait_abortable(v_full, (n_blk + j) & 1, s_abort);
+            if (!ok) break;
+            umma::fence_after_sync();
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks)
+              umma::mma_bf16_ts(tmem + kColO, tmem + kColS + ks * 8, umma::desc_mnmajor(v_addr, ks), idesc_kn, j > 0 || ks > 0);
+            umma::mma_commit(o_done);
+            umma::mma_commit(v_empty);
+            // the tensor pipe runs in issue order, so the next scores may overwrite P right away
+            if (j + 1 < blocks) ok = issue_scores(j + 1);
+          }
+          if (!ok) break;
+          n_blk += blocks;
+        }
+      }
+    } else {
+      const int q4 = warp & 3, rr = q4 * 32 + lane;
+      const uint32_t lane_base = tmem + (uint32_t(q4 * 32) << 16);
+      constexpr float kLazy = 8.f;
+      const int ncb = (d + 31) >> 5;
+      const float scale = a.scale_log2e;
+      for (int p = 0; p < count; ++p) {
+        const Piece* pc = &sh->pieces[p];
+        const int blocks = pc->b1 - pc->b0, b0 = pc->b0, len = pc->len;
+        const int rows = pc->n * a.G - pc->row0;                 // of this tile, kRT at most count
+        // last slot this row sees, and the least of the tile's rows
+        const int base = len - pc->n;
+        const int last = cost.causal ? min(base + (pc->row0 + rr) / a.G, len - 1) : len - 1;
+        const int first_last = cost.causal ? min(base + pc->row0 / a.G, len - 1) : len - 1;
+        float m_ref = -INFINITY, l_run = 0.f;
+        uint32_t sv[4][32];
+        bool ok = true;
+        for (int j = 0; j < blocks; ++j) {
+          ok = mbar_wait_abortable(s_ready, (n_blk + j) & 1, s_abort);
+          if (!__all_sync(0xffffffffu, ok)) break;
+          umma::fence_after_sync();
+          const int k0 = (b0 + j) * kKB;
+#pragma unroll
+          for (int cb = 0; cb < 4; ++cb) umma::tmem_ld32(lane_base + kColS + cb * 32, sv[cb]);
+          umma::tmem_wait_ld();
+          if (k0 + kKB - 1 > first_last) {
+            const int lim = last - k0;
+#pragma unroll
+            for (int cb = 0; cb < 4; ++cb)
+#pragma unroll
+              for (int c = 0; c < 32; ++c)
+                if (cb * 32 + c > lim) sv[cb][c] = 0xff800000u;
+          }
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int cb = 0; cb < 4; ++cb)
+#pragma unroll
+            for (int c = 0; c < 32; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(sv[cb][c]));
+          const float m_blk = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
+          float alpha = 1.f;
+          if (m_blk > m_ref + kLazy || m_ref == -INFINITY) {
+            const float m_new = fmaxf(m_ref, m_blk);
+            alpha = (m_new == -INFINITY) ? 1.f : ex2_approx(m_ref - m_new);
+            m_ref = m_new;
+          }
+          const float neg_m = (m_ref == -INFINITY) ? 0.f : -m_ref;
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int cb = 0; cb < 4; ++cb) {
+            uint32_t w[16];
+#pragma unroll
+            for (int c = 0; c < 32; c += 2) {
+              const float p0 = ex2_approx(fmaf(__uint_as_float(sv[cb][c]), scale, neg_m));
+              const float p1 = ex2_approx(fmaf(__uint_as_float(sv[cb][c + 1]), scale, neg_m));
+              sum[(c >> 1) & 3] += p0 + p1;
+              w[c >> 1] = pack_bf16x2(p0, p1);
+            }
+            umma::tmem_st16(lane_base + kColS + cb * 16, w);
+          }
+          l_run = fmaf(l_run, alpha, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+          umma::tmem_wait_st();
+          if (k0 + kKB > len) {
+            // the request's last block: value rows that nobody has written
+            ok = mbar_wait_abortable(v_full, (n_blk + j) & 1, s_abort);
+            if (!__all_sync(0xffffffffu, ok)) break;
+            if (k0 + rr >= len)
+              for (int c = 0; c < halves * 8; ++c)
+                *reinterpret_cast<uint4*>(smem + kOffV + umma::tile_chunk_offset(rr, c * 8)) = make_uint4(0, 0, 0, 0);
+            fence_proxy_async_smem();
+          }
+          if (j > 0) {
+            ok = mbar_wait_abortable(o_done, (n_blk + j - 1) & 1, s_abort);
+            if (!__all_sync(0xffffffffu, ok)) break;
+            umma::fence_after_sync();
+            if (!__all_sync(0xffffffffu, alpha == 1.f)) {
+#pragma unroll
+              for (int cb = 0; cb < 4; ++cb)
+                if (cb < ncb) umma::tmem_ld32(lane_base + kColO + cb * 32, sv[cb]);
+              umma::tmem_wait_ld();
+#pragma unroll
+              for (int cb = 0; cb < 4; ++cb) {
+                if (cb < ncb) {
+#pragma unroll
+                  for (int c = 0; c < 32; ++c) sv[cb][c] = __float_as_uint(__uint_as_float(sv[cb][c]) * alpha);
+                  umma::tmem_st32(lane_base + kColO + cb * 32, sv[cb]);
+                }
+              }
+              umma::tmem_wait_st();
+            }
+          }
+          umma::fence_before_sync();
+          mbar_arrive(p_ready);
+        }
+        if (!__all_sync(0xffffffffu, ok)) break;
+        ok = mbar_wait_abortable(o_done, (n_blk + blocks - 1) & 1, s_abort);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        umma::fence_after_sync();
+        n_blk += blocks;
+#pragma unroll
+        for (int cb = 0; cb < 4; ++cb)
+          if (cb < ncb) umma::tmem_ld32(lane_base + kColO + cb * 32, sv[cb]);
+        umma::tmem_wait_ld();
+        if (rr < rows) {
+          const int row = pc->row0 + rr;
+          if (pc->whole) {
+            const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+            const long long at = (long long)(pc->t0 + row / a.G) * (a.G * a.Hkv) + pc->h * a.G + row % a.G;
+            __nv_bfloat16* dst = a.o + at * d;
+#pragma unroll
+            for (int cb = 0; cb < 4; ++cb) {
+#pragma unroll
+              for (int c = 0; c < 32; c += 8) {
+                if (cb * 32 + c >= d) continue;
+                uint32_t w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  w[i] = pack_bf16x2(__uint_as_float(sv[cb][c + 2 * i]) * inv, __uint_as_float(sv[cb][c + 2 * i + 1]) * inv);
+                *reinterpret_cast<uint4*>(dst + cb * 32 + c) = make_uint4(w[0], w[1], w[2], w[3]);
+              }
+            }
+            if (a.lse2) a.lse2[at] = l_run > 0.f ? m_ref + log2f(l_run) : INFINITY;
+          } else {
+            float* slot = scratch.parts + paged_slot_floats(kRT, d) * (2 * cta + (b0 == 0));
+            slot[rr] = m_ref;
+            slot[kRT + rr] = l_run;
+            float* dst = slot + 2 * kRT + rr * d;
+#pragma unroll
+            for (int cb = 0; cb < 4; ++cb) {
+#pragma unroll
+              for (int c = 0; c < 32; c += 4)
+                if (cb * 32 + c < d)
+                  *reinterpret_cast<uint4*>(dst + cb * 32 + c) = make_uint4(sv[cb][c], sv[cb][c + 1], sv[cb][c + 2], sv[cb][c + 3]);
+            }
+          }
+        }
+      }
+    }
+    // the batch's pieces may be listed anew once every role is through with them
+    __syncwarp();
+    umma::fence_before_sync();
+    __syncthreads();
+    umma::fence_after_sync();
+    if (count < kBatch || *s_abort) break;
+  }
+  if (*s_abort) {
+    // loads in flight land before the shared memory goes (a bounded wait, too)
+    if (tid == 0) {
+      if (sh->loads_k) mbar_wait_bounded(k_full, (sh->loads_k - 1) & 1);
+      if (sh->loads_v) mbar_wait_bounded(v_full, (sh->loads_v - 1) & 1);
+      if (batch.status) atomicExch(batch.status, CB2_WAIT_TIMEOUT);
+    }
+    __syncthreads();
+  }
+  if (warp == 1) {
+    __syncwarp();
+    umma::tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// Pools as a 4-D tensor {d, page_size, Hkv, n_pages}; box = 64 columns of a page, 128 rows at most.
+int make_pool_map(CUtensorMap* out, const void* base, int d, int page_size, int Hkv, int n_pages, long long page_stride) {
+  using Fn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                          const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static Fn fn = nullptr;
+  if (!fn) {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess || !p)
+      return CB2_LAUNCH_FAIL;
+    fn = reinterpret_cast<Fn>(p);
+  }
+  const cuuint64_t dims[4] = {cuuint64_t(d), cuuint64_t(page_size), cuuint64_t(Hkv), cuuint64_t(n_pages)};
+  const cuuint64_t strides[3] = {cuuint64_t(d) * 2, cuuint64_t(page_size) * d * 2, cuuint64_t(page_stride) * 2};
+  const cuuint32_t box[4] = {64, cuuint32_t(page_size < 128 ? page_size : 128), 1, 1};
+  const cuuint32_t step[4] = {1, 1, 1, 1};
+  const CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, step,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? CB2_OK : CB2_LAUNCH_FAIL;
+}
+
+constexpr int kCtas = 2 * kNumSMs;
+
+}  // namespace
+
+size_t paged_tc_scratch_bytes(int d) { return paged_scratch_bytes(kCtas, kRT, d); }
+
+// Requests of more than `few` packed rows; partial carriers are left in `scratch` (kRT rows a slot, kCtas shares).
+int paged_tc_run(const PagedRows& rows, const PagedPools& pools, const PagedBatch& batch, int causal, int few, void* o, float* lse2,
+                 void* scratch, PagedScratch* parts, int* n_cta, int* rt, cudaStream_t st) {
+  CUtensorMap mk, mv;
+  int rc = make_pool_map(&mk, pools.k, pools.d, 1 << batch.page_log2, pools.Hkv, batch.n_pages, pools.k_page_stride);
+  if (rc == CB2_OK) rc = make_pool_map(&mv, pools.v, pools.d, 1 << batch.page_log2, pools.Hkv, batch.n_pages, pools.v_page_stride);
+  if (rc != CB2_OK) return rc;
+  if (cudaFuncSetAttribute(paged_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmemBytes)) != cudaSuccess)
+    return CB2_LAUNCH_FAIL;
+  *parts = paged_scratch(scratch, kCtas);
+  *n_cta = kCtas;
+  *rt = kRT;
+  const TcArgs a{static_cast<const __nv_bfloat16*>(rows.q), rows.q_token, rows.q_head, static_cast<__nv_bfloat16*>(o), lse2,
+                 rows.scale_log2e, rows.G, rows.Hkv, pools.d};
+  const PagedCost<kRT, kKB> cost{rows.G, rows.Hkv, causal, kPagedChunk, few};
+  paged_tc_kernel<<<kCtas, kThreads, kSmemBytes, st>>>(mk, mv, a, batch, cost, *parts);
+  CB2_LAUNCH_CHECK();
+  return CB2_OK;
+}
+
+}  // namespace cb2
