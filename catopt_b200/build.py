@@ -36,6 +36,7 @@ SOURCES = [
     "device_wait.cu",
     "om_paged.cu",
     "om_paged_tc.cu",
+    "om_paged_few.cu",
     "paged_append.cu",
     "paged_evict.cu",
 ]

@@ -312,17 +312,43 @@ paged_weights_fma_kernel(PagedRows rows, PagedPools pools, PagedBatch batch, Pag
 // CTAs of the FMA kernel: three per SM hold its shared memory for d = 128.
 constexpr int kFmaCtas = kNumSMs * 3;
 
-struct Plan {
-  size_t lse, parts, total;
-};
-
 size_t up16(size_t n) { return (n + 15) & ~size_t(15); }
 
-Plan plan(int n_tokens, int Hq, int d, bool weights, int dtype) {
-  Plan p;
+// Which kernels a bf16 call takes.  A request of at most `few` packed rows is bound by reading its keys and
+// goes to the streaming kernel, whose products hold 8 or 16 rows; the others go to the tensor-core tiles.
+struct Plan {
+  int few;                     // 0: no streaming kernel
+  bool chunks;
+  size_t lse, scores, parts, total;
+};
+
+// Attention weight of few rows is summed from scores that the streaming kernel leaves in scratch (4 bytes per
+// row and key, against 2 d bytes for reading the keys again), up to this size.
+constexpr size_t kMostScores = size_t(256) << 20;
+
+Plan plan(int n_tokens, int R, int Hq, int Hkv, int d, int max_q, int max_k, bool weights, int dtype) {
+  Plan p{};
+  const int G = Hq / Hkv;
   p.lse = weights ? up16(size_t(n_tokens) * Hq * 4) : 0;
-  p.parts = up16(dtype == CB2_BF16 ? paged_tc_scratch_bytes(d) : paged_scratch_bytes(kFmaCtas, kRT, d));
-  p.total = p.lse + p.parts;
+  if (dtype == CB2_F32) {
+    p.parts = paged_scratch_bytes(kFmaCtas, kRT, d);
+  } else {
+    const int64_t rows = int64_t(max_q) * G;
+    if (rows <= 16) {
+      p.few = rows <= 8 ? 8 : 16;
+    } else {
+      p.chunks = true;
+      p.few = R == 1 || G > 16 ? 0 : (G <= 8 ? 8 : 16);       // the single tokens of a mixed batch
+    }
+    p.parts = p.chunks ? paged_tc_scratch_bytes(d) : 0;
+    if (p.few && paged_few_scratch_bytes(d) > p.parts) p.parts = paged_few_scratch_bytes(d);   // one after the other
+    if (weights && p.few) {
+      const size_t s = size_t(R) * Hkv * p.few * max_k * 4;
+      p.scores = s <= kMostScores ? up16(s) : 0;
+    }
+  }
+  p.parts = up16(p.parts);
+  p.total = p.lse + p.scores + p.parts;
   return p;
 }
 
@@ -365,12 +391,23 @@ int run_f32(const PagedRows& rows, const PagedPools& pools, const PagedBatch& ba
 int run_bf16(const PagedRows& rows, const PagedPools& pools, const PagedBatch& batch, int causal, __nv_bfloat16* o, float* weights,
              char* scratch, const Plan& p, cudaStream_t st) {
   float* lse2 = weights ? reinterpret_cast<float*>(scratch) : nullptr;
+  float* scores = p.scores ? reinterpret_cast<float*>(scratch + p.lse) : nullptr;
+  char* parts = scratch + p.lse + p.scores;
   PagedScratch ws;
-  int n_cta, rt;
-  int rc = paged_tc_run(rows, pools, batch, causal, 0, o, lse2, scratch + p.lse, &ws, &n_cta, &rt, st);
-  if (rc == CB2_OK) rc = join(rt, n_cta, ws, o, lse2, batch, rows, pools.d, st);
-  const PagedCost<kRT, kKB> cost{rows.G, rows.Hkv, causal, kPagedAll, 0};
-  if (rc == CB2_OK && weights) rc = fma_weights<__nv_bfloat16>(rows, pools, batch, cost, lse2, weights, st);
+  int n_cta, rt, rc = CB2_OK;
+  if (p.chunks) {
+    rc = paged_tc_run(rows, pools, batch, causal, p.few, o, lse2, parts, &ws, &n_cta, &rt, st);
+    if (rc == CB2_OK) rc = join(rt, n_cta, ws, o, lse2, batch, rows, pools.d, st);
+    if (rc == CB2_OK && weights)
+      rc = fma_weights<__nv_bfloat16>(rows, pools, batch, {rows.G, rows.Hkv, causal, kPagedChunk, p.few}, lse2, weights, st);
+  }
+  if (rc == CB2_OK && p.few) {
+    rc = paged_few_run(rows, pools, batch, causal, p.few, o, lse2, scores, parts, &ws, &n_cta, &rt, st);
+    if (rc == CB2_OK) rc = join(rt, n_cta, ws, o, lse2, batch, rows, pools.d, st);
+    if (rc == CB2_OK && scores) rc = paged_few_weights_run(rows, batch, causal, p.few, scores, lse2, weights, st);
+    if (rc == CB2_OK && weights && !scores)
+      rc = fma_weights<__nv_bfloat16>(rows, pools, batch, {rows.G, rows.Hkv, causal, kPagedFew, p.few}, lse2, weights, st);
+  }
   return rc;
 }
 
@@ -388,7 +425,7 @@ extern "C" size_t cb2_om_paged_scratch_bytes(int n_tokens, int R, int Hq, int Hk
   using namespace cb2;
   if (!sizes_ok(n_tokens, R, Hq, Hkv, d, max_q, max_k) || n_tokens == 0) return 0;
   if (dtype != CB2_F32 && dtype != CB2_BF16) return 0;
-  return plan(n_tokens, Hq, d, weights != 0, dtype).total;
+  return plan(n_tokens, R, Hq, Hkv, d, max_q, max_k, weights != 0, dtype).total;
 }
 
 extern "C" int cb2_om_paged_fwd(const void* q, long long q_token_stride, long long q_head_stride, const void* k_pages,
@@ -411,11 +448,11 @@ extern "C" int cb2_om_paged_fwd(const void* q, long long q_token_stride, long lo
   if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(o) || !aligned16(scratch) ||
       q_token_stride % vec || q_head_stride % vec || k_page_stride % vec || v_page_stride % vec)
     return CB2_BAD_ALIGN;
-  const Plan p = plan(n_tokens, Hq, d, weights != nullptr, dtype);
+  const Plan p = plan(n_tokens, R, Hq, Hkv, d, max_q, max_k, weights != nullptr, dtype);
   if (scratch_bytes < p.total) return CB2_SCRATCH_TOO_SMALL;
   int page_log2 = 0;
   while ((1 << page_log2) < page_size) ++page_log2;
-  const PagedBatch batch{block_table, seq_lens, cu_q, R, max_pages, n_pages, page_log2, n_tokens, max_k, dev_status};
+  const PagedBatch batch{block_table, seq_lens, cu_q, R, max_pages, n_pages, page_log2, n_tokens, max_q, max_k, dev_status};
   const PagedPools pools{k_pages, v_pages, k_page_stride, v_page_stride, Hkv, d};
   const PagedRows rows{q, q_token_stride, q_head_stride, Hq / Hkv, Hkv, scale * 1.4426950408889634f};
   cudaStream_t st = static_cast<cudaStream_t>(stream);

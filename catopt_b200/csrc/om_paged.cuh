@@ -24,7 +24,7 @@ struct PagedBatch {
   const int* table;   // [R, max_pages]
   const int* lens;    // [R] cached keys, the new tokens included
   const int* cu;      // [R+1] first row of each request in q
-  int R, max_pages, n_pages, page_log2, n_tokens, max_k;
+  int R, max_pages, n_pages, page_log2, n_tokens, max_q, max_k;
   int* status;
 };
 
@@ -54,7 +54,7 @@ __device__ __forceinline__ PagedReq paged_request(const PagedBatch& b, int r) {
   const int c0 = __ldg(b.cu + r), c1 = __ldg(b.cu + r + 1), l = __ldg(b.lens + r);
   PagedReq q;
   q.t0 = min(max(c0, 0), b.n_tokens);
-  q.n = max(min(c1, b.n_tokens) - q.t0, 0);
+  q.n = min(max(min(c1, b.n_tokens) - q.t0, 0), b.max_q);
   q.len = min(max(l, 0), b.max_k);
   if (q.t0 != c0 || q.t0 + q.n != c1 || q.len != l) paged_flag(b);
   return q;
@@ -308,5 +308,13 @@ inline PagedScratch paged_scratch(void* base, int n_cta) {
 size_t paged_tc_scratch_bytes(int d);
 int paged_tc_run(const PagedRows& rows, const PagedPools& pools, const PagedBatch& batch, int causal, int few, void* o,
                  float* lse2, void* scratch, PagedScratch* parts, int* n_cta, int* rt, cudaStream_t st);
+
+// om_paged_few.cu: requests of at most `few` (8 or 16) packed rows (bf16), one pass over K and V.  scores (may be
+// NULL): [R, Hkv, few, max_k] floats for paged_few_weights_run.
+size_t paged_few_scratch_bytes(int d);
+int paged_few_run(const PagedRows& rows, const PagedPools& pools, const PagedBatch& batch, int causal, int few, void* o,
+                  float* lse2, float* scores, void* scratch, PagedScratch* parts, int* n_cta, int* rt, cudaStream_t st);
+int paged_few_weights_run(const PagedRows& rows, const PagedBatch& batch, int causal, int few, const float* scores,
+                          const float* lse2, float* weights, cudaStream_t st);
 
 }  // namespace cb2

@@ -239,7 +239,7 @@ extern "C" int cb2_paged_append(const void* q, long long q_token_stride, long lo
     return CB2_BAD_ALIGN;
   int page_log2 = 0;
   while ((1 << page_log2) < page_size) ++page_log2;
-  const PagedBatch batch{block_table, seq_lens, cu_q, R, max_pages, n_pages, page_log2, n_tokens, max_pages * page_size, dev_status};
+  const PagedBatch batch{block_table, seq_lens, cu_q, R, max_pages, n_pages, page_log2, n_tokens, n_tokens, max_pages * page_size, dev_status};
   AppendArgs a{q, k, v, q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride, q_out,
                k_pages, v_pages, k_page_stride, v_page_stride, weights, positions, q_weight, k_weight, cos, sin, table_rows,
                rotary, interleaved, eps, Hq, Hkv, d, 1};

@@ -215,7 +215,7 @@ extern "C" int cb2_paged_evict(void* k_pages, void* v_pages, long long k_page_st
   if (!aligned16(k_pages) || !aligned16(v_pages) || k_page_stride * esz % 16 || v_page_stride * esz % 16) return CB2_BAD_ALIGN;
   int page_log2 = 0;
   while ((1 << page_log2) < page_size) ++page_log2;
-  const PagedBatch batch{block_table, seq_lens, nullptr, R, max_pages, n_pages, page_log2, 0, max_k, dev_status};
+  const PagedBatch batch{block_table, seq_lens, nullptr, R, max_pages, n_pages, page_log2, 0, 0, max_k, dev_status};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const EvictArgs e{weights, Hkv, budget, keep_first, keep_last, kept, new_lens};
   paged_select_kernel<<<dim3(Hkv, R), kSelThreads, 0, st>>>(e, batch);

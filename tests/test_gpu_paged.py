@@ -46,7 +46,7 @@ def run_attend(dev, new, lens, kv, group, d, page, dtype, causal=True, weights=F
 
 RAGGED = [
     ([1], [1]), ([1, 1, 0, 1], [7, 130, 0, 513]), ([5, 1, 17], [5, 64, 400]), ([3, 0, 1, 2], [0, 0, 1, 1]),
-    ([40, 1, 129], [170, 259, 129]), ([300], [1000]),
+    ([40, 1, 129], [170, 259, 129]), ([300], [1000]), ([2, 4, 1, 3], [2, 70, 500, 33]),
 ]
 
 
@@ -75,6 +75,23 @@ def test_attention_strided_rows_and_spaced_pages(dev, dtype):
                          ids=["long", "many", "two", "chunk", "r300"])
 def test_attention_work_cut_over_keys(dev, dtype, new, lens, kv, group):
     run_attend(dev, new, lens, kv, group, 128 if kv == 2 else 64, 16, dtype, weights=True, fill=float("inf"))
+
+
+def test_weights_when_the_bound_on_keys_is_far_off(dev):
+    # scores of 2.3 million possible keys are not kept: the weights are computed from the keys again
+    from catopt_b200 import ops
+
+    lens, new = [700, 5], [1, 1]
+    c = ref.make_cache(lens, 2, 256, 64, BF, dev, 8)
+    wide = torch.full((2, 9000), -1, dtype=torch.int32, device=dev)
+    wide[:, :c["table"].shape[1]] = c["table"]
+    q = torch.randn(2, 8, 64, device=dev).to(BF)
+    w = torch.zeros(c["k"].shape[:3], device=dev)
+    o = ops.om_paged_fwd(q, c["k"], c["v"], wide, c["lens"], ref.offsets(new, dev), 1, weights=w)
+    ops.check_device_status(dev)
+    want, tol, ww, wtol = ref.attend(q, c, new, lens, 0.125, True)
+    close(o, want, tol, "o")
+    close(w, ww, wtol, "weights")
 
 
 def test_large_scores_and_ties(dev):
@@ -121,11 +138,11 @@ def test_attention_graph_follows_lengths(dev):
     outs, graphs = [], []
     with torch.cuda.stream(stream):
         for _ in range(2):
-            ops.om_paged_fwd(q, c["k"], c["v"], c["table"], c["lens"], cu, 5, max_k=300, weights=w)
+            ops.om_paged_fwd(q, c["k"], c["v"], c["table"], c["lens"], cu, 6, max_k=300, weights=w)
         for _ in range(2):
             gph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(gph, stream=stream):
-                outs.append(ops.om_paged_fwd(q, c["k"], c["v"], c["table"], c["lens"], cu, 5, max_k=300, weights=w))
+                outs.append(ops.om_paged_fwd(q, c["k"], c["v"], c["table"], c["lens"], cu, 6, max_k=300, weights=w))
             graphs.append(gph)
     torch.cuda.synchronize()
     for new, lens in (([1, 5], [300, 90]), ([4, 2], [77, 10]), ([6, 0], [250, 0])):
@@ -168,6 +185,7 @@ def test_bad_indices_are_reported(dev):
         bad(lens=torch.tensor([-3, 70], dtype=torch.int32, device=dev))
         bad(cu_q=torch.tensor([0, 1, 900], dtype=torch.int32, device=dev))
         bad(cu_q=torch.tensor([-7, 1, 3], dtype=torch.int32, device=dev))
+        bad(cu_q=torch.tensor([0, 0, 3], dtype=torch.int32, device=dev))      # three new tokens where two were promised
         k = torch.randn(3, 2, 64, device=dev).to(dtype)
         t = c["table"].clone()
         t[1, 4] = c["k"].shape[0]
