@@ -101,10 +101,7 @@ paged_fma_kernel(const PagedRows rows, const PagedPools pools, const PagedBatch 
   constexpr int kLdP = kKB + 4;
   const int cta = blockIdx.x, n_cta = gridDim.x;
   const PagedShare share = paged_find_share<kThreads>(batch, cost, cta, n_cta, &find);
-  if (tid == 0) {
-    scratch.joins[cta].r = -1;
-    if (cta == 0) *scratch.total = share.total;
-  }
+  if (tid == 0) scratch.joins[cta].r = -1;
   const int ty = tid / 16, tx = tid % 16, lane = tid % 32, wq = tid / 32;
   for (PagedWalk<PagedCost<kRT, kKB>> w(batch, cost, share); w.valid(); w.next()) {
     w.clip();
@@ -200,7 +197,7 @@ paged_fma_kernel(const PagedRows rows, const PagedPools pools, const PagedBatch 
         if (lse2 && lane == 0) lse2[at] = lr > 0.f ? ml[rr] + log2f(lr) : INFINITY;
       }
     } else {
-      if (tid == 0 && w.b0 == 0) paged_write_join(w, share.total, cta, n_cta, scratch.joins);
+      if (tid == 0 && w.b0 == 0) paged_write_join(w, share.total, cta, share.n_share, scratch.joins);
       float* slot = scratch.parts + paged_slot_floats(kRT, d) * (2 * cta + (w.b0 == 0));
       if (tid < kRT) {
         slot[tid] = ml[tid];
@@ -215,42 +212,74 @@ paged_fma_kernel(const PagedRows rows, const PagedPools pools, const PagedBatch 
   }
 }
 
-// Joins the partial carriers of a unit in share order: m = max m_c, l = sum l_c 2^(m_c - m), a likewise.
-// Block (c, y) takes rows [16 y, 16 y + 16) of the unit that starts in share c; warp = row, lane = 4 columns.
+// Joins the partial carriers of a unit: m = max m_c, l = sum l_c 2^(m_c - m), a likewise, over the shares
+// c .. last, none of them empty.  Block (c, y) takes rows [16 y, 16 y + 16) of the unit that starts in share c.
+// A warp holds one row, a lane four columns; with few rows several warps share a row's shares (every
+// `stride`-th one) and meet in shared memory, always in the same order.
+constexpr int kJoinWarps = 16;
+
 template <class T>
-__global__ void __launch_bounds__(512)
-paged_combine_kernel(int rt, PagedScratch scratch, T* __restrict__ o, float* __restrict__ lse2, PagedBatch batch, int G,
+__global__ void __launch_bounds__(kJoinWarps * 32)
+paged_combine_kernel(int rt, const PagedScratch scratch, T* __restrict__ o, float* __restrict__ lse2, const PagedBatch batch, int G,
                      int Hkv, int d) {
-  const int c = blockIdx.x, n_cta = gridDim.x, lane = threadIdx.x & 31;
+  __shared__ float sh_m[kJoinWarps], sh_l[kJoinWarps];
+  __shared__ __align__(16) float sh_a[kJoinWarps][128];
+  const int c = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const PagedJoin j = scratch.joins[c];
   if (j.r < 0) return;
   const PagedReq q = paged_request(batch, j.r);
-  const int rr = blockIdx.y * 16 + (threadIdx.x >> 5), row = j.tile * rt + rr;
-  if (row >= q.n * G) return;
-  const long long total = *scratch.total;
+  const int row_first = j.tile * rt + blockIdx.y * kJoinWarps;
+  const int n_rows = min(kJoinWarps, q.n * G - row_first);
+  if (n_rows <= 0) return;
+  int stride = 1;                                        // warps a row
+  while (stride * 2 * n_rows <= kJoinWarps) stride *= 2;
+  const int rr = warp / stride, part = warp % stride;
+  const bool live = rr < n_rows;
   const size_t slot = paged_slot_floats(rt, d);
-  float m = -INFINITY;
-  for (int s = c + lane; s <= j.last; s += 32)
-    if (paged_cut(total, s, n_cta) < paged_cut(total, s + 1, n_cta)) m = fmaxf(m, scratch.parts[slot * (2 * s + (s == c)) + rr]);
-#pragma unroll
-  for (int off = 16; off; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
-  const float ref = m == -INFINITY ? 0.f : m;
-  float l = 0.f;
+  const float* base = scratch.parts + (live ? blockIdx.y * kJoinWarps + rr : 0);
+  auto slot_of = [&](int s) { return base + slot * (2 * s + (s == c)); };
+  float m = -INFINITY, l = 0.f;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (live) {
+    for (int s = c + part + lane * stride; s <= j.last; s += 32 * stride) m = fmaxf(m, *slot_of(s));
+#pragma unroll
+    for (int off = 16; off; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+    const float ref = m == -INFINITY ? 0.f : m;
+    const int row = blockIdx.y * kJoinWarps + rr;
 #pragma unroll 4
-  for (int s = c; s <= j.last; ++s) {
-    if (paged_cut(total, s, n_cta) == paged_cut(total, s + 1, n_cta)) continue;   // an empty share left nothing
-    const float* p = scratch.parts + slot * (2 * s + (s == c));
-    const float f = ex2_approx(p[rr] - ref);
-    l += p[rt + rr] * f;
-    if (4 * lane < d) {
-      const float4 v = *reinterpret_cast<const float4*>(p + 2 * rt + rr * d + 4 * lane);
-      a.x += v.x * f;
-      a.y += v.y * f;
-      a.z += v.z * f;
-      a.w += v.w * f;
+    for (int s = c + part; s <= j.last; s += stride) {
+      const float* p = slot_of(s);
+      const float f = ex2_approx(p[0] - ref);
+      l += p[rt] * f;
+      if (4 * lane < d) {
+        const float4 v = *reinterpret_cast<const float4*>(p - row + 2 * rt + row * d + 4 * lane);
+        a.x += v.x * f;
+        a.y += v.y * f;
+        a.z += v.z * f;
+        a.w += v.w * f;
+      }
     }
   }
+  if (stride > 1) {
+    *reinterpret_cast<float4*>(&sh_a[warp][4 * lane]) = a;
+    if (lane == 0) {
+      sh_m[warp] = m;
+      sh_l[warp] = l;
+    }
+    __syncthreads();
+    if (part != 0 || !live) return;
+    for (int w = warp + 1; w < warp + stride; ++w) {
+      const float m_new = fmaxf(m, sh_m[w]);
+      const float ref = m_new == -INFINITY ? 0.f : m_new;
+      const float f0 = ex2_approx(m - ref), f1 = ex2_approx(sh_m[w] - ref);
+      const float4 v = *reinterpret_cast<const float4*>(&sh_a[w][4 * lane]);
+      m = m_new;
+      l = l * f0 + sh_l[w] * f1;
+      a = make_float4(a.x * f0 + v.x * f1, a.y * f0 + v.y * f1, a.z * f0 + v.z * f1, a.w * f0 + v.w * f1);
+    }
+  }
+  if (!live) return;
+  const int row = row_first + rr;
   const float inv = l > 0.f ? 1.f / l : 0.f;
   const long long at = (long long)(q.t0 + row / G) * (G * Hkv) + j.h * G + row % G;
   if (4 * lane < d) store4(o + at * d + 4 * lane, make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv));
@@ -355,7 +384,7 @@ Plan plan(int n_tokens, int R, int Hq, int Hkv, int d, int max_q, int max_k, boo
 template <class T>
 int join(int rt, int n_cta, const PagedScratch& ws, T* o, float* lse2, const PagedBatch& batch, const PagedRows& rows, int d,
          cudaStream_t st) {
-  paged_combine_kernel<T><<<dim3(n_cta, rt / 16), 512, 0, st>>>(rt, ws, o, lse2, batch, rows.G, rows.Hkv, d);
+  paged_combine_kernel<T><<<dim3(n_cta, rt / kJoinWarps), kJoinWarps * 32, 0, st>>>(rt, ws, o, lse2, batch, rows.G, rows.Hkv, d);
   CB2_LAUNCH_CHECK();
   return CB2_OK;
 }
@@ -374,7 +403,7 @@ int fma_weights(const PagedRows& rows, const PagedPools& pools, const PagedBatch
 
 int run_f32(const PagedRows& rows, const PagedPools& pools, const PagedBatch& batch, int causal, float* o, float* weights,
             char* scratch, const Plan& p, cudaStream_t st) {
-  const PagedCost<kRT, kKB> cost{rows.G, rows.Hkv, causal, kPagedAll, 0};
+  const PagedCost<kRT, kKB> cost{rows.G, rows.Hkv, causal, kPagedAll, 0, 2};
   float* lse2 = weights ? reinterpret_cast<float*>(scratch) : nullptr;
   const PagedScratch ws = paged_scratch(scratch + p.lse, kFmaCtas);
   const int d = pools.d, ld = d + 4;
@@ -399,14 +428,14 @@ int run_bf16(const PagedRows& rows, const PagedPools& pools, const PagedBatch& b
     rc = paged_tc_run(rows, pools, batch, causal, p.few, o, lse2, parts, &ws, &n_cta, &rt, st);
     if (rc == CB2_OK) rc = join(rt, n_cta, ws, o, lse2, batch, rows, pools.d, st);
     if (rc == CB2_OK && weights)
-      rc = fma_weights<__nv_bfloat16>(rows, pools, batch, {rows.G, rows.Hkv, causal, kPagedChunk, p.few}, lse2, weights, st);
+      rc = fma_weights<__nv_bfloat16>(rows, pools, batch, {rows.G, rows.Hkv, causal, kPagedChunk, p.few, 1}, lse2, weights, st);
   }
   if (rc == CB2_OK && p.few) {
     rc = paged_few_run(rows, pools, batch, causal, p.few, o, lse2, scores, parts, &ws, &n_cta, &rt, st);
     if (rc == CB2_OK) rc = join(rt, n_cta, ws, o, lse2, batch, rows, pools.d, st);
     if (rc == CB2_OK && scores) rc = paged_few_weights_run(rows, batch, causal, p.few, scores, lse2, weights, st);
     if (rc == CB2_OK && weights && !scores)
-      rc = fma_weights<__nv_bfloat16>(rows, pools, batch, {rows.G, rows.Hkv, causal, kPagedFew, p.few}, lse2, weights, st);
+      rc = fma_weights<__nv_bfloat16>(rows, pools, batch, {rows.G, rows.Hkv, causal, kPagedFew, p.few, 1}, lse2, weights, st);
   }
   return rc;
 }

@@ -106,6 +106,7 @@ enum { kPagedAll = 0, kPagedFew = 1, kPagedChunk = 2 };
 template <int RT, int KB>
 struct PagedCost {
   int G, Hkv, causal, which, few;
+  int min_blocks;          // a share holds at least so many: fewer CTAs work on a short line
   __device__ __forceinline__ bool takes(const PagedReq& q) const {
     if (q.n == 0) return false;
     return which == kPagedAll || (which == kPagedFew) == (q.n * G <= few);
@@ -143,6 +144,7 @@ struct PagedFindSmem {
 // Start of this CTA's share [lo, hi) of the line: request and offset in it.  All T threads call it.
 struct PagedShare {
   long long total, lo, hi;
+  int n_share;      // shares that are not empty: [0, n_share)
   int r;            // request that holds lo
   long long off;    // lo - start of that request
 };
@@ -179,8 +181,12 @@ __device__ PagedShare paged_find_share(const PagedBatch& b, const Cost& cost, in
     total += block_total;
   }
   out.total = total;
-  out.lo = paged_cut(total, cta, n_cta);
-  out.hi = paged_cut(total, cta + 1, n_cta);
+  out.n_share = int(max(1ll, min((long long)n_cta, total / cost.min_blocks)));
+  out.lo = out.hi = total;
+  if (cta < out.n_share) {
+    out.lo = paged_cut(total, cta, out.n_share);
+    out.hi = paged_cut(total, cta + 1, out.n_share);
+  }
   if (tid == 0) {
     s->r = 0;
     s->off = 0;
@@ -276,30 +282,28 @@ __device__ __forceinline__ float ex2_approx(float x) {
   return y;
 }
 
-__device__ __forceinline__ void paged_write_join(const PagedWalkState& w, long long total, int cta, int n_cta, PagedJoin* joins) {
+__device__ __forceinline__ void paged_write_join(const PagedWalkState& w, long long total, int cta, int n_share, PagedJoin* joins) {
   // called for a piece with b0 == 0 and b1 < nb: the unit's last block sits at cur + nb - 1
   PagedJoin j;
   j.r = w.r;
   j.h = w.h;
   j.tile = w.tile;
-  j.last = int(((w.cur + w.nb) * n_cta - 1) / total);
+  j.last = int(((w.cur + w.nb) * n_share - 1) / total);
   joins[cta] = j;
 }
 
-// Scratch of one attention kernel of n_cta shares: the line's length, the joins, the partial carriers.
+// Scratch of one attention kernel of n_cta shares: the joins, the partial carriers.
 struct PagedScratch {
-  long long* total;
   PagedJoin* joins;
   float* parts;
 };
 __host__ __device__ inline size_t paged_scratch_bytes(int n_cta, int rt, int d) {
-  return 16 + size_t(n_cta) * sizeof(PagedJoin) + size_t(n_cta) * 2 * paged_slot_floats(rt, d) * 4;
+  return size_t(n_cta) * sizeof(PagedJoin) + size_t(n_cta) * 2 * paged_slot_floats(rt, d) * 4;
 }
 inline PagedScratch paged_scratch(void* base, int n_cta) {
   PagedScratch s;
-  s.total = static_cast<long long*>(base);
-  s.joins = reinterpret_cast<PagedJoin*>(static_cast<char*>(base) + 16);
-  s.parts = reinterpret_cast<float*>(static_cast<char*>(base) + 16 + size_t(n_cta) * sizeof(PagedJoin));
+  s.joins = static_cast<PagedJoin*>(base);
+  s.parts = reinterpret_cast<float*>(static_cast<char*>(base) + size_t(n_cta) * sizeof(PagedJoin));
   return s;
 }
 

@@ -73,10 +73,7 @@ paged_few_kernel(const PagedRows rows, const PagedPools pools, const PagedBatch 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int cta = blockIdx.x, n_cta = gridDim.x, d = pools.d, G = rows.G;
   const PagedShare share = paged_find_share<kThreads>(batch, cost, cta, n_cta, &find);
-  if (tid == 0) {
-    scratch.joins[cta].r = -1;
-    if (cta == 0) *scratch.total = share.total;
-  }
+  if (tid == 0) scratch.joins[cta].r = -1;
   unsigned char* ring = smem + warp * R::kWarpBytes;
   const uint32_t ring_addr = smem_u32(ring);
   const int ps_log2 = batch.page_log2, ps = 1 << ps_log2;
@@ -279,7 +276,7 @@ paged_few_kernel(const PagedRows rows, const PagedPools pools, const PagedBatch 
       }
     __syncthreads();
     const bool whole = w.b0 == 0 && w.b1 == w.nb;
-    if (!whole && w.b0 == 0 && tid == 0) paged_write_join(w, share.total, cta, n_cta, scratch.joins);
+    if (!whole && w.b0 == 0 && tid == 0) paged_write_join(w, share.total, cta, share.n_share, scratch.joins);
     float* slot = scratch.parts + paged_slot_floats(kRT, d) * (2 * cta + (w.b0 == 0));
     for (int row = 0; row < n_rows; ++row) {
       float mm = -INFINITY;
@@ -309,27 +306,31 @@ paged_few_kernel(const PagedRows rows, const PagedPools pools, const PagedBatch 
   }
 }
 
-// weight[key] += sum over the packed rows of 2^(score - lse), from the scores that the kernel above left; the
-// same shares, a thread a key.
-__global__ void __launch_bounds__(kThreads)
+// weight[key] += sum over the packed rows of 2^(score - lse), from the scores that the kernel above left: a
+// thread a key, the same line cut into more shares (one block or a few each, so that all loads are in flight).
+constexpr int kWeightThreads = 256, kWeightCtas = 8 * kNumSMs;
+
+__global__ void __launch_bounds__(kWeightThreads)
 paged_few_weights_kernel(const PagedBatch batch, const Cost cost, const float* __restrict__ scores, const float* __restrict__ lse2,
                          float* __restrict__ weights) {
   __shared__ PagedFindSmem find;
-  const PagedShare share = paged_find_share<kThreads>(batch, cost, blockIdx.x, gridDim.x, &find);
-  const int G = cost.G, ps = 1 << batch.page_log2;
+  __shared__ float sh_lse[kRT];
+  const PagedShare share = paged_find_share<kWeightThreads>(batch, cost, blockIdx.x, gridDim.x, &find);
+  const int G = cost.G, ps = 1 << batch.page_log2, tid = threadIdx.x;
   for (PagedWalk<Cost> w(batch, cost, share); w.valid(); w.next()) {
     w.clip();
     const float* sc = scores + ((long long)w.r * cost.Hkv + w.h) * cost.few * batch.max_k;
     const int n_rows = w.q.n * G, end = min(w.b1 * kKB, w.q.len);
-    for (int j = w.b0 * kKB + threadIdx.x; j < end; j += kThreads) {
-      float sum = 0.f;
-#pragma unroll 4
-      for (int row = 0; row < n_rows; ++row) {
-        const float z = __ldg(lse2 + (long long)(w.q.t0 + row / G) * (G * cost.Hkv) + w.h * G + row % G);
-        sum += ex2_approx(sc[(long long)row * batch.max_k + j] - z);
-      }
+    __syncthreads();
+    if (tid < n_rows) sh_lse[tid] = __ldg(lse2 + (long long)(w.q.t0 + tid / G) * (G * cost.Hkv) + w.h * G + tid % G);
+    __syncthreads();
+    for (int j = w.b0 * kKB + tid; j < end; j += kWeightThreads) {
       const int page = paged_page(batch, w.r, j >> batch.page_log2);
-      weights[((long long)page * cost.Hkv + w.h) * ps + (j & (ps - 1))] += sum;
+      float* at = weights + ((long long)page * cost.Hkv + w.h) * ps + (j & (ps - 1));
+      float sum = 0.f;
+#pragma unroll 8
+      for (int row = 0; row < n_rows; ++row) sum += ex2_approx(__ldg(sc + (long long)row * batch.max_k + j) - sh_lse[row]);
+      *at += sum;
     }
   }
 }
@@ -354,7 +355,8 @@ int paged_few_run(const PagedRows& rows, const PagedPools& pools, const PagedBat
   *parts = paged_scratch(scratch, kCtas);
   *n_cta = kCtas;
   *rt = kRT;
-  const Cost cost{rows.G, rows.Hkv, causal, kPagedFew, few};
+  // 256 keys a share at least: four tiles a warp, less than that is mostly start and join
+  const Cost cost{rows.G, rows.Hkv, causal, kPagedFew, few, 4};
   __nv_bfloat16* out = static_cast<__nv_bfloat16*>(o);
   if (pools.d <= 64)
     return few <= 8 ? launch<4, 1>(rows, pools, batch, cost, out, lse2, scores, *parts, st)
@@ -365,8 +367,8 @@ int paged_few_run(const PagedRows& rows, const PagedPools& pools, const PagedBat
 
 int paged_few_weights_run(const PagedRows& rows, const PagedBatch& batch, int causal, int few, const float* scores, const float* lse2,
                           float* weights, cudaStream_t st) {
-  const Cost cost{rows.G, rows.Hkv, causal, kPagedFew, few};
-  paged_few_weights_kernel<<<kCtas, kThreads, 0, st>>>(batch, cost, scores, lse2, weights);
+  const Cost cost{rows.G, rows.Hkv, causal, kPagedFew, few, 2};
+  paged_few_weights_kernel<<<kWeightCtas, kWeightThreads, 0, st>>>(batch, cost, scores, lse2, weights);
   CB2_LAUNCH_CHECK();
   return CB2_OK;
 }

@@ -40,6 +40,7 @@ struct Smem {
   int loads_k, loads_v;     // issued so far
   PagedWalkState walk;
   long long total;
+  int n_share;
   Piece pieces[kBatch];
   PagedFindSmem find;
 };
@@ -101,12 +102,12 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   }
   {
     const PagedShare share = paged_find_share<kThreads>(batch, cost, cta, n_cta, &sh->find);
-    if (cta == 0 && tid == 0) *scratch.total = share.total;
     if (warp == 0) {
       const PagedWalk<PagedCost<kRT, kKB>> walk(batch, cost, share);
       if (lane == 0) {
         sh->walk = walk;
         sh->total = share.total;
+        sh->n_share = share.n_share;
       }
     }
   }
@@ -128,7 +129,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         if (lane == 0) {
           const bool whole = walk.b0 == 0 && walk.b1 == walk.nb;
           sh->pieces[count] = Piece{walk.r, walk.h, walk.tile * kRT, walk.q.t0, walk.q.n, walk.q.len, walk.b0, walk.b1, whole};
-          if (walk.b0 == 0 && !whole) paged_write_join(walk, sh->total, cta, n_cta, scratch.joins);
+          if (walk.b0 == 0 && !whole) paged_write_join(walk, sh->total, cta, sh->n_share, scratch.joins);
         }
       }
       if (lane == 0) {
@@ -427,7 +428,7 @@ int paged_tc_run(const PagedRows& rows, const PagedPools& pools, const PagedBatc
   *rt = kRT;
   const TcArgs a{static_cast<const __nv_bfloat16*>(rows.q), rows.q_token, rows.q_head, static_cast<__nv_bfloat16*>(o), lse2,
                  rows.scale_log2e, rows.G, rows.Hkv, pools.d};
-  const PagedCost<kRT, kKB> cost{rows.G, rows.Hkv, causal, kPagedChunk, few};
+  const PagedCost<kRT, kKB> cost{rows.G, rows.Hkv, causal, kPagedChunk, few, 2};
   paged_tc_kernel<<<kCtas, kThreads, kSmemBytes, st>>>(mk, mv, a, batch, cost, *parts);
   CB2_LAUNCH_CHECK();
   return CB2_OK;

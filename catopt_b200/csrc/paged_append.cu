@@ -14,6 +14,7 @@ namespace cb2 {
 namespace {
 
 constexpr int kThreads = 256, kGroups = kThreads / 16;
+constexpr int kAhead = 4;     // rows a group has in flight
 
 struct AppendArgs {
   const void *q, *k, *v;
@@ -124,86 +125,95 @@ paged_append_kernel(const AppendArgs a, const PagedBatch batch) {
   const bool in = gl * 8 < d;
   const int ps = 1 << batch.page_log2;
 
-  float cs[8], sn[8], wq[8], wk[8];
+  float cs[8], sn[8];
+  Raw<T> wq, wk;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) cs[i] = 1.f, sn[i] = 0.f, wq[i] = wk[i] = 1.f;
-  if (in) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int e = gl * 8 + i;
-      if (e < a.rot) {
-        const int f = a.interleaved ? e >> 1 : (e < half ? e : e - half);
-        const bool first = a.interleaved ? !(e & 1) : e < half;
-        cs[i] = __ldg(a.cos + (long long)here.position * half + f);
-        const float s = __ldg(a.sin + (long long)here.position * half + f);
-        sn[i] = first ? -s : s;          // y = x cos + partner * sn
-      }
-    }
-    Raw<T> r;
-    if (a.q_weight) {
-      r.load(static_cast<const T*>(a.q_weight) + gl * 8);
-      r.unpack(wq);
-    }
-    if (a.k_weight) {
-      r.load(static_cast<const T*>(a.k_weight) + gl * 8);
-      r.unpack(wk);
+  for (int i = 0; i < 8; ++i) {
+    const int e = gl * 8 + i;
+    cs[i] = 1.f, sn[i] = 0.f;
+    if (e < a.rot) {
+      const int f = a.interleaved ? e >> 1 : (e < half ? e : e - half);
+      const bool first = a.interleaved ? !(e & 1) : e < half;
+      cs[i] = __ldg(a.cos + (long long)here.position * half + f);
+      const float s = __ldg(a.sin + (long long)here.position * half + f);
+      sn[i] = first ? -s : s;          // y = x cos + partner * sn
     }
   }
+  if (in && a.q_weight) wq.load(static_cast<const T*>(a.q_weight) + gl * 8);
+  if (in && a.k_weight) wk.load(static_cast<const T*>(a.k_weight) + gl * 8);
   const int n_rows = a.Hq + 2 * a.Hkv;
-  for (int row = group % per_token; row < n_rows; row += per_token) {
-    const bool is_q = row < a.Hq, is_v = row >= a.Hq + a.Hkv;
-    const int h = is_q ? row : (is_v ? row - a.Hq - a.Hkv : row - a.Hq);
-    Raw<T> raw;
-    if (in) {
-      const T* src = is_q ? static_cast<const T*>(a.q) + t * a.q_token + h * a.q_head
-                   : is_v ? static_cast<const T*>(a.v) + t * a.v_token + h * a.v_head
-                          : static_cast<const T*>(a.k) + t * a.k_token + h * a.k_head;
-      raw.load(src + gl * 8);
-    }
-    if (!is_v) {
-      float x[8] = {};
-      if (in) raw.unpack(x);
-      if (is_q ? a.q_weight != nullptr : a.k_weight != nullptr) {
-        float ss = 0.f;
+  for (int row0 = group % per_token; row0 < n_rows; row0 += kAhead * per_token) {
+    Raw<T> raw[kAhead];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
-#pragma unroll
-        for (int off = 8; off; off >>= 1) ss += __shfl_xor_sync(half_mask, ss, off);
-        const float inv = rsqrtf(ss / float(d) + a.eps);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] *= inv * (is_q ? wq[i] : wk[i]);
+    for (int u = 0; u < kAhead; ++u) {
+      const int row = row0 + u * per_token;
+      if (in && row < n_rows) {
+        const bool is_q = row < a.Hq, is_v = row >= a.Hq + a.Hkv;
+        const T* src = is_q ? static_cast<const T*>(a.q) + t * a.q_token + row * a.q_head
+                       : is_v ? static_cast<const T*>(a.v) + t * a.v_token + (row - a.Hq - a.Hkv) * a.v_head
+                              : static_cast<const T*>(a.k) + t * a.k_token + (row - a.Hq) * a.k_head;
+        raw[u].load(src + gl * 8);
       }
-      if (a.rot) {
-        float y[8];
-        if (a.interleaved) {
+    }
 #pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] = x[i ^ 1];
-        } else {
-          // the partner lies rot/2 columns away, in another lane: through shared memory
-          float* mine = rows[group];
-          __syncwarp(half_mask);
-          *reinterpret_cast<float4*>(mine + gl * 8) = make_float4(x[0], x[1], x[2], x[3]);
-          *reinterpret_cast<float4*>(mine + gl * 8 + 4) = make_float4(x[4], x[5], x[6], x[7]);
-          __syncwarp(half_mask);
+    for (int u = 0; u < kAhead; ++u) {
+      const int row = row0 + u * per_token;
+      if (row >= n_rows) break;
+      const bool is_q = row < a.Hq, is_v = row >= a.Hq + a.Hkv;
+      const int h = is_q ? row : (is_v ? row - a.Hq - a.Hkv : row - a.Hq);
+      if (!is_v) {
+        float x[8] = {};
+        if (in) raw[u].unpack(x);
+        if (is_q ? a.q_weight != nullptr : a.k_weight != nullptr) {
+          float ss = 0.f, weight[8] = {};
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int e = gl * 8 + i;
-            y[i] = e < a.rot ? mine[e < half ? e + half : e - half] : 0.f;
-          }
+          for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
+#pragma unroll
+          for (int off = 8; off; off >>= 1) ss += __shfl_xor_sync(half_mask, ss, off);
+          const float inv = rsqrtf(ss / float(d) + a.eps);
+          if (in) (is_q ? wq : wk).unpack(weight);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] *= inv * weight[i];
         }
+        if (a.rot) {
+          float y[8];
+          if (a.interleaved) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = fmaf(y[i], sn[i], x[i] * cs[i]);
+            for (int i = 0; i < 8; ++i) y[i] = x[i ^ 1];
+          } else {
+            // the partner lies rot/2 columns away, in another lane: through shared memory
+            float* mine = rows[group];
+            __syncwarp(half_mask);
+            *reinterpret_cast<float4*>(mine + gl * 8) = make_float4(x[0], x[1], x[2], x[3]);
+            *reinterpret_cast<float4*>(mine + gl * 8 + 4) = make_float4(x[4], x[5], x[6], x[7]);
+            __syncwarp(half_mask);
+            if ((half & 7) == 0) {       // a lane's eight columns have their partners in one lane
+              const int e = gl * 8 < half ? gl * 8 + half : (gl * 8 < a.rot ? gl * 8 - half : 0);
+              const float4 lo = *reinterpret_cast<const float4*>(mine + e), hi = *reinterpret_cast<const float4*>(mine + e + 4);
+              y[0] = lo.x, y[1] = lo.y, y[2] = lo.z, y[3] = lo.w, y[4] = hi.x, y[5] = hi.y, y[6] = hi.z, y[7] = hi.w;
+            } else {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const int e = gl * 8 + i;
+                y[i] = e < a.rot ? mine[e < half ? e + half : e - half] : 0.f;
+              }
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (gl * 8 + i < a.rot) x[i] = fmaf(y[i], sn[i], x[i] * cs[i]);
+        }
+        raw[u].pack(x);
       }
-      raw.pack(x);
-    }
-    if (!in) continue;
-    if (is_q) {
-      raw.store(static_cast<T*>(a.q_out) + ((long long)t * a.Hq + h) * d + gl * 8);
-    } else if (here.page >= 0) {
-      T* pool = static_cast<T*>(is_v ? a.v_pages : a.k_pages);
-      const long long at = here.page * (is_v ? a.v_page_stride : a.k_page_stride) + (long long)(h * ps + here.slot) * d;
-      raw.store(pool + at + gl * 8);
-      if (is_v && a.weights && gl == 0) a.weights[((long long)here.page * a.Hkv + h) * ps + here.slot] = 0.f;
+      if (!in) continue;
+      if (is_q) {
+        raw[u].store(static_cast<T*>(a.q_out) + ((long long)t * a.Hq + h) * d + gl * 8);
+      } else if (here.page >= 0) {
+        T* pool = static_cast<T*>(is_v ? a.v_pages : a.k_pages);
+        const long long at = here.page * (is_v ? a.v_page_stride : a.k_page_stride) + (long long)(h * ps + here.slot) * d;
+        raw[u].store(pool + at + gl * 8);
+        if (is_v && a.weights && gl == 0) a.weights[((long long)here.page * a.Hkv + h) * ps + here.slot] = 0.f;
+      }
     }
   }
 }
@@ -243,9 +253,9 @@ extern "C" int cb2_paged_append(const void* q, long long q_token_stride, long lo
   AppendArgs a{q, k, v, q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride, q_out,
                k_pages, v_pages, k_page_stride, v_page_stride, weights, positions, q_weight, k_weight, cos, sin, table_rows,
                rotary, interleaved, eps, Hq, Hkv, d, 1};
-  // Few tokens: sixteen groups share one token's heads (latency).  Many: a pair of groups keeps a token,
-  // so that its angles are loaded once for half of its heads.
-  while (a.tokens_per_cta < 8 && n_tokens / (2 * a.tokens_per_cta) >= 2 * kNumSMs) a.tokens_per_cta *= 2;
+  // Few tokens: sixteen groups share one token's heads (latency).  Many: four groups keep a token, so that its
+  // angles are loaded once for a quarter of its heads.
+  while (a.tokens_per_cta < 4 && n_tokens / (2 * a.tokens_per_cta) >= 2 * kNumSMs) a.tokens_per_cta *= 2;
   const unsigned grid = unsigned((n_tokens + a.tokens_per_cta - 1) / a.tokens_per_cta);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == CB2_BF16)

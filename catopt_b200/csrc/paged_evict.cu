@@ -13,7 +13,8 @@
 namespace cb2 {
 namespace {
 
-constexpr int kSelThreads = 512, kMoveThreads = 256, kMoveRows = 64;
+constexpr int kSelThreads = 1024, kMoveThreads = 256, kMoveRows = 64;
+constexpr int kMostHeld = 48 * 1024;       // keys that fit shared memory beside the histogram
 
 // Unsigned key of the same order as the float: NaN lowest, -0 and +0 the same.
 __device__ __forceinline__ uint32_t weight_key(float w) {
@@ -27,6 +28,7 @@ struct EvictArgs {
   int Hkv, budget, first, last;
   int* kept;        // [R, Hkv, budget]
   int* new_lens;    // [R]
+  int held;         // keys of a request that shared memory holds
 };
 
 struct WeightReader {
@@ -39,10 +41,24 @@ struct WeightReader {
   }
 };
 
+// Positions among the true flags of a block, thread order: exclusive rank and total.
+__device__ __forceinline__ int block_rank(bool flag, int* warp_count, int& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const unsigned b = __ballot_sync(0xffffffffu, flag);
+  if (lane == 0) warp_count[warp] = __popc(b);
+  __syncthreads();
+  const int c = warp_count[lane];                       // kSelThreads / 32 = 32 warps
+  const int before = __reduce_add_sync(0xffffffffu, lane < warp ? c : 0);
+  total = __reduce_add_sync(0xffffffffu, c);
+  return before + __popc(b & ((1u << lane) - 1));
+}
+static_assert(kSelThreads == 1024, "block_rank reads one count a lane");
+
 __global__ void __launch_bounds__(kSelThreads)
 paged_select_kernel(const EvictArgs a, const PagedBatch batch) {
+  extern __shared__ uint32_t sh_keys[];                 // [held]
   __shared__ int hist[256];
-  __shared__ int warp_keep[kSelThreads / 32], warp_tie[kSelThreads / 32];
+  __shared__ int warp_count[2][2][32];
   __shared__ uint32_t s_prefix;
   __shared__ int s_need;
   const int h = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -56,20 +72,29 @@ paged_select_kernel(const EvictArgs a, const PagedBatch batch) {
   }
   const WeightReader key{batch, a.weights, r, h, a.Hkv};
   const int lo = a.first, hi = len - a.last;             // first + last <= budget < len
-  // the (budget - first - last)-th largest key of [lo, hi), byte by byte
+  const int want = a.budget - a.first - a.last;          // of [lo, hi)
+  const int held = min(a.held, len);
+#pragma unroll 4
+  for (int j = tid; j < held; j += kSelThreads) sh_keys[j] = key(j);
+  auto key_at = [&](int j) { return j < held ? sh_keys[j] : key(j); };
   if (tid == 0) {
     s_prefix = 0;
-    s_need = a.budget - a.first - a.last;
+    s_need = want;
   }
   __syncthreads();
-  const bool any = a.budget - a.first - a.last > 0;
-  for (int shift = 24; any && shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256; i += kSelThreads) hist[i] = 0;
+  // the want-th largest key of [lo, hi), byte by byte
+  for (int shift = 24; want > 0 && shift >= 0; shift -= 8) {
+    if (tid < 256) hist[tid] = 0;
     __syncthreads();
     const uint32_t prefix = s_prefix, mask = shift == 24 ? 0u : ~0u << (shift + 8);
-    for (int j = lo + tid; j < hi; j += kSelThreads) {
-      const uint32_t k = key(j);
-      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255u], 1);
+    for (int j0 = lo; j0 < hi; j0 += kSelThreads) {
+      const int j = j0 + tid;
+      const uint32_t k = j < hi ? key_at(j) : 0u;
+      const bool in = j < hi && (k & mask) == prefix;
+      const unsigned bin = in ? (k >> shift) & 255u : 256u;
+      // weights share their leading bytes: one addition for all lanes of a bin
+      const unsigned peers = __match_any_sync(0xffffffffu, bin);
+      if (in && lane == __ffs(peers) - 1) atomicAdd(&hist[bin], __popc(peers));
     }
     __syncthreads();
     if (warp == 0) {
@@ -103,41 +128,27 @@ paged_select_kernel(const EvictArgs a, const PagedBatch batch) {
     __syncthreads();
   }
   const uint32_t cut = s_prefix;
-  const int ties = any ? s_need : 0;       // how many keys equal to the cut are kept, the lowest slots first
-  int base_keep = 0, base_tie = 0;
-  for (int j0 = 0; j0 < len; j0 += kSelThreads) {
+  const int ties = want > 0 ? s_need : 0;  // how many keys equal to the cut are kept, the lowest slots first
+  int base_keep = 0, base_tie = 0, phase = 0;
+  for (int j0 = 0; j0 < len; j0 += kSelThreads, phase ^= 1) {
     const int j = j0 + tid;
     bool keep = false, tie = false;
     if (j < len) {
       if (j < lo || j >= hi) {
         keep = true;
-      } else if (any) {
-        const uint32_t k = key(j);
+      } else if (want > 0) {
+        const uint32_t k = key_at(j);
         keep = k > cut;
         tie = k == cut;
       }
     }
-    const unsigned below = (1u << lane) - 1;
-    const unsigned bt = __ballot_sync(0xffffffffu, tie);
-    if (lane == 0) warp_tie[warp] = __popc(bt);
-    __syncthreads();
-    int tb = base_tie, tt = 0;
-    for (int w = 0; w < kSelThreads / 32; ++w) {
-      if (w < warp) tb += warp_tie[w];
-      tt += warp_tie[w];
-    }
-    if (tie && tb + __popc(bt & below) < ties) keep = true;
-    const unsigned bk = __ballot_sync(0xffffffffu, keep);
-    if (lane == 0) warp_keep[warp] = __popc(bk);
-    __syncthreads();
-    int kb = base_keep, kt = 0;
-    for (int w = 0; w < kSelThreads / 32; ++w) {
-      if (w < warp) kb += warp_keep[w];
-      kt += warp_keep[w];
-    }
-    if (keep) kept[kb + __popc(bk & below)] = j;
-    base_keep += kt;
-    base_tie += tt;
+    int n_tie, n_keep;
+    const int tie_rank = base_tie + block_rank(tie, warp_count[phase][0], n_tie);
+    keep |= tie && tie_rank < ties;
+    const int rank = base_keep + block_rank(keep, warp_count[phase][1], n_keep);
+    if (keep) kept[rank] = j;
+    base_keep += n_keep;
+    base_tie += n_tie;
   }
 }
 
@@ -217,8 +228,10 @@ extern "C" int cb2_paged_evict(void* k_pages, void* v_pages, long long k_page_st
   while ((1 << page_log2) < page_size) ++page_log2;
   const PagedBatch batch{block_table, seq_lens, nullptr, R, max_pages, n_pages, page_log2, 0, 0, max_k, dev_status};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const EvictArgs e{weights, Hkv, budget, keep_first, keep_last, kept, new_lens};
-  paged_select_kernel<<<dim3(Hkv, R), kSelThreads, 0, st>>>(e, batch);
+  const EvictArgs e{weights, Hkv, budget, keep_first, keep_last, kept, new_lens, max_k < kMostHeld ? max_k : kMostHeld};
+  if (cudaFuncSetAttribute(paged_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostHeld * 4) != cudaSuccess)
+    return CB2_LAUNCH_FAIL;
+  paged_select_kernel<<<dim3(Hkv, R), kSelThreads, size_t(e.held) * 4, st>>>(e, batch);
   CB2_LAUNCH_CHECK();
   const MoveArgs m{static_cast<char*>(k_pages), static_cast<char*>(v_pages), k_page_stride * esz, v_page_stride * esz, weights,
                    kept, new_table, new_pages, Hkv, budget, d * esz};

@@ -678,46 +678,80 @@ def gated_contract(s: torch.Tensor, g: torch.Tensor, v: torch.Tensor) -> torch.T
 
 
 # --------------------------------------------------------------------------- paged cache
+# A step of a decode loop costs the GPU a few microseconds, so these wrappers keep their checks cheap: one call
+# per tensor for its place, no views, the stream's handle without a stream object.
+def _here(what: str, dev: int, *tensors: torch.Tensor) -> None:
+    for t in tensors:
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise B200Error("catopt_b200 executors take CUDA tensors only (no CPU fallback)")
+        if t.get_device() != dev:
+            raise B200Error(f"{what}: tensor on {t.device} but the current device is cuda:{dev}")
+
+
+def _status_ptr(what: str, dev: int) -> int:
+    w = _status_words.get(dev)
+    if w is None:
+        if torch.cuda.is_current_stream_capturing():
+            raise B200Error(f"{what}: the first call on a device allocates its status word and must not be captured")
+        w = device_status(torch.device("cuda", dev))
+    return w.data_ptr()
+
+
+def _current(what: str, t: torch.Tensor) -> int:
+    """The current device, on which every tensor of the call has to be."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise B200Error("catopt_b200 executors take CUDA tensors only (no CPU fallback)")
+    return torch.cuda.current_device()
+
+
+def _bound(what: str, name: str, value: int, most: int) -> int:
+    if not 0 <= value <= most:
+        raise B200Error(f"{what}: {name}={value} is outside 0..{most}")
+    return int(value)
+
+
+def _raw_stream(dev: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(dev)
+
+
 def _no_grad_asked(what: str, *tensors: torch.Tensor | None) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise B200Error(f"{what} serves a cache and has no gradient: call it under torch.no_grad()")
 
 
-def _pools(what: str, k_pages: torch.Tensor, v_pages: torch.Tensor) -> tuple[int, int]:
-    """Page strides (elements) of two pools ``[n_pages, Hkv, page_size, d]`` that are dense inside a page."""
-    require_device(k_pages, v_pages)
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype or 0 in k_pages.shape:
+def _pools(what: str, dev: int, k_pages: torch.Tensor, v_pages: torch.Tensor) -> tuple[int, int, int, int, int, int]:
+    """``(n_pages, Hkv, page_size, d, stride of a K page, of a V page)`` of two pools that are dense inside a page."""
+    _here(what, dev, k_pages, v_pages)
+    shape = k_pages.shape
+    if len(shape) != 4 or shape != v_pages.shape or k_pages.dtype != v_pages.dtype or 0 in shape:
         raise B200Error(f"{what}: k_pages and v_pages are [n_pages, Hkv, page_size, d] of one shape and dtype")
-    n, hkv, ps, d = k_pages.shape
+    n, hkv, ps, d = shape
     page = hkv * ps * d
     strides = []
     for pool in (k_pages, v_pages):
-        if not pool[0].is_contiguous() or (n > 1 and pool.stride(0) < page):
+        sn, sh, sp, sd = pool.stride()
+        if (sd != 1 and d > 1) or (sp != d and ps > 1) or (sh != ps * d and hkv > 1) or (sn < page and n > 1):
             raise B200Error(f"{what}: a page [Hkv, page_size, d] must be contiguous")
-        strides.append(pool.stride(0) if n > 1 else page)
-    return strides[0], strides[1]
+        strides.append(sn if n > 1 else page)
+    return n, hkv, ps, d, strides[0], strides[1]
 
 
-def _page_weights(what: str, weights: torch.Tensor, k_pages: torch.Tensor) -> None:
-    require_cuda(weights)
-    if weights.dtype != torch.float32 or weights.shape != k_pages.shape[:3]:
-        raise B200Error(f"{what}: weights are float32 [n_pages, Hkv, page_size]")
+def _dense(what: str, dev: int, name: str, t: torch.Tensor, dtype: torch.dtype, *shape: int) -> int:
+    """Address of a contiguous tensor of this shape and type on the current device."""
+    if not isinstance(t, torch.Tensor) or t.get_device() != dev:
+        _here(what, dev, t)
+    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous():
+        raise B200Error(f"{what}: {name} is a contiguous {dtype} {list(shape)}, got {t.dtype} {list(t.shape)}")
+    return t.data_ptr()
 
 
-def _index(what: str, name: str, t: torch.Tensor, shape: tuple) -> None:
-    require_cuda(t)
-    if t.dtype != torch.int32 or tuple(t.shape) != shape:
-        raise B200Error(f"{what}: {name} is int32 {list(shape)}, got {t.dtype} {list(t.shape)}")
-
-
-def _ragged_batch(what: str, block_table: torch.Tensor, seq_lens: torch.Tensor, cu_q: torch.Tensor) -> tuple[int, int]:
+def _ragged_batch(what: str, dev: int, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                  cu_q: torch.Tensor) -> tuple[int, int, int, int, int]:
     if block_table.dim() != 2 or 0 in block_table.shape:
         raise B200Error(f"{what}: block_table is int32 [R, max_pages]")
     R, max_pages = block_table.shape
-    _index(what, "block_table", block_table, (R, max_pages))
-    _index(what, "seq_lens", seq_lens, (R,))
-    _index(what, "cu_q", cu_q, (R + 1,))
-    return R, max_pages
+    return (R, max_pages, _dense(what, dev, "block_table", block_table, torch.int32, R, max_pages),
+            _dense(what, dev, "seq_lens", seq_lens, torch.int32, R), _dense(what, dev, "cu_q", cu_q, torch.int32, R + 1))
 
 
 def _token_rows(t: torch.Tensor) -> torch.Tensor:
@@ -729,12 +763,10 @@ def _token_rows(t: torch.Tensor) -> torch.Tensor:
     return t
 
 
-def _dense_out(what: str, out: torch.Tensor | None, q: torch.Tensor) -> torch.Tensor:
+def _dense_out(what: str, dev: int, out: torch.Tensor | None, q: torch.Tensor) -> torch.Tensor:
     if out is None:
         return torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    require_cuda(out)
-    if out.shape != q.shape or out.dtype != q.dtype:
-        raise B200Error(f"{what}: out must have the shape and dtype of q")
+    _dense(what, dev, "out", out, q.dtype, *q.shape)
     return out
 
 
@@ -755,46 +787,45 @@ def paged_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_pag
     rotary/2)``, or ``(2i, 2i+1)`` if ``interleaved``.  ``weights`` (float32 ``[n_pages, Hkv, page_size]``) is
     zeroed at the new slots.  Returns the normed and rotated ``q`` (rows behind ``cu_q[R]`` are not written)."""
     what = "paged_append"
-    require_device(q, k, v)
-    ks, vs = _pools(what, k_pages, v_pages)
-    R, max_pages = _ragged_batch(what, block_table, seq_lens, cu_q)
-    n_pages, hkv, ps, d = k_pages.shape
-    if k.dim() != 3 or tuple(k.shape[1:]) != (hkv, d) or v.shape != k.shape or not (k.dtype == v.dtype == k_pages.dtype):
+    dev = _current(what, k_pages)
+    n_pages, hkv, ps, d, ks, vs = _pools(what, dev, k_pages, v_pages)
+    R, max_pages, table, lens, cu = _ragged_batch(what, dev, block_table, seq_lens, cu_q)
+    dt = k_pages.dtype
+    _here(what, dev, k, v)
+    n = k.shape[0] if k.dim() == 3 else -1
+    if n < 0 or k.shape[1] != hkv or k.shape[2] != d or v.shape != k.shape or k.dtype != dt or v.dtype != dt:
         raise B200Error(f"{what}: k and v are [n_tokens, {hkv}, {d}] of the pools' dtype")
-    n = k.shape[0]
-    if q is not None and (q.dim() != 3 or q.shape[0] != n or q.shape[2] != d or q.dtype != k.dtype):
-        raise B200Error(f"{what}: q is [n_tokens, Hq, {d}] of the dtype of k")
-    for w in (q_weight, k_weight):
-        if w is not None:
-            require_cuda(w)
-            if tuple(w.shape) != (d,) or w.dtype != k.dtype:
-                raise B200Error(f"{what}: norm weights are [{d}] of the dtype of k")
+    w_ptr = None if weights is None else _dense(what, dev, "weights", weights, torch.float32, n_pages, hkv, ps)
+    qw = None if q_weight is None else _dense(what, dev, "q_weight", q_weight, dt, d)
+    kw = None if k_weight is None else _dense(what, dev, "k_weight", k_weight, dt, d)
     rotary = rows = 0
+    cos_ptr = sin_ptr = pos_ptr = None
     if cos is not None or sin is not None or positions is not None:
         if cos is None or sin is None or positions is None:
             raise B200Error(f"{what}: rotation takes cos, sin and positions")
-        require_cuda(cos, sin)
-        if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32 or \
-                0 in cos.shape or 2 * cos.shape[1] > d:
+        if cos.dim() != 2 or 0 in cos.shape or 2 * cos.shape[1] > d:
             raise B200Error(f"{what}: cos and sin are float32 [rows, rotary/2], rotary <= {d}")
-        _index(what, "positions", positions, (n,))
-        rows, rotary = cos.shape[0], 2 * cos.shape[1]
-    if weights is not None:
-        _page_weights(what, weights, k_pages)
+        rows, half = cos.shape
+        rotary = 2 * half
+        cos_ptr = _dense(what, dev, "cos", cos, torch.float32, rows, half)
+        sin_ptr = _dense(what, dev, "sin", sin, torch.float32, rows, half)
+        pos_ptr = _dense(what, dev, "positions", positions, torch.int32, n)
     _no_grad_asked(what, q, k, v, q_weight, k_weight, cos, sin)
-    k, v = _token_rows(k), _token_rows(v)
+    res, hq, q_args = None, 0, (None, 0, 0)
     if q is not None:
-        res = _dense_out(what, out, q)
+        _here(what, dev, q)
+        if q.dim() != 3 or q.shape[0] != n or q.shape[2] != d or q.dtype != dt:
+            raise B200Error(f"{what}: q is [n_tokens, Hq, {d}] of the dtype of k")
+        hq = q.shape[1]
+        res = _dense_out(what, dev, out, q)
         q = _token_rows(q)
-        qa = (q.data_ptr(), q.stride(0), q.stride(1))
-    else:
-        res, qa = None, (None, 0, 0)
+        q_args = (q.data_ptr(), q.stride(0), q.stride(1))
+    k, v = _token_rows(k), _token_rows(v)
     rc = _lib.load().cb2_paged_append(
-        *qa, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), _ptr(res), k_pages.data_ptr(),
-        v_pages.data_ptr(), ks, vs, _ptr(weights), block_table.data_ptr(), seq_lens.data_ptr(), cu_q.data_ptr(),
-        _ptr(positions), _ptr(q_weight), _ptr(k_weight), float(eps), _ptr(cos), _ptr(sin), rows, rotary,
-        1 if interleaved else 0, n, R, 0 if q is None else q.shape[1], hkv, d, ps, n_pages, max_pages, dtype_code(k.dtype),
-        device_status(k.device).data_ptr(), stream_ptr())
+        *q_args, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+        None if res is None else res.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, w_ptr, table, lens, cu, pos_ptr,
+        qw, kw, eps, cos_ptr, sin_ptr, rows, rotary, 1 if interleaved else 0, n, R, hq, hkv, d, ps, n_pages, max_pages,
+        dtype_code(dt), _status_ptr(what, dev), _raw_stream(dev))
     check(rc, "cb2_paged_append")
     return res
 
@@ -814,29 +845,29 @@ def om_paged_fwd(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     ``weights`` (float32 ``[n_pages, Hkv, page_size]``): the softmax probability that every cached key gets, summed
     over rows and the heads of its group, is added to it.  ``scale`` defaults to ``1/sqrt(d)``."""
     what = "om_paged_fwd"
-    require_device(q)
-    ks, vs = _pools(what, k_pages, v_pages)
-    R, max_pages = _ragged_batch(what, block_table, seq_lens, cu_q)
-    n_pages, hkv, ps, d = k_pages.shape
-    if q.dim() != 3 or q.shape[2] != d or q.dtype != k_pages.dtype or q.shape[1] == 0 or q.shape[1] % hkv:
+    dev = _current(what, k_pages)
+    n_pages, hkv, ps, d, ks, vs = _pools(what, dev, k_pages, v_pages)
+    R, max_pages, table, lens, cu = _ragged_batch(what, dev, block_table, seq_lens, cu_q)
+    _here(what, dev, q)
+    dt = q.dtype
+    if q.dim() != 3 or q.shape[2] != d or dt != k_pages.dtype or q.shape[1] == 0 or q.shape[1] % hkv:
         raise B200Error(f"{what}: q is [n_tokens, Hq, {d}] of the pools' dtype, Hq a multiple of {hkv}")
-    if weights is not None:
-        _page_weights(what, weights, k_pages)
+    w_ptr = None if weights is None else _dense(what, dev, "weights", weights, torch.float32, n_pages, hkv, ps)
     _no_grad_asked(what, q, k_pages, v_pages)
-    res = _dense_out(what, out, q)
+    res = _dense_out(what, dev, out, q)
     q = _token_rows(q)
     n, hq = q.shape[0], q.shape[1]
-    max_k = max_pages * ps if max_k is None else int(max_k)
-    code, w = dtype_code(q.dtype), 0 if weights is None else 1
+    max_q = _bound(what, "max_q", max_q, (1 << 31) - 1)
+    max_k = _bound(what, "max_k", max_pages * ps if max_k is None else max_k, min(max_pages * ps, 1 << 30))
+    code = dtype_code(dt)
     lib = _lib.load()
-    need = lib.cb2_om_paged_scratch_bytes(n, R, hq, hkv, d, max_q, max_k, w, code)
+    need = lib.cb2_om_paged_scratch_bytes(n, R, hq, hkv, d, max_q, max_k, 0 if weights is None else 1, code)
     # a buffer of its own for every call: two captured graphs, or two streams, never share one
     scratch = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)
     rc = lib.cb2_om_paged_fwd(q.data_ptr(), q.stride(0), q.stride(1), k_pages.data_ptr(), v_pages.data_ptr(), ks, vs,
-                              res.data_ptr(), _ptr(weights), block_table.data_ptr(), seq_lens.data_ptr(), cu_q.data_ptr(),
-                              n, R, hq, hkv, d, ps, n_pages, max_pages, int(max_q), max_k,
-                              1.0 / float(d) ** 0.5 if scale is None else float(scale), 1 if causal else 0, code,
-                              scratch.data_ptr(), need, device_status(q.device).data_ptr(), stream_ptr())
+                              res.data_ptr(), w_ptr, table, lens, cu, n, R, hq, hkv, d, ps, n_pages, max_pages, max_q, max_k,
+                              d ** -0.5 if scale is None else scale, 1 if causal else 0, code, scratch.data_ptr(), need,
+                              _status_ptr(what, dev), _raw_stream(dev))
     check(rc, "cb2_om_paged_fwd")
     return res
 
@@ -852,24 +883,25 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, weights: torch.Ten
     none of which may belong to a request of this call; the old pages stay as they are.  Returns ``(kept, new_lens)``:
     int32 ``[R, Hkv, budget]``, the old slot of every new one and -1 behind the last, and int32 ``[R]``."""
     what = "paged_evict"
-    ks, vs = _pools(what, k_pages, v_pages)
+    dev = _current(what, k_pages)
+    n_pages, hkv, ps, d, ks, vs = _pools(what, dev, k_pages, v_pages)
     if block_table.dim() != 2 or 0 in block_table.shape or new_table.dim() != 2 or 0 in new_table.shape:
         raise B200Error(f"{what}: block_table and new_table are int32 [R, pages]")
     R, max_pages = block_table.shape
-    _index(what, "block_table", block_table, (R, max_pages))
-    _index(what, "seq_lens", seq_lens, (R,))
-    _index(what, "new_table", new_table, (R, new_table.shape[1]))
-    _page_weights(what, weights, k_pages)
-    n_pages, hkv, ps, d = k_pages.shape
-    max_k = max_pages * ps if max_k is None else int(max_k)
-    if budget < 1 or new_table.shape[1] * ps < budget:
-        raise B200Error(f"{what}: a budget of {budget} keys does not fit {new_table.shape[1]} pages of {ps}")
+    new_pages = new_table.shape[1]
+    table = _dense(what, dev, "block_table", block_table, torch.int32, R, max_pages)
+    lens = _dense(what, dev, "seq_lens", seq_lens, torch.int32, R)
+    to = _dense(what, dev, "new_table", new_table, torch.int32, R, new_pages)
+    w_ptr = _dense(what, dev, "weights", weights, torch.float32, n_pages, hkv, ps)
+    _no_grad_asked(what, k_pages, v_pages, weights)
+    max_k = _bound(what, "max_k", max_pages * ps if max_k is None else max_k, min(max_pages * ps, 1 << 30))
+    keep_first, keep_last = (_bound(what, name, x, budget) for name, x in (("keep_first", keep_first), ("keep_last", keep_last)))
+    if budget < 1 or new_pages * ps < budget:
+        raise B200Error(f"{what}: a budget of {budget} keys does not fit {new_pages} pages of {ps}")
     kept = torch.empty(R, hkv, budget, dtype=torch.int32, device=k_pages.device)
     new_lens = torch.empty(R, dtype=torch.int32, device=k_pages.device)
-    rc = _lib.load().cb2_paged_evict(k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, weights.data_ptr(),
-                                     block_table.data_ptr(), seq_lens.data_ptr(), new_table.data_ptr(), kept.data_ptr(),
-                                     new_lens.data_ptr(), R, hkv, d, ps, n_pages, max_pages, new_table.shape[1], max_k,
-                                     int(budget), int(keep_first), int(keep_last), dtype_code(k_pages.dtype),
-                                     device_status(k_pages.device).data_ptr(), stream_ptr())
+    rc = _lib.load().cb2_paged_evict(k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, w_ptr, table, lens, to, kept.data_ptr(),
+                                     new_lens.data_ptr(), R, hkv, d, ps, n_pages, max_pages, new_pages, max_k, budget, keep_first,
+                                     keep_last, dtype_code(k_pages.dtype), _status_ptr(what, dev), _raw_stream(dev))
     check(rc, "cb2_paged_evict")
     return kept, new_lens
