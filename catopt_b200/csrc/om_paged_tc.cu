@@ -9,9 +9,9 @@
 // Only a block that some row of the tile may not see whole is masked, per element.  Of the last block of a
 // request the value rows behind its length are zeroed in shared memory, since 0 x NaN is NaN.
 //
-// Roles: warp 0 = loads (pages by TMA: one box per page and 64 columns, each lane its own page; the packed
-// query rows by 16-byte asynchronous copies, since a tile may start inside a token's group), warp 1 = MMA issue
-// and TMEM owner, warps 2..5 = softmax.  The pieces of a share are listed in shared memory in batches, so that
+// Roles: warp 0 = loads (pages by TMA: one box per page and 64 columns, each lane its own page), warp 1 = MMA
+// issue and TMEM owner, warps 2..5 = softmax and the query rows (16-byte asynchronous copies, since a tile may start
+// inside a token's group; a piece's rows are fetched during the last softmax of the piece before).  The pieces of a share are listed in shared memory in batches, so that
 // the softmax threads spend no registers on the walk.  Every wait is bounded.
 #include "om_paged.cuh"
 #include "umma.cuh"
@@ -25,7 +25,7 @@ constexpr int kBatch = 32;                // pieces listed at a time
 constexpr uint32_t kTile = umma::kTileBytes;
 constexpr uint32_t kOffQ = 0, kOffK = kTile, kOffV = 2 * kTile;
 constexpr uint32_t kOffBars = 3 * kTile;
-constexpr int kNumBars = 10;
+constexpr int kNumBars = 8;
 constexpr uint32_t kColS = 0, kColO = 128, kTmemCols = 256;
 
 struct Piece {
@@ -75,8 +75,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kOffBars);
-  uint64_t *k_full = bars, *k_empty = bars + 1, *v_full = bars + 2, *v_empty = bars + 3, *q_full = bars + 4, *q_empty = bars + 5,
-           *s_ready = bars + 6, *p_ready = bars + 7, *o_done = bars + 8;
+  uint64_t *k_full = bars, *k_empty = bars + 1, *v_full = bars + 2, *v_empty = bars + 3, *q_full = bars + 4,
+           *s_ready = bars + 5, *p_ready = bars + 6, *o_done = bars + 7;
   Smem* sh = reinterpret_cast<Smem*>(smem + kOffMisc);
   volatile int* s_abort = &sh->abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -87,8 +87,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     mbar_init(k_empty, 1);
     mbar_init(v_full, 1);
     mbar_init(v_empty, 1);
-    mbar_init(q_full, 32);
-    mbar_init(q_empty, 1);
+    mbar_init(q_full, 128);
     mbar_init(s_ready, 1);
     mbar_init(p_ready, 128);
     mbar_init(o_done, 1);
@@ -142,7 +141,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
 
     if (warp == 0) {
       const int ps_log2 = batch.page_log2, box_log2 = min(ps_log2, 7), boxes = kKB >> box_log2;
-      for (int p = 0; p < count; ++p, ++n_piece) {
+      for (int p = 0; p < count; ++p) {
         const Piece pc = sh->pieces[p];
         const int blocks = pc.b1 - pc.b0;
         auto load_block = [&](int j, const CUtensorMap* map, unsigned char* dst, uint64_t* full, uint64_t* empty) -> bool {
@@ -168,21 +167,6 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
           return true;
         };
         if (!load_block(0, &map_k, smem + kOffK, k_full, k_empty)) break;
-        // the packed rows of the tile
-        bool ok = n_piece == 0 || mbar_wait_abortable(q_empty, (n_piece - 1) & 1, s_abort);
-        if (!__all_sync(0xffffffffu, ok)) break;
-        const int chunks = halves * 8, rows = pc.n * a.G - pc.row0;
-        for (int e = lane; e < kRT * chunks; e += 32) {
-          const int rr = e / chunks, col = (e % chunks) * 8;
-          const bool there = rr < rows && col < d;
-          const int row = pc.row0 + (there ? rr : 0);
-          const __nv_bfloat16* src = a.q + (pc.t0 + row / a.G) * a.q_token + (pc.h * a.G + row % a.G) * a.q_head + (there ? col : 0);
-          cp_async16_or_zero(q_addr + umma::tile_chunk_offset(rr, col), src, there);
-        }
-        cp_async_commit();
-        cp_async_wait_all();
-        fence_proxy_async_smem();
-        mbar_arrive(q_full);
         if (!load_block(0, &map_v, smem + kOffV, v_full, v_empty)) break;
         bool fine = true;
         for (int j = 1; fine && j < blocks; ++j)
@@ -206,7 +190,6 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
                 umma::mma_bf16(tmem + kColS, umma::desc_kmajor(q_addr, ks), umma::desc_kmajor(k_addr, ks), idesc_kk, ks > 0);
             umma::mma_commit(s_ready);
             umma::mma_commit(k_empty);
-            if (j == blocks - 1) umma::mma_commit(q_empty);
             return true;
           };
           bool ok = mbar_wait_abortable(q_full, n_piece & 1, s_abort) && issue_scores(0);
@@ -232,6 +215,31 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       constexpr float kLazy = 8.f;
       const int ncb = (d + 31) >> 5;
       const float scale = a.scale_log2e;
+      // The 32 packed rows of this warp, into the query tile: the row's place is worked out by one lane, its
+      // chunks are copied by 8 or 16 neighbouring ones.
+      auto load_rows = [&](const Piece* pc) {
+        const int row = pc->row0 + rr;
+        const bool there = row < pc->n * a.G;
+        const int tok = there ? row / a.G : 0, g = there ? row - tok * a.G : 0;
+        const long long at = (pc->t0 + tok) * a.q_token + (pc->h * a.G + g) * a.q_head;
+        const int chunks = halves * 8, per_copy = 32 / chunks, col = (lane % chunks) * 8;
+        for (int i = 0; i < 32; i += per_copy) {
+          const int from = i + lane / chunks;
+          const long long off = __shfl_sync(0xffffffffu, at, from);
+          const bool ok = __shfl_sync(0xffffffffu, there, from) && col < d;
+          cp_async16_or_zero(q_addr + umma::tile_chunk_offset(q4 * 32 + from, col), a.q + off + (ok ? col : 0), ok);
+        }
+        cp_async_commit();
+      };
+      auto rows_there = [&] {
+        cp_async_wait_all();
+        fence_proxy_async_smem();
+        mbar_arrive(q_full);
+      };
+      if (count > 0) {
+        load_rows(&sh->pieces[0]);
+        rows_there();
+      }
       for (int p = 0; p < count; ++p) {
         const Piece* pc = &sh->pieces[p];
         const int blocks = pc->b1 - pc->b0, b0 = pc->b0, len = pc->len;
@@ -248,6 +256,9 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
           if (!__all_sync(0xffffffffu, ok)) break;
           umma::fence_after_sync();
           const int k0 = (b0 + j) * kKB;
+          // the last scores of this piece are out, so the next piece's rows may take its place
+          const bool next_rows = j == blocks - 1 && p + 1 < count;
+          if (next_rows) load_rows(pc + 1);
 #pragma unroll
           for (int cb = 0; cb < 4; ++cb) umma::tmem_ld32(lane_base + kColS + cb * 32, sv[cb]);
           umma::tmem_wait_ld();
@@ -318,6 +329,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
           }
           umma::fence_before_sync();
           mbar_arrive(p_ready);
+          if (next_rows) rows_there();
         }
         if (!__all_sync(0xffffffffu, ok)) break;
         ok = mbar_wait_abortable(o_done, (n_blk + blocks - 1) & 1, s_abort);
