@@ -1,32 +1,52 @@
 // Attention over a paged key/value cache on the tensor cores (bf16), for requests with many packed rows
-// (chunks of prompts): the work line of om_paged.cuh with tiles of 128 packed rows and 128-key blocks.
+// (chunks of prompts): the work line of om_paged.cuh with tiles of 128 packed rows and 64-key blocks.
 //
-// A CTA keeps two to an SM (half of the tensor memory and of the shared memory each), so one's softmax runs
-// while the other's products are on the tensor core, and walks its share of the line:
-//   MMA1  S = Q K_j^T -> TMEM;   P = 2^(S scale - m) as bf16 over S, l and the running m in registers (thread
-//   = row = TMEM lane);   MMA2  O += P V_j with P read from TMEM.
-// The reference point m follows the maximum lazily (when it moved by more than 2^8), so O is rarely rescaled.
+// Two CTAs share an SM (half of the tensor memory and of the shared memory each); a CTA walks its share of the line:
+//   MMA1  S = Q K_j^T -> TMEM, two blocks ahead of the softmax (two S buffers of 64 columns);
+//   softmax   P = 2^(S scale - m) as bf16 over S, l and the running m in registers (thread = row = TMEM lane);
+//   MMA2  O += P V_j, P read from TMEM.
+// With S ready before it is asked for, the softmax warps never wait for the tensor core, which finds the next
+// block's P after every product: one exponential per score (16 a clock and SM) and the products (1024 clocks per
+// 128 x 128 scores either way) overlap.  The reference point m follows the maximum lazily (when it moved by
+// more than 2^8), so O is rarely rescaled, and only then does the softmax wait for the product before.
 // Only a block that some row of the tile may not see whole is masked, per element.  Of the last block of a
 // request the value rows behind its length are zeroed in shared memory, since 0 x NaN is NaN.
 //
 // Roles: warp 0 = loads (pages by TMA: one box per page and 64 columns, each lane its own page), warp 1 = MMA
 // issue and TMEM owner, warps 2..5 = softmax and the query rows (16-byte asynchronous copies, since a tile may start
-// inside a token's group; a piece's rows are fetched during the last softmax of the piece before).  The pieces of a share are listed in shared memory in batches, so that
-// the softmax threads spend no registers on the walk.  Every wait is bounded.
+// inside a token's group; a piece's rows are fetched during the last softmax of the piece before).  The
+// pieces of a share are listed in shared memory in batches, so that the softmax threads spend no registers on
+// the walk.  Every wait is bounded.
 #include "om_paged.cuh"
 #include "umma.cuh"
 
 namespace cb2 {
 namespace {
 
-constexpr int kRT = 128, kKB = 128;
+constexpr int kRT = 128, kKB = 64;
 constexpr int kThreads = 192;
 constexpr int kBatch = 32;                // pieces listed at a time
-constexpr uint32_t kTile = umma::kTileBytes;
-constexpr uint32_t kOffQ = 0, kOffK = kTile, kOffV = 2 * kTile;
-constexpr uint32_t kOffBars = 3 * kTile;
-constexpr int kNumBars = 8;
+constexpr uint32_t kQTile = umma::kTileBytes;            // 128 x 128 bf16
+constexpr uint32_t kSub = 64 * 128;                      // 64 keys x 64 columns
+constexpr uint32_t kKvTile = 2 * kSub;
+constexpr uint32_t kOffQ = 0, kOffK = kQTile, kOffV = kOffK + 2 * kKvTile;
+constexpr uint32_t kOffBars = kOffV + 2 * kKvTile;
+constexpr int kNumBars = 15;
 constexpr uint32_t kColS = 0, kColO = 128, kTmemCols = 256;
+
+// Byte offset of the 16-byte chunk of columns [col, col + 8) of a key row in a 64-key tile.
+__device__ __forceinline__ uint32_t kv_chunk_offset(uint32_t row, uint32_t col) {
+  return (col >> 6) * kSub + row * 128u + ((((col & 63u) >> 3) ^ (row & 7u)) << 4);
+}
+__device__ __forceinline__ uint64_t desc_k(uint32_t tile, int ks) {      // K-major, 16 columns a step
+  return umma::smem_desc(tile + (ks >> 2) * kSub + (ks & 3) * 32u, 16u, 1024u);
+}
+__device__ __forceinline__ uint64_t desc_v(uint32_t tile, int ks) {      // MN-major, 16 keys a step
+  return umma::smem_desc(tile + ks * 2048u, kSub, 1024u);
+}
+
+// arguments of a wait: where to see that another role gave up, the budget, and the line to report
+#define CB2_SITE s_abort, kDefaultWaitNs, __LINE__
 
 struct Piece {
   int r, h, row0, t0, n, len, b0, b1;
@@ -75,22 +95,24 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kOffBars);
-  uint64_t *k_full = bars, *k_empty = bars + 1, *v_full = bars + 2, *v_empty = bars + 3, *q_full = bars + 4,
-           *s_ready = bars + 5, *p_ready = bars + 6, *o_done = bars + 7;
+  uint64_t *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 6;      // two slots each
+  uint64_t *s_ready = bars + 8, *p_ready = bars + 10, *o_done = bars + 12, *q_full = bars + 14;
   Smem* sh = reinterpret_cast<Smem*>(smem + kOffMisc);
   volatile int* s_abort = &sh->abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int cta = blockIdx.x, n_cta = gridDim.x;
 
   if (tid == 0) {
-    mbar_init(k_full, 1);
-    mbar_init(k_empty, 1);
-    mbar_init(v_full, 1);
-    mbar_init(v_empty, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 1);
+      mbar_init(&s_ready[i], 1);
+      mbar_init(&p_ready[i], 128);
+      mbar_init(&o_done[i], 1);
+    }
     mbar_init(q_full, 128);
-    mbar_init(s_ready, 1);
-    mbar_init(p_ready, 128);
-    mbar_init(o_done, 1);
     sh->abort = sh->loads_k = sh->loads_v = 0;
     scratch.joins[cta].r = -1;
     mbar_fence_init();
@@ -140,70 +162,72 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     const int count = sh->count;
 
     if (warp == 0) {
-      const int ps_log2 = batch.page_log2, box_log2 = min(ps_log2, 7), boxes = kKB >> box_log2;
+      const int ps_log2 = batch.page_log2, box_log2 = min(ps_log2, 6), boxes = kKB >> box_log2;
       for (int p = 0; p < count; ++p) {
         const Piece pc = sh->pieces[p];
         const int blocks = pc.b1 - pc.b0;
-        auto load_block = [&](int j, const CUtensorMap* map, unsigned char* dst, uint64_t* full, uint64_t* empty) -> bool {
-          const int k0 = (pc.b0 + j) * kKB;
+        bool fine = true;
+        for (int j = 0; fine && j < blocks; ++j, ++n_blk) {
+          const int k0 = (pc.b0 + j) * kKB, slot = n_blk & 1;
           const bool mine = lane < boxes && k0 + (lane << box_log2) < pc.len;
           int page = 0;
           if (mine) page = paged_page(batch, pc.r, (k0 + (lane << box_log2)) >> ps_log2);
           const unsigned have = __ballot_sync(0xffffffffu, mine);
-          bool ok = true;
-          if (n_blk + j > 0) ok = mbar_wait_abortable(empty, (n_blk + j - 1) & 1, s_abort);
-          if (!__all_sync(0xffffffffu, ok)) return false;
-          const uint32_t box_bytes = 128u << box_log2;
-          if (lane == 0) {
-            mbar_arrive_expect_tx(full, __popc(have) * halves * box_bytes);
-            ++*(full == k_full ? &sh->loads_k : &sh->loads_v);
+          const uint32_t box_bytes = 128u << box_log2, bytes = __popc(have) * halves * box_bytes;
+          const int y = ps_log2 > 6 ? k0 & ((1 << ps_log2) - 1) : 0;       // inside a page longer than a block
+          for (int kv = 0; fine && kv < 2; ++kv) {
+            uint64_t *full = kv ? &v_full[slot] : &k_full[slot], *empty = kv ? &v_empty[slot] : &k_empty[slot];
+            bool ok = n_blk < 2 || mbar_wait_abortable(empty, ((n_blk >> 1) - 1) & 1, CB2_SITE);
+            fine = __all_sync(0xffffffffu, ok);
+            if (!fine) break;
+            if (lane == 0) {
+              mbar_arrive_expect_tx(full, bytes);
+              ++*(kv ? &sh->loads_v : &sh->loads_k);
+            }
+            __syncwarp();
+            if (mine) {
+              unsigned char* dst = smem + (kv ? kOffV : kOffK) + slot * kKvTile + lane * box_bytes;
+              for (int hf = 0; hf < halves; ++hf)
+                tma_load_4d(dst + hf * kSub, kv ? &map_v : &map_k, hf * 64, y, pc.h, page, full);
+            }
           }
-          __syncwarp();
-          if (mine) {
-            const int y = k0 & ((1 << ps_log2) - 1);       // inside the page when pages are longer than a block
-            for (int hf = 0; hf < halves; ++hf)
-              tma_load_4d(dst + hf * umma::kSubTileBytes + lane * box_bytes, map, hf * 64, ps_log2 > 7 ? y : 0, pc.h, page, full);
-          }
-          return true;
-        };
-        if (!load_block(0, &map_k, smem + kOffK, k_full, k_empty)) break;
-        if (!load_block(0, &map_v, smem + kOffV, v_full, v_empty)) break;
-        bool fine = true;
-        for (int j = 1; fine && j < blocks; ++j)
-          fine = load_block(j, &map_k, smem + kOffK, k_full, k_empty) && load_block(j, &map_v, smem + kOffV, v_full, v_empty);
+        }
         if (!fine) break;
-        n_blk += blocks;
       }
     } else if (warp == 1) {
       if (lane == 0) {
         const int ksteps = (d + 15) >> 4;
-        constexpr uint32_t idesc_kk = umma::instr_desc_bf16(128, 128, false, false);
+        constexpr uint32_t idesc_kk = umma::instr_desc_bf16(128, kKB, false, false);
         const uint32_t idesc_kn = umma::instr_desc_bf16(128, uint32_t(d + 15) & ~15u, false, true);
         for (int p = 0; p < count; ++p, ++n_piece) {
           const int blocks = sh->pieces[p].b1 - sh->pieces[p].b0;
           auto issue_scores = [&](int j) -> bool {
-            if (!mbar_wait_abortable(k_full, (n_blk + j) & 1, s_abort)) return false;
+            const uint32_t n = n_blk + j, slot = n & 1;
+            if (!mbar_wait_abortable(&k_full[slot], (n >> 1) & 1, CB2_SITE)) return false;
             umma::fence_after_sync();
 #pragma unroll
             for (int ks = 0; ks < 8; ++ks)
               if (ks < ksteps)
-                umma::mma_bf16(tmem + kColS, umma::desc_kmajor(q_addr, ks), umma::desc_kmajor(k_addr, ks), idesc_kk, ks > 0);
-            umma::mma_commit(s_ready);
-            umma::mma_commit(k_empty);
+                umma::mma_bf16(tmem + kColS + slot * kKB, umma::desc_kmajor(q_addr, ks), desc_k(k_addr + slot * kKvTile, ks), idesc_kk,
+                               ks > 0);
+            umma::mma_commit(&s_ready[slot]);
+            umma::mma_commit(&k_empty[slot]);
             return true;
           };
-          bool ok = mbar_wait_abortable(q_full, n_piece & 1, s_abort) && issue_scores(0);
+          bool ok = mbar_wait_abortable(q_full, n_piece & 1, CB2_SITE) && issue_scores(0) && (blocks < 2 || issue_scores(1));
           for (int j = 0; ok && j < blocks; ++j) {
-            ok = mbar_wait_abortable(p_ready, (n_blk + j) & 1, s_abort) && mbar_wait_abortable(v_full, (n_blk + j) & 1, s_abort);
+            const uint32_t n = n_blk + j, slot = n & 1;
+            ok = mbar_wait_abortable(&p_ready[slot], (n >> 1) & 1, CB2_SITE) && mbar_wait_abortable(&v_full[slot], (n >> 1) & 1, CB2_SITE);
             if (!ok) break;
             umma::fence_after_sync();
 #pragma unroll
-            for (int ks = 0; ks < 8; ++ks)
-              umma::mma_bf16_ts(tmem + kColO, tmem + kColS + ks * 8, umma::desc_mnmajor(v_addr, ks), idesc_kn, j > 0 || ks > 0);
-            umma::mma_commit(o_done);
-            umma::mma_commit(v_empty);
-            // the tensor pipe runs in issue order, so the next scores may overwrite P right away
-            if (j + 1 < blocks) ok = issue_scores(j + 1);
+            for (int ks = 0; ks < kKB / 16; ++ks)
+              umma::mma_bf16_ts(tmem + kColO, tmem + kColS + slot * kKB + ks * 8, desc_v(v_addr + slot * kKvTile, ks), idesc_kn,
+                                j > 0 || ks > 0);
+            umma::mma_commit(&o_done[slot]);
+            umma::mma_commit(&v_empty[slot]);
+            // the tensor pipe runs in issue order, so the scores after next may overwrite P right away
+            if (j + 2 < blocks) ok = issue_scores(j + 2);
           }
           if (!ok) break;
           n_blk += blocks;
@@ -249,30 +273,32 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         const int last = cost.causal ? min(base + (pc->row0 + rr) / a.G, len - 1) : len - 1;
         const int first_last = cost.causal ? min(base + pc->row0 / a.G, len - 1) : len - 1;
         float m_ref = -INFINITY, l_run = 0.f;
-        uint32_t sv[4][32];
         bool ok = true;
         for (int j = 0; j < blocks; ++j) {
-          ok = mbar_wait_abortable(s_ready, (n_blk + j) & 1, s_abort);
+          const uint32_t n = n_blk + j, slot = n & 1;
+          const uint32_t s_cols = lane_base + kColS + slot * kKB;
+          ok = mbar_wait_abortable(&s_ready[slot], (n >> 1) & 1, CB2_SITE);
           if (!__all_sync(0xffffffffu, ok)) break;
           umma::fence_after_sync();
           const int k0 = (b0 + j) * kKB;
           // the last scores of this piece are out, so the next piece's rows may take its place
           const bool next_rows = j == blocks - 1 && p + 1 < count;
           if (next_rows) load_rows(pc + 1);
+          uint32_t sv[2][32];
 #pragma unroll
-          for (int cb = 0; cb < 4; ++cb) umma::tmem_ld32(lane_base + kColS + cb * 32, sv[cb]);
+          for (int cb = 0; cb < 2; ++cb) umma::tmem_ld32(s_cols + cb * 32, sv[cb]);
           umma::tmem_wait_ld();
           if (k0 + kKB - 1 > first_last) {
             const int lim = last - k0;
 #pragma unroll
-            for (int cb = 0; cb < 4; ++cb)
+            for (int cb = 0; cb < 2; ++cb)
 #pragma unroll
               for (int c = 0; c < 32; ++c)
                 if (cb * 32 + c > lim) sv[cb][c] = 0xff800000u;
           }
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int cb = 0; cb < 4; ++cb)
+          for (int cb = 0; cb < 2; ++cb)
 #pragma unroll
             for (int c = 0; c < 32; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(sv[cb][c]));
           const float m_blk = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
@@ -285,7 +311,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
           const float neg_m = (m_ref == -INFINITY) ? 0.f : -m_ref;
           float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int cb = 0; cb < 4; ++cb) {
+          for (int cb = 0; cb < 2; ++cb) {
             uint32_t w[16];
 #pragma unroll
             for (int c = 0; c < 32; c += 2) {
@@ -294,84 +320,78 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
               sum[(c >> 1) & 3] += p0 + p1;
               w[c >> 1] = pack_bf16x2(p0, p1);
             }
-            umma::tmem_st16(lane_base + kColS + cb * 16, w);
+            umma::tmem_st16(s_cols + cb * 16, w);
           }
           l_run = fmaf(l_run, alpha, (sum[0] + sum[1]) + (sum[2] + sum[3]));
           umma::tmem_wait_st();
           if (k0 + kKB > len) {
             // the request's last block: value rows that nobody has written
-            ok = mbar_wait_abortable(v_full, (n_blk + j) & 1, s_abort);
+            ok = mbar_wait_abortable(&v_full[slot], (n >> 1) & 1, CB2_SITE);
             if (!__all_sync(0xffffffffu, ok)) break;
-            if (k0 + rr >= len)
-              for (int c = 0; c < halves * 8; ++c)
-                *reinterpret_cast<uint4*>(smem + kOffV + umma::tile_chunk_offset(rr, c * 8)) = make_uint4(0, 0, 0, 0);
+            const int row = rr & (kKB - 1);
+            if (k0 + row >= len && (rr >> 6) < halves)
+              for (int c = 0; c < 8; ++c)
+                *reinterpret_cast<uint4*>(smem + kOffV + slot * kKvTile + kv_chunk_offset(row, (rr >> 6) * 64 + c * 8)) =
+                    make_uint4(0, 0, 0, 0);
             fence_proxy_async_smem();
           }
-          if (j > 0) {
-            ok = mbar_wait_abortable(o_done, (n_blk + j - 1) & 1, s_abort);
+          // O <- O alpha once the product before has landed.  This wait is often skipped, so the products
+          // alternate between two barriers: of one barrier's phases, all but the awaited one are then known to be over
+          if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+            ok = mbar_wait_abortable(&o_done[slot ^ 1], ((n - 1) >> 1) & 1, CB2_SITE);
             if (!__all_sync(0xffffffffu, ok)) break;
             umma::fence_after_sync();
-            if (!__all_sync(0xffffffffu, alpha == 1.f)) {
-#pragma unroll
-              for (int cb = 0; cb < 4; ++cb)
-                if (cb < ncb) umma::tmem_ld32(lane_base + kColO + cb * 32, sv[cb]);
+            for (int cb = 0; cb < ncb; ++cb) {
+              umma::tmem_ld32(lane_base + kColO + cb * 32, sv[0]);
               umma::tmem_wait_ld();
 #pragma unroll
-              for (int cb = 0; cb < 4; ++cb) {
-                if (cb < ncb) {
-#pragma unroll
-                  for (int c = 0; c < 32; ++c) sv[cb][c] = __float_as_uint(__uint_as_float(sv[cb][c]) * alpha);
-                  umma::tmem_st32(lane_base + kColO + cb * 32, sv[cb]);
-                }
-              }
-              umma::tmem_wait_st();
+              for (int c = 0; c < 32; ++c) sv[0][c] = __float_as_uint(__uint_as_float(sv[0][c]) * alpha);
+              umma::tmem_st32(lane_base + kColO + cb * 32, sv[0]);
             }
+            umma::tmem_wait_st();
           }
           umma::fence_before_sync();
-          mbar_arrive(p_ready);
+          mbar_arrive(&p_ready[slot]);
           if (next_rows) rows_there();
         }
         if (!__all_sync(0xffffffffu, ok)) break;
-        ok = mbar_wait_abortable(o_done, (n_blk + blocks - 1) & 1, s_abort);
+        n_blk += blocks;
+        ok = mbar_wait_abortable(&o_done[(n_blk - 1) & 1], ((n_blk - 1) >> 1) & 1, CB2_SITE);
         if (!__all_sync(0xffffffffu, ok)) break;
         umma::fence_after_sync();
-        n_blk += blocks;
+        const bool live = rr < rows, whole = pc->whole;
+        const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+        const int row = pc->row0 + rr;
+        const long long at = (long long)(pc->t0 + row / a.G) * (a.G * a.Hkv) + pc->h * a.G + row % a.G;
+        float* slot = scratch.parts + paged_slot_floats(kRT, d) * (2 * cta + (b0 == 0));
+        for (int cb = 0; cb < ncb; ++cb) {
+          uint32_t sv[32];
+          __syncwarp();
+          umma::tmem_ld32(lane_base + kColO + cb * 32, sv);
+          umma::tmem_wait_ld();
+          if (!live) continue;
+          if (whole) {
+            __nv_bfloat16* dst = a.o + at * d + cb * 32;
 #pragma unroll
-        for (int cb = 0; cb < 4; ++cb)
-          if (cb < ncb) umma::tmem_ld32(lane_base + kColO + cb * 32, sv[cb]);
-        umma::tmem_wait_ld();
-        if (rr < rows) {
-          const int row = pc->row0 + rr;
-          if (pc->whole) {
-            const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
-            const long long at = (long long)(pc->t0 + row / a.G) * (a.G * a.Hkv) + pc->h * a.G + row % a.G;
-            __nv_bfloat16* dst = a.o + at * d;
+            for (int c = 0; c < 32; c += 8) {
+              if (cb * 32 + c >= d) continue;
+              uint32_t w[4];
 #pragma unroll
-            for (int cb = 0; cb < 4; ++cb) {
-#pragma unroll
-              for (int c = 0; c < 32; c += 8) {
-                if (cb * 32 + c >= d) continue;
-                uint32_t w[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                  w[i] = pack_bf16x2(__uint_as_float(sv[cb][c + 2 * i]) * inv, __uint_as_float(sv[cb][c + 2 * i + 1]) * inv);
-                *reinterpret_cast<uint4*>(dst + cb * 32 + c) = make_uint4(w[0], w[1], w[2], w[3]);
-              }
+              for (int i = 0; i < 4; ++i)
+                w[i] = pack_bf16x2(__uint_as_float(sv[c + 2 * i]) * inv, __uint_as_float(sv[c + 2 * i + 1]) * inv);
+              *reinterpret_cast<uint4*>(dst + c) = make_uint4(w[0], w[1], w[2], w[3]);
             }
-            if (a.lse2) a.lse2[at] = l_run > 0.f ? m_ref + log2f(l_run) : INFINITY;
           } else {
-            float* slot = scratch.parts + paged_slot_floats(kRT, d) * (2 * cta + (b0 == 0));
-            slot[rr] = m_ref;
-            slot[kRT + rr] = l_run;
-            float* dst = slot + 2 * kRT + rr * d;
+            float* dst = slot + 2 * kRT + rr * d + cb * 32;
 #pragma unroll
-            for (int cb = 0; cb < 4; ++cb) {
-#pragma unroll
-              for (int c = 0; c < 32; c += 4)
-                if (cb * 32 + c < d)
-                  *reinterpret_cast<uint4*>(dst + cb * 32 + c) = make_uint4(sv[cb][c], sv[cb][c + 1], sv[cb][c + 2], sv[cb][c + 3]);
-            }
+            for (int c = 0; c < 32; c += 4)
+              if (cb * 32 + c < d) *reinterpret_cast<uint4*>(dst + c) = make_uint4(sv[c], sv[c + 1], sv[c + 2], sv[c + 3]);
           }
+        }
+        if (live && whole && a.lse2) a.lse2[at] = l_run > 0.f ? m_ref + log2f(l_run) : INFINITY;
+        if (live && !whole) {
+          slot[rr] = m_ref;
+          slot[kRT + rr] = l_run;
         }
       }
     }
@@ -385,9 +405,9 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   if (*s_abort) {
     // loads in flight land before the shared memory goes (a bounded wait, too)
     if (tid == 0) {
-      if (sh->loads_k) mbar_wait_bounded(k_full, (sh->loads_k - 1) & 1);
-      if (sh->loads_v) mbar_wait_bounded(v_full, (sh->loads_v - 1) & 1);
-      if (batch.status) atomicExch(batch.status, CB2_WAIT_TIMEOUT);
+      for (int n = max(sh->loads_k - 2, 0); n < sh->loads_k; ++n) mbar_wait_bounded(&k_full[n & 1], (n >> 1) & 1);
+      for (int n = max(sh->loads_v - 2, 0); n < sh->loads_v; ++n) mbar_wait_bounded(&v_full[n & 1], (n >> 1) & 1);
+      if (batch.status) atomicExch(batch.status, CB2_WAIT_TIMEOUT | (*s_abort << 8));     // which wait: its source line
     }
     __syncthreads();
   }
@@ -397,7 +417,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   }
 }
 
-// Pools as a 4-D tensor {d, page_size, Hkv, n_pages}; box = 64 columns of a page, 128 rows at most.
+// Pools as a 4-D tensor {d, page_size, Hkv, n_pages}; box = 64 columns of a page, 64 rows at most.
 int make_pool_map(CUtensorMap* out, const void* base, int d, int page_size, int Hkv, int n_pages, long long page_stride) {
   using Fn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                           const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -412,7 +432,7 @@ int make_pool_map(CUtensorMap* out, const void* base, int d, int page_size, int 
   }
   const cuuint64_t dims[4] = {cuuint64_t(d), cuuint64_t(page_size), cuuint64_t(Hkv), cuuint64_t(n_pages)};
   const cuuint64_t strides[3] = {cuuint64_t(d) * 2, cuuint64_t(page_size) * d * 2, cuuint64_t(page_stride) * 2};
-  const cuuint32_t box[4] = {64, cuuint32_t(page_size < 128 ? page_size : 128), 1, 1};
+  const cuuint32_t box[4] = {64, cuuint32_t(page_size < kKB ? page_size : kKB), 1, 1};
   const cuuint32_t step[4] = {1, 1, 1, 1};
   const CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, step,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -440,7 +460,7 @@ int paged_tc_run(const PagedRows& rows, const PagedPools& pools, const PagedBatc
   *rt = kRT;
   const TcArgs a{static_cast<const __nv_bfloat16*>(rows.q), rows.q_token, rows.q_head, static_cast<__nv_bfloat16*>(o), lse2,
                  rows.scale_log2e, rows.G, rows.Hkv, pools.d};
-  const PagedCost<kRT, kKB> cost{rows.G, rows.Hkv, causal, kPagedChunk, few, 2};
+  const PagedCost<kRT, kKB> cost{rows.G, rows.Hkv, causal, kPagedChunk, few, 4};
   paged_tc_kernel<<<kCtas, kThreads, kSmemBytes, st>>>(mk, mv, a, batch, cost, *parts);
   CB2_LAUNCH_CHECK();
   return CB2_OK;

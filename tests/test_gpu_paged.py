@@ -71,8 +71,9 @@ def test_attention_strided_rows_and_spaced_pages(dev, dtype):
 
 @pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("new,lens,kv,group", [([1], [20000], 1, 2), ([1] * 37, [(97 * i) % 700 + 1 for i in range(37)], 2, 4),
-                                               ([2], [9001], 2, 7), ([64], [6000], 1, 4), ([1] * 300, [3 + i % 50 for i in range(300)], 1, 1)],
-                         ids=["long", "many", "two", "chunk", "r300"])
+                                               ([2], [9001], 2, 7), ([64], [6000], 1, 4), ([1] * 300, [3 + i % 50 for i in range(300)], 1, 1),
+                                               ([509, 1, 411, 314], [2048, 700, 1363, 679], 2, 4), ([1100], [6000], 2, 3)],
+                         ids=["long", "many", "two", "chunk", "r300", "pieces", "long-pieces"])
 def test_attention_work_cut_over_keys(dev, dtype, new, lens, kv, group):
     run_attend(dev, new, lens, kv, group, 128 if kv == 2 else 64, 16, dtype, weights=True, fill=float("inf"))
 
