@@ -212,78 +212,118 @@ paged_fma_kernel(const PagedRows rows, const PagedPools pools, const PagedBatch 
   }
 }
 
-// Joins the partial carriers of a unit: m = max m_c, l = sum l_c 2^(m_c - m), a likewise, over the shares
-// c .. last, none of them empty.  Block (c, y) takes rows [16 y, 16 y + 16) of the unit that starts in share c.
-// A warp holds one row, a lane four columns; with few rows several warps share a row's shares (every
+// Joins the partial carriers of a unit, (m, l, a) + (m', l', a') with both scaled to the larger m, over the
+// shares c .. last, none of them empty.  Block (c, y) takes rows [RB y, RB y + RB) of the unit that starts in share c.
+// A warp holds one row at a time, a lane four columns; with few rows several warps share a row's shares (every
 // `stride`-th one) and meet in shared memory, always in the same order.
 constexpr int kJoinWarps = 16;
 
+struct Carrier {
+  float m, l;
+  float4 a;
+  __device__ __forceinline__ void add(float m1, float l1, const float4& v) {
+    const float m_new = fmaxf(m, m1), ref = m_new == -INFINITY ? 0.f : m_new;
+    const float f0 = ex2_approx(m - ref), f1 = ex2_approx(m1 - ref);
+    m = m_new;
+    l = l * f0 + l1 * f1;
+    a = make_float4(a.x * f0 + v.x * f1, a.y * f0 + v.y * f1, a.z * f0 + v.z * f1, a.w * f0 + v.w * f1);
+  }
+};
+
 template <class T>
 __global__ void __launch_bounds__(kJoinWarps * 32)
-paged_combine_kernel(int rt, const PagedScratch scratch, T* __restrict__ o, float* __restrict__ lse2, const PagedBatch batch, int G,
-                     int Hkv, int d) {
+paged_combine_kernel(const PagedScratch scratch, T* __restrict__ o, float* __restrict__ lse2, const PagedBatch batch, int G, int Hkv,
+                     int d) {
+  static_assert(kRT == kJoinWarps, "a warp a row");
   __shared__ float sh_m[kJoinWarps], sh_l[kJoinWarps];
   __shared__ __align__(16) float sh_a[kJoinWarps][128];
   const int c = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const PagedJoin j = scratch.joins[c];
   if (j.r < 0) return;
   const PagedReq q = paged_request(batch, j.r);
-  const int row_first = j.tile * rt + blockIdx.y * kJoinWarps;
-  const int n_rows = min(kJoinWarps, q.n * G - row_first);
-  if (n_rows <= 0) return;
+  const int row_first = j.tile * kRT, n_rows = min(kRT, q.n * G - row_first);
   int stride = 1;                                        // warps a row
   while (stride * 2 * n_rows <= kJoinWarps) stride *= 2;
-  const int rr = warp / stride, part = warp % stride;
-  const bool live = rr < n_rows;
-  const size_t slot = paged_slot_floats(rt, d);
-  const float* base = scratch.parts + (live ? blockIdx.y * kJoinWarps + rr : 0);
-  auto slot_of = [&](int s) { return base + slot * (2 * s + (s == c)); };
-  float m = -INFINITY, l = 0.f;
-  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (live) {
-    for (int s = c + part + lane * stride; s <= j.last; s += 32 * stride) m = fmaxf(m, *slot_of(s));
-#pragma unroll
-    for (int off = 16; off; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
-    const float ref = m == -INFINITY ? 0.f : m;
-    const int row = blockIdx.y * kJoinWarps + rr;
+  const int rr = warp / stride, part = warp % stride, col = 4 * lane;
+  const size_t slot = paged_slot_floats(kRT, d);
+  Carrier x{-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+  if (rr < n_rows) {
+    const float* base = scratch.parts + rr;
 #pragma unroll 4
     for (int s = c + part; s <= j.last; s += stride) {
-      const float* p = slot_of(s);
-      const float f = ex2_approx(p[0] - ref);
-      l += p[rt] * f;
-      if (4 * lane < d) {
-        const float4 v = *reinterpret_cast<const float4*>(p - row + 2 * rt + row * d + 4 * lane);
-        a.x += v.x * f;
-        a.y += v.y * f;
-        a.z += v.z * f;
-        a.w += v.w * f;
-      }
+      const float* p = base + slot * (2 * s + (s == c));
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (col < d) v = *reinterpret_cast<const float4*>(p - rr + 2 * kRT + rr * d + col);
+      x.add(p[0], p[kRT], v);
     }
   }
   if (stride > 1) {
-    *reinterpret_cast<float4*>(&sh_a[warp][4 * lane]) = a;
+    *reinterpret_cast<float4*>(&sh_a[warp][col]) = x.a;
     if (lane == 0) {
-      sh_m[warp] = m;
-      sh_l[warp] = l;
+      sh_m[warp] = x.m;
+      sh_l[warp] = x.l;
     }
     __syncthreads();
-    if (part != 0 || !live) return;
-    for (int w = warp + 1; w < warp + stride; ++w) {
-      const float m_new = fmaxf(m, sh_m[w]);
-      const float ref = m_new == -INFINITY ? 0.f : m_new;
-      const float f0 = ex2_approx(m - ref), f1 = ex2_approx(sh_m[w] - ref);
-      const float4 v = *reinterpret_cast<const float4*>(&sh_a[w][4 * lane]);
-      m = m_new;
-      l = l * f0 + sh_l[w] * f1;
-      a = make_float4(a.x * f0 + v.x * f1, a.y * f0 + v.y * f1, a.z * f0 + v.z * f1, a.w * f0 + v.w * f1);
+    if (part != 0) return;
+    for (int w = warp + 1; w < warp + stride; ++w) x.add(sh_m[w], sh_l[w], *reinterpret_cast<const float4*>(&sh_a[w][col]));
+  }
+  if (rr >= n_rows) return;
+  const int row = row_first + rr;
+  const float inv = x.l > 0.f ? 1.f / x.l : 0.f;
+  const long long at = (long long)(q.t0 + row / G) * (G * Hkv) + j.h * G + row % G;
+  if (col < d) store4(o + at * d + col, make_float4(x.a.x * inv, x.a.y * inv, x.a.z * inv, x.a.w * inv));
+  if (lse2 && lane == 0) lse2[at] = x.l > 0.f ? x.m + log2f(x.l) : INFINITY;
+}
+
+// The same for tiles of 128 rows, a stored [d / 4][128][4]: block (c, y) takes 32 of the rows, a lane one row, a warp
+// every eighth group of four columns; the result is turned in shared memory into whole rows.
+constexpr int kTileRows = 128, kTileWarps = 8;
+
+__global__ void __launch_bounds__(kTileWarps * 32)
+paged_combine_tiles_kernel(const PagedScratch scratch, __nv_bfloat16* __restrict__ o, float* __restrict__ lse2, const PagedBatch batch,
+                           int G, int Hkv, int d) {
+  __shared__ __align__(16) __nv_bfloat16 sh[32][128 + 8];
+  __shared__ long long sh_at[32];
+  const int c = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const PagedJoin j = scratch.joins[c];
+  if (j.r < 0) return;
+  const PagedReq q = paged_request(batch, j.r);
+  const int in_tile = blockIdx.y * 32 + lane, row = j.tile * kTileRows + in_tile;
+  const int n_rows = min(32, q.n * G - j.tile * kTileRows - int(blockIdx.y) * 32);
+  if (n_rows <= 0) return;
+  const size_t slot = paged_slot_floats(kTileRows, d);
+  constexpr int kGroups = 128 / 4 / kTileWarps;
+  Carrier x[kGroups];
+#pragma unroll
+  for (int k = 0; k < kGroups; ++k) x[k] = Carrier{-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+  if (lane < n_rows) {
+    for (int s = c; s <= j.last; ++s) {
+      const float* p = scratch.parts + slot * (2 * s + (s == c)) + in_tile;
+      float4 v[kGroups];
+#pragma unroll
+      for (int k = 0; k < kGroups; ++k) {
+        const int c4 = warp + k * kTileWarps;
+        v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (c4 * 4 < d) v[k] = *reinterpret_cast<const float4*>(p - in_tile + 2 * kTileRows + (c4 * kTileRows + in_tile) * 4);
+      }
+      const float m1 = p[0], l1 = p[kTileRows];
+#pragma unroll
+      for (int k = 0; k < kGroups; ++k) x[k].add(m1, l1, v[k]);
+    }
+    const float inv = x[0].l > 0.f ? 1.f / x[0].l : 0.f;
+#pragma unroll
+    for (int k = 0; k < kGroups; ++k)
+      store4(&sh[lane][(warp + k * kTileWarps) * 4], make_float4(x[k].a.x * inv, x[k].a.y * inv, x[k].a.z * inv, x[k].a.w * inv));
+    if (warp == 0) {
+      const long long at = (long long)(q.t0 + row / G) * (G * Hkv) + j.h * G + row % G;
+      sh_at[lane] = at;
+      if (lse2) lse2[at] = x[0].l > 0.f ? x[0].m + log2f(x[0].l) : INFINITY;
     }
   }
-  if (!live) return;
-  const int row = row_first + rr;
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  const long long at = (long long)(q.t0 + row / G) * (G * Hkv) + j.h * G + row % G;
-  if (4 * lane < d) store4(o + at * d + 4 * lane, make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv));
-  if (lse2 && lane == 0) lse2[at] = l > 0.f ? m + log2f(l) : INFINITY;
+  __syncthreads();
+  const int col = (threadIdx.x & 15) * 8;
+  for (int rr = threadIdx.x >> 4; rr < n_rows; rr += kTileWarps * 2)
+    if (col < d) *reinterpret_cast<uint4*>(o + sh_at[rr] * d + col) = *reinterpret_cast<const uint4*>(&sh[rr][col]);
 }
 
 // weight[key] += sum over rows of 2^(score - lse): a share of (request, kv head, key block) units per CTA,
@@ -382,9 +422,15 @@ Plan plan(int n_tokens, int R, int Hq, int Hkv, int d, int max_q, int max_k, boo
 }
 
 template <class T>
-int join(int rt, int n_cta, const PagedScratch& ws, T* o, float* lse2, const PagedBatch& batch, const PagedRows& rows, int d,
-         cudaStream_t st) {
-  paged_combine_kernel<T><<<dim3(n_cta, rt / kJoinWarps), kJoinWarps * 32, 0, st>>>(rt, ws, o, lse2, batch, rows.G, rows.Hkv, d);
+int join(int n_cta, const PagedScratch& ws, T* o, float* lse2, const PagedBatch& batch, const PagedRows& rows, int d, cudaStream_t st) {
+  paged_combine_kernel<T><<<n_cta, kJoinWarps * 32, 0, st>>>(ws, o, lse2, batch, rows.G, rows.Hkv, d);
+  CB2_LAUNCH_CHECK();
+  return CB2_OK;
+}
+
+int join_tiles(int n_cta, const PagedScratch& ws, __nv_bfloat16* o, float* lse2, const PagedBatch& batch, const PagedRows& rows, int d,
+               cudaStream_t st) {
+  paged_combine_tiles_kernel<<<dim3(n_cta, kTileRows / 32), kTileWarps * 32, 0, st>>>(ws, o, lse2, batch, rows.G, rows.Hkv, d);
   CB2_LAUNCH_CHECK();
   return CB2_OK;
 }
@@ -412,7 +458,7 @@ int run_f32(const PagedRows& rows, const PagedPools& pools, const PagedBatch& ba
     return CB2_LAUNCH_FAIL;
   paged_fma_kernel<float><<<kFmaCtas, kThreads, smem, st>>>(rows, pools, batch, cost, o, lse2, ws);
   CB2_LAUNCH_CHECK();
-  int rc = join(kRT, kFmaCtas, ws, o, lse2, batch, rows, d, st);
+  int rc = join(kFmaCtas, ws, o, lse2, batch, rows, d, st);
   if (rc == CB2_OK && weights) rc = fma_weights<float>(rows, pools, batch, cost, lse2, weights, st);
   return rc;
 }
@@ -423,16 +469,16 @@ int run_bf16(const PagedRows& rows, const PagedPools& pools, const PagedBatch& b
   float* scores = p.scores ? reinterpret_cast<float*>(scratch + p.lse) : nullptr;
   char* parts = scratch + p.lse + p.scores;
   PagedScratch ws;
-  int n_cta, rt, rc = CB2_OK;
+  int n_cta, rc = CB2_OK;
   if (p.chunks) {
-    rc = paged_tc_run(rows, pools, batch, causal, p.few, o, lse2, parts, &ws, &n_cta, &rt, st);
-    if (rc == CB2_OK) rc = join(rt, n_cta, ws, o, lse2, batch, rows, pools.d, st);
+    rc = paged_tc_run(rows, pools, batch, causal, p.few, o, lse2, parts, &ws, &n_cta, st);
+    if (rc == CB2_OK) rc = join_tiles(n_cta, ws, o, lse2, batch, rows, pools.d, st);
     if (rc == CB2_OK && weights)
       rc = fma_weights<__nv_bfloat16>(rows, pools, batch, {rows.G, rows.Hkv, causal, kPagedChunk, p.few, 1}, lse2, weights, st);
   }
   if (rc == CB2_OK && p.few) {
-    rc = paged_few_run(rows, pools, batch, causal, p.few, o, lse2, scores, parts, &ws, &n_cta, &rt, st);
-    if (rc == CB2_OK) rc = join(rt, n_cta, ws, o, lse2, batch, rows, pools.d, st);
+    rc = paged_few_run(rows, pools, batch, causal, p.few, o, lse2, scores, parts, &ws, &n_cta, st);
+    if (rc == CB2_OK) rc = join(n_cta, ws, o, lse2, batch, rows, pools.d, st);
     if (rc == CB2_OK && scores) rc = paged_few_weights_run(rows, batch, causal, p.few, scores, lse2, weights, st);
     if (rc == CB2_OK && weights && !scores)
       rc = fma_weights<__nv_bfloat16>(rows, pools, batch, {rows.G, rows.Hkv, causal, kPagedFew, p.few, 1}, lse2, weights, st);

@@ -100,6 +100,22 @@ __device__ inline long long lattice_sum(unsigned n, unsigned m, unsigned a, unsi
   return sum;
 }
 
+// The same for the steps that a tile count of a power of two gives, without Euclid's divisions.
+//   m = a k:  floor((a i + b) / m) = floor((i + c) / k), c = floor(b / a): a difference of two sums of floor(j / k);
+//   a = m k:  floor((a i + b) / m) = k i + floor(b / m).
+__device__ __forceinline__ long long stair_sum(unsigned n, unsigned m, unsigned a, unsigned b) {
+  if (m >= a && m % a == 0) {
+    const unsigned k = m / a, c = b / a;
+    auto upto = [k](unsigned x) {
+      const unsigned q = x / k, r = x - q * k;
+      return (long long)k * ((long long)q * (q - 1) / 2) + (long long)q * r;     // q = 0 gives 0
+    };
+    return upto(n + c) - upto(c);
+  }
+  if (a % m == 0) return (long long)(a / m) * ((long long)n * (n - 1) / 2) + (long long)n * (b / m);
+  return lattice_sum(n, m, a, b);
+}
+
 // The requests that a kernel takes: all of them, those with at most `few` packed rows, or the others.
 enum { kPagedAll = 0, kPagedFew = 1, kPagedChunk = 2 };
 
@@ -124,7 +140,7 @@ struct PagedCost {
     const int base = q.len - q.n, nt = tiles(q);
     if (!causal || base < 0) return (long long)k * all_blocks(q);
     const int m = min(k, nt - 1);
-    long long s = lattice_sum(m, unsigned(G) * KB, RT, RT - 1 + unsigned(G) * (base + KB));
+    long long s = stair_sum(m, unsigned(G) * KB, RT, RT - 1 + unsigned(G) * (base + KB));
     if (k == nt) s += all_blocks(q);
     return s;
   }
@@ -149,7 +165,10 @@ struct PagedShare {
   long long off;    // lo - start of that request
 };
 
-__device__ __forceinline__ long long paged_cut(long long total, int c, int n) { return total * c / n; }
+__device__ __forceinline__ long long paged_cut(long long total, int c, int n) {
+  if (total < (1 << 20) && n <= 4096) return unsigned(total) * unsigned(c) / unsigned(n);     // without a 64-bit division
+  return total * c / n;
+}
 
 template <int T, class Cost>
 __device__ PagedShare paged_find_share(const PagedBatch& b, const Cost& cost, int cta, int n_cta, PagedFindSmem* s) {
@@ -181,7 +200,7 @@ __device__ PagedShare paged_find_share(const PagedBatch& b, const Cost& cost, in
     total += block_total;
   }
   out.total = total;
-  out.n_share = int(max(1ll, min((long long)n_cta, total / cost.min_blocks)));
+  out.n_share = total >= (long long)n_cta * cost.min_blocks ? n_cta : max(1, int(unsigned(total) / unsigned(cost.min_blocks)));
   out.lo = out.hi = total;
   if (cta < out.n_share) {
     out.lo = paged_cut(total, cta, out.n_share);
@@ -273,7 +292,8 @@ struct PagedJoin {
   int r, h, tile, last;     // r < 0: none; last = share that holds the unit's last block
 };
 // Partial carriers: share c owns slot 2c (a piece that does not start its unit) and 2c + 1 (a piece
-// that starts a unit and does not finish it).  Slot: m[RT], l[RT], a[RT][d], fp32, m in log2 units.
+// that starts a unit and does not finish it).  Slot: m[RT], l[RT], a, fp32, m in log2 units; a is [RT][d], or
+// [d / 4][RT][4] for tiles of 128 rows, whose writers hold a row a thread.
 __host__ __device__ __forceinline__ size_t paged_slot_floats(int rt, int d) { return size_t(rt) * (d + 2); }
 
 __device__ __forceinline__ float ex2_approx(float x) {
@@ -288,7 +308,8 @@ __device__ __forceinline__ void paged_write_join(const PagedWalkState& w, long l
   j.r = w.r;
   j.h = w.h;
   j.tile = w.tile;
-  j.last = int(((w.cur + w.nb) * n_share - 1) / total);
+  const long long x = (w.cur + w.nb) * n_share - 1;
+  j.last = x < (1ll << 32) ? int(unsigned(x) / unsigned(total)) : int(x / total);
   joins[cta] = j;
 }
 
@@ -308,16 +329,16 @@ inline PagedScratch paged_scratch(void* base, int n_cta) {
 }
 
 // om_paged_tc.cu: requests of more than `few` packed rows (bf16), on the tensor cores.  What it leaves for
-// the join: row tiles of *rt rows, *n_cta shares.
+// the join: tiles of 128 rows, *n_cta shares.
 size_t paged_tc_scratch_bytes(int d);
 int paged_tc_run(const PagedRows& rows, const PagedPools& pools, const PagedBatch& batch, int causal, int few, void* o,
-                 float* lse2, void* scratch, PagedScratch* parts, int* n_cta, int* rt, cudaStream_t st);
+                 float* lse2, void* scratch, PagedScratch* parts, int* n_cta, cudaStream_t st);
 
 // om_paged_few.cu: requests of at most `few` (8 or 16) packed rows (bf16), one pass over K and V.  scores (may be
 // NULL): [R, Hkv, few, max_k] floats for paged_few_weights_run.
 size_t paged_few_scratch_bytes(int d);
 int paged_few_run(const PagedRows& rows, const PagedPools& pools, const PagedBatch& batch, int causal, int few, void* o,
-                  float* lse2, float* scores, void* scratch, PagedScratch* parts, int* n_cta, int* rt, cudaStream_t st);
+                  float* lse2, float* scores, void* scratch, PagedScratch* parts, int* n_cta, cudaStream_t st);
 int paged_few_weights_run(const PagedRows& rows, const PagedBatch& batch, int causal, int few, const float* scores,
                           const float* lse2, float* weights, cudaStream_t st);
 

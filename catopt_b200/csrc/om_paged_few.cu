@@ -351,10 +351,9 @@ int launch(const PagedRows& rows, const PagedPools& pools, const PagedBatch& bat
 size_t paged_few_scratch_bytes(int d) { return paged_scratch_bytes(kCtas, kRT, d); }
 
 int paged_few_run(const PagedRows& rows, const PagedPools& pools, const PagedBatch& batch, int causal, int few, void* o, float* lse2,
-                  float* scores, void* scratch, PagedScratch* parts, int* n_cta, int* rt, cudaStream_t st) {
+                  float* scores, void* scratch, PagedScratch* parts, int* n_cta, cudaStream_t st) {
   *parts = paged_scratch(scratch, kCtas);
   *n_cta = kCtas;
-  *rt = kRT;
   // 256 keys a share at least: four tiles a warp, less than that is mostly start and join
   const Cost cost{rows.G, rows.Hkv, causal, kPagedFew, few, 4};
   __nv_bfloat16* out = static_cast<__nv_bfloat16*>(o);

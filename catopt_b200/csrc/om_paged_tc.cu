@@ -20,6 +20,8 @@
 #include "om_paged.cuh"
 #include "umma.cuh"
 
+#include <type_traits>
+
 namespace cb2 {
 namespace {
 
@@ -30,7 +32,9 @@ constexpr uint32_t kQTile = umma::kTileBytes;            // 128 x 128 bf16
 constexpr uint32_t kSub = 64 * 128;                      // 64 keys x 64 columns
 constexpr uint32_t kKvTile = 2 * kSub;
 constexpr uint32_t kOffQ = 0, kOffK = kQTile, kOffV = kOffK + 2 * kKvTile;
-constexpr uint32_t kOffBars = kOffV + 2 * kKvTile;
+constexpr uint32_t kOffStage = kOffV + 2 * kKvTile;      // a warp's 32 rows x 32 columns of output
+constexpr uint32_t kStagePitch = 80, kStageBytes = 32 * kStagePitch;
+constexpr uint32_t kOffBars = kOffStage + 4 * kStageBytes;
 constexpr int kNumBars = 15;
 constexpr uint32_t kColS = 0, kColO = 128, kTmemCols = 256;
 
@@ -120,6 +124,10 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   if (warp == 1) {
     __syncwarp();
     umma::tmem_alloc(&sh->tmem, kTmemCols);
+  }
+  if (tid == 32) {
+    umma::tma_prefetch_desc(&map_k);
+    umma::tma_prefetch_desc(&map_v);
   }
   {
     const PagedShare share = paged_find_share<kThreads>(batch, cost, cta, n_cta, &sh->find);
@@ -239,20 +247,29 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       constexpr float kLazy = 8.f;
       const int ncb = (d + 31) >> 5;
       const float scale = a.scale_log2e;
-      // The 32 packed rows of this warp, into the query tile: the row's place is worked out by one lane, its
-      // chunks are copied by 8 or 16 neighbouring ones.
+      // The 32 packed rows of this warp, into the query tile: a lane works out the place of one row, 8 or 16
+      // neighbouring lanes copy its chunks (a copy instruction then touches two or four rows, not 32).
       auto load_rows = [&](const Piece* pc) {
         const int row = pc->row0 + rr;
         const bool there = row < pc->n * a.G;
         const int tok = there ? row / a.G : 0, g = there ? row - tok * a.G : 0;
         const long long at = (pc->t0 + tok) * a.q_token + (pc->h * a.G + g) * a.q_head;
-        const int chunks = halves * 8, per_copy = 32 / chunks, col = (lane % chunks) * 8;
-        for (int i = 0; i < 32; i += per_copy) {
-          const int from = i + lane / chunks;
-          const long long off = __shfl_sync(0xffffffffu, at, from);
-          const bool ok = __shfl_sync(0xffffffffu, there, from) && col < d;
-          cp_async16_or_zero(q_addr + umma::tile_chunk_offset(q4 * 32 + from, col), a.q + off + (ok ? col : 0), ok);
-        }
+        const unsigned have = __ballot_sync(0xffffffffu, there);
+        auto copy = [&](auto chunks) {
+          constexpr int kChunks = decltype(chunks)::value, kRows = 32 / kChunks;
+          const int c = lane % kChunks;
+#pragma unroll
+          for (int i = 0; i < 32; i += kRows) {
+            const int from = i + lane / kChunks;
+            const long long off = __shfl_sync(0xffffffffu, at, from);
+            const bool ok = ((have >> from) & 1) && c * 8 < d;
+            cp_async16_or_zero(q_addr + umma::tile_chunk_offset(q4 * 32 + from, c * 8), a.q + off + (ok ? c * 8 : 0), ok);
+          }
+        };
+        if (halves == 2)
+          copy(std::integral_constant<int, 16>{});
+        else
+          copy(std::integral_constant<int, 8>{});
         cp_async_commit();
       };
       auto rows_there = [&] {
@@ -364,29 +381,39 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         const int row = pc->row0 + rr;
         const long long at = (long long)(pc->t0 + row / a.G) * (a.G * a.Hkv) + pc->h * a.G + row % a.G;
         float* slot = scratch.parts + paged_slot_floats(kRT, d) * (2 * cta + (b0 == 0));
+        unsigned char* stage = smem + kOffStage + q4 * kStageBytes;
         for (int cb = 0; cb < ncb; ++cb) {
           uint32_t sv[32];
-          __syncwarp();
           umma::tmem_ld32(lane_base + kColO + cb * 32, sv);
           umma::tmem_wait_ld();
-          if (!live) continue;
           if (whole) {
-            __nv_bfloat16* dst = a.o + at * d + cb * 32;
+            // 32 columns of 32 rows, turned in shared memory so that a store covers 64 bytes of 8 rows
 #pragma unroll
-            for (int c = 0; c < 32; c += 8) {
-              if (cb * 32 + c >= d) continue;
+            for (int c = 0; c < 4; ++c) {
               uint32_t w[4];
 #pragma unroll
               for (int i = 0; i < 4; ++i)
-                w[i] = pack_bf16x2(__uint_as_float(sv[c + 2 * i]) * inv, __uint_as_float(sv[c + 2 * i + 1]) * inv);
-              *reinterpret_cast<uint4*>(dst + c) = make_uint4(w[0], w[1], w[2], w[3]);
+                w[i] = pack_bf16x2(__uint_as_float(sv[c * 8 + 2 * i]) * inv, __uint_as_float(sv[c * 8 + 2 * i + 1]) * inv);
+              *reinterpret_cast<uint4*>(stage + lane * kStagePitch + c * 16) = make_uint4(w[0], w[1], w[2], w[3]);
             }
-          } else {
-            float* dst = slot + 2 * kRT + rr * d + cb * 32;
+            __syncwarp();
+            const int col = cb * 32 + (lane & 3) * 8;
 #pragma unroll
-            for (int c = 0; c < 32; c += 4)
-              if (cb * 32 + c < d) *reinterpret_cast<uint4*>(dst + c) = make_uint4(sv[c], sv[c + 1], sv[c + 2], sv[c + 3]);
+            for (int i = 0; i < 4; ++i) {
+              const int r8 = i * 8 + (lane >> 2);
+              const uint4 v = *reinterpret_cast<const uint4*>(stage + r8 * kStagePitch + (lane & 3) * 16);
+              const long long to = __shfl_sync(0xffffffffu, at, r8);
+              if (q4 * 32 + r8 < rows && col < d) *reinterpret_cast<uint4*>(a.o + to * d + col) = v;
+            }
+            __syncwarp();
+          } else if (live) {
+            float* dst = slot + 2 * kRT + (cb * 8 * kRT + rr) * 4;
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+              if (cb * 32 + c * 4 < d)
+                *reinterpret_cast<uint4*>(dst + c * kRT * 4) = make_uint4(sv[4 * c], sv[4 * c + 1], sv[4 * c + 2], sv[4 * c + 3]);
           }
+          __syncwarp();
         }
         if (live && whole && a.lse2) a.lse2[at] = l_run > 0.f ? m_ref + log2f(l_run) : INFINITY;
         if (live && !whole) {
@@ -448,7 +475,7 @@ size_t paged_tc_scratch_bytes(int d) { return paged_scratch_bytes(kCtas, kRT, d)
 
 // Requests of more than `few` packed rows; partial carriers are left in `scratch` (kRT rows a slot, kCtas shares).
 int paged_tc_run(const PagedRows& rows, const PagedPools& pools, const PagedBatch& batch, int causal, int few, void* o, float* lse2,
-                 void* scratch, PagedScratch* parts, int* n_cta, int* rt, cudaStream_t st) {
+                 void* scratch, PagedScratch* parts, int* n_cta, cudaStream_t st) {
   CUtensorMap mk, mv;
   int rc = make_pool_map(&mk, pools.k, pools.d, 1 << batch.page_log2, pools.Hkv, batch.n_pages, pools.k_page_stride);
   if (rc == CB2_OK) rc = make_pool_map(&mv, pools.v, pools.d, 1 << batch.page_log2, pools.Hkv, batch.n_pages, pools.v_page_stride);
@@ -457,7 +484,6 @@ int paged_tc_run(const PagedRows& rows, const PagedPools& pools, const PagedBatc
     return CB2_LAUNCH_FAIL;
   *parts = paged_scratch(scratch, kCtas);
   *n_cta = kCtas;
-  *rt = kRT;
   const TcArgs a{static_cast<const __nv_bfloat16*>(rows.q), rows.q_token, rows.q_head, static_cast<__nv_bfloat16*>(o), lse2,
                  rows.scale_log2e, rows.G, rows.Hkv, pools.d};
   const PagedCost<kRT, kKB> cost{rows.G, rows.Hkv, causal, kPagedChunk, few, 4};
