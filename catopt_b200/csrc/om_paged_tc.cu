@@ -42,11 +42,30 @@ constexpr uint32_t kColS = 0, kColO = 128, kTmemCols = 256;
 __device__ __forceinline__ uint32_t kv_chunk_offset(uint32_t row, uint32_t col) {
   return (col >> 6) * kSub + row * 128u + ((((col & 63u) >> 3) ^ (row & 7u)) << 4);
 }
-__device__ __forceinline__ uint64_t desc_k(uint32_t tile, int ks) {      // K-major, 16 columns a step
-  return umma::smem_desc(tile + (ks >> 2) * kSub + (ks & 3) * 32u, 16u, 1024u);
+// Shared-memory descriptors: the high word is the same for every step, the low word moves by the step's offset.
+__device__ __forceinline__ uint64_t desc_step(uint64_t base, uint32_t bytes) {
+  return (base & 0xffffffff00000000ull) | (uint32_t(base) + (bytes >> 4));
 }
-__device__ __forceinline__ uint64_t desc_v(uint32_t tile, int ks) {      // MN-major, 16 keys a step
-  return umma::smem_desc(tile + ks * 2048u, kSub, 1024u);
+__device__ __forceinline__ constexpr uint32_t q_step(int ks) { return (ks >> 2) * umma::kSubTileBytes + (ks & 3) * 32u; }   // 16 columns
+__device__ __forceinline__ constexpr uint32_t k_step(int ks) { return (ks >> 2) * kSub + (ks & 3) * 32u; }
+__device__ __forceinline__ constexpr uint32_t v_step(int ks) { return ks * 2048u; }                                         // 16 keys
+
+// Registers that a TMEM load has filled, after the wait for it: arithmetic on them cannot be moved ahead of this.
+__device__ __forceinline__ void loaded(uint32_t (&r)[32]) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 8)
+    asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]),
+                 "+r"(r[i + 7]));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 
 // arguments of a wait: where to see that another role gave up, the budget, and the line to report
@@ -207,17 +226,20 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         const int ksteps = (d + 15) >> 4;
         constexpr uint32_t idesc_kk = umma::instr_desc_bf16(128, kKB, false, false);
         const uint32_t idesc_kn = umma::instr_desc_bf16(128, uint32_t(d + 15) & ~15u, false, true);
+        const uint64_t q_desc = umma::smem_desc(q_addr, 16u, 1024u);
+        const uint64_t k_desc[2] = {umma::smem_desc(k_addr, 16u, 1024u), umma::smem_desc(k_addr + kKvTile, 16u, 1024u)};
+        const uint64_t v_desc[2] = {umma::smem_desc(v_addr, kSub, 1024u), umma::smem_desc(v_addr + kKvTile, kSub, 1024u)};
         for (int p = 0; p < count; ++p, ++n_piece) {
           const int blocks = sh->pieces[p].b1 - sh->pieces[p].b0;
           auto issue_scores = [&](int j) -> bool {
             const uint32_t n = n_blk + j, slot = n & 1;
             if (!mbar_wait_abortable(&k_full[slot], (n >> 1) & 1, CB2_SITE)) return false;
             umma::fence_after_sync();
+            const uint64_t kd = slot ? k_desc[1] : k_desc[0];
 #pragma unroll
             for (int ks = 0; ks < 8; ++ks)
               if (ks < ksteps)
-                umma::mma_bf16(tmem + kColS + slot * kKB, umma::desc_kmajor(q_addr, ks), desc_k(k_addr + slot * kKvTile, ks), idesc_kk,
-                               ks > 0);
+                umma::mma_bf16(tmem + kColS + slot * kKB, desc_step(q_desc, q_step(ks)), desc_step(kd, k_step(ks)), idesc_kk, ks > 0);
             umma::mma_commit(&s_ready[slot]);
             umma::mma_commit(&k_empty[slot]);
             return true;
@@ -228,10 +250,10 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
             ok = mbar_wait_abortable(&p_ready[slot], (n >> 1) & 1, CB2_SITE) && mbar_wait_abortable(&v_full[slot], (n >> 1) & 1, CB2_SITE);
             if (!ok) break;
             umma::fence_after_sync();
+            const uint64_t vd = slot ? v_desc[1] : v_desc[0];
 #pragma unroll
             for (int ks = 0; ks < kKB / 16; ++ks)
-              umma::mma_bf16_ts(tmem + kColO, tmem + kColS + slot * kKB + ks * 8, desc_v(v_addr + slot * kKvTile, ks), idesc_kn,
-                                j > 0 || ks > 0);
+              umma::mma_bf16_ts(tmem + kColO, tmem + kColS + slot * kKB + ks * 8, desc_step(vd, v_step(ks)), idesc_kn, j > 0 || ks > 0);
             umma::mma_commit(&o_done[slot]);
             umma::mma_commit(&v_empty[slot]);
             // the tensor pipe runs in issue order, so the scores after next may overwrite P right away
@@ -305,6 +327,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
 #pragma unroll
           for (int cb = 0; cb < 2; ++cb) umma::tmem_ld32(s_cols + cb * 32, sv[cb]);
           umma::tmem_wait_ld();
+          loaded(sv[0]);
+          loaded(sv[1]);
           if (k0 + kKB - 1 > first_last) {
             const int lim = last - k0;
 #pragma unroll
@@ -313,12 +337,12 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
               for (int c = 0; c < 32; ++c)
                 if (cb * 32 + c > lim) sv[cb][c] = 0xff800000u;
           }
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          float mx[4];
 #pragma unroll
-          for (int cb = 0; cb < 2; ++cb)
+          for (int i = 0; i < 4; ++i) mx[i] = fmaxf(__uint_as_float(sv[0][i]), __uint_as_float(sv[1][i]));
 #pragma unroll
-            for (int c = 0; c < 32; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(sv[cb][c]));
-          const float m_blk = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
+          for (int c = 4; c < 32; ++c) mx[c & 3] = max3(mx[c & 3], __uint_as_float(sv[0][c]), __uint_as_float(sv[1][c]));
+          const float m_blk = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * scale;
           float alpha = 1.f;
           if (m_blk > m_ref + kLazy || m_ref == -INFINITY) {
             const float m_new = fmaxf(m_ref, m_blk);
@@ -326,20 +350,25 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
             m_ref = m_new;
           }
           const float neg_m = (m_ref == -INFINITY) ? 0.f : -m_ref;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          const uint64_t scale2 = umma::f2_pack(scale, scale), neg2 = umma::f2_pack(neg_m, neg_m);
+          uint64_t sum2[2] = {0ull, 0ull};
 #pragma unroll
           for (int cb = 0; cb < 2; ++cb) {
             uint32_t w[16];
 #pragma unroll
             for (int c = 0; c < 32; c += 2) {
-              const float p0 = ex2_approx(fmaf(__uint_as_float(sv[cb][c]), scale, neg_m));
-              const float p1 = ex2_approx(fmaf(__uint_as_float(sv[cb][c + 1]), scale, neg_m));
-              sum[(c >> 1) & 3] += p0 + p1;
+              const uint64_t x = umma::f2_fma(umma::f2_pack(__uint_as_float(sv[cb][c]), __uint_as_float(sv[cb][c + 1])), scale2, neg2);
+              float x0, x1;
+              umma::f2_unpack(x, x0, x1);
+              const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+              sum2[(c >> 1) & 1] = f2_add(sum2[(c >> 1) & 1], umma::f2_pack(p0, p1));
               w[c >> 1] = pack_bf16x2(p0, p1);
             }
             umma::tmem_st16(s_cols + cb * 16, w);
           }
-          l_run = fmaf(l_run, alpha, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+          float s0, s1;
+          umma::f2_unpack(f2_add(sum2[0], sum2[1]), s0, s1);
+          l_run = fmaf(l_run, alpha, s0 + s1);
           umma::tmem_wait_st();
           if (k0 + kKB > len) {
             // the request's last block: value rows that nobody has written
@@ -361,6 +390,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
             for (int cb = 0; cb < ncb; ++cb) {
               umma::tmem_ld32(lane_base + kColO + cb * 32, sv[0]);
               umma::tmem_wait_ld();
+              loaded(sv[0]);
 #pragma unroll
               for (int c = 0; c < 32; ++c) sv[0][c] = __float_as_uint(__uint_as_float(sv[0][c]) * alpha);
               umma::tmem_st32(lane_base + kColO + cb * 32, sv[0]);
@@ -386,6 +416,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
           uint32_t sv[32];
           umma::tmem_ld32(lane_base + kColO + cb * 32, sv);
           umma::tmem_wait_ld();
+          loaded(sv);
           if (whole) {
             // 32 columns of 32 rows, turned in shared memory so that a store covers 64 bytes of 8 rows
 #pragma unroll
