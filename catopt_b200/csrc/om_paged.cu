@@ -10,6 +10,7 @@ namespace cb2 {
 namespace {
 
 constexpr int kRT = 16, kKB = 64, kThreads = 128;
+using Cost = PagedCost<kRT, kKB, 1>;
 
 template <class T>
 __device__ __forceinline__ float4 load4(const T* p);
@@ -88,7 +89,7 @@ __device__ __forceinline__ int last_slot(const PagedReq& q, int row, int G, int 
 
 template <class T>
 __global__ void __launch_bounds__(kThreads)
-paged_fma_kernel(const PagedRows rows, const PagedPools pools, const PagedBatch batch, const PagedCost<kRT, kKB> cost, T* __restrict__ o,
+paged_fma_kernel(const PagedRows rows, const PagedPools pools, const PagedBatch batch, const Cost cost, T* __restrict__ o,
                  float* __restrict__ lse2, PagedScratch scratch) {
   extern __shared__ __align__(16) float sm[];
   __shared__ PagedFindSmem find;
@@ -103,7 +104,7 @@ paged_fma_kernel(const PagedRows rows, const PagedPools pools, const PagedBatch 
   const PagedShare share = paged_find_share<kThreads>(batch, cost, cta, n_cta, &find);
   if (tid == 0) scratch.joins[cta].r = -1;
   const int ty = tid / 16, tx = tid % 16, lane = tid % 32, wq = tid / 32;
-  for (PagedWalk<PagedCost<kRT, kKB>> w(batch, cost, share); w.valid(); w.next()) {
+  for (PagedWalk<Cost> w(batch, cost, share); w.valid(); w.next()) {
     w.clip();
     const int row0 = w.tile * kRT;
     __syncthreads();
@@ -330,7 +331,7 @@ paged_combine_tiles_kernel(const PagedScratch scratch, __nv_bfloat16* __restrict
 // every key of a block summed by one CTA over all rows in order.
 template <class T>
 __global__ void __launch_bounds__(kThreads)
-paged_weights_fma_kernel(PagedRows rows, PagedPools pools, PagedBatch batch, PagedCost<kRT, kKB> cost,
+paged_weights_fma_kernel(PagedRows rows, PagedPools pools, PagedBatch batch, Cost cost,
                          const float* __restrict__ lse2, float* __restrict__ weights) {
   extern __shared__ __align__(16) float sm[];
   const int d = pools.d, ld = d + 4, tid = threadIdx.x;
@@ -416,6 +417,7 @@ Plan plan(int n_tokens, int R, int Hq, int Hkv, int d, int max_q, int max_k, boo
       p.scores = s <= kMostScores ? up16(s) : 0;
     }
   }
+  if (weights && dtype == CB2_BF16 && paged_weights_tc_scratch_bytes() > p.parts) p.parts = paged_weights_tc_scratch_bytes();
   p.parts = up16(p.parts);
   p.total = p.lse + p.scores + p.parts;
   return p;
@@ -436,7 +438,7 @@ int join_tiles(int n_cta, const PagedScratch& ws, __nv_bfloat16* o, float* lse2,
 }
 
 template <class T>
-int fma_weights(const PagedRows& rows, const PagedPools& pools, const PagedBatch& batch, const PagedCost<kRT, kKB>& cost,
+int fma_weights(const PagedRows& rows, const PagedPools& pools, const PagedBatch& batch, const Cost& cost,
                 const float* lse2, float* weights, cudaStream_t st) {
   const int ld = pools.d + 4, smem = (kRT * ld + kKB * ld + 8 * kKB) * 4;
   if (cudaFuncSetAttribute(paged_weights_fma_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
@@ -449,7 +451,7 @@ int fma_weights(const PagedRows& rows, const PagedPools& pools, const PagedBatch
 
 int run_f32(const PagedRows& rows, const PagedPools& pools, const PagedBatch& batch, int causal, float* o, float* weights,
             char* scratch, const Plan& p, cudaStream_t st) {
-  const PagedCost<kRT, kKB> cost{rows.G, rows.Hkv, causal, kPagedAll, 0, 2};
+  const Cost cost{rows.G, rows.Hkv, causal, kPagedAll, 0, 2};
   float* lse2 = weights ? reinterpret_cast<float*>(scratch) : nullptr;
   const PagedScratch ws = paged_scratch(scratch + p.lse, kFmaCtas);
   const int d = pools.d, ld = d + 4;
@@ -473,15 +475,14 @@ int run_bf16(const PagedRows& rows, const PagedPools& pools, const PagedBatch& b
   if (p.chunks) {
     rc = paged_tc_run(rows, pools, batch, causal, p.few, o, lse2, parts, &ws, &n_cta, st);
     if (rc == CB2_OK) rc = join_tiles(n_cta, ws, o, lse2, batch, rows, pools.d, st);
-    if (rc == CB2_OK && weights)
-      rc = fma_weights<__nv_bfloat16>(rows, pools, batch, {rows.G, rows.Hkv, causal, kPagedChunk, p.few, 1}, lse2, weights, st);
+    if (rc == CB2_OK && weights) rc = paged_weights_tc_run(rows, pools, batch, causal, kPagedChunk, p.few, lse2, weights, parts, st);
   }
   if (rc == CB2_OK && p.few) {
     rc = paged_few_run(rows, pools, batch, causal, p.few, o, lse2, scores, parts, &ws, &n_cta, st);
     if (rc == CB2_OK) rc = join(n_cta, ws, o, lse2, batch, rows, pools.d, st);
     if (rc == CB2_OK && scores) rc = paged_few_weights_run(rows, batch, causal, p.few, scores, lse2, weights, st);
     if (rc == CB2_OK && weights && !scores)
-      rc = fma_weights<__nv_bfloat16>(rows, pools, batch, {rows.G, rows.Hkv, causal, kPagedFew, p.few, 1}, lse2, weights, st);
+      rc = paged_weights_tc_run(rows, pools, batch, causal, kPagedFew, p.few, lse2, weights, parts, st);
   }
   return rc;
 }

@@ -119,8 +119,10 @@ __device__ __forceinline__ long long stair_sum(unsigned n, unsigned m, unsigned 
 // The requests that a kernel takes: all of them, those with at most `few` packed rows, or the others.
 enum { kPagedAll = 0, kPagedFew = 1, kPagedChunk = 2 };
 
-template <int RT, int KB>
+// OV: what starting and ending a unit costs, in blocks; a unit takes OV + blocks of the line.
+template <int RT, int KB, int OV>
 struct PagedCost {
+  static constexpr int kOv = OV;
   int G, Hkv, causal, which, few;
   int min_blocks;          // a share holds at least so many: fewer CTAs work on a short line
   __device__ __forceinline__ bool takes(const PagedReq& q) const {
@@ -135,14 +137,14 @@ struct PagedCost {
     if (!causal || base < 0 || i == tiles(q) - 1) return all_blocks(q);
     return int((unsigned(i) * RT + RT - 1 + unsigned(G) * (base + KB)) / (unsigned(G) * KB));
   }
-  // blocks of the first `k` tiles of one kv head
+  // length of the first `k` tiles of one kv head
   __device__ __forceinline__ long long before(const PagedReq& q, int k) const {
     const int base = q.len - q.n, nt = tiles(q);
-    if (!causal || base < 0) return (long long)k * all_blocks(q);
+    if (!causal || base < 0) return (long long)k * (all_blocks(q) + OV);
     const int m = min(k, nt - 1);
     long long s = stair_sum(m, unsigned(G) * KB, RT, RT - 1 + unsigned(G) * (base + KB));
     if (k == nt) s += all_blocks(q);
-    return s;
+    return s + (long long)k * OV;
   }
   __device__ __forceinline__ long long of_request(const PagedReq& q) const {
     if (!takes(q)) return 0;
@@ -265,13 +267,21 @@ struct PagedWalk : PagedWalkState {
     }
     tile = lo;
     nb = cost.blocks(q, tile);
-    b0 = int(rest - cost.before(q, tile));
+    b0 = int(rest - cost.before(q, tile)) - Cost::kOv;
+    enter();
   }
   __device__ bool valid() const { return cur < hi; }
   __device__ void clip() { b1 = int(min((long long)nb, b0 + (hi - cur))); }
+  // past the unit's overhead, to its first block (a share may end before)
+  __device__ void enter() {
+    if (b0 < 0) {
+      cur -= b0;
+      b0 = 0;
+    }
+  }
   __device__ void next() {
     cur += b1 - b0;
-    b0 = 0;
+    b0 = -Cost::kOv;
     if (cur >= hi) return;
     if (++tile == cost.tiles(q)) {
       tile = 0;
@@ -284,6 +294,7 @@ struct PagedWalk : PagedWalkState {
       }
     }
     nb = cost.blocks(q, tile);
+    enter();
   }
 };
 
@@ -296,6 +307,10 @@ struct PagedJoin {
 // [d / 4][RT][4] for tiles of 128 rows, whose writers hold a row a thread.
 __host__ __device__ __forceinline__ size_t paged_slot_floats(int rt, int d) { return size_t(rt) * (d + 2); }
 
+// 16-byte asynchronous copy that writes zeros when `there` is false.
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
 __device__ __forceinline__ float ex2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -303,7 +318,7 @@ __device__ __forceinline__ float ex2_approx(float x) {
 }
 
 __device__ __forceinline__ void paged_write_join(const PagedWalkState& w, long long total, int cta, int n_share, PagedJoin* joins) {
-  // called for a piece with b0 == 0 and b1 < nb: the unit's last block sits at cur + nb - 1
+  // called for a piece with b0 == 0 and b1 < nb: the unit's last block sits at cur + nb - 1 of the line
   PagedJoin j;
   j.r = w.r;
   j.h = w.h;
@@ -341,5 +356,10 @@ int paged_few_run(const PagedRows& rows, const PagedPools& pools, const PagedBat
                   float* lse2, float* scores, void* scratch, PagedScratch* parts, int* n_cta, cudaStream_t st);
 int paged_few_weights_run(const PagedRows& rows, const PagedBatch& batch, int causal, int few, const float* scores,
                           const float* lse2, float* weights, cudaStream_t st);
+
+// om_paged_weights.cu: attention weight of the requests of class `which` (bf16), from their lse.
+size_t paged_weights_tc_scratch_bytes();
+int paged_weights_tc_run(const PagedRows& rows, const PagedPools& pools, const PagedBatch& batch, int causal, int which, int few,
+                         const float* lse2, float* weights, void* scratch, cudaStream_t st);
 
 }  // namespace cb2

@@ -19,11 +19,8 @@ constexpr int kRT = 16, kKB = 64, kTileKeys = 16;
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kCtas = 2 * kNumSMs;
 
-using Cost = PagedCost<kRT, kKB>;
+using Cost = PagedCost<kRT, kKB, 1>;
 
-__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool there) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
 template <int N>
 __device__ __forceinline__ void cp_async_wait_group() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");

@@ -20,13 +20,13 @@
 #include "om_paged.cuh"
 #include "umma.cuh"
 
-#include <type_traits>
-
 namespace cb2 {
 namespace {
 
 constexpr int kRT = 128, kKB = 64;
 constexpr int kThreads = 192;
+// Rows in, scores of the first blocks, results out: as long as four blocks.
+using Cost = PagedCost<kRT, kKB, 4>;
 constexpr int kBatch = 32;                // pieces listed at a time
 constexpr uint32_t kQTile = umma::kTileBytes;            // 128 x 128 bf16
 constexpr uint32_t kSub = 64 * 128;                      // 64 keys x 64 columns
@@ -42,32 +42,18 @@ constexpr uint32_t kColS = 0, kColO = 128, kTmemCols = 256;
 __device__ __forceinline__ uint32_t kv_chunk_offset(uint32_t row, uint32_t col) {
   return (col >> 6) * kSub + row * 128u + ((((col & 63u) >> 3) ^ (row & 7u)) << 4);
 }
-// Shared-memory descriptors: the high word is the same for every step, the low word moves by the step's offset.
-__device__ __forceinline__ uint64_t desc_step(uint64_t base, uint32_t bytes) {
-  return (base & 0xffffffff00000000ull) | (uint32_t(base) + (bytes >> 4));
+__device__ __forceinline__ uint64_t desc_k(uint32_t tile, int ks) {      // K-major, 16 columns a step
+  return umma::smem_desc(tile + (ks >> 2) * kSub + (ks & 3) * 32u, 16u, 1024u);
 }
-__device__ __forceinline__ constexpr uint32_t q_step(int ks) { return (ks >> 2) * umma::kSubTileBytes + (ks & 3) * 32u; }   // 16 columns
-__device__ __forceinline__ constexpr uint32_t k_step(int ks) { return (ks >> 2) * kSub + (ks & 3) * 32u; }
-__device__ __forceinline__ constexpr uint32_t v_step(int ks) { return ks * 2048u; }                                         // 16 keys
+__device__ __forceinline__ uint64_t desc_v(uint32_t tile, int ks) {      // MN-major, 16 keys a step
+  return umma::smem_desc(tile + ks * 2048u, kSub, 1024u);
+}
 
-// Registers that a TMEM load has filled, after the wait for it: arithmetic on them cannot be moved ahead of this.
-__device__ __forceinline__ void loaded(uint32_t (&r)[32]) {
-#pragma unroll
-  for (int i = 0; i < 32; i += 8)
-    asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]),
-                 "+r"(r[i + 7]));
-}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float y;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
 }
-__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-
 // arguments of a wait: where to see that another role gave up, the budget, and the line to report
 #define CB2_SITE s_abort, kDefaultWaitNs, __LINE__
 
@@ -100,21 +86,9 @@ struct TcArgs {
   int G, Hkv, d;
 };
 
-__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* m, int x, int y, int z, int w, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
-          smem_u32(dst)),
-      "l"(m), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
-      : "memory");
-}
-// 16-byte asynchronous copy that writes zeros when `there` is false.
-__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool there) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
-
 __global__ void __launch_bounds__(kThreads, 2)
 paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const TcArgs a,
-                const PagedBatch batch, const PagedCost<kRT, kKB> cost, const PagedScratch scratch) {
+                const PagedBatch batch, const Cost cost, const PagedScratch scratch) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kOffBars);
@@ -151,7 +125,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   {
     const PagedShare share = paged_find_share<kThreads>(batch, cost, cta, n_cta, &sh->find);
     if (warp == 0) {
-      const PagedWalk<PagedCost<kRT, kKB>> walk(batch, cost, share);
+      const PagedWalk<Cost> walk(batch, cost, share);
       if (lane == 0) {
         sh->walk = walk;
         sh->total = share.total;
@@ -169,7 +143,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   uint32_t n_blk = 0, n_piece = 0;        // blocks and pieces this role has gone through: the barriers' phases
   for (;;) {
     if (warp == 0) {
-      PagedWalk<PagedCost<kRT, kKB>> walk(batch, cost, sh->walk);
+      PagedWalk<Cost> walk(batch, cost, sh->walk);
       __syncwarp();
       int count = 0;
       for (; count < kBatch && walk.valid(); ++count, walk.next()) {
@@ -215,53 +189,60 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
             if (mine) {
               unsigned char* dst = smem + (kv ? kOffV : kOffK) + slot * kKvTile + lane * box_bytes;
               for (int hf = 0; hf < halves; ++hf)
-                tma_load_4d(dst + hf * kSub, kv ? &map_v : &map_k, hf * 64, y, pc.h, page, full);
+                umma::tma_load_4d(dst + hf * kSub, kv ? &map_v : &map_k, hf * 64, y, pc.h, page, full);
             }
           }
         }
         if (!fine) break;
       }
     } else if (warp == 1) {
-      if (lane == 0) {
-        const int ksteps = (d + 15) >> 4;
-        constexpr uint32_t idesc_kk = umma::instr_desc_bf16(128, kKB, false, false);
-        const uint32_t idesc_kn = umma::instr_desc_bf16(128, uint32_t(d + 15) & ~15u, false, true);
-        const uint64_t q_desc = umma::smem_desc(q_addr, 16u, 1024u);
-        const uint64_t k_desc[2] = {umma::smem_desc(k_addr, 16u, 1024u), umma::smem_desc(k_addr + kKvTile, 16u, 1024u)};
-        const uint64_t v_desc[2] = {umma::smem_desc(v_addr, kSub, 1024u), umma::smem_desc(v_addr + kKvTile, kSub, 1024u)};
-        for (int p = 0; p < count; ++p, ++n_piece) {
-          const int blocks = sh->pieces[p].b1 - sh->pieces[p].b0;
-          auto issue_scores = [&](int j) -> bool {
+      // the whole warp walks and waits, one lane issues
+      const int ksteps = (d + 15) >> 4;
+      constexpr uint32_t idesc_kk = umma::instr_desc_bf16(128, kKB, false, false);
+      const uint32_t idesc_kn = umma::instr_desc_bf16(128, uint32_t(d + 15) & ~15u, false, true);
+      auto wait = [&](uint64_t* bar, uint32_t parity, int site) {
+        return __all_sync(0xffffffffu, mbar_wait_abortable(bar, parity, s_abort, kDefaultWaitNs, site));
+      };
+      for (int p = 0; p < count; ++p, ++n_piece) {
+        const int blocks = sh->pieces[p].b1 - sh->pieces[p].b0;
+        bool ok = wait(q_full, n_piece & 1, __LINE__);
+        // scores run two blocks ahead; the tensor pipe runs in issue order, so those of block j + 2 may overwrite P of
+        // block j right behind the product that reads it
+        for (int j = -2; ok && j < blocks; ++j) {
+          if (j >= 0) {
             const uint32_t n = n_blk + j, slot = n & 1;
-            if (!mbar_wait_abortable(&k_full[slot], (n >> 1) & 1, CB2_SITE)) return false;
-            umma::fence_after_sync();
-            const uint64_t kd = slot ? k_desc[1] : k_desc[0];
-#pragma unroll
-            for (int ks = 0; ks < 8; ++ks)
-              if (ks < ksteps)
-                umma::mma_bf16(tmem + kColS + slot * kKB, desc_step(q_desc, q_step(ks)), desc_step(kd, k_step(ks)), idesc_kk, ks > 0);
-            umma::mma_commit(&s_ready[slot]);
-            umma::mma_commit(&k_empty[slot]);
-            return true;
-          };
-          bool ok = mbar_wait_abortable(q_full, n_piece & 1, CB2_SITE) && issue_scores(0) && (blocks < 2 || issue_scores(1));
-          for (int j = 0; ok && j < blocks; ++j) {
-            const uint32_t n = n_blk + j, slot = n & 1;
-            ok = mbar_wait_abortable(&p_ready[slot], (n >> 1) & 1, CB2_SITE) && mbar_wait_abortable(&v_full[slot], (n >> 1) & 1, CB2_SITE);
+            ok = wait(&p_ready[slot], (n >> 1) & 1, __LINE__) && wait(&v_full[slot], (n >> 1) & 1, __LINE__);
             if (!ok) break;
             umma::fence_after_sync();
-            const uint64_t vd = slot ? v_desc[1] : v_desc[0];
+            if (lane == 0) {
+              const uint32_t tile = v_addr + slot * kKvTile;
 #pragma unroll
-            for (int ks = 0; ks < kKB / 16; ++ks)
-              umma::mma_bf16_ts(tmem + kColO, tmem + kColS + slot * kKB + ks * 8, desc_step(vd, v_step(ks)), idesc_kn, j > 0 || ks > 0);
-            umma::mma_commit(&o_done[slot]);
-            umma::mma_commit(&v_empty[slot]);
-            // the tensor pipe runs in issue order, so the scores after next may overwrite P right away
-            if (j + 2 < blocks) ok = issue_scores(j + 2);
+              for (int ks = 0; ks < kKB / 16; ++ks)
+                umma::mma_bf16_ts(tmem + kColO, tmem + kColS + slot * kKB + ks * 8, desc_v(tile, ks), idesc_kn, j > 0 || ks > 0);
+              umma::mma_commit(&o_done[slot]);
+              umma::mma_commit(&v_empty[slot]);
+            }
+            __syncwarp();
           }
-          if (!ok) break;
-          n_blk += blocks;
+          if (j + 2 < blocks) {
+            const uint32_t n = n_blk + j + 2, slot = n & 1;
+            ok = wait(&k_full[slot], (n >> 1) & 1, __LINE__);
+            if (!ok) break;
+            umma::fence_after_sync();
+            if (lane == 0) {
+              const uint32_t tile = k_addr + slot * kKvTile;
+#pragma unroll
+              for (int ks = 0; ks < 8; ++ks)
+                if (ks < ksteps)
+                  umma::mma_bf16(tmem + kColS + slot * kKB, umma::desc_kmajor(q_addr, ks), desc_k(tile, ks), idesc_kk, ks > 0);
+              umma::mma_commit(&s_ready[slot]);
+              umma::mma_commit(&k_empty[slot]);
+            }
+            __syncwarp();
+          }
         }
+        if (!ok) break;
+        n_blk += blocks;
       }
     } else {
       const int q4 = warp & 3, rr = q4 * 32 + lane;
@@ -277,21 +258,16 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         const int tok = there ? row / a.G : 0, g = there ? row - tok * a.G : 0;
         const long long at = (pc->t0 + tok) * a.q_token + (pc->h * a.G + g) * a.q_head;
         const unsigned have = __ballot_sync(0xffffffffu, there);
-        auto copy = [&](auto chunks) {
-          constexpr int kChunks = decltype(chunks)::value, kRows = 32 / kChunks;
-          const int c = lane % kChunks;
-#pragma unroll
-          for (int i = 0; i < 32; i += kRows) {
-            const int from = i + lane / kChunks;
-            const long long off = __shfl_sync(0xffffffffu, at, from);
-            const bool ok = ((have >> from) & 1) && c * 8 < d;
-            cp_async16_or_zero(q_addr + umma::tile_chunk_offset(q4 * 32 + from, c * 8), a.q + off + (ok ? c * 8 : 0), ok);
-          }
-        };
-        if (halves == 2)
-          copy(std::integral_constant<int, 16>{});
-        else
-          copy(std::integral_constant<int, 8>{});
+        const int chunks = halves * 8, c = lane & (chunks - 1), sub = lane / chunks, step = 32 / chunks;
+        const bool col = c * 8 < d;
+        const uint32_t dst = q_addr + q4 * 32 * 128u + (c >> 3) * umma::kSubTileBytes;
+        // not unrolled: at a kernel's start every instruction line is a miss
+#pragma unroll 1
+        for (int from = sub; from < 32; from += step) {
+          const long long off = __shfl_sync(0xffffffffu, at, from);
+          const bool ok = ((have >> from) & 1) && col;
+          cp_async16_or_zero(dst + from * 128u + (((c & 7) ^ (from & 7)) << 4), a.q + off + (ok ? c * 8 : 0), ok);
+        }
         cp_async_commit();
       };
       auto rows_there = [&] {
@@ -327,8 +303,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
 #pragma unroll
           for (int cb = 0; cb < 2; ++cb) umma::tmem_ld32(s_cols + cb * 32, sv[cb]);
           umma::tmem_wait_ld();
-          loaded(sv[0]);
-          loaded(sv[1]);
+          umma::tmem_loaded(sv[0]);
+          umma::tmem_loaded(sv[1]);
           if (k0 + kKB - 1 > first_last) {
             const int lim = last - k0;
 #pragma unroll
@@ -361,13 +337,13 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
               float x0, x1;
               umma::f2_unpack(x, x0, x1);
               const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
-              sum2[(c >> 1) & 1] = f2_add(sum2[(c >> 1) & 1], umma::f2_pack(p0, p1));
+              sum2[(c >> 1) & 1] = umma::f2_add(sum2[(c >> 1) & 1], umma::f2_pack(p0, p1));
               w[c >> 1] = pack_bf16x2(p0, p1);
             }
             umma::tmem_st16(s_cols + cb * 16, w);
           }
           float s0, s1;
-          umma::f2_unpack(f2_add(sum2[0], sum2[1]), s0, s1);
+          umma::f2_unpack(umma::f2_add(sum2[0], sum2[1]), s0, s1);
           l_run = fmaf(l_run, alpha, s0 + s1);
           umma::tmem_wait_st();
           if (k0 + kKB > len) {
@@ -390,7 +366,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
             for (int cb = 0; cb < ncb; ++cb) {
               umma::tmem_ld32(lane_base + kColO + cb * 32, sv[0]);
               umma::tmem_wait_ld();
-              loaded(sv[0]);
+              umma::tmem_loaded(sv[0]);
 #pragma unroll
               for (int c = 0; c < 32; ++c) sv[0][c] = __float_as_uint(__uint_as_float(sv[0][c]) * alpha);
               umma::tmem_st32(lane_base + kColO + cb * 32, sv[0]);
@@ -416,7 +392,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
           uint32_t sv[32];
           umma::tmem_ld32(lane_base + kColO + cb * 32, sv);
           umma::tmem_wait_ld();
-          loaded(sv);
+          umma::tmem_loaded(sv);
           if (whole) {
             // 32 columns of 32 rows, turned in shared memory so that a store covers 64 bytes of 8 rows
 #pragma unroll
@@ -475,8 +451,12 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   }
 }
 
+constexpr int kCtas = 2 * kNumSMs;
+
+}  // namespace
+
 // Pools as a 4-D tensor {d, page_size, Hkv, n_pages}; box = 64 columns of a page, 64 rows at most.
-int make_pool_map(CUtensorMap* out, const void* base, int d, int page_size, int Hkv, int n_pages, long long page_stride) {
+int paged_pool_map(CUtensorMap* out, const void* base, int d, int page_size, int Hkv, int n_pages, long long page_stride) {
   using Fn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                           const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
   static Fn fn = nullptr;
@@ -490,7 +470,7 @@ int make_pool_map(CUtensorMap* out, const void* base, int d, int page_size, int 
   }
   const cuuint64_t dims[4] = {cuuint64_t(d), cuuint64_t(page_size), cuuint64_t(Hkv), cuuint64_t(n_pages)};
   const cuuint64_t strides[3] = {cuuint64_t(d) * 2, cuuint64_t(page_size) * d * 2, cuuint64_t(page_stride) * 2};
-  const cuuint32_t box[4] = {64, cuuint32_t(page_size < kKB ? page_size : kKB), 1, 1};
+  const cuuint32_t box[4] = {64, cuuint32_t(page_size < 64 ? page_size : 64), 1, 1};
   const cuuint32_t step[4] = {1, 1, 1, 1};
   const CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, step,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -498,18 +478,14 @@ int make_pool_map(CUtensorMap* out, const void* base, int d, int page_size, int 
   return r == CUDA_SUCCESS ? CB2_OK : CB2_LAUNCH_FAIL;
 }
 
-constexpr int kCtas = 2 * kNumSMs;
-
-}  // namespace
-
 size_t paged_tc_scratch_bytes(int d) { return paged_scratch_bytes(kCtas, kRT, d); }
 
 // Requests of more than `few` packed rows; partial carriers are left in `scratch` (kRT rows a slot, kCtas shares).
 int paged_tc_run(const PagedRows& rows, const PagedPools& pools, const PagedBatch& batch, int causal, int few, void* o, float* lse2,
                  void* scratch, PagedScratch* parts, int* n_cta, cudaStream_t st) {
   CUtensorMap mk, mv;
-  int rc = make_pool_map(&mk, pools.k, pools.d, 1 << batch.page_log2, pools.Hkv, batch.n_pages, pools.k_page_stride);
-  if (rc == CB2_OK) rc = make_pool_map(&mv, pools.v, pools.d, 1 << batch.page_log2, pools.Hkv, batch.n_pages, pools.v_page_stride);
+  int rc = paged_pool_map(&mk, pools.k, pools.d, 1 << batch.page_log2, pools.Hkv, batch.n_pages, pools.k_page_stride);
+  if (rc == CB2_OK) rc = paged_pool_map(&mv, pools.v, pools.d, 1 << batch.page_log2, pools.Hkv, batch.n_pages, pools.v_page_stride);
   if (rc != CB2_OK) return rc;
   if (cudaFuncSetAttribute(paged_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmemBytes)) != cudaSuccess)
     return CB2_LAUNCH_FAIL;
@@ -517,7 +493,7 @@ int paged_tc_run(const PagedRows& rows, const PagedPools& pools, const PagedBatc
   *n_cta = kCtas;
   const TcArgs a{static_cast<const __nv_bfloat16*>(rows.q), rows.q_token, rows.q_head, static_cast<__nv_bfloat16*>(o), lse2,
                  rows.scale_log2e, rows.G, rows.Hkv, pools.d};
-  const PagedCost<kRT, kKB> cost{rows.G, rows.Hkv, causal, kPagedChunk, few, 4};
+  const Cost cost{rows.G, rows.Hkv, causal, kPagedChunk, few, 4};
   paged_tc_kernel<<<kCtas, kThreads, kSmemBytes, st>>>(mk, mv, a, batch, cost, *parts);
   CB2_LAUNCH_CHECK();
   return CB2_OK;
