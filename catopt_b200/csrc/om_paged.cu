@@ -517,6 +517,7 @@ extern "C" int cb2_om_paged_fwd(const void* q, long long q_token_stride, long lo
   if (int64_t(max_pages) * page_size < max_k || !(scale > 0.f) || scale > 3e38f) return CB2_BAD_SHAPE;
   const long long page = (long long)Hkv * page_size * d;
   if (k_page_stride < page || v_page_stride < page || q_token_stride < 0 || q_head_stride < 0) return CB2_BAD_SHAPE;
+  if ((n_tokens > 1 && q_token_stride == 0) || (Hq > 1 && q_head_stride == 0)) return CB2_BAD_SHAPE;
   if (dtype != CB2_BF16 && dtype != CB2_F32) return CB2_UNSUPPORTED_DTYPE;
   if (n_tokens == 0) return CB2_OK;
   if (!q || !o || !scratch) return CB2_NULL_PTR;

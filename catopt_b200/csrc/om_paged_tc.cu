@@ -457,17 +457,8 @@ constexpr int kCtas = 2 * kNumSMs;
 
 // Pools as a 4-D tensor {d, page_size, Hkv, n_pages}; box = 64 columns of a page, 64 rows at most.
 int paged_pool_map(CUtensorMap* out, const void* base, int d, int page_size, int Hkv, int n_pages, long long page_stride) {
-  using Fn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                          const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-  static Fn fn = nullptr;
-  if (!fn) {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
-        q != cudaDriverEntryPointSuccess || !p)
-      return CB2_LAUNCH_FAIL;
-    fn = reinterpret_cast<Fn>(p);
-  }
+  const umma::EncodeTiledFn fn = umma::encode_tiled();
+  if (!fn) return CB2_LAUNCH_FAIL;
   const cuuint64_t dims[4] = {cuuint64_t(d), cuuint64_t(page_size), cuuint64_t(Hkv), cuuint64_t(n_pages)};
   const cuuint64_t strides[3] = {cuuint64_t(d) * 2, cuuint64_t(page_size) * d * 2, cuuint64_t(page_stride) * 2};
   const cuuint32_t box[4] = {64, cuuint32_t(page_size < 64 ? page_size : 64), 1, 1};

@@ -7,9 +7,11 @@
 // the attention costs.  Unit of the work line = (request, kv head, 128-key block), cost = the 64-row tiles that
 // see it; a unit cut between shares leaves 128 partial sums a share, added in share order.
 //
-// Roles: warp 0 = the key block (pages by TMA), warp 1 = MMA issue and TMEM owner, warps 2..5 = sums, warps 6, 7 = rows
-// of a tile (16-byte asynchronous copies), their -lse and the last slot each sees.  A ring of three stages holds
-// row tile, -lse and S together; two CTAs share an SM.  Every wait is bounded.
+// A row tile is T = 64 / G whole tokens of a group (64 heads of one token when G > 64), so that one TMA box of q brings
+// it; columns past T G stay zero.  Roles: warp 0 = the key block (pages by TMA), warp 1 = MMA issue and TMEM owner,
+// warps 2..5 = sums, warp 6 = row tiles, their -lse and the last slot each row sees (copying the rows by 16-byte
+// asynchronous copies took 2.8 k cycles a tile and set the pace).  A ring of four stages holds row tile, -lse and S
+// together; two CTAs share an SM.  Every wait is bounded.
 #include "om_paged.cuh"
 #include "umma.cuh"
 
@@ -18,8 +20,8 @@ int paged_pool_map(CUtensorMap* out, const void* base, int d, int page_size, int
 
 namespace {
 
-constexpr int kKeys = 128, kRows = 64, kStages = 3;
-constexpr int kThreads = 256;
+constexpr int kKeys = 128, kRows = 64, kStages = 4;
+constexpr int kThreads = 224;
 constexpr int kCtas = 2 * kNumSMs;
 constexpr uint32_t kSub = 64 * 128;                       // 64 rows x 64 columns of a row tile
 constexpr uint32_t kRowTile = 2 * kSub;
@@ -32,20 +34,21 @@ constexpr uint32_t kTmemCols = 256;
 struct KeyCost {
   static constexpr int kOv = 2;
   int G, Hkv, causal, which, few, min_blocks;
+  int T, per_token;         // tokens a row tile, row tiles a token: one of them is 1
   __device__ __forceinline__ bool takes(const PagedReq& q) const {
     if (q.n == 0 || q.len == 0) return false;
     return which == kPagedAll || (which == kPagedFew) == (q.n * G <= few);
   }
-  __device__ __forceinline__ int row_tiles(const PagedReq& q) const { return (q.n * G + kRows - 1) / kRows; }
+  __device__ __forceinline__ int row_tiles(const PagedReq& q) const { return (q.n + T - 1) / T * per_token; }
   __device__ __forceinline__ int first_row_tile(const PagedReq& q, int i) const {
-    return causal ? int(unsigned(max(i * kKeys - (q.len - q.n), 0)) * G / kRows) : 0;
+    return causal ? max(i * kKeys - (q.len - q.n), 0) / T * per_token : 0;
   }
   __device__ __forceinline__ int tiles(const PagedReq& q) const { return (q.len + kKeys - 1) / kKeys; }
   __device__ __forceinline__ int blocks(const PagedReq& q, int i) const { return row_tiles(q) - first_row_tile(q, i); }
   __device__ __forceinline__ long long before(const PagedReq& q, int k) const {
     long long s = (long long)k * (row_tiles(q) + kOv);
     const int base = q.len - q.n, i1 = base < 0 ? 0 : base / kKeys + 1;       // first block that not all rows see
-    if (causal && k > i1) s -= stair_sum(k - i1, kRows, unsigned(kKeys) * G, unsigned(i1 * kKeys - base) * G);
+    if (causal && k > i1) s -= stair_sum(k - i1, T, kKeys, unsigned(i1 * kKeys - base)) * per_token;
     return s;
   }
   __device__ __forceinline__ long long of_request(const PagedReq& q) const { return takes(q) ? before(q, tiles(q)) * Hkv : 0; }
@@ -59,14 +62,13 @@ constexpr int kBatch = 16;
 
 struct Smem {
   uint32_t tmem;
-  int abort, count, loads_k, n_share;
+  int abort, count, loads_k, loads_q, n_share;
   long long total;
   PagedWalkState walk;
   Piece pieces[kBatch];
   PagedFindSmem find;
   float neg_lse[kStages][kRows];
   int last[kStages][kRows];
-  long long row_at[2][32];
 };
 constexpr uint32_t kOffMisc = (kOffBars + kNumBars * 8 + 15) & ~15u;
 constexpr uint32_t kSmemBytes = kOffMisc + uint32_t(sizeof(Smem)) + 1024;
@@ -77,7 +79,7 @@ __device__ __forceinline__ uint64_t desc_rows(uint32_t tile, int ks) {
 }
 
 __global__ void __launch_bounds__(kThreads, 2)
-paged_weights_tc_kernel(const __grid_constant__ CUtensorMap map_k, const PagedRows rows, const int d, const PagedBatch batch,
+paged_weights_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_q, const PagedRows rows, const int d, const PagedBatch batch,
                         const KeyCost cost, const float* __restrict__ lse2, float* __restrict__ weights, PagedJoin* __restrict__ joins,
                         float* __restrict__ parts) {
   extern __shared__ unsigned char smem_raw[];
@@ -91,13 +93,13 @@ paged_weights_tc_kernel(const __grid_constant__ CUtensorMap map_k, const PagedRo
 
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(&q_full[i], 64);
+      mbar_init(&q_full[i], 33);           // the TMA box and the 32 lanes that write -lse
       mbar_init(&s_ready[i], 1);
       mbar_init(&s_empty[i], 128);
     }
     mbar_init(k_full, 1);
     mbar_init(k_empty, 1);
-    sh->abort = sh->loads_k = 0;
+    sh->abort = sh->loads_k = sh->loads_q = 0;
     joins[cta].r = -1;
     mbar_fence_init();
   }
@@ -105,6 +107,10 @@ paged_weights_tc_kernel(const __grid_constant__ CUtensorMap map_k, const PagedRo
     __syncwarp();
     umma::tmem_alloc(&sh->tmem, kTmemCols);
   }
+  // columns that no box writes count as rows of zeros
+  for (uint32_t e = tid; e < kStages * kRowTile / 16; e += kThreads)
+    *reinterpret_cast<uint4*>(smem + kOffQ + e * 16) = make_uint4(0, 0, 0, 0);
+  fence_proxy_async_smem();
   {
     const PagedShare share = paged_find_share<kThreads>(batch, cost, cta, n_cta, &sh->find);
     if (warp == 0) {
@@ -218,8 +224,9 @@ paged_weights_tc_kernel(const __grid_constant__ CUtensorMap map_k, const PagedRo
           umma::tmem_wait_ld();
           umma::tmem_loaded(sv[0]);
           umma::tmem_loaded(sv[1]);
-          // rows that do not see the whole key block: hidden per element
-          if (cost.causal && base + (pc->tile0 + i) * kRows / G < pc->k0 + kKeys - 1) {
+          // rows that do not see the whole key block, or are not of this request: hidden per element
+          const int tok0 = (pc->tile0 + i) / cost.per_token * cost.T;
+          if ((cost.causal && base + tok0 < pc->k0 + kKeys - 1) || tok0 + cost.T > pc->n || cost.per_token > 1) {
 #pragma unroll
             for (int cb = 0; cb < 2; ++cb)
 #pragma unroll
@@ -255,50 +262,49 @@ paged_weights_tc_kernel(const __grid_constant__ CUtensorMap map_k, const PagedRo
         }
       }
     } else {
-      // rows of the tiles, 32 a warp: a lane works out one row's place, then 8 or 16 neighbouring lanes copy its chunks
-      const int lw = warp - 6, lt = lw * 32 + lane;
-      const int chunks = halves * 8, c = lane & (chunks - 1), sub = lane / chunks, step = 32 / chunks;
-      const uint32_t dst = q_addr + lw * 32 * 128u + (c >> 3) * kSub;
-      const __nv_bfloat16* qb = static_cast<const __nv_bfloat16*>(rows.q);
-      uint32_t issued = n_tile;          // tiles whose copies have been issued; n_tile: handed to the MMA warp
+      // columns lane and lane + 32 of a tile: token and head inside it
+      const int hb = min(G, kRows);
+      const int tok_of[2] = {lane / hb, (lane + 32) / hb}, g_of[2] = {lane % hb, (lane + 32) % hb};
+      float z[2];
+      int last[2];
+      auto look_up = [&](const Piece& pc, int i) {           // a tile ahead
+        const int tile = pc.tile0 + i, tok0 = tile / cost.per_token * cost.T, g0 = tile % cost.per_token * kRows;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int tok = tok0 + tok_of[e], g = g0 + g_of[e];
+          const bool there = tok_of[e] < cost.T && tok < pc.n && g < G;
+          z[e] = there ? __ldg(lse2 + (long long)(pc.t0 + tok) * (G * rows.Hkv) + pc.h * G + g) : INFINITY;
+          last[e] = there ? (cost.causal ? min(pc.len - pc.n + tok, pc.len - 1) : pc.len - 1) : -1;
+        }
+      };
+      if (count > 0) look_up(sh->pieces[0], 0);
       for (int p = 0; p < count; ++p) {
         const Piece pc = sh->pieces[p];
         bool ok = true;
-        for (int i = 0; i < pc.tiles; ++i, ++issued) {
-          const uint32_t st = stage_of(issued);
-          if (issued >= kStages) ok = mbar_wait_abortable(&s_empty[st], phase_of(issued - kStages), s_abort, kDefaultWaitNs, __LINE__);
+        for (int i = 0; i < pc.tiles; ++i, ++n_tile) {
+          const uint32_t st = stage_of(n_tile);
+          if (n_tile >= kStages) ok = mbar_wait_abortable(&s_empty[st], phase_of(n_tile - kStages), s_abort, kDefaultWaitNs, __LINE__);
           if (!__all_sync(0xffffffffu, ok)) break;
-          const int row = (pc.tile0 + i) * kRows + lt;
-          const bool there = row < pc.n * G;
-          const int tok = there ? row / G : 0, g = there ? row - tok * G : 0;
-          const float z = there ? __ldg(lse2 + (long long)(pc.t0 + tok) * (G * rows.Hkv) + pc.h * G + g) : INFINITY;
-          sh->neg_lse[st][lt] = -z;
-          sh->last[st][lt] = cost.causal ? min(pc.len - pc.n + tok, pc.len - 1) : pc.len - 1;
-          sh->row_at[lw][lane] = there ? (pc.t0 + tok) * rows.q_token + (pc.h * G + g) * rows.q_head : -1;
-          __syncwarp();
-#pragma unroll 4
-          for (int r = sub; r < 32; r += step) {
-            const long long at = sh->row_at[lw][r];
-            const bool have = at >= 0 && c * 8 < d;
-            cp_async16_or_zero(dst + st * kRowTile + r * 128u + (((c & 7) ^ (r & 7)) << 4), qb + (have ? at + c * 8 : 0), have);
+          if (lane == 0) {
+            const int tile = pc.tile0 + i;
+            mbar_arrive_expect_tx(&q_full[st], halves * hb * cost.T * 128);
+            ++sh->loads_q;
+            for (int hf = 0; hf < halves; ++hf)
+              umma::tma_load_3d(smem + kOffQ + st * kRowTile + hf * kSub, &map_q, hf * 64, pc.h * G + tile % cost.per_token * kRows,
+                                pc.t0 + tile / cost.per_token * cost.T, &q_full[st]);
           }
-          cp_async_commit();
-          // the tile before this one has landed
-          if (issued > n_tile) {
-            cp_async_wait_one();
-            fence_proxy_async_smem();
-            mbar_arrive(&q_full[stage_of(n_tile)]);
-            ++n_tile;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            sh->neg_lse[st][lane + 32 * e] = -z[e];
+            sh->last[st][lane + 32 * e] = last[e];
           }
-          __syncwarp();            // row_at is read
+          mbar_arrive(&q_full[st]);
+          if (i + 1 < pc.tiles)
+            look_up(pc, i + 1);
+          else if (p + 1 < count)
+            look_up(sh->pieces[p + 1], 0);
         }
         if (!__all_sync(0xffffffffu, ok)) break;
-      }
-      if (issued > n_tile) {
-        cp_async_wait_all();
-        fence_proxy_async_smem();
-        mbar_arrive(&q_full[stage_of(n_tile)]);
-        ++n_tile;
       }
     }
     __syncwarp();
@@ -309,7 +315,9 @@ paged_weights_tc_kernel(const __grid_constant__ CUtensorMap map_k, const PagedRo
   }
   if (*s_abort) {
     if (tid == 0) {
-      if (sh->loads_k) mbar_wait_bounded(k_full, (sh->loads_k - 1) & 1);      // a load in flight lands before the memory goes
+      // loads in flight land before the shared memory goes (bounded waits, too)
+      if (sh->loads_k) mbar_wait_bounded(k_full, (sh->loads_k - 1) & 1);
+      for (int n = max(sh->loads_q - kStages, 0); n < sh->loads_q; ++n) mbar_wait_bounded(&q_full[stage_of(n)], phase_of(n));
       if (batch.status) atomicExch(batch.status, CB2_WAIT_TIMEOUT | (*s_abort << 8));
     }
     __syncthreads();
@@ -342,15 +350,19 @@ size_t paged_weights_tc_scratch_bytes() { return size_t(kCtas) * (sizeof(PagedJo
 
 int paged_weights_tc_run(const PagedRows& rows, const PagedPools& pools, const PagedBatch& batch, int causal, int which, int few,
                          const float* lse2, float* weights, void* scratch, cudaStream_t st) {
-  CUtensorMap mk;
-  const int rc = paged_pool_map(&mk, pools.k, pools.d, 1 << batch.page_log2, pools.Hkv, batch.n_pages, pools.k_page_stride);
+  CUtensorMap mk, mq;
+  int rc = paged_pool_map(&mk, pools.k, pools.d, 1 << batch.page_log2, pools.Hkv, batch.n_pages, pools.k_page_stride);
+  // q as {d, Hq, n_tokens}: a box holds T tokens of a group
+  const int Hq = rows.G * rows.Hkv, T = rows.G < kRows ? kRows / rows.G : 1;
+  const long long head = Hq > 1 ? rows.q_head : pools.d, token = batch.n_tokens > 1 ? rows.q_token : (long long)Hq * pools.d;
+  if (rc == CB2_OK) rc = umma::make_map_3d_strided(&mq, rows.q, pools.d, Hq, batch.n_tokens, head, token, 64, rows.G < kRows ? rows.G : kRows, T);
   if (rc != CB2_OK) return rc;
   if (cudaFuncSetAttribute(paged_weights_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmemBytes)) != cudaSuccess)
     return CB2_LAUNCH_FAIL;
-  const KeyCost cost{rows.G, rows.Hkv, causal, which, few, 4};
+  const KeyCost cost{rows.G, rows.Hkv, causal, which, few, 4, T, rows.G > kRows ? (rows.G + kRows - 1) / kRows : 1};
   PagedJoin* joins = static_cast<PagedJoin*>(scratch);
   float* parts = reinterpret_cast<float*>(joins + kCtas);
-  paged_weights_tc_kernel<<<kCtas, kThreads, kSmemBytes, st>>>(mk, rows, pools.d, batch, cost, lse2, weights, joins, parts);
+  paged_weights_tc_kernel<<<kCtas, kThreads, kSmemBytes, st>>>(mk, mq, rows, pools.d, batch, cost, lse2, weights, joins, parts);
   CB2_LAUNCH_CHECK();
   paged_weights_join_kernel<<<kCtas, kKeys, 0, st>>>(batch, rows.Hkv, joins, parts, weights);
   CB2_LAUNCH_CHECK();

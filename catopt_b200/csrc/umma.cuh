@@ -166,21 +166,25 @@ __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* tmap) {
 // A box that reaches past an extent is filled with zeros on load and clipped on store.  The
 // encoder is taken from the driver through the runtime's entry-point query, so the library
 // does not link against the driver library directly.
-inline int make_map_3d(CUtensorMap* out, const void* base, bool is_bf16, uint64_t d0, uint64_t d1,
-                       uint64_t d2, uint32_t b0, uint32_t b1, bool swizzle128 = false) {
-  using Fn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                          const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
-                          CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
-                          CUtensorMapFloatOOBfill);
-  static Fn fn = nullptr;
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+inline EncodeTiledFn encode_tiled() {
+  static EncodeTiledFn fn = nullptr;
   if (!fn) {
     void* p = nullptr;
     cudaDriverEntryPointQueryResult q;
     if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
         q != cudaDriverEntryPointSuccess || !p)
-      return CB2_LAUNCH_FAIL;
-    fn = reinterpret_cast<Fn>(p);
+      return nullptr;
+    fn = reinterpret_cast<EncodeTiledFn>(p);
   }
+  return fn;
+}
+inline int make_map_3d(CUtensorMap* out, const void* base, bool is_bf16, uint64_t d0, uint64_t d1,
+                       uint64_t d2, uint32_t b0, uint32_t b1, bool swizzle128 = false) {
+  const EncodeTiledFn fn = encode_tiled();
+  if (!fn) return CB2_LAUNCH_FAIL;
   const uint64_t esz = is_bf16 ? 2 : 4;
   const cuuint64_t gdim[3] = {d0, d1, d2};
   const cuuint64_t gstride[2] = {d0 * esz, d0 * d1 * esz};
@@ -191,6 +195,20 @@ inline int make_map_3d(CUtensorMap* out, const void* base, bool is_bf16, uint64_
                         CU_TENSOR_MAP_INTERLEAVE_NONE,
                         swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? CB2_OK : CB2_LAUNCH_FAIL;
+}
+// bf16 tensor {d0, d1, d2} with strides s1, s2 (elements, multiples of 8), box {b0, b1, b2}, 128-byte swizzle.
+inline int make_map_3d_strided(CUtensorMap* out, const void* base, uint64_t d0, uint64_t d1, uint64_t d2, uint64_t s1,
+                               uint64_t s2, uint32_t b0, uint32_t b1, uint32_t b2) {
+  const EncodeTiledFn fn = encode_tiled();
+  if (!fn) return CB2_LAUNCH_FAIL;
+  const cuuint64_t gdim[3] = {d0, d1, d2};
+  const cuuint64_t gstride[2] = {s1 * 2, s2 * 2};
+  const cuuint32_t box[3] = {b0, b1, b2};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), gdim, gstride, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? CB2_OK : CB2_LAUNCH_FAIL;
 }
 

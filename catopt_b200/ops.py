@@ -758,7 +758,8 @@ def _token_rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` ``[n_tokens, heads, d]`` as the kernels read it: 16-byte steps between heads and tokens (a view
     that has them is read in place)."""
     unit = 16 // t.element_size()
-    if t.numel() and (t.stride(2) != 1 or t.stride(0) % unit or t.stride(1) % unit or t.data_ptr() % 16):
+    st, sh, sd = t.stride()
+    if t.numel() and (sd != 1 or st % unit or sh % unit or st == 0 or sh == 0 or t.data_ptr() % 16):
         return t.clone(memory_format=torch.contiguous_format)
     return t
 

@@ -448,8 +448,8 @@ int cb2_paged_append(const void* q, long long q_token_stride, long long q_head_s
  * over the slots j <= seq_lens[r] - n_r + i that row i of request r sees (causal != 0), or all
  * of its slots.  A row that sees no key (seq_lens[r] = 0, or less than n_r) is 0.  What the
  * slots behind seq_lens[r] hold, NaN included, has no effect.
- * q: [n_tokens, Hq, d] with token and head strides in elements; o: [n_tokens, Hq, d] dense,
- * apart from q.  max_q: no request has more new tokens; max_k: none more cached keys.
+ * q: [n_tokens, Hq, d] with token and head strides in elements (none 0); o: [n_tokens, Hq, d]
+ * dense, apart from q.  max_q: no request has more new tokens; max_k: none more cached keys.
  * weights (may be NULL): weights[key] += sum over the rows that see it, and the heads of its
  * group, of the softmax probability.  Results do not depend on the order in which CTAs run.
  * Products of bf16 tensors accumulate in fp32 and probabilities are rounded to bf16 for the

@@ -78,6 +78,12 @@ def test_attention_work_cut_over_keys(dev, dtype, new, lens, kv, group):
     run_attend(dev, new, lens, kv, group, 128 if kv == 2 else 64, 16, dtype, weights=True, fill=float("inf"))
 
 
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("group", [20, 72, 128])
+def test_many_heads_on_one(dev, dtype, group):
+    run_attend(dev, [1, 0, 7, 40], [300, 5, 200, 150], 1 if group > 20 else 2, group, 64, 16, dtype, weights=True)
+
+
 def test_weights_when_the_bound_on_keys_is_far_off(dev):
     # scores of 2.3 million possible keys are not kept: the weights are computed from the keys again
     from catopt_b200 import ops

@@ -31,7 +31,7 @@ NULL, SHAPE, ALIGN, DTYPE, SCRATCH = 6, 1, 2, 3, 7
     (dict(R=0), SHAPE), (dict(Hq=3), SHAPE), (dict(Hkv=0), SHAPE), (dict(d=60), SHAPE), (dict(d=136), SHAPE), (dict(page=12), SHAPE),
     (dict(page=4), SHAPE), (dict(page=2048), SHAPE), (dict(max_k=33), SHAPE), (dict(max_k=0), SHAPE), (dict(max_q=-1), SHAPE),
     (dict(n_pages=0), SHAPE), (dict(scale=0.0), SHAPE), (dict(scale=float("nan")), SHAPE), (dict(scale=float("inf")), SHAPE),
-    (dict(ks=2040), SHAPE), (dict(n=1 << 30), SHAPE), (dict(dtype=7), DTYPE), (dict(q=P + 2), ALIGN), (dict(qt=252), ALIGN),
+    (dict(ks=2040), SHAPE), (dict(qt=0), SHAPE), (dict(qh=0), SHAPE), (dict(n=1 << 30), SHAPE), (dict(dtype=7), DTYPE), (dict(q=P + 2), ALIGN), (dict(qt=252), ALIGN),
     (dict(v=P + 8), ALIGN), (dict(bytes=16), SCRATCH),
 ], ids=str)
 def test_attention_refusals(lib, change, want):
