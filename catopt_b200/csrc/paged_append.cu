@@ -6,15 +6,17 @@
 //   slot len - n + i of request r <- k', v ;  attention weight there <- 0 ;  q' -> q_out
 //
 // Bound by memory: every row is read once and written once.  Sixteen lanes hold one head's row, eight
-// elements each, so the sum of squares is four shuffles; the lanes' columns are the same for every head of
-// a token, so its cos / sin and the norm weights are loaded once and stay in registers across the heads.
+// elements each as two chunks of four, so the sum of squares is four shuffles.  Which columns a lane holds is chosen so
+// that both elements of a rotated pair are in one lane: neighbouring chunks for interleaved pairs, chunks half a row
+// apart for pairs (i, i + d/2); only a rotation of part of the columns in halves exchanges through shared
+// memory.  A lane's columns are the same for every head of a token, so its angles and norm weights are loaded once.
 #include "om_paged.cuh"
 
 namespace cb2 {
 namespace {
 
 constexpr int kThreads = 256, kGroups = kThreads / 16;
-constexpr int kAhead = 4;     // rows a group has in flight
+constexpr int kAhead = 4;     // rows of q a group has in flight
 
 struct AppendArgs {
   const void *q, *k, *v;
@@ -31,15 +33,25 @@ struct AppendArgs {
   int Hq, Hkv, d, tokens_per_cta;
 };
 
+// How the columns of a row are paired by the rotation.
+enum { kNone, kInterleaved, kHalves, kExchange };
+
+// Eight elements of a row: columns [o0, o0 + 4) and [o1, o1 + 4).
 template <class T>
 struct Raw;
 template <>
 struct Raw<__nv_bfloat16> {
-  uint4 u;
-  __device__ __forceinline__ void load(const __nv_bfloat16* p) { u = *reinterpret_cast<const uint4*>(p); }
-  __device__ __forceinline__ void store(__nv_bfloat16* p) const { *reinterpret_cast<uint4*>(p) = u; }
+  uint2 a, b;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p, int o0, int o1) {
+    a = *reinterpret_cast<const uint2*>(p + o0);
+    b = *reinterpret_cast<const uint2*>(p + o1);
+  }
+  __device__ __forceinline__ void store(__nv_bfloat16* p, int o0, int o1) const {
+    *reinterpret_cast<uint2*>(p + o0) = a;
+    *reinterpret_cast<uint2*>(p + o1) = b;
+  }
   __device__ __forceinline__ void unpack(float (&x)[8]) const {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    const uint32_t w[4] = {a.x, a.y, b.x, b.y};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       x[2 * i] = bf16lo_to_f32(w[i]);
@@ -47,19 +59,20 @@ struct Raw<__nv_bfloat16> {
     }
   }
   __device__ __forceinline__ void pack(const float (&x)[8]) {
-    u = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
+    a = make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
+    b = make_uint2(pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
   }
 };
 template <>
 struct Raw<float> {
   float4 a, b;
-  __device__ __forceinline__ void load(const float* p) {
-    a = *reinterpret_cast<const float4*>(p);
-    b = *reinterpret_cast<const float4*>(p + 4);
+  __device__ __forceinline__ void load(const float* p, int o0, int o1) {
+    a = *reinterpret_cast<const float4*>(p + o0);
+    b = *reinterpret_cast<const float4*>(p + o1);
   }
-  __device__ __forceinline__ void store(float* p) const {
-    *reinterpret_cast<float4*>(p) = a;
-    *reinterpret_cast<float4*>(p + 4) = b;
+  __device__ __forceinline__ void store(float* p, int o0, int o1) const {
+    *reinterpret_cast<float4*>(p + o0) = a;
+    *reinterpret_cast<float4*>(p + o1) = b;
   }
   __device__ __forceinline__ void unpack(float (&x)[8]) const {
     x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
@@ -76,11 +89,53 @@ struct TokenPlace {
   int live;
 };
 
-template <class T>
+// Norm and rotation of the eight elements that a lane holds; `mine`: this row's place in shared memory (kExchange).
+template <int MODE>
+__device__ __forceinline__ void turn(float (&x)[8], bool norm, const float (&w)[8], float inv_d, float eps, const float (&cs)[8],
+                                     const float (&sn)[8], unsigned half_mask, float* mine, int gl, int rot) {
+  if (norm) {
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
+#pragma unroll
+    for (int off = 8; off; off >>= 1) ss += __shfl_xor_sync(half_mask, ss, off);
+    const float inv = rsqrtf(ss * inv_d + eps);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] *= inv * w[i];
+  }
+  if (MODE == kInterleaved) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      const float a = x[i], b = x[i + 1];
+      x[i] = fmaf(-b, sn[i >> 1], a * cs[i >> 1]);
+      x[i + 1] = fmaf(a, sn[i >> 1], b * cs[i >> 1]);
+    }
+  } else if (MODE == kHalves) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float a = x[i], b = x[i + 4];
+      x[i] = fmaf(-b, sn[i], a * cs[i]);
+      x[i + 4] = fmaf(a, sn[i], b * cs[i]);
+    }
+  } else if (MODE == kExchange) {
+    const int half = rot / 2;
+    __syncwarp(half_mask);
+    *reinterpret_cast<float4*>(mine + gl * 8) = make_float4(x[0], x[1], x[2], x[3]);
+    *reinterpret_cast<float4*>(mine + gl * 8 + 4) = make_float4(x[4], x[5], x[6], x[7]);
+    __syncwarp(half_mask);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int e = gl * 8 + i;
+      if (e < rot) x[i] = fmaf(mine[e < half ? e + half : e - half], sn[i], x[i] * cs[i]);
+    }
+  }
+}
+
+template <class T, int MODE>
 __global__ void __launch_bounds__(kThreads)
 paged_append_kernel(const AppendArgs a, const PagedBatch batch) {
   __shared__ TokenPlace place[kGroups];
-  __shared__ __align__(16) float rows[kGroups][128];
+  __shared__ __align__(16) float rows[MODE == kExchange ? kGroups : 1][128];
   const int tid = threadIdx.x, group = tid / 16, gl = tid % 16;
   const int t_first = blockIdx.x * a.tokens_per_cta;
   const int t_count = min(a.tokens_per_cta, batch.n_tokens - t_first);
@@ -125,97 +180,99 @@ paged_append_kernel(const AppendArgs a, const PagedBatch batch) {
   const bool in = gl * 8 < d;
   const int ps = 1 << batch.page_log2;
 
-  float cs[8], sn[8];
-  Raw<T> wq, wk;
+  const int o0 = MODE == kHalves ? gl * 4 : gl * 8, o1 = MODE == kHalves ? half + gl * 4 : gl * 8 + 4;
+  // what the group reads first is on its way before the angles are looked up
+  const int sub = group % per_token;
+  const T* qp = static_cast<const T*>(a.q) + t * a.q_token;
+  const T* kp = static_cast<const T*>(a.k) + t * a.k_token;
+  const T* vp = static_cast<const T*>(a.v) + t * a.v_token;
+  Raw<T> rq[kAhead], rk, rv;
+  auto fetch_q = [&](int h0) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int e = gl * 8 + i;
-    cs[i] = 1.f, sn[i] = 0.f;
-    if (e < a.rot) {
-      const int f = a.interleaved ? e >> 1 : (e < half ? e : e - half);
-      const bool first = a.interleaved ? !(e & 1) : e < half;
-      cs[i] = __ldg(a.cos + (long long)here.position * half + f);
-      const float s = __ldg(a.sin + (long long)here.position * half + f);
-      sn[i] = first ? -s : s;          // y = x cos + partner * sn
-    }
+    for (int u = 0; u < kAhead; ++u)
+      if (in && h0 + u * per_token < a.Hq) rq[u].load(qp + (h0 + u * per_token) * a.q_head, o0, o1);
+  };
+  fetch_q(sub);
+  if (in && sub < a.Hkv) {
+    rk.load(kp + sub * a.k_head, o0, o1);
+    rv.load(vp + sub * a.v_head, o0, o1);
   }
-  if (in && a.q_weight) wq.load(static_cast<const T*>(a.q_weight) + gl * 8);
-  if (in && a.k_weight) wk.load(static_cast<const T*>(a.k_weight) + gl * 8);
-  const int n_rows = a.Hq + 2 * a.Hkv;
-  for (int row0 = group % per_token; row0 < n_rows; row0 += kAhead * per_token) {
-    Raw<T> raw[kAhead];
+  float cs[8], sn[8], w[8];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int row = row0 + u * per_token;
-      if (in && row < n_rows) {
-        const bool is_q = row < a.Hq, is_v = row >= a.Hq + a.Hkv;
-        const T* src = is_q ? static_cast<const T*>(a.q) + t * a.q_token + row * a.q_head
-                       : is_v ? static_cast<const T*>(a.v) + t * a.v_token + (row - a.Hq - a.Hkv) * a.v_head
-                              : static_cast<const T*>(a.k) + t * a.k_token + (row - a.Hq) * a.k_head;
-        raw[u].load(src + gl * 8);
-      }
+  for (int i = 0; i < 8; ++i) cs[i] = 1.f, sn[i] = 0.f, w[i] = 0.f;
+  const float* ct = a.cos + (long long)here.position * half;
+  const float* st = a.sin + (long long)here.position * half;
+  if (MODE == kInterleaved || MODE == kHalves) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int f = gl * 4 + i;
+      if (f < half) cs[i] = __ldg(ct + f), sn[i] = __ldg(st + f);
     }
+  } else if (MODE == kExchange) {
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int row = row0 + u * per_token;
-      if (row >= n_rows) break;
-      const bool is_q = row < a.Hq, is_v = row >= a.Hq + a.Hkv;
-      const int h = is_q ? row : (is_v ? row - a.Hq - a.Hkv : row - a.Hq);
-      if (!is_v) {
-        float x[8] = {};
-        if (in) raw[u].unpack(x);
-        if (is_q ? a.q_weight != nullptr : a.k_weight != nullptr) {
-          float ss = 0.f, weight[8] = {};
-#pragma unroll
-          for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
-#pragma unroll
-          for (int off = 8; off; off >>= 1) ss += __shfl_xor_sync(half_mask, ss, off);
-          const float inv = rsqrtf(ss / float(d) + a.eps);
-          if (in) (is_q ? wq : wk).unpack(weight);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] *= inv * weight[i];
-        }
-        if (a.rot) {
-          float y[8];
-          if (a.interleaved) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = x[i ^ 1];
-          } else {
-            // the partner lies rot/2 columns away, in another lane: through shared memory
-            float* mine = rows[group];
-            __syncwarp(half_mask);
-            *reinterpret_cast<float4*>(mine + gl * 8) = make_float4(x[0], x[1], x[2], x[3]);
-            *reinterpret_cast<float4*>(mine + gl * 8 + 4) = make_float4(x[4], x[5], x[6], x[7]);
-            __syncwarp(half_mask);
-            if ((half & 7) == 0) {       // a lane's eight columns have their partners in one lane
-              const int e = gl * 8 < half ? gl * 8 + half : (gl * 8 < a.rot ? gl * 8 - half : 0);
-              const float4 lo = *reinterpret_cast<const float4*>(mine + e), hi = *reinterpret_cast<const float4*>(mine + e + 4);
-              y[0] = lo.x, y[1] = lo.y, y[2] = lo.z, y[3] = lo.w, y[4] = hi.x, y[5] = hi.y, y[6] = hi.z, y[7] = hi.w;
-            } else {
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const int e = gl * 8 + i;
-                y[i] = e < a.rot ? mine[e < half ? e + half : e - half] : 0.f;
-              }
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (gl * 8 + i < a.rot) x[i] = fmaf(y[i], sn[i], x[i] * cs[i]);
-        }
-        raw[u].pack(x);
-      }
-      if (!in) continue;
-      if (is_q) {
-        raw[u].store(static_cast<T*>(a.q_out) + ((long long)t * a.Hq + h) * d + gl * 8);
-      } else if (here.page >= 0) {
-        T* pool = static_cast<T*>(is_v ? a.v_pages : a.k_pages);
-        const long long at = here.page * (is_v ? a.v_page_stride : a.k_page_stride) + (long long)(h * ps + here.slot) * d;
-        raw[u].store(pool + at + gl * 8);
-        if (is_v && a.weights && gl == 0) a.weights[((long long)here.page * a.Hkv + h) * ps + here.slot] = 0.f;
+    for (int i = 0; i < 8; ++i) {
+      const int e = gl * 8 + i;
+      if (e < a.rot) {
+        const float s = __ldg(st + (e < half ? e : e - half));
+        cs[i] = __ldg(ct + (e < half ? e : e - half));
+        sn[i] = e < half ? -s : s;          // x' = x cos + partner * sn
       }
     }
   }
+  const float inv_d = 1.f / float(d);
+  float* mine = rows[MODE == kExchange ? group : 0];
+  auto weight = [&](const void* p) {
+    Raw<T> r;
+    if (in && p) {
+      r.load(static_cast<const T*>(p), o0, o1);
+      r.unpack(w);
+    }
+  };
+  weight(a.q_weight);
+  T* qo = static_cast<T*>(a.q_out) + (long long)t * a.Hq * d;
+  for (int h0 = sub; h0 < a.Hq; h0 += kAhead * per_token) {
+    if (h0 != sub) fetch_q(h0);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int h = h0 + u * per_token;
+      if (h >= a.Hq) break;
+      float x[8] = {};
+      if (in) rq[u].unpack(x);
+      turn<MODE>(x, a.q_weight != nullptr, w, inv_d, a.eps, cs, sn, half_mask, mine, gl, a.rot);
+      rq[u].pack(x);
+      if (in) rq[u].store(qo + h * d, o0, o1);
+    }
+  }
+  if (here.page < 0) return;
+  weight(a.k_weight);
+  T* ko = static_cast<T*>(a.k_pages) + here.page * a.k_page_stride + here.slot * d;
+  T* vo = static_cast<T*>(a.v_pages) + here.page * a.v_page_stride + here.slot * d;
+  for (int h = sub; h < a.Hkv; h += per_token) {
+    if (in && h != sub) {
+      rk.load(kp + h * a.k_head, o0, o1);
+      rv.load(vp + h * a.v_head, o0, o1);
+    }
+    const int at = h * ps * d;          // Hkv * page_size * d is a page: below 2^31
+    if (in) rv.store(vo + at, o0, o1);
+    float x[8] = {};
+    if (in) rk.unpack(x);
+    turn<MODE>(x, a.k_weight != nullptr, w, inv_d, a.eps, cs, sn, half_mask, mine, gl, a.rot);
+    rk.pack(x);
+    if (in) rk.store(ko + at, o0, o1);
+    if (a.weights && gl == 0) a.weights[((long long)here.page * a.Hkv + h) * ps + here.slot] = 0.f;
+  }
+}
+
+template <class T>
+int launch(int mode, unsigned grid, const AppendArgs& a, const PagedBatch& batch, cudaStream_t st) {
+  switch (mode) {
+    case kNone: paged_append_kernel<T, kNone><<<grid, kThreads, 0, st>>>(a, batch); break;
+    case kInterleaved: paged_append_kernel<T, kInterleaved><<<grid, kThreads, 0, st>>>(a, batch); break;
+    case kHalves: paged_append_kernel<T, kHalves><<<grid, kThreads, 0, st>>>(a, batch); break;
+    default: paged_append_kernel<T, kExchange><<<grid, kThreads, 0, st>>>(a, batch);
+  }
+  CB2_LAUNCH_CHECK();
+  return CB2_OK;
 }
 
 }  // namespace
@@ -235,7 +292,7 @@ extern "C" int cb2_paged_append(const void* q, long long q_token_stride, long lo
   if (page_size < 8 || page_size > 1024 || (page_size & (page_size - 1)) || int64_t(max_pages) * page_size > (1 << 30)) return CB2_BAD_SHAPE;
   if (rotary < 0 || rotary > d || rotary % 2 || (rotary && table_rows < 1) || !(eps >= 0.f)) return CB2_BAD_SHAPE;
   const long long page = (long long)Hkv * page_size * d;
-  if (k_page_stride < page || v_page_stride < page || q_token_stride < 0 || q_head_stride < 0 || k_token_stride < 0 ||
+  if (page >= (1ll << 31) || k_page_stride < page || v_page_stride < page || q_token_stride < 0 || q_head_stride < 0 || k_token_stride < 0 ||
       k_head_stride < 0 || v_token_stride < 0 || v_head_stride < 0)
     return CB2_BAD_SHAPE;
   if (dtype != CB2_BF16 && dtype != CB2_F32) return CB2_UNSUPPORTED_DTYPE;
@@ -258,10 +315,6 @@ extern "C" int cb2_paged_append(const void* q, long long q_token_stride, long lo
   while (a.tokens_per_cta < 4 && n_tokens / (2 * a.tokens_per_cta) >= 2 * kNumSMs) a.tokens_per_cta *= 2;
   const unsigned grid = unsigned((n_tokens + a.tokens_per_cta - 1) / a.tokens_per_cta);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == CB2_BF16)
-    paged_append_kernel<__nv_bfloat16><<<grid, kThreads, 0, st>>>(a, batch);
-  else
-    paged_append_kernel<float><<<grid, kThreads, 0, st>>>(a, batch);
-  CB2_LAUNCH_CHECK();
-  return CB2_OK;
+  const int mode = !rotary ? kNone : interleaved ? kInterleaved : rotary == d ? kHalves : kExchange;
+  return dtype == CB2_BF16 ? launch<__nv_bfloat16>(mode, grid, a, batch, st) : launch<float>(mode, grid, a, batch, st);
 }
