@@ -715,8 +715,10 @@ def _raw_stream(dev: int) -> int:
 
 
 def _no_grad_asked(what: str, *tensors: torch.Tensor | None) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise B200Error(f"{what} serves a cache and has no gradient: call it under torch.no_grad()")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise B200Error(f"{what} serves a cache and has no gradient: call it under torch.no_grad()")
 
 
 def _pools(what: str, dev: int, k_pages: torch.Tensor, v_pages: torch.Tensor) -> tuple[int, int, int, int, int, int]:
@@ -736,11 +738,11 @@ def _pools(what: str, dev: int, k_pages: torch.Tensor, v_pages: torch.Tensor) ->
     return n, hkv, ps, d, strides[0], strides[1]
 
 
-def _dense(what: str, dev: int, name: str, t: torch.Tensor, dtype: torch.dtype, *shape: int) -> int:
+def _dense(what: str, dev: int, name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple) -> int:
     """Address of a contiguous tensor of this shape and type on the current device."""
     if not isinstance(t, torch.Tensor) or t.get_device() != dev:
         _here(what, dev, t)
-    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous():
+    if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
         raise B200Error(f"{what}: {name} is a contiguous {dtype} {list(shape)}, got {t.dtype} {list(t.shape)}")
     return t.data_ptr()
 
@@ -750,24 +752,27 @@ def _ragged_batch(what: str, dev: int, block_table: torch.Tensor, seq_lens: torc
     if block_table.dim() != 2 or 0 in block_table.shape:
         raise B200Error(f"{what}: block_table is int32 [R, max_pages]")
     R, max_pages = block_table.shape
-    return (R, max_pages, _dense(what, dev, "block_table", block_table, torch.int32, R, max_pages),
-            _dense(what, dev, "seq_lens", seq_lens, torch.int32, R), _dense(what, dev, "cu_q", cu_q, torch.int32, R + 1))
+    return (R, max_pages, _dense(what, dev, "block_table", block_table, torch.int32, (R, max_pages)),
+            _dense(what, dev, "seq_lens", seq_lens, torch.int32, (R,)), _dense(what, dev, "cu_q", cu_q, torch.int32, (R + 1,)))
 
 
-def _token_rows(t: torch.Tensor) -> torch.Tensor:
-    """``t`` ``[n_tokens, heads, d]`` as the kernels read it: 16-byte steps between heads and tokens (a view
-    that has them is read in place)."""
+def _token_rows(t: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
+    """``t`` ``[n_tokens, heads, d]`` as the kernels read it, 16-byte steps between heads and tokens (a view that has
+    them is read in place), its address and its token and head strides."""
     unit = 16 // t.element_size()
     st, sh, sd = t.stride()
-    if t.numel() and (sd != 1 or st % unit or sh % unit or st == 0 or sh == 0 or t.data_ptr() % 16):
-        return t.clone(memory_format=torch.contiguous_format)
-    return t
+    ptr = t.data_ptr()
+    if (sd != 1 or st % unit or sh % unit or st == 0 or sh == 0 or ptr % 16) and t.numel():
+        t = t.clone(memory_format=torch.contiguous_format)
+        st, sh, _ = t.stride()
+        ptr = t.data_ptr()
+    return t, ptr, st, sh
 
 
 def _dense_out(what: str, dev: int, out: torch.Tensor | None, q: torch.Tensor) -> torch.Tensor:
     if out is None:
         return torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    _dense(what, dev, "out", out, q.dtype, *q.shape)
+    _dense(what, dev, "out", out, q.dtype, q.shape)
     return out
 
 
@@ -796,9 +801,9 @@ def paged_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_pag
     n = k.shape[0] if k.dim() == 3 else -1
     if n < 0 or k.shape[1] != hkv or k.shape[2] != d or v.shape != k.shape or k.dtype != dt or v.dtype != dt:
         raise B200Error(f"{what}: k and v are [n_tokens, {hkv}, {d}] of the pools' dtype")
-    w_ptr = None if weights is None else _dense(what, dev, "weights", weights, torch.float32, n_pages, hkv, ps)
-    qw = None if q_weight is None else _dense(what, dev, "q_weight", q_weight, dt, d)
-    kw = None if k_weight is None else _dense(what, dev, "k_weight", k_weight, dt, d)
+    w_ptr = None if weights is None else _dense(what, dev, "weights", weights, torch.float32, (n_pages, hkv, ps))
+    qw = None if q_weight is None else _dense(what, dev, "q_weight", q_weight, dt, (d,))
+    kw = None if k_weight is None else _dense(what, dev, "k_weight", k_weight, dt, (d,))
     rotary = rows = 0
     cos_ptr = sin_ptr = pos_ptr = None
     if cos is not None or sin is not None or positions is not None:
@@ -808,9 +813,9 @@ def paged_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_pag
             raise B200Error(f"{what}: cos and sin are float32 [rows, rotary/2], rotary <= {d}")
         rows, half = cos.shape
         rotary = 2 * half
-        cos_ptr = _dense(what, dev, "cos", cos, torch.float32, rows, half)
-        sin_ptr = _dense(what, dev, "sin", sin, torch.float32, rows, half)
-        pos_ptr = _dense(what, dev, "positions", positions, torch.int32, n)
+        cos_ptr = _dense(what, dev, "cos", cos, torch.float32, (rows, half))
+        sin_ptr = _dense(what, dev, "sin", sin, torch.float32, (rows, half))
+        pos_ptr = _dense(what, dev, "positions", positions, torch.int32, (n,))
     _no_grad_asked(what, q, k, v, q_weight, k_weight, cos, sin)
     res, hq, q_args = None, 0, (None, 0, 0)
     if q is not None:
@@ -819,12 +824,11 @@ def paged_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_pag
             raise B200Error(f"{what}: q is [n_tokens, Hq, {d}] of the dtype of k")
         hq = q.shape[1]
         res = _dense_out(what, dev, out, q)
-        q = _token_rows(q)
-        q_args = (q.data_ptr(), q.stride(0), q.stride(1))
-    k, v = _token_rows(k), _token_rows(v)
+        q, *q_args = _token_rows(q)
+    k, *k_args = _token_rows(k)
+    v, *v_args = _token_rows(v)
     rc = _lib.load().cb2_paged_append(
-        *q_args, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-        None if res is None else res.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, w_ptr, table, lens, cu, pos_ptr,
+        *q_args, *k_args, *v_args, None if res is None else res.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, w_ptr, table, lens, cu, pos_ptr,
         qw, kw, eps, cos_ptr, sin_ptr, rows, rotary, 1 if interleaved else 0, n, R, hq, hkv, d, ps, n_pages, max_pages,
         dtype_code(dt), _status_ptr(what, dev), _raw_stream(dev))
     check(rc, "cb2_paged_append")
@@ -853,11 +857,11 @@ def om_paged_fwd(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     dt = q.dtype
     if q.dim() != 3 or q.shape[2] != d or dt != k_pages.dtype or q.shape[1] == 0 or q.shape[1] % hkv:
         raise B200Error(f"{what}: q is [n_tokens, Hq, {d}] of the pools' dtype, Hq a multiple of {hkv}")
-    w_ptr = None if weights is None else _dense(what, dev, "weights", weights, torch.float32, n_pages, hkv, ps)
+    w_ptr = None if weights is None else _dense(what, dev, "weights", weights, torch.float32, (n_pages, hkv, ps))
     _no_grad_asked(what, q, k_pages, v_pages)
     res = _dense_out(what, dev, out, q)
-    q = _token_rows(q)
-    n, hq = q.shape[0], q.shape[1]
+    q, *q_args = _token_rows(q)
+    n, hq, _ = q.shape
     max_q = _bound(what, "max_q", max_q, (1 << 31) - 1)
     max_k = _bound(what, "max_k", max_pages * ps if max_k is None else max_k, min(max_pages * ps, 1 << 30))
     code = dtype_code(dt)
@@ -865,7 +869,7 @@ def om_paged_fwd(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     need = lib.cb2_om_paged_scratch_bytes(n, R, hq, hkv, d, max_q, max_k, 0 if weights is None else 1, code)
     # a buffer of its own for every call: two captured graphs, or two streams, never share one
     scratch = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)
-    rc = lib.cb2_om_paged_fwd(q.data_ptr(), q.stride(0), q.stride(1), k_pages.data_ptr(), v_pages.data_ptr(), ks, vs,
+    rc = lib.cb2_om_paged_fwd(*q_args, k_pages.data_ptr(), v_pages.data_ptr(), ks, vs,
                               res.data_ptr(), w_ptr, table, lens, cu, n, R, hq, hkv, d, ps, n_pages, max_pages, max_q, max_k,
                               d ** -0.5 if scale is None else scale, 1 if causal else 0, code, scratch.data_ptr(), need,
                               _status_ptr(what, dev), _raw_stream(dev))
@@ -890,10 +894,10 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, weights: torch.Ten
         raise B200Error(f"{what}: block_table and new_table are int32 [R, pages]")
     R, max_pages = block_table.shape
     new_pages = new_table.shape[1]
-    table = _dense(what, dev, "block_table", block_table, torch.int32, R, max_pages)
-    lens = _dense(what, dev, "seq_lens", seq_lens, torch.int32, R)
-    to = _dense(what, dev, "new_table", new_table, torch.int32, R, new_pages)
-    w_ptr = _dense(what, dev, "weights", weights, torch.float32, n_pages, hkv, ps)
+    table = _dense(what, dev, "block_table", block_table, torch.int32, (R, max_pages))
+    lens = _dense(what, dev, "seq_lens", seq_lens, torch.int32, (R,))
+    to = _dense(what, dev, "new_table", new_table, torch.int32, (R, new_pages))
+    w_ptr = _dense(what, dev, "weights", weights, torch.float32, (n_pages, hkv, ps))
     _no_grad_asked(what, k_pages, v_pages, weights)
     max_k = _bound(what, "max_k", max_pages * ps if max_k is None else max_k, min(max_pages * ps, 1 << 30))
     keep_first, keep_last = (_bound(what, name, x, budget) for name, x in (("keep_first", keep_first), ("keep_last", keep_last)))

@@ -415,8 +415,8 @@ int cb2_om_bias_step(const void* q, const void* k, const void* v, const float* b
  * [R]) and the pages block_table[r][0 .. ceil(seq_lens[r] / page_size)) (int32
  * [R, max_pages]; later entries are not read).  Key slot j is row j % page_size of page
  * block_table[r][j / page_size]; new token i takes slot seq_lens[r] - n_r + i.  A request
- * without new tokens takes no part in append and attention.  Rows of q behind cu_q[R] are
- * not read and the rows of the outputs there not written.
+ * without new tokens takes no part in append and attention.  Rows of q, k and v behind
+ * cu_q[R] have no effect, and the rows of the outputs there are not written.
  * All index tensors are device memory and are read by the kernels, so a captured graph
  * follows them.  A length, offset, position or page id out of range leads to no access out
  * of bounds: it is clamped or skipped, the outputs of that request are then unspecified, and
