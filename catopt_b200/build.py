@@ -37,6 +37,7 @@ SOURCES = [
     "om_paged.cu",
     "om_paged_tc.cu",
     "om_paged_few.cu",
+    "om_paged_fma.cu",
     "om_paged_weights.cu",
     "paged_append.cu",
     "paged_evict.cu",

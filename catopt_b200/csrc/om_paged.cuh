@@ -116,8 +116,8 @@ __device__ __forceinline__ long long stair_sum(unsigned n, unsigned m, unsigned 
   return lattice_sum(n, m, a, b);
 }
 
-// The requests that a kernel takes: all of them, those with at most `few` packed rows, or the others.
-enum { kPagedAll = 0, kPagedFew = 1, kPagedChunk = 2 };
+// The requests that a kernel takes: those with at most `few` packed rows, or the others.
+enum { kPagedFew, kPagedChunk };
 
 // OV: what starting and ending a unit costs, in blocks; a unit takes OV + blocks of the line.
 template <int RT, int KB, int OV>
@@ -127,7 +127,7 @@ struct PagedCost {
   int min_blocks;          // a share holds at least so many: fewer CTAs work on a short line
   __device__ __forceinline__ bool takes(const PagedReq& q) const {
     if (q.n == 0) return false;
-    return which == kPagedAll || (which == kPagedFew) == (q.n * G <= few);
+    return (which == kPagedFew) == (q.n * G <= few);
   }
   __device__ __forceinline__ int tiles(const PagedReq& q) const { return (q.n * G + RT - 1) / RT; }
   __device__ __forceinline__ int all_blocks(const PagedReq& q) const { return max(1, (q.len + KB - 1) / KB); }
@@ -361,5 +361,12 @@ int paged_few_weights_run(const PagedRows& rows, const PagedBatch& batch, int ca
 size_t paged_weights_tc_scratch_bytes();
 int paged_weights_tc_run(const PagedRows& rows, const PagedPools& pools, const PagedBatch& batch, int causal, int which, int few,
                          const float* lse2, float* weights, void* scratch, cudaStream_t st);
+
+// om_paged_fma.cu: fp32.  Row tiles of rt = 8, 16 or 64; scores as for the streaming kernel.
+size_t paged_fma_scratch_bytes(int rt, int d);
+int paged_fma_run(int rt, const PagedRows& rows, const PagedPools& pools, const PagedBatch& batch, int causal, int which, int few,
+                  float* o, float* lse2, float* kept_scores, void* scratch, PagedScratch* parts, int* n_cta, cudaStream_t st);
+int paged_weights_fma_run(const PagedRows& rows, const PagedPools& pools, const PagedBatch& batch, int causal, int which, int few,
+                          const float* lse2, float* weights, cudaStream_t st);
 
 }  // namespace cb2

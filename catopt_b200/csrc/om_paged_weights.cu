@@ -37,7 +37,7 @@ struct KeyCost {
   int T, per_token;         // tokens a row tile, row tiles a token: one of them is 1
   __device__ __forceinline__ bool takes(const PagedReq& q) const {
     if (q.n == 0 || q.len == 0) return false;
-    return which == kPagedAll || (which == kPagedFew) == (q.n * G <= few);
+    return (which == kPagedFew) == (q.n * G <= few);
   }
   __device__ __forceinline__ int row_tiles(const PagedReq& q) const { return (q.n + T - 1) / T * per_token; }
   __device__ __forceinline__ int first_row_tile(const PagedReq& q, int i) const {
