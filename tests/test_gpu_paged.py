@@ -292,3 +292,145 @@ def test_evict(dev, dtype, lens, budget, first, last, kv, d, page):
     bits = {2: torch.int16, 4: torch.int32}
     for got, exp in zip((c["k"], c["v"], w), want):
         assert torch.equal(got.view(bits[got.element_size()]), exp.view(bits[exp.element_size()]))
+
+
+# --------------------------------------------------------------------------- together
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+def test_decode_loop(dev, dtype):
+    """Prompts in chunks, single tokens, an eviction, more tokens, a request that ends and one that begins: every output
+    against 64-bit attention over lists of keys kept beside the cache."""
+    from catopt_b200 import ops
+    from catopt_b200.paged import PagedCache
+
+    kv, group, d, layers = 2, 4, 64, 2
+    hq = kv * group
+    g = torch.Generator(device=dev).manual_seed(77)
+    cache = PagedCache(layers, 64, 16, kv, d, dtype=dtype, device=dev, track_weights=True)
+    ang = torch.arange(400, device=dev, dtype=torch.float64)[:, None] * 10000.0 ** (-torch.arange(d // 2, device=dev, dtype=torch.float64) / (d // 2))
+    cos, sin = ang.cos().float(), ang.sin().float()
+    qw, kw = ((1 + 0.1 * torch.randn(d, generator=g, device=dev)).to(dtype) for _ in range(2))
+    kept_keys = {}       # (request, layer, head) -> [keys], [values], [weights] in 64 bits
+
+    def step(new):
+        batch = cache.begin(new)
+        n = sum(new.values())
+        for layer in range(layers):
+            x = torch.randn(n, hq + 2 * kv, d, generator=g, device=dev).to(dtype)
+            q, k, v = x[:, :hq], x[:, hq:hq + kv], x[:, hq + kv:]
+            qq = cache.append(layer, batch, q, k, v, q_weight=qw, k_weight=kw, cos=cos, sin=sin)
+            o = cache.attend(layer, batch, qq)
+            want_q, tol_q = ref.turned(q, qw, 1e-6, cos, sin, batch.positions, False)
+            close(qq, want_q, tol_q, "q")
+            want_k, _ = ref.turned(k, kw, 1e-6, cos, sin, batch.positions, False)
+            want_k = want_k.to(dtype).double()          # what a cache of this type holds
+            at = 0
+            for r, m in new.items():
+                for h in range(kv):
+                    ks, vs, ws = kept_keys.setdefault((r, layer, h), ([], [], []))
+                    ks += list(want_k[at:at + m, h])
+                    vs += list(v[at:at + m, h].double())
+                    ws += [0.0] * m
+                    if not m:
+                        continue
+                    K, V = torch.stack(ks), torch.stack(vs)
+                    s = torch.einsum("tgd,jd->gtj", qq[at:at + m, h * group:(h + 1) * group].double(), K) * d ** -0.5
+                    t = len(ks) - m + torch.arange(m, device=dev)
+                    s = s.masked_fill(torch.arange(len(ks), device=dev)[None, None] > t[None, :, None], float("-inf"))
+                    p = torch.softmax(s, -1)
+                    want = torch.einsum("gtj,jd->tgd", p, V)
+                    spread = torch.einsum("gtj,jd->tgd", p, V.abs())
+                    # a cached key may be one step of the type off its 64-bit rounding: 2 half steps of each score, 8 of
+                    # which in magnitude are at most the sums below
+                    dot = torch.einsum("tgd,jd->tgj", qq[at:at + m, h * group:(h + 1) * group].double().abs(), K.abs()).amax(-1, keepdim=True) * d ** -0.5
+                    rel = 2 * dot * (2 * ref.half_step(dtype) + (d + 4) * ref.U32) + 2.0 ** -20
+                    close(o[at:at + m, h * group:(h + 1) * group], want, spread * (rel + 2 * ref.half_step(dtype)) + 1e-6, "o")
+                    ws[:] = (torch.tensor(ws, dtype=torch.float64, device=dev) + p.sum((0, 1))).tolist()
+                at += m
+
+    a, b = cache.open(), cache.open()
+    step({a: 37, b: 90})
+    step({b: 33, a: 1})
+    for _ in range(3):
+        step({a: 1, b: 1})
+    kept = cache.evict([a, b], 48, keep_first=2, keep_last=8)
+    assert cache.length(a) == 41 and cache.length(b) == 48 and cache.position(b) == 126
+    for layer in range(layers):
+        for h in range(kv):
+            ks, vs, ws = kept_keys[b, layer, h]
+            j = kept[layer][0, h].tolist()
+            out = [i for i in range(len(ks)) if i not in j]
+            assert j[:2] == [0, 1] and j[-8:] == list(range(118, 126)) and j == sorted(j) and len(set(j)) == 48
+            # the lightest kept key is not lighter than the heaviest evicted one, up to the rounding of the sums
+            assert min(ws[i] for i in j[2:-8]) >= max(ws[i] for i in out) * (1 - (2.0 ** -4 if dtype == BF else 2.0 ** -12))
+            kept_keys[b, layer, h] = [ks[i] for i in j], [vs[i] for i in j], [ws[i] for i in j]
+    step({a: 1, b: 1})
+    step({b: 20, a: 3})
+    cache.close(a)
+    c = cache.open()
+    step({c: 50, b: 1})
+    step({c: 0, b: 2})
+    ops.check_device_status(dev)
+
+
+def test_calls_on_two_streams(dev):
+    """Calls on different streams share nothing; tensors of another stream's making are ordered by the caller."""
+    from catopt_b200 import ops
+
+    c = ref.make_cache([1500, 700], 2, 16, 64, BF, dev, 9)
+    cu = ref.offsets([1, 120], dev)
+    qs = [torch.randn(121, 8, 64, device=dev).to(BF) for _ in range(2)]
+    want = [ops.om_paged_fwd(q, c["k"], c["v"], c["table"], c["lens"], cu, 120) for q in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(20):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(ops.om_paged_fwd(qs[i], c["k"], c["v"], c["table"], c["lens"], cu, 120))
+    torch.cuda.synchronize()
+    ops.check_device_status(dev)
+    assert all(torch.equal(o, want[i]) for i in range(2) for o in got[i])
+
+
+def test_gradients_are_refused(dev):
+    from catopt_b200 import B200Error, ops
+
+    c = ref.make_cache([20], 1, 16, 64, BF, dev, 10)
+    cu = ref.offsets([1], dev)
+    q = torch.randn(1, 2, 64, device=dev).to(BF).requires_grad_()
+    with pytest.raises(B200Error, match="no_grad"):
+        ops.om_paged_fwd(q, c["k"], c["v"], c["table"], c["lens"], cu, 1)
+    with torch.no_grad():
+        ops.om_paged_fwd(q, c["k"], c["v"], c["table"], c["lens"], cu, 1)
+    k = torch.randn(1, 1, 64, device=dev).to(BF)
+    with pytest.raises(B200Error, match="no_grad"):
+        ops.paged_append(q, k, k, c["k"], c["v"], c["table"], c["lens"], cu)
+
+
+def test_wrong_arguments_are_refused(dev):
+    from catopt_b200 import B200Error, ops
+
+    c = ref.make_cache([20, 9], 2, 16, 64, BF, dev, 12)
+    cu = ref.offsets([1, 1], dev)
+    q = torch.randn(2, 4, 64, device=dev).to(BF)
+    k = torch.randn(2, 2, 64, device=dev).to(BF)
+    ok = dict(q=q, k_pages=c["k"], v_pages=c["v"], block_table=c["table"], seq_lens=c["lens"], cu_q=cu, max_q=1)
+    ops.om_paged_fwd(**ok)
+    for bad in (dict(q=q[:, :3]), dict(q=q.float()), dict(q=q[..., :32]), dict(v_pages=c["v"][:-1]), dict(k_pages=c["k"].transpose(1, 2)),
+                dict(block_table=c["table"].long()), dict(seq_lens=c["lens"][:1]), dict(cu_q=cu[:2]), dict(max_k=1 << 20), dict(max_q=-1),
+                dict(scale=-1.0), dict(weights=torch.zeros(3, device=dev)), dict(out=torch.empty_like(q).float()), dict(seq_lens=c["lens"].cpu())):
+        with pytest.raises(B200Error):
+            ops.om_paged_fwd(**{**ok, **bad})
+    ok = dict(q=q, k=k, v=k, k_pages=c["k"], v_pages=c["v"], block_table=c["table"], seq_lens=c["lens"], cu_q=cu)
+    table = torch.zeros(8, 16, device=dev)
+    for bad in (dict(k=k[:1]), dict(v=k.float()), dict(q=q[:1]), dict(cos=table), dict(cos=table, sin=table), dict(q_weight=torch.ones(64, device=dev)),
+                dict(cos=table, sin=table, positions=torch.zeros(3, dtype=torch.int32, device=dev)), dict(eps=-1.0),
+                dict(cos=table.repeat(1, 4), sin=table.repeat(1, 4), positions=cu[:2])):
+        with pytest.raises(B200Error):
+            ops.paged_append(**{**ok, **bad})
+    w = torch.zeros(c["k"].shape[:3], device=dev)
+    to = torch.zeros(2, 1, dtype=torch.int32, device=dev)
+    for bad in (dict(budget=17), dict(budget=0), dict(budget=8, keep_first=9), dict(budget=8, keep_first=4, keep_last=5), dict(budget=8, max_k=1 << 20)):
+        with pytest.raises(B200Error):
+            ops.paged_evict(c["k"], c["v"], w, c["table"], c["lens"], to, **bad)
+    ops.check_device_status(dev)

@@ -75,3 +75,55 @@ def test_host_tensors_are_refused():
         ops.paged_append(None, torch.zeros(1, 2, 64), torch.zeros(1, 2, 64), pool, pool, i, i[0], torch.zeros(2, dtype=torch.int32))
     with pytest.raises(B200Error):
         ops.paged_evict(pool, pool, pool[..., 0], i, i[0], i, 4)
+
+
+# --------------------------------------------------------------------------- the cache's bookkeeping
+def make(**kw):
+    from catopt_b200.paged import PagedCache
+
+    return PagedCache(**{**dict(n_layers=1, n_pages=10, page_size=8, n_kv_heads=1, head_dim=8, device="cpu", track_weights=True), **kw})
+
+
+def test_cache_hands_out_and_takes_back_pages():
+    from catopt_b200 import B200Error
+
+    c = make()
+    a, b = c.open(), c.open()
+    s = c.begin({a: 9, b: 0})
+    assert s.table.tolist()[0][:2] == [0, 1] and s.table.tolist()[1] == [-1, -1]
+    assert s.seq_lens.tolist() == [9, 0] and s.cu_q.tolist() == [0, 9, 9] and s.positions.tolist() == list(range(9))
+    assert (s.n_tokens, s.max_q, s.max_k) == (9, 9, 9)
+    s = c.begin({b: 8, a: 7})                        # a's last page still has room, b fills one
+    assert c.free_pages == 7 and s.seq_lens.tolist() == [8, 16]
+    assert s.positions.tolist() == list(range(8)) + list(range(9, 16)) and s.requests == (b, a)
+    with pytest.raises(B200Error, match="pages"):
+        c.begin({a: 8, b: 100})
+    assert c.length(a) == 16 and c.length(b) == 8 and c.free_pages == 7          # nothing has changed
+    used = set(s.table.flatten().tolist()) - {-1}
+    assert len(used) == 3
+    c.close(a)
+    assert c.free_pages == 9
+    with pytest.raises(B200Error, match="not open"):
+        c.begin({a: 1})
+    again = c.begin({c.open(): 72})
+    assert not set(again.table.flatten().tolist()) & set(s.table[0].tolist()[:1])     # b's page stays b's
+    assert c.free_pages == 0
+
+
+def test_cache_refusals():
+    from catopt_b200 import B200Error
+
+    for bad in (dict(page_size=12), dict(page_size=4), dict(head_dim=132), dict(head_dim=12), dict(n_pages=0), dict(dtype=torch.float16)):
+        with pytest.raises(B200Error):
+            make(**bad)
+    c = make()
+    r = c.open()
+    for call in (lambda: c.begin({}), lambda: c.begin({r: -1}), lambda: c.begin({99: 1}), lambda: c.evict([r, r], 4),
+                 lambda: c.evict([r], 0), lambda: c.evict([r], 4, keep_first=3, keep_last=2), lambda: make(track_weights=False).evict([], 4)):
+        with pytest.raises(B200Error):
+            call()
+    assert c.evict([r], 4) == []                     # not longer than the budget: nothing to do
+    c.begin({r: 60})                                 # 8 of 10 pages
+    with pytest.raises(B200Error, match="free"):
+        c.evict([r], 20)                             # the kept keys need 3 fresh ones
+    assert c.length(r) == 60 and c.free_pages == 2
