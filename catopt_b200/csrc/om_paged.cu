@@ -39,6 +39,8 @@ paged_combine_kernel(int rt, const PagedScratch scratch, T* __restrict__ o, floa
   __shared__ float sh_m[kJoinWarps], sh_l[kJoinWarps];
   __shared__ __align__(16) float sh_a[kJoinWarps][128];
   const int c = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  let_next();
+  after_previous();
   const PagedJoin j = scratch.joins[c];
   if (j.r < 0) return;
   const PagedReq q = paged_request(batch, j.r);
@@ -87,6 +89,8 @@ paged_combine_tiles_kernel(const PagedScratch scratch, __nv_bfloat16* __restrict
   __shared__ __align__(16) __nv_bfloat16 sh[32][128 + 8];
   __shared__ long long sh_at[32];
   const int c = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  let_next();
+  after_previous();
   const PagedJoin j = scratch.joins[c];
   if (j.r < 0) return;
   const PagedReq q = paged_request(batch, j.r);
@@ -130,8 +134,13 @@ paged_combine_tiles_kernel(const PagedScratch scratch, __nv_bfloat16* __restrict
 
 size_t up16(size_t n) { return (n + 15) & ~size_t(15); }
 
-// Which kernels a call takes.  A request of at most `few` packed rows is bound by reading its keys and goes to the
-// streaming kernel (bf16: products with 8 or 16 rows; fp32: tiles of 8 or 16 rows), the others go to the wide tiles.
+// Which kernels a call takes.  Requests of at most `few` packed rows are bound by reading their keys: a batch of
+// nothing else goes to the streaming kernel (bf16: products with 8 or 16 rows; fp32: tiles of 8 or 16 rows).  A batch
+// with chunks goes to the wide tiles as a whole in bf16: their line takes single tokens at the pace of memory, too, and
+// the two launches more of the streaming kernel never paid (31 single tokens on up to 16384 keys beside a chunk of 64:
+// 237 us with one kernel, 255 with both; 21 on up to 2048 beside three chunks: 45 and 62).  In fp32 a row that is not
+// there costs as much as one that is, so there the few rows of a mixed batch have the narrow tiles, unless the batch is
+// sure to be small (15 single tokens on up to 4096 keys: 351 us with both, 466 with one; 12 on 512: 75 and 71).
 struct Plan {
   int few;                     // 0: no streaming kernel
   bool chunks;
@@ -150,7 +159,8 @@ Plan plan(int n_tokens, int R, int Hq, int Hkv, int d, int max_q, int max_k, boo
     p.few = rows <= 8 ? 8 : 16;
   } else {
     p.chunks = true;
-    p.few = R == 1 || G > 16 ? 0 : (G <= 8 ? 8 : 16);       // the single tokens of a mixed batch
+    const int64_t blocks = int64_t(R) * Hkv * (1 + (max_k + 63) / 64);
+    if (dtype == CB2_F32 && R > 1 && G <= 16 && blocks > 8 * kNumSMs) p.few = G <= 8 ? 8 : 16;
   }
   p.lse = weights ? up16(size_t(n_tokens) * Hq * 4) : 0;
   if (weights && p.few) {
@@ -174,16 +184,13 @@ Plan plan(int n_tokens, int R, int Hq, int Hkv, int d, int max_q, int max_k, boo
 template <class T>
 int join(int rt, int n_cta, const PagedScratch& ws, T* o, float* lse2, const PagedBatch& batch, const PagedRows& rows, int d,
          cudaStream_t st) {
-  paged_combine_kernel<T><<<dim3(n_cta, (rt + kJoinWarps - 1) / kJoinWarps), kJoinWarps * 32, 0, st>>>(rt, ws, o, lse2, batch, rows.G, rows.Hkv, d);
-  CB2_LAUNCH_CHECK();
-  return CB2_OK;
+  return launch_next(paged_combine_kernel<T>, dim3(n_cta, (rt + kJoinWarps - 1) / kJoinWarps), kJoinWarps * 32, st, rt, ws, o, lse2, batch,
+                     rows.G, rows.Hkv, d);
 }
 
 int join_tiles(int n_cta, const PagedScratch& ws, __nv_bfloat16* o, float* lse2, const PagedBatch& batch, const PagedRows& rows, int d,
                cudaStream_t st) {
-  paged_combine_tiles_kernel<<<dim3(n_cta, kTileRows / 32), kTileWarps * 32, 0, st>>>(ws, o, lse2, batch, rows.G, rows.Hkv, d);
-  CB2_LAUNCH_CHECK();
-  return CB2_OK;
+  return launch_next(paged_combine_tiles_kernel, dim3(n_cta, kTileRows / 32), kTileWarps * 32, st, ws, o, lse2, batch, rows.G, rows.Hkv, d);
 }
 
 int run_f32(const PagedRows& rows, const PagedPools& pools, const PagedBatch& batch, int causal, float* o, float* weights,

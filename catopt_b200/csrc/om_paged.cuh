@@ -14,9 +14,44 @@
 //         (m, l, a) per share, which paged_combine_kernel joins in share order (no atomics: the same
 //         inputs give the same bits).
 #pragma once
+#include <atomic>
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace cb2 {
+
+// Lets a kernel use `bytes` of dynamic shared memory, asked for once per device (`done`: one bit each): a decode step is
+// short enough for the question to show.
+inline bool allow_smem(const void* kernel, int bytes, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const unsigned long long bit = dev < 64 ? 1ull << dev : 0ull;
+  if (done.load(std::memory_order_relaxed) & bit) return true;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return true;
+}
+
+// A kernel that reads what the kernel before it leaves is launched while that one still runs (programmatic dependent
+// launch): it waits with after_previous() at its top, and the one before has called let_next() at its own.  Of a chain, every
+// kernel waits in all of its blocks, so what the last one sees is complete.
+__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <class... Args>
+inline int launch_next(void (*kernel)(Args...), dim3 grid, unsigned threads, cudaStream_t st, std::common_type_t<Args>... args) {
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? CB2_OK : CB2_LAUNCH_FAIL;
+}
 
 // The index tensors of a ragged batch.  Values out of range are clamped where they are read and
 // reported as CB2_BAD_INDEX, so that no index tensor can lead to an access out of bounds.

@@ -69,6 +69,7 @@ paged_few_kernel(const PagedRows rows, const PagedPools pools, const PagedBatch 
   __shared__ float sh_m[kWarps][kRT], sh_l[kWarps][kRT];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int cta = blockIdx.x, n_cta = gridDim.x, d = pools.d, G = rows.G;
+  let_next();
   const PagedShare share = paged_find_share<kThreads>(batch, cost, cta, n_cta, &find);
   if (tid == 0) scratch.joins[cta].r = -1;
   unsigned char* ring = smem + warp * R::kWarpBytes;
@@ -314,6 +315,8 @@ paged_few_weights_kernel(const PagedBatch batch, const Cost cost, const float* _
   __shared__ float sh_lse[kRT];
   const PagedShare share = paged_find_share<kWeightThreads>(batch, cost, blockIdx.x, gridDim.x, &find);
   const int G = cost.G, ps = 1 << batch.page_log2, tid = threadIdx.x;
+  let_next();
+  after_previous();          // (the share comes from index tensors alone)
   for (PagedWalk<Cost> w(batch, cost, share); w.valid(); w.next()) {
     w.clip();
     const float* sc = scores + ((long long)w.r * cost.Hkv + w.h) * cost.few * batch.max_k;
@@ -336,8 +339,8 @@ template <int KS, int NB>
 int launch(const PagedRows& rows, const PagedPools& pools, const PagedBatch& batch, const Cost& cost, __nv_bfloat16* o, float* lse2,
            float* scores, const PagedScratch& ws, cudaStream_t st) {
   constexpr int smem = Ring<KS>::kSmem;
-  if (cudaFuncSetAttribute(paged_few_kernel<KS, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-    return CB2_LAUNCH_FAIL;
+  static std::atomic<unsigned long long> done{0};
+  if (!allow_smem(reinterpret_cast<const void*>(paged_few_kernel<KS, NB>), smem, done)) return CB2_LAUNCH_FAIL;
   paged_few_kernel<KS, NB><<<kCtas, kThreads, smem, st>>>(rows, pools, batch, cost, o, lse2, scores, ws);
   CB2_LAUNCH_CHECK();
   return CB2_OK;
@@ -364,9 +367,7 @@ int paged_few_run(const PagedRows& rows, const PagedPools& pools, const PagedBat
 int paged_few_weights_run(const PagedRows& rows, const PagedBatch& batch, int causal, int few, const float* scores, const float* lse2,
                           float* weights, cudaStream_t st) {
   const Cost cost{rows.G, rows.Hkv, causal, kPagedFew, few, 2};
-  paged_few_weights_kernel<<<kWeightCtas, kWeightThreads, 0, st>>>(batch, cost, scores, lse2, weights);
-  CB2_LAUNCH_CHECK();
-  return CB2_OK;
+  return launch_next(paged_few_weights_kernel, dim3(kWeightCtas), kWeightThreads, st, batch, cost, scores, lse2, weights);
 }
 
 }  // namespace cb2

@@ -84,6 +84,7 @@ paged_fma_kernel(const PagedRows rows, const PagedPools pools, const PagedBatch 
   float* Ps = Vs + 2 * kKB * d;                              // [RT][kLdP]
   float* stat = Ps + RT * kLdP;                              // rescaling of a block, then m and l
   const int cta = blockIdx.x, n_cta = gridDim.x;
+  let_next();
   const PagedShare share = paged_find_share<kThreads>(batch, cost, cta, n_cta, &find);
   if (tid == 0) scratch.joins[cta].r = -1;
   const int ty = tid / KX, tx = tid % KX, cg = tid % CG, rg = tid / CG;
@@ -309,8 +310,8 @@ template <int RT, int CG>
 int launch(const PagedRows& rows, const PagedPools& pools, const PagedBatch& batch, const typename Tile<RT>::Cost& cost, float* o,
            float* lse2, float* kept_scores, const PagedScratch& ws, cudaStream_t st) {
   const int smem = Tile<RT>::smem_bytes(pools.d);
-  if (cudaFuncSetAttribute(paged_fma_kernel<RT, CG>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-    return CB2_LAUNCH_FAIL;
+  static std::atomic<unsigned long long> done{0};
+  if (!allow_smem(reinterpret_cast<const void*>(paged_fma_kernel<RT, CG>), Tile<RT>::smem_bytes(CG * 4), done)) return CB2_LAUNCH_FAIL;
   paged_fma_kernel<RT, CG><<<Tile<RT>::ctas(pools.d), Tile<RT>::kThreads, smem, st>>>(rows, pools, batch, cost, o, lse2, kept_scores, ws);
   CB2_LAUNCH_CHECK();
   return CB2_OK;
@@ -344,7 +345,8 @@ int paged_fma_run(int rt, const PagedRows& rows, const PagedPools& pools, const 
 int paged_weights_fma_run(const PagedRows& rows, const PagedPools& pools, const PagedBatch& batch, int causal, int which, int few,
                           const float* lse2, float* weights, cudaStream_t st) {
   const int ld = pools.d + 4, smem = (kKB * ld + 2 * kWRows * ld + 16 * kKB) * 4;
-  if (cudaFuncSetAttribute(paged_weights_fma_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+  static std::atomic<unsigned long long> done{0};
+  if (!allow_smem(reinterpret_cast<const void*>(paged_weights_fma_kernel), (kKB * 132 + 2 * kWRows * 132 + 16 * kKB) * 4, done))
     return CB2_LAUNCH_FAIL;
   const Tile<64>::Cost cost{rows.G, rows.Hkv, causal, which, few, 1};
   const dim3 grid((batch.max_k + kKB - 1) / kKB, rows.Hkv, batch.R < 256 ? batch.R : 256);

@@ -99,6 +99,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int cta = blockIdx.x, n_cta = gridDim.x;
 
+  let_next();
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&k_full[i], 1);
@@ -478,8 +479,8 @@ int paged_tc_run(const PagedRows& rows, const PagedPools& pools, const PagedBatc
   int rc = paged_pool_map(&mk, pools.k, pools.d, 1 << batch.page_log2, pools.Hkv, batch.n_pages, pools.k_page_stride);
   if (rc == CB2_OK) rc = paged_pool_map(&mv, pools.v, pools.d, 1 << batch.page_log2, pools.Hkv, batch.n_pages, pools.v_page_stride);
   if (rc != CB2_OK) return rc;
-  if (cudaFuncSetAttribute(paged_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmemBytes)) != cudaSuccess)
-    return CB2_LAUNCH_FAIL;
+  static std::atomic<unsigned long long> done{0};
+  if (!allow_smem(reinterpret_cast<const void*>(paged_tc_kernel), kSmemBytes, done)) return CB2_LAUNCH_FAIL;
   *parts = paged_scratch(scratch, kCtas);
   *n_cta = kCtas;
   const TcArgs a{static_cast<const __nv_bfloat16*>(rows.q), rows.q_token, rows.q_head, static_cast<__nv_bfloat16*>(o), lse2,

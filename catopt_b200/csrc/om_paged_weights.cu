@@ -91,6 +91,7 @@ paged_weights_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int cta = blockIdx.x, n_cta = gridDim.x;
 
+  let_next();
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&q_full[i], 33);           // the TMA box and the 32 lanes that write -lse
@@ -333,6 +334,7 @@ __global__ void __launch_bounds__(kKeys)
 paged_weights_join_kernel(const PagedBatch batch, int Hkv, const PagedJoin* __restrict__ joins, const float* __restrict__ parts,
                           float* __restrict__ weights) {
   const int c = blockIdx.x, key = threadIdx.x;
+  after_previous();
   const PagedJoin jn = joins[c];
   if (jn.r < 0) return;
   const int len = min(max(__ldg(batch.lens + jn.r), 0), batch.max_k), j = jn.tile * kKeys + key, ps = 1 << batch.page_log2;
@@ -357,16 +359,15 @@ int paged_weights_tc_run(const PagedRows& rows, const PagedPools& pools, const P
   const long long head = Hq > 1 ? rows.q_head : pools.d, token = batch.n_tokens > 1 ? rows.q_token : (long long)Hq * pools.d;
   if (rc == CB2_OK) rc = umma::make_map_3d_strided(&mq, rows.q, pools.d, Hq, batch.n_tokens, head, token, 64, rows.G < kRows ? rows.G : kRows, T);
   if (rc != CB2_OK) return rc;
-  if (cudaFuncSetAttribute(paged_weights_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmemBytes)) != cudaSuccess)
-    return CB2_LAUNCH_FAIL;
+  static std::atomic<unsigned long long> done{0};
+  if (!allow_smem(reinterpret_cast<const void*>(paged_weights_tc_kernel), kSmemBytes, done)) return CB2_LAUNCH_FAIL;
   const KeyCost cost{rows.G, rows.Hkv, causal, which, few, 4, T, rows.G > kRows ? (rows.G + kRows - 1) / kRows : 1};
   PagedJoin* joins = static_cast<PagedJoin*>(scratch);
   float* parts = reinterpret_cast<float*>(joins + kCtas);
   paged_weights_tc_kernel<<<kCtas, kThreads, kSmemBytes, st>>>(mk, mq, rows, pools.d, batch, cost, lse2, weights, joins, parts);
   CB2_LAUNCH_CHECK();
-  paged_weights_join_kernel<<<kCtas, kKeys, 0, st>>>(batch, rows.Hkv, joins, parts, weights);
-  CB2_LAUNCH_CHECK();
-  return CB2_OK;
+  return launch_next(paged_weights_join_kernel, dim3(kCtas), kKeys, st, batch, rows.Hkv, static_cast<const PagedJoin*>(joins),
+                     static_cast<const float*>(parts), weights);
 }
 
 }  // namespace cb2

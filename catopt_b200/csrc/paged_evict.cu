@@ -62,6 +62,7 @@ paged_select_kernel(const EvictArgs a, const PagedBatch batch) {
   __shared__ uint32_t s_prefix;
   __shared__ int s_need;
   const int h = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  let_next();
   const int l0 = __ldg(batch.lens + r), len = min(max(l0, 0), batch.max_k);
   if (len != l0) paged_flag(batch);
   int* kept = a.kept + ((long long)r * a.Hkv + h) * a.budget;
@@ -166,6 +167,7 @@ paged_move_kernel(const MoveArgs a, const PagedBatch batch) {
   __shared__ long long src[kMoveRows], dst[kMoveRows];    // (page * 2^32 + slot), -1: nothing
   const int r = blockIdx.z, h = blockIdx.y, i0 = blockIdx.x * kMoveRows, tid = threadIdx.x;
   const int ps = 1 << batch.page_log2;
+  after_previous();
   if (tid < kMoveRows) {
     const int i = i0 + tid;
     long long s = -1, t = -1;
@@ -229,13 +231,11 @@ extern "C" int cb2_paged_evict(void* k_pages, void* v_pages, long long k_page_st
   const PagedBatch batch{block_table, seq_lens, nullptr, R, max_pages, n_pages, page_log2, 0, 0, max_k, dev_status};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const EvictArgs e{weights, Hkv, budget, keep_first, keep_last, kept, new_lens, max_k < kMostHeld ? max_k : kMostHeld};
-  if (cudaFuncSetAttribute(paged_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostHeld * 4) != cudaSuccess)
-    return CB2_LAUNCH_FAIL;
+  static std::atomic<unsigned long long> done{0};
+  if (!allow_smem(reinterpret_cast<const void*>(paged_select_kernel), kMostHeld * 4, done)) return CB2_LAUNCH_FAIL;
   paged_select_kernel<<<dim3(Hkv, R), kSelThreads, size_t(e.held) * 4, st>>>(e, batch);
   CB2_LAUNCH_CHECK();
   const MoveArgs m{static_cast<char*>(k_pages), static_cast<char*>(v_pages), k_page_stride * esz, v_page_stride * esz, weights,
                    kept, new_table, new_pages, Hkv, budget, d * esz};
-  paged_move_kernel<<<dim3((budget + kMoveRows - 1) / kMoveRows, Hkv, R), kMoveThreads, 0, st>>>(m, batch);
-  CB2_LAUNCH_CHECK();
-  return CB2_OK;
+  return launch_next(paged_move_kernel, dim3((budget + kMoveRows - 1) / kMoveRows, Hkv, R), kMoveThreads, st, m, batch);
 }

@@ -10,6 +10,7 @@ one stream do, which stream order makes safe.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import torch
 
@@ -789,7 +790,7 @@ def paged_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_pag
     ``cu_q[r]:cu_q[r+1]`` and take its slots ``seq_lens[r] - n_r ..`` (``seq_lens`` counts them already), slot j
     being row ``j % page_size`` of page ``block_table[r, j // page_size]`` of the pools ``[n_pages, Hkv, page_size,
     d]``.  ``q_weight``/``k_weight [d]``: root-mean-square norm of each head; ``cos``/``sin`` float32 ``[rows,
-    rotary/2]`` with ``positions`` int32 ``[n]``: rotation of the first ``rotary`` columns in pairs ``(i, i +
+    rotary/2]`` with ``positions`` int32 ``[n]`` (read only then): rotation of the first ``rotary`` columns in pairs ``(i, i +
     rotary/2)``, or ``(2i, 2i+1)`` if ``interleaved``.  ``weights`` (float32 ``[n_pages, Hkv, page_size]``) is
     zeroed at the new slots.  Returns the normed and rotated ``q`` (rows behind ``cu_q[R]`` are not written)."""
     what = "paged_append"
@@ -806,7 +807,7 @@ def paged_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_pag
     kw = None if k_weight is None else _dense(what, dev, "k_weight", k_weight, dt, (d,))
     rotary = rows = 0
     cos_ptr = sin_ptr = pos_ptr = None
-    if cos is not None or sin is not None or positions is not None:
+    if cos is not None or sin is not None:
         if cos is None or sin is None or positions is None:
             raise B200Error(f"{what}: rotation takes cos, sin and positions")
         if cos.dim() != 2 or 0 in cos.shape or 2 * cos.shape[1] > d:
@@ -833,6 +834,11 @@ def paged_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_pag
         dtype_code(dt), _status_ptr(what, dev), _raw_stream(dev))
     check(rc, "cb2_paged_append")
     return res
+
+
+@functools.lru_cache(maxsize=4096)
+def _paged_scratch_bytes(*sizes: int) -> int:
+    return _lib.load().cb2_om_paged_scratch_bytes(*sizes)
 
 
 def om_paged_fwd(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
@@ -866,7 +872,7 @@ def om_paged_fwd(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     max_k = _bound(what, "max_k", max_pages * ps if max_k is None else max_k, min(max_pages * ps, 1 << 30))
     code = dtype_code(dt)
     lib = _lib.load()
-    need = lib.cb2_om_paged_scratch_bytes(n, R, hq, hkv, d, max_q, max_k, 0 if weights is None else 1, code)
+    need = _paged_scratch_bytes(n, R, hq, hkv, d, max_q, max_k, 0 if weights is None else 1, code)
     # a buffer of its own for every call: two captured graphs, or two streams, never share one
     scratch = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)
     rc = lib.cb2_om_paged_fwd(*q_args, k_pages.data_ptr(), v_pages.data_ptr(), ks, vs,

@@ -79,6 +79,12 @@ def test_attention_work_cut_over_keys(dev, dtype, new, lens, kv, group):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+def test_chunk_beside_many_single_tokens(dev, dtype):
+    # enough keys for both kernels of a mixed batch in fp32
+    run_attend(dev, [40] + [1] * 30 + [5], [400 + 7 * i for i in range(32)], 8, 2, 64, 16, dtype, weights=True)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("group", [20, 72, 128])
 def test_many_heads_on_one(dev, dtype, group):
     run_attend(dev, [1, 0, 7, 40], [300, 5, 200, 150], 1 if group > 20 else 2, group, 64, 16, dtype, weights=True)
