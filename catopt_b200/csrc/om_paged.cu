@@ -34,8 +34,7 @@ struct Carrier {
 
 template <class T>
 __global__ void __launch_bounds__(kJoinWarps * 32)
-paged_combine_kernel(int rt, const PagedScratch scratch, T* __restrict__ o, float* __restrict__ lse2, const PagedBatch batch, int G,
-                     int Hkv, int d) {
+paged_combine_kernel(int rt, const PagedScratch scratch, T* __restrict__ o, float* __restrict__ lse2, int G, int Hkv, int d) {
   __shared__ float sh_m[kJoinWarps], sh_l[kJoinWarps];
   __shared__ __align__(16) float sh_a[kJoinWarps][128];
   const int c = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -43,8 +42,7 @@ paged_combine_kernel(int rt, const PagedScratch scratch, T* __restrict__ o, floa
   after_previous();
   const PagedJoin j = scratch.joins[c];
   if (j.r < 0) return;
-  const PagedReq q = paged_request(batch, j.r);
-  const int in_tile = blockIdx.y * kJoinWarps, row_first = j.tile * rt + in_tile, n_rows = min(kJoinWarps, q.n * G - row_first);
+  const int in_tile = blockIdx.y * kJoinWarps, row_first = j.tile * rt + in_tile, n_rows = min(kJoinWarps, j.n * G - row_first);
   if (n_rows <= 0) return;
   int stride = 1;                                        // warps a row
   while (stride * 2 * n_rows <= kJoinWarps) stride *= 2;
@@ -53,7 +51,7 @@ paged_combine_kernel(int rt, const PagedScratch scratch, T* __restrict__ o, floa
   Carrier x{-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
   if (rr < n_rows) {
     const float* base = scratch.parts + in_tile + rr;
-#pragma unroll 4
+#pragma unroll 8
     for (int s = c + part; s <= j.last; s += stride) {
       const float* p = base + slot * (2 * s + (s == c));
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -74,7 +72,7 @@ paged_combine_kernel(int rt, const PagedScratch scratch, T* __restrict__ o, floa
   if (rr >= n_rows) return;
   const int row = row_first + rr;
   const float inv = x.l > 0.f ? 1.f / x.l : 0.f;
-  const long long at = (long long)(q.t0 + row / G) * (G * Hkv) + j.h * G + row % G;
+  const long long at = (long long)(j.t0 + row / G) * (G * Hkv) + j.h * G + row % G;
   if (col < d) store4(o + at * d + col, make_float4(x.a.x * inv, x.a.y * inv, x.a.z * inv, x.a.w * inv));
   if (lse2 && lane == 0) lse2[at] = x.l > 0.f ? x.m + log2f(x.l) : INFINITY;
 }
@@ -84,8 +82,7 @@ paged_combine_kernel(int rt, const PagedScratch scratch, T* __restrict__ o, floa
 constexpr int kTileRows = 128, kTileWarps = 8;
 
 __global__ void __launch_bounds__(kTileWarps * 32)
-paged_combine_tiles_kernel(const PagedScratch scratch, __nv_bfloat16* __restrict__ o, float* __restrict__ lse2, const PagedBatch batch,
-                           int G, int Hkv, int d) {
+paged_combine_tiles_kernel(const PagedScratch scratch, __nv_bfloat16* __restrict__ o, float* __restrict__ lse2, int G, int Hkv, int d) {
   __shared__ __align__(16) __nv_bfloat16 sh[32][128 + 8];
   __shared__ long long sh_at[32];
   const int c = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -93,9 +90,8 @@ paged_combine_tiles_kernel(const PagedScratch scratch, __nv_bfloat16* __restrict
   after_previous();
   const PagedJoin j = scratch.joins[c];
   if (j.r < 0) return;
-  const PagedReq q = paged_request(batch, j.r);
   const int in_tile = blockIdx.y * 32 + lane, row = j.tile * kTileRows + in_tile;
-  const int n_rows = min(32, q.n * G - j.tile * kTileRows - int(blockIdx.y) * 32);
+  const int n_rows = min(32, j.n * G - j.tile * kTileRows - int(blockIdx.y) * 32);
   if (n_rows <= 0) return;
   const size_t slot = paged_slot_floats(kTileRows, d);
   constexpr int kGroups = 128 / 4 / kTileWarps;
@@ -121,7 +117,7 @@ paged_combine_tiles_kernel(const PagedScratch scratch, __nv_bfloat16* __restrict
     for (int k = 0; k < kGroups; ++k)
       store4(&sh[lane][(warp + k * kTileWarps) * 4], make_float4(x[k].a.x * inv, x[k].a.y * inv, x[k].a.z * inv, x[k].a.w * inv));
     if (warp == 0) {
-      const long long at = (long long)(q.t0 + row / G) * (G * Hkv) + j.h * G + row % G;
+      const long long at = (long long)(j.t0 + row / G) * (G * Hkv) + j.h * G + row % G;
       sh_at[lane] = at;
       if (lse2) lse2[at] = x[0].l > 0.f ? x[0].m + log2f(x[0].l) : INFINITY;
     }
@@ -164,7 +160,7 @@ Plan plan(int n_tokens, int R, int Hq, int Hkv, int d, int max_q, int max_k, boo
   }
   p.lse = weights ? up16(size_t(n_tokens) * Hq * 4) : 0;
   if (weights && p.few) {
-    const size_t s = size_t(R) * Hkv * p.few * max_k * 4;
+    const size_t s = size_t(R) * Hkv * p.few * paged_score_stride(max_k) * 4;
     p.scores = s <= kMostScores ? up16(s) : 0;
   }
   auto at_least = [&p](size_t n) { p.parts = n > p.parts ? n : p.parts; };      // the kernels use it one after the other
@@ -182,15 +178,13 @@ Plan plan(int n_tokens, int R, int Hq, int Hkv, int d, int max_q, int max_k, boo
 }
 
 template <class T>
-int join(int rt, int n_cta, const PagedScratch& ws, T* o, float* lse2, const PagedBatch& batch, const PagedRows& rows, int d,
-         cudaStream_t st) {
-  return launch_next(paged_combine_kernel<T>, dim3(n_cta, (rt + kJoinWarps - 1) / kJoinWarps), kJoinWarps * 32, st, rt, ws, o, lse2, batch,
-                     rows.G, rows.Hkv, d);
+int join(int rt, int n_cta, const PagedScratch& ws, T* o, float* lse2, const PagedRows& rows, int d, cudaStream_t st) {
+  return launch_next(paged_combine_kernel<T>, dim3(n_cta, (rt + kJoinWarps - 1) / kJoinWarps), kJoinWarps * 32, st, rt, ws, o, lse2, rows.G,
+                     rows.Hkv, d);
 }
 
-int join_tiles(int n_cta, const PagedScratch& ws, __nv_bfloat16* o, float* lse2, const PagedBatch& batch, const PagedRows& rows, int d,
-               cudaStream_t st) {
-  return launch_next(paged_combine_tiles_kernel, dim3(n_cta, kTileRows / 32), kTileWarps * 32, st, ws, o, lse2, batch, rows.G, rows.Hkv, d);
+int join_tiles(int n_cta, const PagedScratch& ws, __nv_bfloat16* o, float* lse2, const PagedRows& rows, int d, cudaStream_t st) {
+  return launch_next(paged_combine_tiles_kernel, dim3(n_cta, kTileRows / 32), kTileWarps * 32, st, ws, o, lse2, rows.G, rows.Hkv, d);
 }
 
 int run_f32(const PagedRows& rows, const PagedPools& pools, const PagedBatch& batch, int causal, float* o, float* weights,
@@ -202,12 +196,12 @@ int run_f32(const PagedRows& rows, const PagedPools& pools, const PagedBatch& ba
   int n_cta, rc = CB2_OK;
   if (p.chunks) {
     rc = paged_fma_run(64, rows, pools, batch, causal, kPagedChunk, p.few, o, lse2, nullptr, parts, &ws, &n_cta, st);
-    if (rc == CB2_OK) rc = join(64, n_cta, ws, o, lse2, batch, rows, pools.d, st);
+    if (rc == CB2_OK) rc = join(64, n_cta, ws, o, lse2, rows, pools.d, st);
     if (rc == CB2_OK && weights) rc = paged_weights_fma_run(rows, pools, batch, causal, kPagedChunk, p.few, lse2, weights, st);
   }
   if (rc == CB2_OK && p.few) {
     rc = paged_fma_run(p.few, rows, pools, batch, causal, kPagedFew, p.few, o, lse2, scores, parts, &ws, &n_cta, st);
-    if (rc == CB2_OK) rc = join(p.few, n_cta, ws, o, lse2, batch, rows, pools.d, st);
+    if (rc == CB2_OK) rc = join(p.few, n_cta, ws, o, lse2, rows, pools.d, st);
     if (rc == CB2_OK && scores) rc = paged_few_weights_run(rows, batch, causal, p.few, scores, lse2, weights, st);
     if (rc == CB2_OK && weights && !scores) rc = paged_weights_fma_run(rows, pools, batch, causal, kPagedFew, p.few, lse2, weights, st);
   }
@@ -223,12 +217,12 @@ int run_bf16(const PagedRows& rows, const PagedPools& pools, const PagedBatch& b
   int n_cta, rc = CB2_OK;
   if (p.chunks) {
     rc = paged_tc_run(rows, pools, batch, causal, p.few, o, lse2, parts, &ws, &n_cta, st);
-    if (rc == CB2_OK) rc = join_tiles(n_cta, ws, o, lse2, batch, rows, pools.d, st);
+    if (rc == CB2_OK) rc = join_tiles(n_cta, ws, o, lse2, rows, pools.d, st);
     if (rc == CB2_OK && weights) rc = paged_weights_tc_run(rows, pools, batch, causal, kPagedChunk, p.few, lse2, weights, parts, st);
   }
   if (rc == CB2_OK && p.few) {
     rc = paged_few_run(rows, pools, batch, causal, p.few, o, lse2, scores, parts, &ws, &n_cta, st);
-    if (rc == CB2_OK) rc = join(16, n_cta, ws, o, lse2, batch, rows, pools.d, st);
+    if (rc == CB2_OK) rc = join(16, n_cta, ws, o, lse2, rows, pools.d, st);
     if (rc == CB2_OK && scores) rc = paged_few_weights_run(rows, batch, causal, p.few, scores, lse2, weights, st);
     if (rc == CB2_OK && weights && !scores)
       rc = paged_weights_tc_run(rows, pools, batch, causal, kPagedFew, p.few, lse2, weights, parts, st);
@@ -271,7 +265,7 @@ extern "C" int cb2_om_paged_fwd(const void* q, long long q_token_stride, long lo
   if (n_tokens == 0) return CB2_OK;
   if (!q || !o || !scratch) return CB2_NULL_PTR;
   const int vec = dtype == CB2_BF16 ? 8 : 4;      // elements in 16 bytes
-  if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(o) || !aligned16(scratch) ||
+  if (!aligned16(q) || !aligned16(weights) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(o) || !aligned16(scratch) ||
       q_token_stride % vec || q_head_stride % vec || k_page_stride % vec || v_page_stride % vec)
     return CB2_BAD_ALIGN;
   const Plan p = plan(n_tokens, R, Hq, Hkv, d, max_q, max_k, weights != nullptr, dtype);

@@ -336,6 +336,7 @@ struct PagedWalk : PagedWalkState {
 // A unit that starts in share c and goes on in the next ones: written by CTA c for the combine kernel.
 struct PagedJoin {
   int r, h, tile, last;     // r < 0: none; last = share that holds the unit's last block
+  int t0, n, pad[2];        // the request's rows
 };
 // Partial carriers: share c owns slot 2c (a piece that does not start its unit) and 2c + 1 (a piece
 // that starts a unit and does not finish it).  Slot: m[RT], l[RT], a, fp32, m in log2 units; a is [RT][d], or
@@ -358,10 +359,16 @@ __device__ __forceinline__ void paged_write_join(const PagedWalkState& w, long l
   j.r = w.r;
   j.h = w.h;
   j.tile = w.tile;
+  j.t0 = w.q.t0;
+  j.n = w.q.n;
+  j.pad[0] = j.pad[1] = 0;
   const long long x = (w.cur + w.nb) * n_share - 1;
   j.last = x < (1ll << 32) ? int(unsigned(x) / unsigned(total)) : int(x / total);
   joins[cta] = j;
 }
+
+// Kept scores of a request, kv head and packed row: so many floats apart, a multiple of four.
+__host__ __device__ __forceinline__ long long paged_score_stride(int max_k) { return (max_k + 3ll) & ~3ll; }
 
 // Scratch of one attention kernel of n_cta shares: the joins, the partial carriers.
 struct PagedScratch {

@@ -201,7 +201,7 @@ paged_few_kernel(const PagedRows rows, const PagedPools pools, const PagedBatch 
           for (int e = 0; e < 4; ++e) {
             const int row = b * 8 + 2 * t + (e & 1), j = k0 + g + 8 * (e >> 1);
             if (row < n_rows && j < len)
-              scores[(((long long)w.r * rows.Hkv + w.h) * cost.few + row) * batch.max_k + j] = s[b][e];
+              scores[(((long long)w.r * rows.Hkv + w.h) * cost.few + row) * paged_score_stride(batch.max_k) + j] = s[b][e];
           }
       }
       if (__any_sync(0xffffffffu, grow)) {
@@ -305,8 +305,9 @@ paged_few_kernel(const PagedRows rows, const PagedPools pools, const PagedBatch 
 }
 
 // weight[key] += sum over the packed rows of 2^(score - lse), from the scores that the kernel above left: a
-// thread a key, the same line cut into more shares (one block or a few each, so that all loads are in flight).
-constexpr int kWeightThreads = 256, kWeightCtas = 8 * kNumSMs;
+// thread four neighbouring keys (they lie in one page), the same line cut into more shares, so that all loads are in
+// flight at once.
+constexpr int kWeightThreads = 256, kWeightCtas = 4 * kNumSMs;
 
 __global__ void __launch_bounds__(kWeightThreads)
 paged_few_weights_kernel(const PagedBatch batch, const Cost cost, const float* __restrict__ scores, const float* __restrict__ lse2,
@@ -315,22 +316,37 @@ paged_few_weights_kernel(const PagedBatch batch, const Cost cost, const float* _
   __shared__ float sh_lse[kRT];
   const PagedShare share = paged_find_share<kWeightThreads>(batch, cost, blockIdx.x, gridDim.x, &find);
   const int G = cost.G, ps = 1 << batch.page_log2, tid = threadIdx.x;
+  const long long stride = paged_score_stride(batch.max_k);
   let_next();
   after_previous();          // (the share comes from index tensors alone)
   for (PagedWalk<Cost> w(batch, cost, share); w.valid(); w.next()) {
     w.clip();
-    const float* sc = scores + ((long long)w.r * cost.Hkv + w.h) * cost.few * batch.max_k;
+    const float* sc = scores + ((long long)w.r * cost.Hkv + w.h) * cost.few * stride;
     const int n_rows = w.q.n * G, end = min(w.b1 * kKB, w.q.len);
     __syncthreads();
     if (tid < n_rows) sh_lse[tid] = __ldg(lse2 + (long long)(w.q.t0 + tid / G) * (G * cost.Hkv) + w.h * G + tid % G);
     __syncthreads();
-    for (int j = w.b0 * kKB + tid; j < end; j += kWeightThreads) {
+    for (int j = w.b0 * kKB + 4 * tid; j < end; j += 4 * kWeightThreads) {
       const int page = paged_page(batch, w.r, j >> batch.page_log2);
       float* at = weights + ((long long)page * cost.Hkv + w.h) * ps + (j & (ps - 1));
-      float sum = 0.f;
-#pragma unroll 8
-      for (int row = 0; row < n_rows; ++row) sum += ex2_approx(__ldg(sc + (long long)row * batch.max_k + j) - sh_lse[row]);
-      *at += sum;
+      const float4 was = *reinterpret_cast<const float4*>(at);
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+      for (int row = 0; row < n_rows; ++row) {
+        const float4 x = __ldg(reinterpret_cast<const float4*>(sc + row * stride + j));
+        const float z = sh_lse[row];
+        sum[0] += ex2_approx(x.x - z);
+        sum[1] += ex2_approx(x.y - z);
+        sum[2] += ex2_approx(x.z - z);
+        sum[3] += ex2_approx(x.w - z);
+      }
+      if (j + 4 <= end) {
+        *reinterpret_cast<float4*>(at) = make_float4(was.x + sum[0], was.y + sum[1], was.z + sum[2], was.w + sum[3]);
+      } else {               // slots behind the length, and scores there, are nobody's
+        at[0] = was.x + sum[0];
+        if (j + 1 < end) at[1] = was.y + sum[1];
+        if (j + 2 < end) at[2] = was.z + sum[2];
+      }
     }
   }
 }

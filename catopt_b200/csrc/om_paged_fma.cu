@@ -150,7 +150,7 @@ paged_fma_kernel(const PagedRows rows, const PagedPools pools, const PagedBatch 
           mx = fmaxf(mx, s[i][k]);
         }
         if (kept_scores && row0 + SR * ty + i < n_rows) {
-          float* to = kept_scores + (((long long)w.r * rows.Hkv + w.h) * cost.few + row0 + SR * ty + i) * batch.max_k + k0 + tx;
+          float* to = kept_scores + (((long long)w.r * rows.Hkv + w.h) * cost.few + row0 + SR * ty + i) * paged_score_stride(batch.max_k) + k0 + tx;
 #pragma unroll
           for (int k = 0; k < KP; ++k)
             if (k0 + tx + KX * k < len) to[KX * k] = s[i][k];

@@ -6,7 +6,7 @@
 // copied whole.  The old pages stay as they are, so shared prefixes are no hazard and the copy needs no order.
 //
 // Two launches.  paged_select_kernel: one CTA per (request, kv head) finds the budget-th weight by radix
-// selection on the weights' order-preserving bit patterns and writes the kept slots in ascending order.
+// selection (11, 11 and 10 bits) on the weights' order-preserving bit patterns and writes the kept slots in ascending order.
 // paged_move_kernel: copies rows, bound by memory (kept rows read once and written once).
 #include "om_paged.cuh"
 
@@ -15,6 +15,7 @@ namespace {
 
 constexpr int kSelThreads = 1024, kMoveThreads = 256, kMoveRows = 64;
 constexpr int kMostHeld = 48 * 1024;       // keys that fit shared memory beside the histogram
+constexpr int kBins = 2048;
 
 // Unsigned key of the same order as the float: NaN lowest, -0 and +0 the same.
 __device__ __forceinline__ uint32_t weight_key(float w) {
@@ -39,6 +40,15 @@ struct WeightReader {
     const int page = paged_page(b, r, j >> b.page_log2), ps = 1 << b.page_log2;
     return weight_key(w[((long long)page * Hkv + h) * ps + (j & (ps - 1))]);
   }
+  // slots j .. j + 3, j a multiple of four
+  __device__ __forceinline__ void four(int j, uint32_t (&k)[4]) const {
+    const int page = paged_page(b, r, j >> b.page_log2), ps = 1 << b.page_log2;
+    const float4 x = *reinterpret_cast<const float4*>(w + ((long long)page * Hkv + h) * ps + (j & (ps - 1)));
+    k[0] = weight_key(x.x);
+    k[1] = weight_key(x.y);
+    k[2] = weight_key(x.z);
+    k[3] = weight_key(x.w);
+  }
 };
 
 // Positions among the true flags of a block, thread order: exclusive rank and total.
@@ -56,8 +66,8 @@ static_assert(kSelThreads == 1024, "block_rank reads one count a lane");
 
 __global__ void __launch_bounds__(kSelThreads)
 paged_select_kernel(const EvictArgs a, const PagedBatch batch) {
-  extern __shared__ uint32_t sh_keys[];                 // [held]
-  __shared__ int hist[256];
+  extern __shared__ __align__(16) uint32_t sh_keys[];                 // [held]
+  __shared__ int hist[kBins];
   __shared__ int warp_count[2][2][32];
   __shared__ uint32_t s_prefix;
   __shared__ int s_need;
@@ -75,55 +85,65 @@ paged_select_kernel(const EvictArgs a, const PagedBatch batch) {
   const int lo = a.first, hi = len - a.last;             // first + last <= budget < len
   const int want = a.budget - a.first - a.last;          // of [lo, hi)
   const int held = min(a.held, len);
-#pragma unroll 4
-  for (int j = tid; j < held; j += kSelThreads) sh_keys[j] = key(j);
+#pragma unroll 2
+  for (int j = 4 * tid; j < held; j += 4 * kSelThreads) {      // four neighbouring slots lie in one page
+    uint32_t k[4];
+    key.four(j, k);
+    *reinterpret_cast<uint4*>(sh_keys + j) = make_uint4(k[0], k[1], k[2], k[3]);
+  }
   auto key_at = [&](int j) { return j < held ? sh_keys[j] : key(j); };
   if (tid == 0) {
     s_prefix = 0;
     s_need = want;
   }
-  __syncthreads();
-  // the want-th largest key of [lo, hi), byte by byte
-  for (int shift = 24; want > 0 && shift >= 0; shift -= 8) {
-    if (tid < 256) hist[tid] = 0;
+  // the want-th largest key of [lo, hi), 11, 11 and 10 bits at a time
+  for (int pass = 0; want > 0 && pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+    const uint32_t mask = pass == 0 ? 0u : ~0u << (shift + bits), bin_mask = (1u << bits) - 1;
+    for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
     __syncthreads();
-    const uint32_t prefix = s_prefix, mask = shift == 24 ? 0u : ~0u << (shift + 8);
+    const uint32_t prefix = s_prefix;
+    const int need = s_need;
     for (int j0 = lo; j0 < hi; j0 += kSelThreads) {
       const int j = j0 + tid;
       const uint32_t k = j < hi ? key_at(j) : 0u;
       const bool in = j < hi && (k & mask) == prefix;
-      const unsigned bin = in ? (k >> shift) & 255u : 256u;
-      // weights share their leading bytes: one addition for all lanes of a bin
-      const unsigned peers = __match_any_sync(0xffffffffu, bin);
-      if (in && lane == __ffs(peers) - 1) atomicAdd(&hist[bin], __popc(peers));
+      const uint32_t bin = (k >> shift) & bin_mask;
+      // many keys may be the same (0, say): the lanes that agree with the first one add together
+      const unsigned all = __ballot_sync(0xffffffffu, in);
+      const uint32_t first = __shfl_sync(0xffffffffu, bin, all ? __ffs(all) - 1 : 0);
+      const unsigned same = __ballot_sync(0xffffffffu, in && bin == first);
+      if (in && bin != first) atomicAdd(&hist[bin], 1);
+      if (same && lane == __ffs(same) - 1) atomicAdd(&hist[first], __popc(same));
     }
     __syncthreads();
-    if (warp == 0) {
-      // bins from the top, eight a lane: the bin in which the need runs out
-      int c[8], sum = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        c[i] = hist[255 - (lane * 8 + i)];
-        sum += c[i];
-      }
-      int incl = sum;
+    // from the top: the 64 bins in which the need runs out (a warp each), then the bin
+    const int top = kBins - 1 - warp * 64;
+    const int c0 = hist[top - lane], c1 = hist[top - 32 - lane];
+    const int mine = __reduce_add_sync(0xffffffffu, c0 + c1);
+    if (lane == 0) warp_count[0][0][warp] = mine;
+    __syncthreads();
+    const int other = warp_count[0][0][lane];
+    const int before = __reduce_add_sync(0xffffffffu, lane < warp ? other : 0);
+    if (before < need && before + mine >= need) {          // one warp
+      int incl0 = c0, incl1 = c1;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += y;
-      }
-      int before = incl - sum;
-      const int need = s_need;
-      __syncwarp();
-      if (before < need && incl >= need) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (before < need && before + c[i] >= need) {
-            s_prefix = prefix | (uint32_t(255 - (lane * 8 + i)) << shift);
-            s_need = need - before;
-          }
-          before += c[i];
+        const int y0 = __shfl_up_sync(0xffffffffu, incl0, o), y1 = __shfl_up_sync(0xffffffffu, incl1, o);
+        if (lane >= o) {
+          incl0 += y0;
+          incl1 += y1;
         }
+      }
+      incl0 += before;
+      incl1 += __shfl_sync(0xffffffffu, incl0, 31);
+      if (incl0 - c0 < need && incl0 >= need) {
+        s_prefix = prefix | (uint32_t(top - lane) << shift);
+        s_need = need - (incl0 - c0);
+      }
+      if (incl1 - c1 < need && incl1 >= need) {
+        s_prefix = prefix | (uint32_t(top - 32 - lane) << shift);
+        s_need = need - (incl1 - c1);
       }
     }
     __syncthreads();
@@ -225,7 +245,7 @@ extern "C" int cb2_paged_evict(void* k_pages, void* v_pages, long long k_page_st
   if (k_page_stride < page || v_page_stride < page) return CB2_BAD_SHAPE;
   if (dtype != CB2_BF16 && dtype != CB2_F32) return CB2_UNSUPPORTED_DTYPE;
   const int esz = dtype == CB2_BF16 ? 2 : 4;
-  if (!aligned16(k_pages) || !aligned16(v_pages) || k_page_stride * esz % 16 || v_page_stride * esz % 16) return CB2_BAD_ALIGN;
+  if (!aligned16(k_pages) || !aligned16(v_pages) || !aligned16(weights) || k_page_stride * esz % 16 || v_page_stride * esz % 16) return CB2_BAD_ALIGN;
   int page_log2 = 0;
   while ((1 << page_log2) < page_size) ++page_log2;
   const PagedBatch batch{block_table, seq_lens, nullptr, R, max_pages, n_pages, page_log2, 0, 0, max_k, dev_status};
@@ -233,7 +253,7 @@ extern "C" int cb2_paged_evict(void* k_pages, void* v_pages, long long k_page_st
   const EvictArgs e{weights, Hkv, budget, keep_first, keep_last, kept, new_lens, max_k < kMostHeld ? max_k : kMostHeld};
   static std::atomic<unsigned long long> done{0};
   if (!allow_smem(reinterpret_cast<const void*>(paged_select_kernel), kMostHeld * 4, done)) return CB2_LAUNCH_FAIL;
-  paged_select_kernel<<<dim3(Hkv, R), kSelThreads, size_t(e.held) * 4, st>>>(e, batch);
+  paged_select_kernel<<<dim3(Hkv, R), kSelThreads, size_t((e.held + 3) & ~3) * 4, st>>>(e, batch);
   CB2_LAUNCH_CHECK();
   const MoveArgs m{static_cast<char*>(k_pages), static_cast<char*>(v_pages), k_page_stride * esz, v_page_stride * esz, weights,
                    kept, new_table, new_pages, Hkv, budget, d * esz};

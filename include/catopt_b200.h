@@ -409,7 +409,8 @@ int cb2_om_bias_step(const void* q, const void* k, const void* v, const float* b
  * Pools k_pages, v_pages: n_pages pages of [Hkv, page_size, d], dense inside a page, the
  * distance between two pages (elements) free; page_size a power of two from 8 to 1024, d a
  * multiple of 8 up to 128.  weights (may be NULL where the comment says so): float
- * [n_pages, Hkv, page_size], the attention weight that each cached key has received.
+ * [n_pages, Hkv, page_size], the attention weight that each cached key has received (16-byte
+ * aligned).
  * A ragged batch of R requests: request r has its new tokens in rows [cu_q[r], cu_q[r+1])
  * of q / k / v (int32 [R+1], ascending), seq_lens[r] cached keys WITH the new tokens (int32
  * [R]) and the pages block_table[r][0 .. ceil(seq_lens[r] / page_size)) (int32

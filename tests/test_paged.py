@@ -32,7 +32,7 @@ NULL, SHAPE, ALIGN, DTYPE, SCRATCH = 6, 1, 2, 3, 7
     (dict(page=4), SHAPE), (dict(page=2048), SHAPE), (dict(max_k=33), SHAPE), (dict(max_k=0), SHAPE), (dict(max_q=-1), SHAPE),
     (dict(n_pages=0), SHAPE), (dict(scale=0.0), SHAPE), (dict(scale=float("nan")), SHAPE), (dict(scale=float("inf")), SHAPE),
     (dict(ks=2040), SHAPE), (dict(qt=0), SHAPE), (dict(qh=0), SHAPE), (dict(n=1 << 30), SHAPE), (dict(dtype=7), DTYPE), (dict(q=P + 2), ALIGN), (dict(qt=252), ALIGN),
-    (dict(v=P + 8), ALIGN), (dict(bytes=16), SCRATCH),
+    (dict(v=P + 8), ALIGN), (dict(w=P + 4), ALIGN), (dict(bytes=16), SCRATCH),
 ], ids=str)
 def test_attention_refusals(lib, change, want):
     assert lib.cb2_om_paged_fwd(*{**ATTEND, **change}.values()) == want
@@ -51,7 +51,7 @@ def test_append_refusals(lib, change, want):
 @pytest.mark.parametrize("change,want", [
     (dict(w=None), NULL), (dict(kept=None), NULL), (dict(budget=0), SHAPE), (dict(budget=17), SHAPE), (dict(first=-1), SHAPE),
     (dict(first=5, last=4), SHAPE), (dict(max_k=40), SHAPE), (dict(R=65536), SHAPE), (dict(page=0), SHAPE), (dict(dtype=5), DTYPE),
-    (dict(k=P + 2), ALIGN), (dict(vs=2052), ALIGN),
+    (dict(k=P + 2), ALIGN), (dict(w=P + 4), ALIGN), (dict(vs=2052), ALIGN),
 ], ids=str)
 def test_evict_refusals(lib, change, want):
     assert lib.cb2_paged_evict(*{**EVICT, **change}.values()) == want
