@@ -5,6 +5,7 @@ built by ``python -m catopt_b200.build``); this package is the thin host side:
 
 * ``ops``        one function per C-ABI entry point, torch CUDA tensors in/out
 * ``executors``  ``nn.Module``s with the reference's batched-executor surface
+* ``paged``      a paged key/value cache for decode loops (append, attention, eviction)
 * ``verify``     the verify gate (``verify_equiv`` / ``verify_module`` / batched)
 * ``sharding``   the batch x head / batch x channel / probe partition over ranks
 * ``sink``       adapter into catopt's ``Sink.executors`` table (needs catopt)

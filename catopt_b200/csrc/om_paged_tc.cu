@@ -17,6 +17,12 @@
 // inside a token's group; a piece's rows are fetched during the last softmax of the piece before).  The
 // pieces of a share are listed in shared memory in batches, so that the softmax threads spend no registers on
 // the walk.  Every wait is bounded.
+//
+// Measured: two chunks of 2048 tokens on 8192 keys in all, 32 heads on 8, d 128: 391 us with the join, 946 TFLOP/s; a
+// piece costs about four blocks' time to start and end, which the line counts.  What bounds a long piece is shared
+// memory: a 64-column product reads Q again for every 64 keys (48 KB a block), P V reads 16 KB, the loads write 32 KB;
+// two CTAs move 192 KB in about 1750 clocks, 110 of 128 bytes a clock.  Tried and slower: 128-key blocks with one S
+// buffer (487 us), part of the exponentials as polynomials on the FMA pipes (+7 %), eight softmax warps (+7 %).
 #include "om_paged.cuh"
 #include "umma.cuh"
 

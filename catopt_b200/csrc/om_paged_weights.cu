@@ -12,6 +12,9 @@
 // warps 2..5 = sums, warp 6 = row tiles, their -lse and the last slot each row sees (copying the rows by 16-byte
 // asynchronous copies took 2.8 k cycles a tile and set the pace).  A ring of four stages holds row tile, -lse and S
 // together; two CTAs share an SM.  Every wait is bounded.
+//
+// Measured: chunks of 1024 and 828 tokens on 4096 and 2896 keys, 32 heads on 8, d 128: 95 us (the attention before it:
+// 126 us); the exponential unit is busy 56 % of the time, the tensor pipe 26 %.  Two threads a key (eight sum warps): 98 us.
 #include "om_paged.cuh"
 #include "umma.cuh"
 
