@@ -71,10 +71,10 @@ paged_combine_kernel(int rt, const PagedScratch scratch, T* __restrict__ o, floa
   }
   if (rr >= n_rows) return;
   const int row = row_first + rr;
-  const float inv = x.l > 0.f ? 1.f / x.l : 0.f;
+  const float inv = x.l == 0.f ? 0.f : 1.f / x.l;      // a NaN sum stays one
   const long long at = (long long)(j.t0 + row / G) * (G * Hkv) + j.h * G + row % G;
   if (col < d) store4(o + at * d + col, make_float4(x.a.x * inv, x.a.y * inv, x.a.z * inv, x.a.w * inv));
-  if (lse2 && lane == 0) lse2[at] = x.l > 0.f ? x.m + log2f(x.l) : INFINITY;
+  if (lse2 && lane == 0) lse2[at] = x.l == 0.f ? INFINITY : x.m + log2f(x.l);
 }
 
 // The same for tiles of 128 rows, a stored [d / 4][128][4]: block (c, y) takes 32 of the rows, a lane one row, a warp
@@ -112,14 +112,14 @@ paged_combine_tiles_kernel(const PagedScratch scratch, __nv_bfloat16* __restrict
 #pragma unroll
       for (int k = 0; k < kGroups; ++k) x[k].add(m1, l1, v[k]);
     }
-    const float inv = x[0].l > 0.f ? 1.f / x[0].l : 0.f;
+    const float inv = x[0].l == 0.f ? 0.f : 1.f / x[0].l;
 #pragma unroll
     for (int k = 0; k < kGroups; ++k)
       store4(&sh[lane][(warp + k * kTileWarps) * 4], make_float4(x[k].a.x * inv, x[k].a.y * inv, x[k].a.z * inv, x[k].a.w * inv));
     if (warp == 0) {
       const long long at = (long long)(j.t0 + row / G) * (G * Hkv) + j.h * G + row % G;
       sh_at[lane] = at;
-      if (lse2) lse2[at] = x[0].l > 0.f ? x[0].m + log2f(x[0].l) : INFINITY;
+      if (lse2) lse2[at] = x[0].l == 0.f ? INFINITY : x[0].m + log2f(x[0].l);
     }
   }
   __syncthreads();
@@ -264,6 +264,7 @@ extern "C" int cb2_om_paged_fwd(const void* q, long long q_token_stride, long lo
   if (dtype != CB2_BF16 && dtype != CB2_F32) return CB2_UNSUPPORTED_DTYPE;
   if (n_tokens == 0) return CB2_OK;
   if (!q || !o || !scratch) return CB2_NULL_PTR;
+  if (q == o) return CB2_BAD_SHAPE;      // rows of q are read after others of o have been written
   const int vec = dtype == CB2_BF16 ? 8 : 4;      // elements in 16 bytes
   if (!aligned16(q) || !aligned16(weights) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(o) || !aligned16(scratch) ||
       q_token_stride % vec || q_head_stride % vec || k_page_stride % vec || v_page_stride % vec)

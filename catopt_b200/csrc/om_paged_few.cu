@@ -293,8 +293,8 @@ paged_few_kernel(const PagedRows rows, const PagedPools pools, const PagedBatch 
       }
       if (whole) {
         const long long at = (long long)(w.q.t0 + row / G) * (G * rows.Hkv) + w.h * G + row % G;
-        if (tid < d) o[at * d + tid] = __float2bfloat16_rn(ll > 0.f ? a / ll : 0.f);
-        if (lse2 && tid == 0) lse2[at] = ll > 0.f ? mm + log2f(ll) : INFINITY;
+        if (tid < d) o[at * d + tid] = __float2bfloat16_rn(ll == 0.f ? 0.f : a / ll)      /* a NaN sum stays one */;
+        if (lse2 && tid == 0) lse2[at] = ll == 0.f ? INFINITY : mm + log2f(ll);
       } else {
         if (tid < d) slot[2 * kRT + row * d + tid] = a;
         if (tid == 0) {

@@ -229,12 +229,12 @@ paged_fma_kernel(const PagedRows rows, const PagedPools pools, const PagedBatch 
     for (int i = 0; i < RP; ++i) {
       const int rr = RP * rg + i, row = row0 + rr;
       if (row >= n_rows) continue;
-      const float lr = stat[RT + rr], inv = whole ? (lr > 0.f ? 1.f / lr : 0.f) : 1.f;
+      const float lr = stat[RT + rr], inv = whole ? (lr == 0.f ? 0.f : 1.f / lr) : 1.f;      // a NaN sum stays one
       const long long at = (long long)(w.q.t0 + row / G) * (G * rows.Hkv) + w.h * G + row % G;
       float* dst = whole ? o + at * d : slot + 2 * RT + rr * d;
       if (4 * cg < d)
         *reinterpret_cast<float4*>(dst + 4 * cg) = make_float4(acc[i][0] * inv, acc[i][1] * inv, acc[i][2] * inv, acc[i][3] * inv);
-      if (whole && lse2 && cg == 0) lse2[at] = lr > 0.f ? stat[rr] + log2f(lr) : INFINITY;
+      if (whole && lse2 && cg == 0) lse2[at] = lr == 0.f ? INFINITY : stat[rr] + log2f(lr);
     }
   }
 }

@@ -390,7 +390,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         if (!__all_sync(0xffffffffu, ok)) break;
         umma::fence_after_sync();
         const bool live = rr < rows, whole = pc->whole;
-        const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+        const float inv = l_run == 0.f ? 0.f : 1.f / l_run;      // a NaN sum stays one
         const int row = pc->row0 + rr;
         const long long at = (long long)(pc->t0 + row / a.G) * (a.G * a.Hkv) + pc->h * a.G + row % a.G;
         float* slot = scratch.parts + paged_slot_floats(kRT, d) * (2 * cta + (b0 == 0));
@@ -429,7 +429,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
           }
           __syncwarp();
         }
-        if (live && whole && a.lse2) a.lse2[at] = l_run > 0.f ? m_ref + log2f(l_run) : INFINITY;
+        if (live && whole && a.lse2) a.lse2[at] = l_run == 0.f ? INFINITY : m_ref + log2f(l_run);
         if (live && !whole) {
           slot[rr] = m_ref;
           slot[kRT + rr] = l_run;

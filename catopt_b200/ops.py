@@ -792,7 +792,8 @@ def paged_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_pag
     d]``.  ``q_weight``/``k_weight [d]``: root-mean-square norm of each head; ``cos``/``sin`` float32 ``[rows,
     rotary/2]`` with ``positions`` int32 ``[n]`` (read only then): rotation of the first ``rotary`` columns in pairs ``(i, i +
     rotary/2)``, or ``(2i, 2i+1)`` if ``interleaved``.  ``weights`` (float32 ``[n_pages, Hkv, page_size]``) is
-    zeroed at the new slots.  Returns the normed and rotated ``q`` (rows behind ``cu_q[R]`` are not written)."""
+    zeroed at the new slots.  Returns the normed and rotated ``q`` (rows behind ``cu_q[R]`` are not written); ``out`` may
+    be a contiguous ``q`` itself."""
     what = "paged_append"
     dev = _current(what, k_pages)
     n_pages, hkv, ps, d, ks, vs = _pools(what, dev, k_pages, v_pages)
@@ -817,7 +818,7 @@ def paged_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_pag
         cos_ptr = _dense(what, dev, "cos", cos, torch.float32, (rows, half))
         sin_ptr = _dense(what, dev, "sin", sin, torch.float32, (rows, half))
         pos_ptr = _dense(what, dev, "positions", positions, torch.int32, (n,))
-    _no_grad_asked(what, q, k, v, q_weight, k_weight, cos, sin)
+    _no_grad_asked(what, q, k, v, k_pages, v_pages, q_weight, k_weight)
     res, hq, q_args = None, 0, (None, 0, 0)
     if q is not None:
         _here(what, dev, q)
@@ -830,7 +831,7 @@ def paged_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_pag
     v, *v_args = _token_rows(v)
     rc = _lib.load().cb2_paged_append(
         *q_args, *k_args, *v_args, None if res is None else res.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, w_ptr, table, lens, cu, pos_ptr,
-        qw, kw, eps, cos_ptr, sin_ptr, rows, rotary, 1 if interleaved else 0, n, R, hq, hkv, d, ps, n_pages, max_pages,
+        qw, kw, float(eps), cos_ptr, sin_ptr, rows, rotary, 1 if interleaved else 0, n, R, hq, hkv, d, ps, n_pages, max_pages,
         dtype_code(dt), _status_ptr(what, dev), _raw_stream(dev))
     check(rc, "cb2_paged_append")
     return res
@@ -854,7 +855,7 @@ def om_paged_fwd(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     (all of them without ``causal``); a row that sees none gives 0.  ``max_q``, ``max_k``: bounds of the requests'
     new tokens and cached keys (``max_k`` defaults to what the table holds); the scratch grows with them.
     ``weights`` (float32 ``[n_pages, Hkv, page_size]``): the softmax probability that every cached key gets, summed
-    over rows and the heads of its group, is added to it.  ``scale`` defaults to ``1/sqrt(d)``."""
+    over rows and the heads of its group, is added to it (requests of one call must not share pages then).  ``scale`` defaults to ``1/sqrt(d)``."""
     what = "om_paged_fwd"
     dev = _current(what, k_pages)
     n_pages, hkv, ps, d, ks, vs = _pools(what, dev, k_pages, v_pages)
@@ -877,7 +878,7 @@ def om_paged_fwd(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     scratch = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)
     rc = lib.cb2_om_paged_fwd(*q_args, k_pages.data_ptr(), v_pages.data_ptr(), ks, vs,
                               res.data_ptr(), w_ptr, table, lens, cu, n, R, hq, hkv, d, ps, n_pages, max_pages, max_q, max_k,
-                              d ** -0.5 if scale is None else scale, 1 if causal else 0, code, scratch.data_ptr(), need,
+                              d ** -0.5 if scale is None else float(scale), 1 if causal else 0, code, scratch.data_ptr(), need,
                               _status_ptr(what, dev), _raw_stream(dev))
     check(rc, "cb2_om_paged_fwd")
     return res
@@ -906,6 +907,7 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, weights: torch.Ten
     w_ptr = _dense(what, dev, "weights", weights, torch.float32, (n_pages, hkv, ps))
     _no_grad_asked(what, k_pages, v_pages, weights)
     max_k = _bound(what, "max_k", max_pages * ps if max_k is None else max_k, min(max_pages * ps, 1 << 30))
+    budget = _bound(what, "budget", budget, (1 << 31) - 1)
     keep_first, keep_last = (_bound(what, name, x, budget) for name, x in (("keep_first", keep_first), ("keep_last", keep_last)))
     if budget < 1 or new_pages * ps < budget:
         raise B200Error(f"{what}: a budget of {budget} keys does not fit {new_pages} pages of {ps}")

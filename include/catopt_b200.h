@@ -432,7 +432,7 @@ int cb2_om_bias_step(const void* q, const void* k, const void* v, const float* b
  * with cos, sin: float [table_rows, rotary/2], row positions[t] (int32 [n_tokens]) for token t.
  * q: [n_tokens, Hq, d] (Hq may be 0, q NULL), k, v: [n_tokens, Hkv, d], each with its token and
  * head strides in elements, so views of a fused projection need no copy; q_out: [n_tokens, Hq,
- * d] dense, apart from q.  Norm weights have the tensors' element type.  Everything is computed
+ * d] dense; it may be q itself where q is dense, but overlap no other operand.  Norm weights have the tensors' element type.  Everything is computed
  * in fp32 and rounded once.  weights (may be NULL): set to 0 at the new slots.  No scratch.
  * Pointers 16-byte aligned, strides multiples of 16 bytes. */
 int cb2_paged_append(const void* q, long long q_token_stride, long long q_head_stride, const void* k,
@@ -452,7 +452,8 @@ int cb2_paged_append(const void* q, long long q_token_stride, long long q_head_s
  * q: [n_tokens, Hq, d] with token and head strides in elements (none 0); o: [n_tokens, Hq, d]
  * dense, apart from q.  max_q: no request has more new tokens; max_k: none more cached keys.
  * weights (may be NULL): weights[key] += sum over the rows that see it, and the heads of its
- * group, of the softmax probability.  Results do not depend on the order in which CTAs run.
+ * group, of the softmax probability; no two requests of the call may then have a page in common
+ * (without weights they may).  Results do not depend on the order in which CTAs run.
  * Products of bf16 tensors accumulate in fp32 and probabilities are rounded to bf16 for the
  * product with v; sums, maxima and accumulators are fp32 throughout.  scale > 0, (n_tokens +
  * max_k + 256) * Hq / Hkv < 2^30.

@@ -58,6 +58,56 @@ def test_attention(dev, dtype, new, lens, kv, group, d, page):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("d", [8, 24, 56, 72, 120])
+def test_attention_head_widths(dev, dtype, d):
+    run_attend(dev, [1, 30, 200], [90, 30, 700], 2, 3, d, 16, dtype, weights=True)
+    run_attend(dev, [1, 2, 1], [90, 300, 70], 2, 3, d, 8, dtype, weights=True)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("new", [1, 40], ids=["step", "chunk"])
+def test_a_nan_that_is_seen_shows(dev, dtype, new):
+    from catopt_b200 import ops
+
+    lens, n = [500, 500], [new, new]
+    c = ref.make_cache(lens, 1, 16, 64, dtype, dev, 13)
+    c["k"][c["table"][1, 3].long(), 0, 5] = float("nan")          # slot 53 of the second request
+    q = torch.randn(2 * new, 4, 64, device=dev).to(dtype)
+    o = ops.om_paged_fwd(q, c["k"], c["v"], c["table"], c["lens"], ref.offsets(n, dev), new)
+    assert o[:new].isfinite().all() and o[new:].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("new,lens", [([1, 1], [200, 130]), ([50, 20], [200, 130])], ids=["step", "chunk"])
+def test_requests_that_share_pages(dev, dtype, new, lens):
+    # the second request's first pages are the first one's: reading them twice is fine
+    from catopt_b200 import ops
+
+    c = ref.make_cache(lens, 2, 16, 64, dtype, dev, 14)
+    c["table"][1, :4] = c["table"][0, :4]
+    q = torch.randn(sum(new), 4, 64, device=dev).to(dtype)
+    o = ops.om_paged_fwd(q, c["k"], c["v"], c["table"], c["lens"], ref.offsets(new, dev), max(new))
+    want, tol, _, _ = ref.attend(q, c, new, lens, 0.125, True)
+    close(o, want, tol, "o")
+
+
+@pytest.mark.parametrize("rot,interleaved", [(64, False), (64, True), (40, False)])
+def test_append_in_place(dev, rot, interleaved):
+    from catopt_b200 import ops
+
+    c = ref.make_cache([300], 2, 16, 64, BF, dev, 15, fill=0.0)
+    q = torch.randn(300, 6, 64, device=dev).to(BF)
+    k = torch.randn(300, 2, 64, device=dev).to(BF)
+    ang = torch.rand(300, rot // 2, device=dev) * 6
+    kw = dict(q_weight=torch.rand(64, device=dev).to(BF), cos=ang.cos(), sin=ang.sin(), interleaved=interleaved,
+              positions=torch.arange(300, dtype=torch.int32, device=dev))
+    cu = ref.offsets([300], dev)
+    want = ops.paged_append(q, k, k, c["k"], c["v"], c["table"], c["lens"], cu, **kw)
+    got = ops.paged_append(q, k, k, c["k"], c["v"], c["table"], c["lens"], cu, out=q, **kw)
+    assert got is q and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("group", [1, 5])
 def test_attention_all_keys_visible(dev, dtype, group):
     # queries against another sequence's states: more rows than keys, too
@@ -424,7 +474,7 @@ def test_wrong_arguments_are_refused(dev):
     ops.om_paged_fwd(**ok)
     for bad in (dict(q=q[:, :3]), dict(q=q.float()), dict(q=q[..., :32]), dict(v_pages=c["v"][:-1]), dict(k_pages=c["k"].transpose(1, 2)),
                 dict(block_table=c["table"].long()), dict(seq_lens=c["lens"][:1]), dict(cu_q=cu[:2]), dict(max_k=1 << 20), dict(max_q=-1),
-                dict(scale=-1.0), dict(weights=torch.zeros(3, device=dev)), dict(out=torch.empty_like(q).float()), dict(seq_lens=c["lens"].cpu())):
+                dict(scale=-1.0), dict(weights=torch.zeros(3, device=dev)), dict(out=q), dict(out=torch.empty_like(q).float()), dict(seq_lens=c["lens"].cpu())):
         with pytest.raises(B200Error):
             ops.om_paged_fwd(**{**ok, **bad})
     ok = dict(q=q, k=k, v=k, k_pages=c["k"], v_pages=c["v"], block_table=c["table"], seq_lens=c["lens"], cu_q=cu)

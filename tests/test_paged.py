@@ -15,7 +15,7 @@ def lib():
 
 P = 4096        # a non-null, aligned address; never read, every call here is refused before a launch
 
-ATTEND = dict(q=P, qt=256, qh=64, k=P, v=P, ks=2 * 16 * 64, vs=2 * 16 * 64, o=P, w=None, table=P, lens=P, cu=P, n=8, R=2, Hq=4,
+ATTEND = dict(q=P, qt=256, qh=64, k=P, v=P, ks=2 * 16 * 64, vs=2 * 16 * 64, o=2 * P, w=None, table=P, lens=P, cu=P, n=8, R=2, Hq=4,
               Hkv=2, d=64, page=16, n_pages=4, max_pages=2, max_q=4, max_k=32, scale=0.125, causal=1, dtype=1, scratch=P,
               bytes=1 << 30, status=None, stream=None)
 APPEND = dict(q=P, qt=256, qh=64, k=P, kt=128, kh=64, v=P, vt=128, vh=64, out=P, kp=P, vp=P, ks=2048, vs=2048, w=None, table=P,
@@ -31,7 +31,7 @@ NULL, SHAPE, ALIGN, DTYPE, SCRATCH = 6, 1, 2, 3, 7
     (dict(R=0), SHAPE), (dict(Hq=3), SHAPE), (dict(Hkv=0), SHAPE), (dict(d=60), SHAPE), (dict(d=136), SHAPE), (dict(page=12), SHAPE),
     (dict(page=4), SHAPE), (dict(page=2048), SHAPE), (dict(max_k=33), SHAPE), (dict(max_k=0), SHAPE), (dict(max_q=-1), SHAPE),
     (dict(n_pages=0), SHAPE), (dict(scale=0.0), SHAPE), (dict(scale=float("nan")), SHAPE), (dict(scale=float("inf")), SHAPE),
-    (dict(ks=2040), SHAPE), (dict(qt=0), SHAPE), (dict(qh=0), SHAPE), (dict(n=1 << 30), SHAPE), (dict(dtype=7), DTYPE), (dict(q=P + 2), ALIGN), (dict(qt=252), ALIGN),
+    (dict(ks=2040), SHAPE), (dict(qt=0), SHAPE), (dict(o=P), SHAPE), (dict(qh=0), SHAPE), (dict(n=1 << 30), SHAPE), (dict(dtype=7), DTYPE), (dict(q=P + 2), ALIGN), (dict(qt=252), ALIGN),
     (dict(v=P + 8), ALIGN), (dict(w=P + 4), ALIGN), (dict(bytes=16), SCRATCH),
 ], ids=str)
 def test_attention_refusals(lib, change, want):
