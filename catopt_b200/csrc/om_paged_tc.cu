@@ -18,11 +18,12 @@
 // pieces of a share are listed in shared memory in batches, so that the softmax threads spend no registers on
 // the walk.  Every wait is bounded.
 //
-// Measured: two chunks of 2048 tokens on 8192 keys in all, 32 heads on 8, d 128: 391 us with the join, 946 TFLOP/s; a
+// Measured: two chunks of 2048 tokens on 8192 keys in all, 32 heads on 8, d 128: 375 us with the join, 987 TFLOP/s; a
 // piece costs about four blocks' time to start and end, which the line counts.  What bounds a long piece is shared
 // memory: a 64-column product reads Q again for every 64 keys (48 KB a block), P V reads 16 KB, the loads write 32 KB;
-// two CTAs move 192 KB in about 1750 clocks, 110 of 128 bytes a clock.  Tried and slower: 128-key blocks with one S
-// buffer (487 us), part of the exponentials as polynomials on the FMA pipes (+7 %), eight softmax warps (+7 %).
+// two CTAs move 192 KB in about 1680 clocks, 115 of 128 bytes a clock.  Tried and slower: 128-key blocks with one S
+// buffer (487 us), two row tiles that share key and value blocks in one CTA of an SM (595 us), part of the
+// exponentials as polynomials on the FMA pipes (+7 %), eight softmax warps (+7 %).
 #include "om_paged.cuh"
 #include "umma.cuh"
 
@@ -203,49 +204,45 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         if (!fine) break;
       }
     } else if (warp == 1) {
-      // the whole warp walks and waits, one lane issues
-      const int ksteps = (d + 15) >> 4;
+      // the whole warp walks, waits and computes the operands (shuffled, which tells the compiler that they are uniform:
+      // 391 -> 375 us at the size above), one lane issues
+      const bool lead = lane == 0;
+      auto uniform = [](uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); };
+      const int ksteps = int(uniform((d + 15) >> 4));
+      const uint32_t d_cols = uniform(tmem), qa = uniform(q_addr), ka = uniform(k_addr), va = uniform(v_addr);
       constexpr uint32_t idesc_kk = umma::instr_desc_bf16(128, kKB, false, false);
       const uint32_t idesc_kn = umma::instr_desc_bf16(128, uint32_t(d + 15) & ~15u, false, true);
       auto wait = [&](uint64_t* bar, uint32_t parity, int site) {
         return __all_sync(0xffffffffu, mbar_wait_abortable(bar, parity, s_abort, kDefaultWaitNs, site));
       };
       for (int p = 0; p < count; ++p, ++n_piece) {
-        const int blocks = sh->pieces[p].b1 - sh->pieces[p].b0;
+        const int blocks = int(uniform(sh->pieces[p].b1 - sh->pieces[p].b0));
         bool ok = wait(q_full, n_piece & 1, __LINE__);
         // scores run two blocks ahead; the tensor pipe runs in issue order, so those of block j + 2 may overwrite P of
         // block j right behind the product that reads it
         for (int j = -2; ok && j < blocks; ++j) {
+          const uint32_t n = uniform(n_blk + j), slot = n & 1;        // (block j + 2 has the same slot)
+          const uint32_t s_cols = d_cols + kColS + slot * kKB, k_tile = ka + slot * kKvTile, v_tile = va + slot * kKvTile;
           if (j >= 0) {
-            const uint32_t n = n_blk + j, slot = n & 1;
             ok = wait(&p_ready[slot], (n >> 1) & 1, __LINE__) && wait(&v_full[slot], (n >> 1) & 1, __LINE__);
             if (!ok) break;
             umma::fence_after_sync();
-            if (lane == 0) {
-              const uint32_t tile = v_addr + slot * kKvTile;
 #pragma unroll
-              for (int ks = 0; ks < kKB / 16; ++ks)
-                umma::mma_bf16_ts(tmem + kColO, tmem + kColS + slot * kKB + ks * 8, desc_v(tile, ks), idesc_kn, j > 0 || ks > 0);
-              umma::mma_commit(&o_done[slot]);
-              umma::mma_commit(&v_empty[slot]);
-            }
-            __syncwarp();
+            for (int ks = 0; ks < kKB / 16; ++ks)
+              umma::mma_bf16_ts_by(lead, d_cols + kColO, s_cols + ks * 8, desc_v(v_tile, ks), idesc_kn, j > 0 || ks > 0);
+            umma::mma_commit_by(lead, &o_done[slot]);
+            umma::mma_commit_by(lead, &v_empty[slot]);
           }
           if (j + 2 < blocks) {
-            const uint32_t n = n_blk + j + 2, slot = n & 1;
-            ok = wait(&k_full[slot], (n >> 1) & 1, __LINE__);
+            ok = wait(&k_full[slot], ((n + 2) >> 1) & 1, __LINE__);
             if (!ok) break;
             umma::fence_after_sync();
-            if (lane == 0) {
-              const uint32_t tile = k_addr + slot * kKvTile;
 #pragma unroll
-              for (int ks = 0; ks < 8; ++ks)
-                if (ks < ksteps)
-                  umma::mma_bf16(tmem + kColS + slot * kKB, umma::desc_kmajor(q_addr, ks), desc_k(tile, ks), idesc_kk, ks > 0);
-              umma::mma_commit(&s_ready[slot]);
-              umma::mma_commit(&k_empty[slot]);
-            }
-            __syncwarp();
+            for (int ks = 0; ks < 8; ++ks)
+              if (ks < ksteps)
+                umma::mma_bf16_by(lead, s_cols, umma::desc_kmajor(qa, ks), desc_k(k_tile, ks), idesc_kk, ks > 0);
+            umma::mma_commit_by(lead, &s_ready[slot]);
+            umma::mma_commit_by(lead, &k_empty[slot]);
           }
         }
         if (!ok) break;

@@ -180,29 +180,29 @@ paged_weights_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
                            pc.h, page, k_full);
       }
     } else if (warp == 1) {
-      const int ksteps = (d + 15) >> 4;
+      // the whole warp computes the operands (shuffled: uniform), one lane issues
+      const bool lead = lane == 0;
+      auto uniform = [](uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); };
+      const int ksteps = int(uniform((d + 15) >> 4));
+      const uint32_t s_cols = uniform(tmem), ka = uniform(k_addr), qa = uniform(q_addr);
       constexpr uint32_t idesc = umma::instr_desc_bf16(kKeys, kRows, false, false);
       auto wait = [&](uint64_t* bar, uint32_t parity, int site) {
         return __all_sync(0xffffffffu, mbar_wait_abortable(bar, parity, s_abort, kDefaultWaitNs, site));
       };
       for (int p = 0; p < count; ++p, ++n_piece) {
-        const int tiles = sh->pieces[p].tiles;
+        const int tiles = int(uniform(sh->pieces[p].tiles));
         bool ok = wait(k_full, n_piece & 1, __LINE__);
         for (int i = 0; ok && i < tiles; ++i, ++n_tile) {
-          const uint32_t st = stage_of(n_tile);
+          const uint32_t st = uniform(stage_of(n_tile)), tile = qa + st * kRowTile;
           ok = wait(&q_full[st], phase_of(n_tile), __LINE__);      // the rows' writers have waited for S to be free
           if (!ok) break;
           umma::fence_after_sync();
-          if (lane == 0) {
-            const uint32_t tile = q_addr + st * kRowTile;
 #pragma unroll
-            for (int ks = 0; ks < 8; ++ks)
-              if (ks < ksteps)
-                umma::mma_bf16(tmem + st * kRows, umma::desc_kmajor(k_addr, ks), desc_rows(tile, ks), idesc, ks > 0);
-            umma::mma_commit(&s_ready[st]);
-            if (i == tiles - 1) umma::mma_commit(k_empty);
-          }
-          __syncwarp();
+          for (int ks = 0; ks < 8; ++ks)
+            if (ks < ksteps)
+              umma::mma_bf16_by(lead, s_cols + st * kRows, umma::desc_kmajor(ka, ks), desc_rows(tile, ks), idesc, ks > 0);
+          umma::mma_commit_by(lead, &s_ready[st]);
+          if (i == tiles - 1) umma::mma_commit_by(lead, k_empty);
         }
         if (!ok) break;
       }
