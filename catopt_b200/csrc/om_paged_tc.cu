@@ -12,13 +12,14 @@
 // Only a block that some row of the tile may not see whole is masked, per element.  Of the last block of a
 // request the value rows behind its length are zeroed in shared memory, since 0 x NaN is NaN.
 //
-// Roles: warp 0 = loads (pages by TMA: one box per page and 64 columns, each lane its own page), warp 1 = MMA
+// Roles: warps 0 and 6 = loads of K and of V (pages by TMA: one box per page and 64 columns, each lane its own page; one
+// warp for both set the pace where a block is many pages: 24 requests on pages of 16, 46 -> 41 us with two), warp 1 = MMA
 // issue and TMEM owner, warps 2..5 = softmax and the query rows (16-byte asynchronous copies, since a tile may start
 // inside a token's group; a piece's rows are fetched during the last softmax of the piece before).  The
 // pieces of a share are listed in shared memory in batches, so that the softmax threads spend no registers on
 // the walk.  Every wait is bounded.
 //
-// Measured: two chunks of 2048 tokens on 8192 keys in all, 32 heads on 8, d 128: 375 us with the join, 987 TFLOP/s; a
+// Measured: two chunks of 2048 tokens on 8192 keys in all, 32 heads on 8, d 128: 372 us with the join, 994 TFLOP/s; a
 // piece costs about four blocks' time to start and end, which the line counts.  What bounds a long piece is shared
 // memory: a 64-column product reads Q again for every 64 keys (48 KB a block), P V reads 16 KB, the loads write 32 KB;
 // two CTAs move 192 KB in about 1680 clocks, 115 of 128 bytes a clock.  Tried and slower: 128-key blocks with one S
@@ -31,7 +32,7 @@ namespace cb2 {
 namespace {
 
 constexpr int kRT = 128, kKB = 64;
-constexpr int kThreads = 192;
+constexpr int kThreads = 224;
 // Rows in, scores of the first blocks, results out: as long as four blocks.
 using Cost = PagedCost<kRT, kKB, 4>;
 constexpr int kBatch = 32;                // pieces listed at a time
@@ -170,38 +171,41 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     __syncthreads();
     const int count = sh->count;
 
-    if (warp == 0) {
+    if (warp == 0 || warp == 6) {
+      const bool is_v = warp == 6;
+      uint64_t *full = is_v ? v_full : k_full, *empty = is_v ? v_empty : k_empty;
+      const CUtensorMap* map = is_v ? &map_v : &map_k;
+      unsigned char* ring = smem + (is_v ? kOffV : kOffK);
       const int ps_log2 = batch.page_log2, box_log2 = min(ps_log2, 6), boxes = kKB >> box_log2;
-      for (int p = 0; p < count; ++p) {
+      const uint32_t box_bytes = 128u << box_log2;
+      bool fine = true;
+      for (int p = 0; fine && p < count; ++p) {
         const Piece pc = sh->pieces[p];
-        const int blocks = pc.b1 - pc.b0;
-        bool fine = true;
-        for (int j = 0; fine && j < blocks; ++j, ++n_blk) {
-          const int k0 = (pc.b0 + j) * kKB, slot = n_blk & 1;
-          const bool mine = lane < boxes && k0 + (lane << box_log2) < pc.len;
-          int page = 0;
-          if (mine) page = paged_page(batch, pc.r, (k0 + (lane << box_log2)) >> ps_log2);
-          const unsigned have = __ballot_sync(0xffffffffu, mine);
-          const uint32_t box_bytes = 128u << box_log2, bytes = __popc(have) * halves * box_bytes;
-          const int y = ps_log2 > 6 ? k0 & ((1 << ps_log2) - 1) : 0;       // inside a page longer than a block
-          for (int kv = 0; fine && kv < 2; ++kv) {
-            uint64_t *full = kv ? &v_full[slot] : &k_full[slot], *empty = kv ? &v_empty[slot] : &k_empty[slot];
-            bool ok = n_blk < 2 || mbar_wait_abortable(empty, ((n_blk >> 1) - 1) & 1, CB2_SITE);
-            fine = __all_sync(0xffffffffu, ok);
-            if (!fine) break;
-            if (lane == 0) {
-              mbar_arrive_expect_tx(full, bytes);
-              ++*(kv ? &sh->loads_v : &sh->loads_k);
-            }
-            __syncwarp();
-            if (mine) {
-              unsigned char* dst = smem + (kv ? kOffV : kOffK) + slot * kKvTile + lane * box_bytes;
-              for (int hf = 0; hf < halves; ++hf)
-                umma::tma_load_4d(dst + hf * kSub, kv ? &map_v : &map_k, hf * 64, y, pc.h, page, full);
-            }
+        // this lane's page of a block, looked up a block ahead
+        auto look_up = [&](int b) {
+          const int k = b * kKB + (lane << box_log2);
+          return lane < boxes && b < pc.b1 && k < pc.len ? paged_page(batch, pc.r, k >> ps_log2) : -1;
+        };
+        int next = look_up(pc.b0);
+        for (int b = pc.b0; b < pc.b1; ++b, ++n_blk) {
+          const int slot = n_blk & 1, page = next;
+          next = look_up(b + 1);
+          const bool mine = page >= 0;
+          const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, mine)) * halves * box_bytes;
+          const int y = ps_log2 > 6 ? (b * kKB) & ((1 << ps_log2) - 1) : 0;       // inside a page longer than a block
+          const bool ok = n_blk < 2 || mbar_wait_abortable(&empty[slot], ((n_blk >> 1) - 1) & 1, CB2_SITE);
+          fine = __all_sync(0xffffffffu, ok);
+          if (!fine) break;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&full[slot], bytes);
+            ++*(is_v ? &sh->loads_v : &sh->loads_k);
+          }
+          __syncwarp();
+          if (mine) {
+            unsigned char* dst = ring + slot * kKvTile + lane * box_bytes;
+            for (int hf = 0; hf < halves; ++hf) umma::tma_load_4d(dst + hf * kSub, map, hf * 64, y, pc.h, page, &full[slot]);
           }
         }
-        if (!fine) break;
       }
     } else if (warp == 1) {
       // the whole warp walks, waits and computes the operands (shuffled, which tells the compiler that they are uniform:
@@ -249,7 +253,9 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         n_blk += blocks;
       }
     } else {
-      const int q4 = warp & 3, rr = q4 * 32 + lane;
+      // lanes q4 * 32 of tensor memory hold the tile's rows from `first_row` on; every second CTA begins in the other half,
+      // so that the few rows of short tiles fall to different quarters of the SM
+      const int q4 = warp & 3, first_row = ((q4 + (cta * 2 < n_cta ? 0 : 2)) & 3) * 32, rr = first_row + lane;
       const uint32_t lane_base = tmem + (uint32_t(q4 * 32) << 16);
       constexpr float kLazy = 8.f;
       const int ncb = (d + 31) >> 5;
@@ -257,6 +263,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       // The 32 packed rows of this warp, into the query tile: a lane works out the place of one row, 8 or 16
       // neighbouring lanes copy its chunks (a copy instruction then touches two or four rows, not 32).
       auto load_rows = [&](const Piece* pc) {
+        if (pc->row0 + first_row >= pc->n * a.G) return;
         const int row = pc->row0 + rr;
         const bool there = row < pc->n * a.G;
         const int tok = there ? row / a.G : 0, g = there ? row - tok * a.G : 0;
@@ -289,6 +296,9 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         const int rows = pc->n * a.G - pc->row0;                 // of this tile, kRT at most count
         // last slot this row sees, and the least of the tile's rows
         const int base = len - pc->n;
+        // a warp without rows only keeps step: what the products make of its lanes is never read (12 chunks of 17 tokens,
+        // d 96: 22.7 -> 21.9 us)
+        const bool busy = first_row < rows;
         const int last = cost.causal ? min(base + (pc->row0 + rr) / a.G, len - 1) : len - 1;
         const int first_last = cost.causal ? min(base + pc->row0 / a.G, len - 1) : len - 1;
         float m_ref = -INFINITY, l_run = 0.f;
@@ -303,53 +313,55 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
           // the last scores of this piece are out, so the next piece's rows may take its place
           const bool next_rows = j == blocks - 1 && p + 1 < count;
           if (next_rows) load_rows(pc + 1);
-          uint32_t sv[2][32];
-#pragma unroll
-          for (int cb = 0; cb < 2; ++cb) umma::tmem_ld32(s_cols + cb * 32, sv[cb]);
-          umma::tmem_wait_ld();
-          umma::tmem_loaded(sv[0]);
-          umma::tmem_loaded(sv[1]);
-          if (k0 + kKB - 1 > first_last) {
-            const int lim = last - k0;
-#pragma unroll
-            for (int cb = 0; cb < 2; ++cb)
-#pragma unroll
-              for (int c = 0; c < 32; ++c)
-                if (cb * 32 + c > lim) sv[cb][c] = 0xff800000u;
-          }
-          float mx[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) mx[i] = fmaxf(__uint_as_float(sv[0][i]), __uint_as_float(sv[1][i]));
-#pragma unroll
-          for (int c = 4; c < 32; ++c) mx[c & 3] = max3(mx[c & 3], __uint_as_float(sv[0][c]), __uint_as_float(sv[1][c]));
-          const float m_blk = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * scale;
           float alpha = 1.f;
-          if (m_blk > m_ref + kLazy || m_ref == -INFINITY) {
-            const float m_new = fmaxf(m_ref, m_blk);
-            alpha = (m_new == -INFINITY) ? 1.f : ex2_approx(m_ref - m_new);
-            m_ref = m_new;
-          }
-          const float neg_m = (m_ref == -INFINITY) ? 0.f : -m_ref;
-          const uint64_t scale2 = umma::f2_pack(scale, scale), neg2 = umma::f2_pack(neg_m, neg_m);
-          uint64_t sum2[2] = {0ull, 0ull};
+          if (busy) {
+            uint32_t sv[2][32];
 #pragma unroll
-          for (int cb = 0; cb < 2; ++cb) {
-            uint32_t w[16];
+            for (int cb = 0; cb < 2; ++cb) umma::tmem_ld32(s_cols + cb * 32, sv[cb]);
+            umma::tmem_wait_ld();
+            umma::tmem_loaded(sv[0]);
+            umma::tmem_loaded(sv[1]);
+            if (k0 + kKB - 1 > first_last) {
+              const int lim = last - k0;
 #pragma unroll
-            for (int c = 0; c < 32; c += 2) {
-              const uint64_t x = umma::f2_fma(umma::f2_pack(__uint_as_float(sv[cb][c]), __uint_as_float(sv[cb][c + 1])), scale2, neg2);
-              float x0, x1;
-              umma::f2_unpack(x, x0, x1);
-              const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
-              sum2[(c >> 1) & 1] = umma::f2_add(sum2[(c >> 1) & 1], umma::f2_pack(p0, p1));
-              w[c >> 1] = pack_bf16x2(p0, p1);
+              for (int cb = 0; cb < 2; ++cb)
+#pragma unroll
+                for (int c = 0; c < 32; ++c)
+                  if (cb * 32 + c > lim) sv[cb][c] = 0xff800000u;
             }
-            umma::tmem_st16(s_cols + cb * 16, w);
+            float mx[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mx[i] = fmaxf(__uint_as_float(sv[0][i]), __uint_as_float(sv[1][i]));
+#pragma unroll
+            for (int c = 4; c < 32; ++c) mx[c & 3] = max3(mx[c & 3], __uint_as_float(sv[0][c]), __uint_as_float(sv[1][c]));
+            const float m_blk = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * scale;
+            if (m_blk > m_ref + kLazy || m_ref == -INFINITY) {
+              const float m_new = fmaxf(m_ref, m_blk);
+              alpha = (m_new == -INFINITY) ? 1.f : ex2_approx(m_ref - m_new);
+              m_ref = m_new;
+            }
+            const float neg_m = (m_ref == -INFINITY) ? 0.f : -m_ref;
+            const uint64_t scale2 = umma::f2_pack(scale, scale), neg2 = umma::f2_pack(neg_m, neg_m);
+            uint64_t sum2[2] = {0ull, 0ull};
+#pragma unroll
+            for (int cb = 0; cb < 2; ++cb) {
+              uint32_t w[16];
+#pragma unroll
+              for (int c = 0; c < 32; c += 2) {
+                const uint64_t x = umma::f2_fma(umma::f2_pack(__uint_as_float(sv[cb][c]), __uint_as_float(sv[cb][c + 1])), scale2, neg2);
+                float x0, x1;
+                umma::f2_unpack(x, x0, x1);
+                const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+                sum2[(c >> 1) & 1] = umma::f2_add(sum2[(c >> 1) & 1], umma::f2_pack(p0, p1));
+                w[c >> 1] = pack_bf16x2(p0, p1);
+              }
+              umma::tmem_st16(s_cols + cb * 16, w);
+            }
+            float s0, s1;
+            umma::f2_unpack(umma::f2_add(sum2[0], sum2[1]), s0, s1);
+            l_run = fmaf(l_run, alpha, s0 + s1);
+            umma::tmem_wait_st();
           }
-          float s0, s1;
-          umma::f2_unpack(umma::f2_add(sum2[0], sum2[1]), s0, s1);
-          l_run = fmaf(l_run, alpha, s0 + s1);
-          umma::tmem_wait_st();
           if (k0 + kKB > len) {
             // the request's last block: value rows that nobody has written
             ok = mbar_wait_abortable(&v_full[slot], (n >> 1) & 1, CB2_SITE);
@@ -363,17 +375,18 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
           }
           // O <- O alpha once the product before has landed.  This wait is often skipped, so the products
           // alternate between two barriers: of one barrier's phases, all but the awaited one are then known to be over
-          if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+          if (busy && j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
             ok = mbar_wait_abortable(&o_done[slot ^ 1], ((n - 1) >> 1) & 1, CB2_SITE);
             if (!__all_sync(0xffffffffu, ok)) break;
             umma::fence_after_sync();
+            uint32_t ov[32];
             for (int cb = 0; cb < ncb; ++cb) {
-              umma::tmem_ld32(lane_base + kColO + cb * 32, sv[0]);
+              umma::tmem_ld32(lane_base + kColO + cb * 32, ov);
               umma::tmem_wait_ld();
-              umma::tmem_loaded(sv[0]);
+              umma::tmem_loaded(ov);
 #pragma unroll
-              for (int c = 0; c < 32; ++c) sv[0][c] = __float_as_uint(__uint_as_float(sv[0][c]) * alpha);
-              umma::tmem_st32(lane_base + kColO + cb * 32, sv[0]);
+              for (int c = 0; c < 32; ++c) ov[c] = __float_as_uint(__uint_as_float(ov[c]) * alpha);
+              umma::tmem_st32(lane_base + kColO + cb * 32, ov);
             }
             umma::tmem_wait_st();
           }
@@ -383,6 +396,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         }
         if (!__all_sync(0xffffffffu, ok)) break;
         n_blk += blocks;
+        if (!busy) continue;
         ok = mbar_wait_abortable(&o_done[(n_blk - 1) & 1], ((n_blk - 1) >> 1) & 1, CB2_SITE);
         if (!__all_sync(0xffffffffu, ok)) break;
         umma::fence_after_sync();
@@ -414,7 +428,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
               const int r8 = i * 8 + (lane >> 2);
               const uint4 v = *reinterpret_cast<const uint4*>(stage + r8 * kStagePitch + (lane & 3) * 16);
               const long long to = __shfl_sync(0xffffffffu, at, r8);
-              if (q4 * 32 + r8 < rows && col < d) *reinterpret_cast<uint4*>(a.o + to * d + col) = v;
+              if (first_row + r8 < rows && col < d) *reinterpret_cast<uint4*>(a.o + to * d + col) = v;
             }
             __syncwarp();
           } else if (live) {
