@@ -13,8 +13,9 @@
 // asynchronous copies took 2.8 k cycles a tile and set the pace).  A ring of four stages holds row tile, -lse and S
 // together; two CTAs share an SM.  Every wait is bounded.
 //
-// Measured: chunks of 1024 and 828 tokens on 4096 and 2896 keys, 32 heads on 8, d 128: 95 us (the attention before it:
-// 126 us); the exponential unit is busy 56 % of the time, the tensor pipe 26 %.  Two threads a key (eight sum warps): 98 us.
+// Measured: chunks of 1024 and 828 tokens on 4096 and 2727 keys, 32 heads on 8, d 128: 85 us (the attention before it:
+// 110 us); the exponential unit is busy about 60 % of the time.  Fetching -lse one tile ahead cost 8 us (the row warp sets the
+// pace), a division in every tile of the sums 3 us.  Two threads a key (eight sum warps), scores in two halves: slower.
 #include "om_paged.cuh"
 #include "umma.cuh"
 
@@ -229,7 +230,7 @@ paged_weights_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
           umma::tmem_loaded(sv[0]);
           umma::tmem_loaded(sv[1]);
           // rows that do not see the whole key block, or are not of this request: hidden per element
-          const int tok0 = (pc->tile0 + i) / cost.per_token * cost.T;
+          const int tok0 = (cost.per_token == 1 ? pc->tile0 + i : (pc->tile0 + i) / cost.per_token) * cost.T;
           if ((cost.causal && base + tok0 < pc->k0 + kKeys - 1) || tok0 + cost.T > pc->n || cost.per_token > 1) {
 #pragma unroll
             for (int cb = 0; cb < 2; ++cb)
@@ -267,49 +268,77 @@ paged_weights_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
       }
     } else {
       // columns lane and lane + 32 of a tile: token and head inside it
-      const int hb = min(G, kRows);
+      const int hb = min(G, kRows), per = cost.per_token;
       const int tok_of[2] = {lane / hb, (lane + 32) / hb}, g_of[2] = {lane % hb, (lane + 32) % hb};
-      float z[2];
-      int last[2];
-      auto look_up = [&](const Piece& pc, int i) {           // a tile ahead
-        const int tile = pc.tile0 + i, tok0 = tile / cost.per_token * cost.T, g0 = tile % cost.per_token * kRows;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int tok = tok0 + tok_of[e], g = g0 + g_of[e];
-          const bool there = tok_of[e] < cost.T && tok < pc.n && g < G;
-          z[e] = there ? __ldg(lse2 + (long long)(pc.t0 + tok) * (G * rows.Hkv) + pc.h * G + g) : INFINITY;
-          last[e] = there ? (cost.causal ? min(pc.len - pc.n + tok, pc.len - 1) : pc.len - 1) : -1;
+      // a tile of the list: T tokens from tok0 on (one, if per > 1: heads from g0 on)
+      struct Cursor {
+        int p, left, tok0, g0;
+      };
+      auto start = [&](Cursor& c) {
+        if (c.p >= count) return;
+        const int tile = sh->pieces[c.p].tile0, tb = per == 1 ? tile : tile / per;
+        c.left = sh->pieces[c.p].tiles;
+        c.tok0 = tb * cost.T;
+        c.g0 = (tile - tb * per) * kRows;
+      };
+      auto advance = [&](Cursor& c) {
+        if (--c.left == 0) {
+          ++c.p;
+          start(c);
+        } else if (per == 1 || (c.g0 += kRows) == per * kRows) {
+          c.g0 = 0;
+          c.tok0 += cost.T;
         }
       };
-      if (count > 0) look_up(sh->pieces[0], 0);
-      for (int p = 0; p < count; ++p) {
-        const Piece pc = sh->pieces[p];
-        bool ok = true;
-        for (int i = 0; i < pc.tiles; ++i, ++n_tile) {
-          const uint32_t st = stage_of(n_tile);
-          if (n_tile >= kStages) ok = mbar_wait_abortable(&s_empty[st], phase_of(n_tile - kStages), s_abort, kDefaultWaitNs, __LINE__);
-          if (!__all_sync(0xffffffffu, ok)) break;
-          if (lane == 0) {
-            const int tile = pc.tile0 + i;
-            mbar_arrive_expect_tx(&q_full[st], halves * hb * cost.T * 128);
-            ++sh->loads_q;
-            for (int hf = 0; hf < halves; ++hf)
-              umma::tma_load_3d(smem + kOffQ + st * kRowTile + hf * kSub, &map_q, hf * 64, pc.h * G + tile % cost.per_token * kRows,
-                                pc.t0 + tile / cost.per_token * cost.T, &q_full[st]);
-          }
+      struct Columns {
+        float z[2];
+        int last[2];
+      };
+      Cursor seen{0, 0, 0, 0};
+      auto look_up = [&](Columns& x) {
+        if (seen.p >= count) return;
+        const Piece* pc = &sh->pieces[seen.p];
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            sh->neg_lse[st][lane + 32 * e] = -z[e];
-            sh->last[st][lane + 32 * e] = last[e];
-          }
-          mbar_arrive(&q_full[st]);
-          if (i + 1 < pc.tiles)
-            look_up(pc, i + 1);
-          else if (p + 1 < count)
-            look_up(sh->pieces[p + 1], 0);
+        for (int e = 0; e < 2; ++e) {
+          const int tok = seen.tok0 + tok_of[e], g = seen.g0 + g_of[e];
+          const bool there = tok_of[e] < cost.T && tok < pc->n && g < G;
+          x.z[e] = there ? __ldg(lse2 + (long long)(pc->t0 + tok) * (G * rows.Hkv) + pc->h * G + g) : INFINITY;
+          x.last[e] = there ? (cost.causal ? min(pc->len - pc->n + tok, pc->len - 1) : pc->len - 1) : -1;
         }
-        if (!__all_sync(0xffffffffu, ok)) break;
-      }
+        advance(seen);
+      };
+      Cursor now{0, 0, 0, 0};
+      auto step = [&](Columns& x) {
+        const uint32_t st = stage_of(n_tile);
+        const bool ok = n_tile < kStages || mbar_wait_abortable(&s_empty[st], phase_of(n_tile - kStages), s_abort, kDefaultWaitNs, __LINE__);
+        if (!__all_sync(0xffffffffu, ok)) return false;
+        if (lane == 0) {
+          const Piece* pc = &sh->pieces[now.p];
+          mbar_arrive_expect_tx(&q_full[st], halves * hb * cost.T * 128);
+          ++sh->loads_q;
+          for (int hf = 0; hf < halves; ++hf)
+            umma::tma_load_3d(smem + kOffQ + st * kRowTile + hf * kSub, &map_q, hf * 64, pc->h * G + now.g0, pc->t0 + now.tok0, &q_full[st]);
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          sh->neg_lse[st][lane + 32 * e] = -x.z[e];
+          sh->last[st][lane + 32 * e] = x.last[e];
+        }
+        mbar_arrive(&q_full[st]);
+        advance(now);
+        ++n_tile;
+        look_up(x);
+        return now.p < count;
+      };
+      // -lse is fetched two tiles ahead (one warp feeds the tiles: its pace is theirs)
+      Columns a, b;
+      start(seen);
+      start(now);
+      look_up(a);
+      look_up(b);
+      if (count > 0)
+        while (step(a) && step(b)) {
+        }
     }
     __syncwarp();
     umma::fence_before_sync();
