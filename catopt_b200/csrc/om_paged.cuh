@@ -181,16 +181,14 @@ struct PagedCost {
     if (k == nt) s += all_blocks(q);
     return s + (long long)k * OV;
   }
-  __device__ __forceinline__ long long of_request(const PagedReq& q) const {
-    if (!takes(q)) return 0;
-    return before(q, tiles(q)) * Hkv;
-  }
+  // length of one kv head of a request
+  __device__ __forceinline__ long long per_head(const PagedReq& q) const { return takes(q) ? before(q, tiles(q)) : 0; }
 };
 
 struct PagedFindSmem {
   long long warp_sum[32];
-  long long carry;
-  long long off;
+  long long per_head, off;
+  PagedReq q;
   int r;
 };
 
@@ -199,6 +197,8 @@ struct PagedShare {
   long long total, lo, hi;
   int n_share;      // shares that are not empty: [0, n_share)
   int r;            // request that holds lo
+  PagedReq q;
+  long long per_head;
   long long off;    // lo - start of that request
 };
 
@@ -212,10 +212,14 @@ __device__ PagedShare paged_find_share(const PagedBatch& b, const Cost& cost, in
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   PagedShare out;
   const int passes = (b.R + T - 1) / T;
+  PagedReq q{0, 0, 0};
+  long long per_head = 0, mine = 0;        // of the request this thread looked at last
   // inclusive prefix of the costs of requests [pass * T, pass * T + T), on top of `carry`
-  auto scan = [&](int pass, long long& mine, long long carry, long long& block_total) -> long long {
+  auto scan = [&](int pass, long long carry, long long& block_total) -> long long {
     const int r = pass * T + tid;
-    mine = r < b.R ? cost.of_request(paged_request(b, r)) : 0;
+    if (r < b.R) q = paged_request(b, r);
+    per_head = r < b.R ? cost.per_head(q) : 0;
+    mine = per_head * cost.Hkv;
     long long x = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -228,12 +232,18 @@ __device__ PagedShare paged_find_share(const PagedBatch& b, const Cost& cost, in
     for (int w = 0; w < warp; ++w) pre += s->warp_sum[w];
     block_total = 0;
     for (int w = 0; w < T / 32; ++w) block_total += s->warp_sum[w];
-    __syncthreads();
+    if (passes > 1) __syncthreads();       // before the sums of the next pass
     return x + pre;
   };
-  long long mine, block_total, incl = 0, total = 0;
+  if (tid == 0) {
+    s->r = 0;
+    s->off = 0;
+    s->per_head = 0;
+    s->q = PagedReq{0, 0, 0};
+  }
+  long long block_total, incl = 0, total = 0;
   for (int p = 0; p < passes; ++p) {
-    incl = scan(p, mine, total, block_total);
+    incl = scan(p, total, block_total);
     total += block_total;
   }
   out.total = total;
@@ -243,25 +253,24 @@ __device__ PagedShare paged_find_share(const PagedBatch& b, const Cost& cost, in
     out.lo = paged_cut(total, cta, out.n_share);
     out.hi = paged_cut(total, cta + 1, out.n_share);
   }
-  if (tid == 0) {
-    s->r = 0;
-    s->off = 0;
-  }
-  __syncthreads();
   long long carry = 0;
   for (int p = 0; p < passes; ++p) {
     if (passes > 1) {
-      incl = scan(p, mine, carry, block_total);
+      incl = scan(p, carry, block_total);
       carry += block_total;
     }
     if (mine > 0 && out.lo >= incl - mine && out.lo < incl) {
       s->r = p * T + tid;
       s->off = out.lo - (incl - mine);
+      s->per_head = per_head;
+      s->q = q;
     }
   }
   __syncthreads();
   out.r = s->r;
   out.off = s->off;
+  out.per_head = s->per_head;
+  out.q = s->q;
   return out;
 }
 
@@ -284,12 +293,10 @@ struct PagedWalk : PagedWalkState {
     hi = s.hi;
     r = s.r;
     h = tile = nb = b0 = b1 = 0;
-    q = PagedReq{0, 0, 0};
+    q = s.q;
     if (cur >= hi) return;
-    q = paged_request(b, r);
-    const long long per_head = cost.before(q, cost.tiles(q));
-    h = int(s.off / per_head);
-    const long long rest = s.off - h * per_head;
+    h = s.off < (1ll << 32) && s.per_head < (1ll << 32) ? int(unsigned(s.off) / unsigned(s.per_head)) : int(s.off / s.per_head);
+    const long long rest = s.off - h * s.per_head;
     // last tile whose start is <= rest: 32 candidates a round, one per lane
     int lo = 0, n = cost.tiles(q);
     const int lane = threadIdx.x & 31;

@@ -55,7 +55,7 @@ struct KeyCost {
     if (causal && k > i1) s -= stair_sum(k - i1, T, kKeys, unsigned(i1 * kKeys - base)) * per_token;
     return s;
   }
-  __device__ __forceinline__ long long of_request(const PagedReq& q) const { return takes(q) ? before(q, tiles(q)) * Hkv : 0; }
+  __device__ __forceinline__ long long per_head(const PagedReq& q) const { return takes(q) ? before(q, tiles(q)) : 0; }
 };
 
 struct Piece {
@@ -71,11 +71,12 @@ struct Smem {
   PagedWalkState walk;
   Piece pieces[kBatch];
   PagedFindSmem find;
-  float neg_lse[kStages][kRows];
+  alignas(16) float neg_lse[kStages][kRows];      // read four at a time
   int last[kStages][kRows];
 };
 constexpr uint32_t kOffMisc = (kOffBars + kNumBars * 8 + 15) & ~15u;
 constexpr uint32_t kSmemBytes = kOffMisc + uint32_t(sizeof(Smem)) + 1024;
+static_assert(alignof(Smem) == 16 && kOffMisc % 16 == 0, "alignment of neg_lse");
 static_assert(2 * kSmemBytes <= 226 * 1024, "two CTAs per SM");
 
 __device__ __forceinline__ uint64_t desc_rows(uint32_t tile, int ks) {
