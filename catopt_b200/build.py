@@ -15,6 +15,7 @@ from pathlib import Path
 HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 LIB = HERE / "libcatopt_b200.so"
+HOST = HERE / "_host.so"
 
 SOURCES = [
     "verify_reduce.cu",
@@ -93,7 +94,27 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     if procs or not LIB.exists():
         cmd = [_nvcc(), "-Wno-deprecated-gpu-targets", "-shared", "-o", str(LIB), *map(str, objs), "-lcudart"]
         subprocess.check_call(cmd)
+    _build_host(force)
     return LIB
+
+
+def _build_host(force: bool) -> None:
+    """``_host.so``: the Python module of ``host_calls.cpp``, against torch's headers and the library beside it."""
+    src = CSRC / "host_calls.cpp"
+    if not force and not _stale(HOST, src):
+        return
+    import sysconfig
+
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(_nvcc()).resolve().parent.parent if Path(_nvcc()).exists() else Path("/usr/local/cuda")
+    include = [root / "include", root / "include/torch/csrc/api/include", sysconfig.get_paths()["include"], cuda / "include"]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           *(x for i in include for x in ("-isystem", str(i))), str(src), "-o", str(HOST),
+           f"-L{HERE}", "-l:libcatopt_b200.so", "-Wl,-rpath,$ORIGIN", f"-L{root / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu",
+           "-lc10", "-lc10_cuda"]
+    subprocess.check_call(cmd)
 
 
 if __name__ == "__main__":

@@ -681,6 +681,18 @@ def gated_contract(s: torch.Tensor, g: torch.Tensor, v: torch.Tensor) -> torch.T
 # --------------------------------------------------------------------------- paged cache
 # A step of a decode loop costs the GPU a few microseconds, so these wrappers keep their checks cheap: one call
 # per tensor for its place, no views, the stream's handle without a stream object.
+@functools.cache
+def _host(name: str):
+    """``name`` of ``host_calls.cpp``: checks and launch of a call that is in order as it stands; NotImplemented for any
+    other, which then goes through the rules below."""
+    _lib.load()
+    try:
+        from . import _host as module
+    except ModuleNotFoundError as e:
+        raise B200Error("_host.so is not built (python -m catopt_b200.build)") from e
+    return getattr(module, name)
+
+
 def _here(what: str, dev: int, *tensors: torch.Tensor) -> None:
     for t in tensors:
         if not isinstance(t, torch.Tensor) or not t.is_cuda:
@@ -794,6 +806,12 @@ def paged_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_pag
     rotary/2)``, or ``(2i, 2i+1)`` if ``interleaved``.  ``weights`` (float32 ``[n_pages, Hkv, page_size]``) is
     zeroed at the new slots.  Returns the normed and rotated ``q`` (rows behind ``cu_q[R]`` are not written); ``out`` may
     be a contiguous ``q`` itself."""
+    res = _host("paged_append")(_status_words, q, k, v, k_pages, v_pages, block_table, seq_lens, cu_q, q_weight, k_weight, eps, cos, sin,
+                                positions, interleaved, weights, out)
+    if res is not NotImplemented:
+        if res.__class__ is int:
+            check(res, "cb2_paged_append")
+        return res
     what = "paged_append"
     dev = _current(what, k_pages)
     n_pages, hkv, ps, d, ks, vs = _pools(what, dev, k_pages, v_pages)
@@ -856,6 +874,11 @@ def om_paged_fwd(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     new tokens and cached keys (``max_k`` defaults to what the table holds); the scratch grows with them.
     ``weights`` (float32 ``[n_pages, Hkv, page_size]``): the softmax probability that every cached key gets, summed
     over rows and the heads of its group, is added to it (requests of one call must not share pages then).  ``scale`` defaults to ``1/sqrt(d)``."""
+    res = _host("om_paged_fwd")(_status_words, q, k_pages, v_pages, block_table, seq_lens, cu_q, max_q, max_k, scale, causal, weights, out)
+    if res is not NotImplemented:
+        if res.__class__ is int:
+            check(res, "cb2_om_paged_fwd")
+        return res
     what = "om_paged_fwd"
     dev = _current(what, k_pages)
     n_pages, hkv, ps, d, ks, vs = _pools(what, dev, k_pages, v_pages)
@@ -894,6 +917,11 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, weights: torch.Ten
     ``weights`` are copied to the pages ``new_table`` (int32 ``[R, >= ceil(budget / page_size)]``) of the same pools,
     none of which may belong to a request of this call; the old pages stay as they are.  Returns ``(kept, new_lens)``:
     int32 ``[R, Hkv, budget]``, the old slot of every new one and -1 behind the last, and int32 ``[R]``."""
+    res = _host("paged_evict")(_status_words, k_pages, v_pages, weights, block_table, seq_lens, new_table, budget, keep_first, keep_last, max_k)
+    if res is not NotImplemented:
+        if res.__class__ is int:
+            check(res, "cb2_paged_evict")
+        return res
     what = "paged_evict"
     dev = _current(what, k_pages)
     n_pages, hkv, ps, d, ks, vs = _pools(what, dev, k_pages, v_pages)

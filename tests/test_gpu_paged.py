@@ -490,3 +490,63 @@ def test_wrong_arguments_are_refused(dev):
         with pytest.raises(B200Error):
             ops.paged_evict(c["k"], c["v"], w, c["table"], c["lens"], to, **bad)
     ops.check_device_status(dev)
+
+
+def test_one_step_calls_and_the_wrappers_agree(dev, monkeypatch):
+    """A call in order is checked and launched in one step (host_calls.cpp); the wrapper's own rules, when they are
+    gone through, give the same answer.  What needs the wrapper is left to it."""
+    from catopt_b200 import ops
+
+    ops.device_status(dev)
+    lens, new = [70, 33], [5, 1]
+    c = ref.make_cache(lens, 2, 16, 64, BF, dev, 3, fill=0.0)
+    cu = ref.offsets(new, dev)
+    g = torch.Generator(device=dev).manual_seed(4)
+    q, k, v = (torch.randn(6, h, 64, generator=g, device=dev).to(BF) for h in (4, 2, 2))
+    cos, sin = (torch.randn(80, 16, generator=g, device=dev) for _ in range(2))
+    pos = torch.arange(6, dtype=torch.int32, device=dev)
+    qw, kw = (torch.randn(64, generator=g, device=dev).to(BF) for _ in range(2))
+    weights = torch.rand(c["k"].shape[:3], generator=g, device=dev)
+    free = [p for p in range(c["k"].shape[0]) if p not in set(c["table"].flatten().tolist())][:2]
+    assert len(free) == 2
+    to = torch.tensor([[p] for p in free], dtype=torch.int32, device=dev)
+
+    def run(**kw_attend):
+        kp, vp, w = c["k"].clone(), c["v"].clone(), weights.clone()
+        turned = ops.paged_append(q, k, v, kp, vp, c["table"], c["lens"], cu, q_weight=qw, k_weight=kw, cos=cos, sin=sin, positions=pos,
+                                  weights=w)
+        none = ops.paged_append(None, k, v, kp, vp, c["table"], c["lens"], cu)
+        out = torch.empty_like(q)
+        o = ops.om_paged_fwd(turned, kp, vp, c["table"], c["lens"], cu, 5, weights=w, out=out, **kw_attend)
+        o2 = ops.om_paged_fwd(turned, kp, vp, c["table"], c["lens"], cu, 5, max_k=70, scale=0.25, causal=False)
+        kept, lens2 = ops.paged_evict(kp, vp, w, c["table"], c["lens"], to, 16, keep_first=2, keep_last=4)
+        assert none is None and o is out
+        ops.check_device_status(dev)
+        return [turned, o, o2, kept, lens2, kp, vp, w]
+
+    taken = []
+    with monkeypatch.context() as m:
+        host = ops._host
+        m.setattr(ops, "_host", lambda name: lambda *a: taken.append(host(name)(*a)) or taken[-1])
+        one = run()
+    assert len(taken) == 5 and not any(x is NotImplemented for x in taken)
+    with monkeypatch.context() as m:
+        m.setattr(ops, "_host", lambda name: lambda *a: NotImplemented)
+        other = run()
+    for a, b in zip(one, other):
+        assert torch.equal(a.nan_to_num(), b.nan_to_num())
+    # not in order as they stand: rows to copy first, numbers of other kinds, gradients, shapes
+    attend = (c["k"], c["v"], c["table"], c["lens"], cu)
+    f = host("om_paged_fwd")
+    assert f(ops._status_words, q.mT.contiguous().mT, *attend, 5, None, None, True, None, None) is NotImplemented
+    assert f(ops._status_words, q, *attend, True, None, None, True, None, None) is NotImplemented
+    assert f(ops._status_words, q, *attend, 5, None, 1, True, None, None) is NotImplemented
+    assert f(ops._status_words, q, *attend, 5, 81 * 16, None, True, None, None) is NotImplemented
+    assert f(ops._status_words, q, *attend, 5, None, None, True, weights[1:], None) is NotImplemented
+    assert f({}, q, *attend, 5, None, None, True, None, None) is NotImplemented
+    assert f(ops._status_words, q.clone().requires_grad_(), *attend, 5, None, None, True, None, None) is NotImplemented
+    assert f(ops._status_words, q[:, :3], *attend, 5, None, None, True, None, None) is NotImplemented
+    with pytest.raises(ops.B200Error):
+        ops.om_paged_fwd(q, *attend, 5, out=q)           # declined by the entry point
+    with pytest.raises(ops.B200Error):
+        ops.om_paged_fwd(q, *attend, 5, scale=float("nan"))

@@ -127,3 +127,16 @@ def test_cache_refusals():
     with pytest.raises(B200Error, match="free"):
         c.evict([r], 20)                             # the kept keys need 3 fresh ones
     assert c.length(r) == 60 and c.free_pages == 2
+
+
+def test_host_calls_leave_what_is_not_in_order(lib):
+    """The one-step form of a call declines whatever it does not know, without an exception: the wrapper then says why."""
+    from catopt_b200 import ops
+
+    t = torch.zeros(2, 2, 16, 64)
+    i = torch.zeros(2, 2, dtype=torch.int32)
+    assert ops._host("om_paged_fwd")() is NotImplemented
+    assert ops._host("om_paged_fwd")({}, t[0], t, t, i, i[0], i[0], 1, None, None, True, None, None) is NotImplemented
+    assert ops._host("om_paged_fwd")(*[None] * 13) is NotImplemented
+    assert ops._host("paged_append")(*["x"] * 18) is NotImplemented
+    assert ops._host("paged_evict")({}, t, t, t, i, i[0], i, 1, 0, 0, 1 << 80) is NotImplemented
