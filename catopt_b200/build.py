@@ -3,7 +3,8 @@
 Run as ``python -m catopt_b200.build`` (or call :func:`build`).  nvcc
 cross-compiles without a GPU, so this also works on a CPU-only machine.  The
 library lands beside this file so that it travels with the source tree and the
-ctypes loader in ``_lib.py`` finds it without any install step.
+ctypes loader in ``_lib.py`` finds it without any install step.  ``_host.so``, the Python module
+that checks and launches a paged-cache call in one step, is compiled next to it with g++.
 """
 from __future__ import annotations
 
