@@ -18,6 +18,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "paged_clamp.cuh"
 
 namespace cb2 {
 
@@ -77,21 +78,13 @@ struct PagedRows {
   float scale_log2e;
 };
 
-struct PagedReq {
-  int t0, n, len;     // first row in q, new tokens, cached keys
-};
-
 __device__ __forceinline__ void paged_flag(const PagedBatch& b) {
   if (b.status) atomicExch(b.status, CB2_BAD_INDEX);
 }
 
 __device__ __forceinline__ PagedReq paged_request(const PagedBatch& b, int r) {
-  const int c0 = __ldg(b.cu + r), c1 = __ldg(b.cu + r + 1), l = __ldg(b.lens + r);
   PagedReq q;
-  q.t0 = min(max(c0, 0), b.n_tokens);
-  q.n = min(max(min(c1, b.n_tokens) - q.t0, 0), b.max_q);
-  q.len = min(max(l, 0), b.max_k);
-  if (q.t0 != c0 || q.t0 + q.n != c1 || q.len != l) paged_flag(b);
+  if (!paged_clamp(__ldg(b.cu + r), __ldg(b.cu + r + 1), __ldg(b.lens + r), b.n_tokens, b.max_q, b.max_k, &q)) paged_flag(b);
   return q;
 }
 

@@ -260,6 +260,30 @@ def test_bad_indices_are_reported(dev):
         assert changed == 1                                    # request 0's token; request 1's have no page
 
 
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("n", [8, 200], ids=["step", "chunk"])
+def test_indices_of_any_content_stay_in_bounds(dev, dtype, n):
+    # extremes of int32, whose differences do not fit it: reported, nothing behind the outputs is written
+    from catopt_b200 import B200Error, ops
+
+    lo, hi = -(1 << 31), (1 << 31) - 1
+    c = ref.make_cache([300, 70], 1, 16, 64, dtype, dev, 16, fill=0.0)
+    q = torch.randn(n, 2, 64, device=dev).to(dtype)
+    k = torch.randn(n, 1, 64, device=dev).to(dtype)
+    rest = [torch.full((n + 64, 2, 64), 5.0, dtype=dtype, device=dev) for _ in range(2)]
+    w = torch.zeros(c["k"].shape[:3], device=dev)
+    for cu in ([0, 5, lo], [0, lo, 5], [lo, 5, n], [0, hi, lo], [5, hi, n], [hi, lo, hi]):
+        for lens in ([300, 70], [lo, hi]):
+            cu_q, seq = (torch.tensor(x, dtype=torch.int32, device=dev) for x in (cu, lens))
+            ops.om_paged_fwd(q, c["k"], c["v"], c["table"], seq, cu_q, n, max_k=300, weights=w, out=rest[0][:n])
+            with pytest.raises(B200Error, match="index"):
+                ops.check_device_status(dev)
+            ops.paged_append(q, k, k, c["k"], c["v"], c["table"], seq, cu_q, weights=w, out=rest[1][:n])
+            torch.cuda.synchronize()
+            ops.device_status(dev).zero_()
+            assert all((x[n:] == 5.0).all() for x in rest)
+
+
 # --------------------------------------------------------------------------- append
 @pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("new,start", [([1], [0]), ([3, 0, 1, 20], [5, 0, 16, 30]), ([700, 1, 2500], [0, 31, 8])],

@@ -1,5 +1,8 @@
 """Paged-cache operators without a GPU: what the entry points refuse."""
 import ctypes as C
+import itertools
+import subprocess
+from pathlib import Path
 
 import pytest
 import torch
@@ -140,3 +143,42 @@ def test_host_calls_leave_what_is_not_in_order(lib):
     assert ops._host("om_paged_fwd")(*[None] * 13) is NotImplemented
     assert ops._host("paged_append")(*["x"] * 18) is NotImplemented
     assert ops._host("paged_evict")({}, t, t, t, i, i[0], i, 1, 0, 0, 1 << 80) is NotImplemented
+
+
+# --------------------------------------------------------------------------- index tensors of any content
+CSRC = Path(__file__).resolve().parent.parent / "catopt_b200" / "csrc"
+INT_MIN, INT_MAX = -(1 << 31), (1 << 31) - 1
+
+
+@pytest.fixture(scope="module")
+def clamp(tmp_path_factory):
+    """The kernels' clamp of a request, compiled for the host: ``f(c0, c1, len, n_tokens, max_q, max_k)``."""
+    d = tmp_path_factory.mktemp("clamp")
+    (d / "clamp.cpp").write_text('#include "paged_clamp.cuh"\nextern "C" int clamp(int a, int b, int l, int n, int q, int k, int* out) {\n'
+                                 "  cb2::PagedReq r;\n  const bool ok = cb2::paged_clamp(a, b, l, n, q, k, &r);\n"
+                                 "  out[0] = r.t0, out[1] = r.n, out[2] = r.len;\n  return ok;\n}\n")
+    subprocess.check_call(["g++", "-O2", "-fwrapv", "-shared", "-fPIC", f"-I{CSRC}", str(d / "clamp.cpp"), "-o", str(d / "clamp.so")])
+    f = C.CDLL(str(d / "clamp.so")).clamp
+
+    def call(*a):
+        out = (C.c_int * 3)()
+        ok = f(*map(C.c_int, a), out)
+        return bool(ok), *out
+
+    return call
+
+
+def test_no_index_leads_out_of_bounds(clamp):
+    values = [INT_MIN, INT_MIN + 1, INT_MIN + 5, INT_MIN + 9, -900, -1, 0, 1, 5, 7, 8, 9, 900, INT_MAX - 8, INT_MAX - 1, INT_MAX]
+    for c0, c1 in itertools.product(values, values):
+        for n_tokens, max_q in ((8, 8), (8, 3), (8, 0), (1, INT_MAX), (INT_MAX, INT_MAX)):
+            ok, t0, n, _ = clamp(c0, c1, 0, n_tokens, max_q, 1)
+            assert 0 <= t0 <= n_tokens and 0 <= n <= max_q and t0 + n <= n_tokens, (c0, c1, n_tokens, max_q, t0, n)
+            good = 0 <= c0 <= c1 <= n_tokens and c1 - c0 <= max_q
+            assert ok == good, (c0, c1, n_tokens, max_q)
+            if good:
+                assert (t0, n) == (c0, c1 - c0)
+    for length in values:
+        for max_k in (1, 8, 1 << 30):
+            ok, _, _, got = clamp(0, 0, length, 8, 8, max_k)
+            assert got == min(max(length, 0), max_k) and ok == (got == length)
