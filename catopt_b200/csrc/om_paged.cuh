@@ -36,7 +36,8 @@ inline bool allow_smem(const void* kernel, int bytes, std::atomic<unsigned long 
 
 // A kernel that reads what the kernel before it leaves is launched while that one still runs (programmatic dependent
 // launch): it waits with after_previous() at its top, and the one before has called let_next() at its own.  Of a chain, every
-// kernel waits in all of its blocks, so what the last one sees is complete.
+// kernel waits in all of its blocks, so what the last one sees is complete.  What the one before writes is read through
+// ordinary pointers: a load that is declared constant (const __restrict__, __ldg) may be moved ahead of the wait.
 __device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

@@ -313,8 +313,7 @@ paged_few_kernel(const PagedRows rows, const PagedPools pools, const PagedBatch 
 constexpr int kWeightThreads = 256, kWeightCtas = 4 * kNumSMs;
 
 __global__ void __launch_bounds__(kWeightThreads)
-paged_few_weights_kernel(const PagedBatch batch, const Cost cost, const float* __restrict__ scores, const float* __restrict__ lse2,
-                         float* __restrict__ weights) {
+paged_few_weights_kernel(const PagedBatch batch, const Cost cost, const float* scores, const float* lse2, float* weights) {
   __shared__ PagedFindSmem find;
   __shared__ float sh_lse[kRT];
   const PagedShare share = paged_find_share<kWeightThreads>(batch, cost, blockIdx.x, gridDim.x, &find);
@@ -327,7 +326,7 @@ paged_few_weights_kernel(const PagedBatch batch, const Cost cost, const float* _
     const float* sc = scores + ((long long)w.r * cost.Hkv + w.h) * cost.few * stride;
     const int n_rows = w.q.n * G, end = min(w.b1 * kKB, w.q.len);
     __syncthreads();
-    if (tid < n_rows) sh_lse[tid] = __ldg(lse2 + (long long)(w.q.t0 + tid / G) * (G * cost.Hkv) + w.h * G + tid % G);
+    if (tid < n_rows) sh_lse[tid] = lse2[(long long)(w.q.t0 + tid / G) * (G * cost.Hkv) + w.h * G + tid % G];
     __syncthreads();
     for (int j = w.b0 * kKB + 4 * tid; j < end; j += 4 * kWeightThreads) {
       const int page = paged_page(batch, w.r, j >> batch.page_log2);
@@ -336,7 +335,7 @@ paged_few_weights_kernel(const PagedBatch batch, const Cost cost, const float* _
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
       for (int row = 0; row < n_rows; ++row) {
-        const float4 x = __ldg(reinterpret_cast<const float4*>(sc + row * stride + j));
+        const float4 x = *reinterpret_cast<const float4*>(sc + row * stride + j);
         const float z = sh_lse[row];
         sum[0] += ex2_approx(x.x - z);
         sum[1] += ex2_approx(x.y - z);

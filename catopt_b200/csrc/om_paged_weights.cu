@@ -364,8 +364,7 @@ paged_weights_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
 
 // Adds up the partial sums of key blocks that were cut between shares, in share order.
 __global__ void __launch_bounds__(kKeys)
-paged_weights_join_kernel(const PagedBatch batch, int Hkv, const PagedJoin* __restrict__ joins, const float* __restrict__ parts,
-                          float* __restrict__ weights) {
+paged_weights_join_kernel(const PagedBatch batch, int Hkv, const PagedJoin* joins, const float* parts, float* weights) {
   const int c = blockIdx.x, key = threadIdx.x;
   after_previous();
   const PagedJoin jn = joins[c];

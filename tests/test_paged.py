@@ -1,6 +1,7 @@
 """Paged-cache operators without a GPU: what the entry points refuse."""
 import ctypes as C
 import itertools
+import re
 import subprocess
 from pathlib import Path
 
@@ -182,3 +183,25 @@ def test_no_index_leads_out_of_bounds(clamp):
         for max_k in (1, 8, 1 << 30):
             ok, _, _, got = clamp(0, 0, length, 8, 8, max_k)
             assert got == min(max(length, 0), max_k) and ok == (got == length)
+
+
+# --------------------------------------------------------------------------- kernels launched while the one before runs
+def waiting_kernels():
+    """``(name, parameters, body)`` of every kernel that waits for the one before it inside itself."""
+    for path in sorted(CSRC.glob("*.cu")):
+        text = path.read_text()
+        for m in re.finditer(r"__global__.*?(\w+)\(([^()]*(?:\([^()]*\)[^()]*)*)\)\s*\{\n(.*?)\n\}\n", text, re.S):
+            if "after_previous()" in m[3]:
+                yield m[1], m[2], m[3]
+
+
+def test_kernels_that_wait_read_ordinarily():
+    """What the kernel before writes while this one is resident is not constant for its lifetime: neither ``const
+    __restrict__`` nor ``__ldg``, which may be moved before the wait.  (Index tensors of the batch, which no
+    kernel of the chain writes, are read so.)"""
+    found = {}
+    for name, params, body in waiting_kernels():
+        constant = [p.strip() for p in params.split(",") if "__restrict__" in p and "const" in p.split("*")[0]]
+        loads = [x for x in re.findall(r"__ldg\((.*)", body) if not re.match(r"(reinterpret_cast<[^>]*>\()?(batch\.(lens|cu|table)|a\.to_table)\b", x)]
+        found[name] = constant + loads
+    assert len(found) >= 5 and not any(found.values()), {k: v for k, v in found.items() if v}
