@@ -248,7 +248,7 @@ PyObject* paged_evict(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const int* table = dense<int>(a[4], dev, at::kInt, {R, max_pages});
     const int* lens = dense<int>(a[5], dev, at::kInt, {R});
     const int* to = dense<int>(a[6], dev, at::kInt, {R, new_pages});
-    const int budget = bounded(a[7], INT_MAX), first = bounded(a[8], budget), last = bounded(a[9], budget);
+    const int budget = bounded(a[7], 1 << 30), first = bounded(a[8], budget), last = bounded(a[9], budget);
     need(budget >= 1 && new_pages * p.ps >= budget && (a[10] != Py_None || max_pages * p.ps <= most));
     const int max_k = a[10] == Py_None ? int(max_pages * p.ps) : bounded(a[10], most);
     int* word = status(a[0], dev);

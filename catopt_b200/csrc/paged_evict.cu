@@ -242,7 +242,8 @@ extern "C" int cb2_paged_evict(void* k_pages, void* v_pages, long long k_page_st
   if (page_size < 8 || page_size > 1024 || (page_size & (page_size - 1)) || max_k < 1 || max_k > (1 << 30) ||
       int64_t(max_pages) * page_size < max_k)
     return CB2_BAD_SHAPE;
-  if (budget < 1 || keep_first < 0 || keep_last < 0 || int64_t(keep_first) + keep_last > budget || int64_t(new_pages) * page_size < budget)
+  // (the kernels step over the budget in 32 bits)
+  if (budget < 1 || budget > (1 << 30) || keep_first < 0 || keep_last < 0 || int64_t(keep_first) + keep_last > budget || int64_t(new_pages) * page_size < budget)
     return CB2_BAD_SHAPE;
   const long long page = (long long)Hkv * page_size * d;
   if (k_page_stride < page || v_page_stride < page) return CB2_BAD_SHAPE;

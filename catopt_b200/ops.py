@@ -935,7 +935,7 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, weights: torch.Ten
     w_ptr = _dense(what, dev, "weights", weights, torch.float32, (n_pages, hkv, ps))
     _no_grad_asked(what, k_pages, v_pages, weights)
     max_k = _bound(what, "max_k", max_pages * ps if max_k is None else max_k, min(max_pages * ps, 1 << 30))
-    budget = _bound(what, "budget", budget, (1 << 31) - 1)
+    budget = _bound(what, "budget", budget, 1 << 30)
     keep_first, keep_last = (_bound(what, name, x, budget) for name, x in (("keep_first", keep_first), ("keep_last", keep_last)))
     if budget < 1 or new_pages * ps < budget:
         raise B200Error(f"{what}: a budget of {budget} keys does not fit {new_pages} pages of {ps}")

@@ -473,7 +473,8 @@ int cb2_om_paged_fwd(const void* q, long long q_token_stride, long long q_head_s
  * new_table[r][..] (int32 [R, new_pages]) of the same pools; none of them may be among the pages of
  * a request of this call.  The old pages stay as they are, so requests may share them.
  * kept: int32 [R, Hkv, budget], the old slot of every new one, -1 behind the last; new_lens: int32
- * [R] = min(seq_lens, budget).  max_k: no request has more cached keys.  No scratch. */
+ * [R] = min(seq_lens, budget).  max_k: no request has more cached keys.  budget <= 2^30.  No
+ * scratch. */
 int cb2_paged_evict(void* k_pages, void* v_pages, long long k_page_stride, long long v_page_stride, float* weights,
                     const int* block_table, const int* seq_lens, const int* new_table, int* kept, int* new_lens, int R,
                     int Hkv, int d, int page_size, int n_pages, int max_pages, int new_pages, int max_k, int budget,

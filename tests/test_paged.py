@@ -61,6 +61,12 @@ def test_evict_refusals(lib, change, want):
     assert lib.cb2_paged_evict(*{**EVICT, **change}.values()) == want
 
 
+@pytest.mark.parametrize("budget", [(1 << 30) + 1, (1 << 31) - 1024, (1 << 31) - 1])
+def test_evict_budget_bound(lib, budget):
+    # a kernel's loop over the budget steps by its threads in 32 bits
+    assert lib.cb2_paged_evict(*{**EVICT, "budget": budget, "new_pages": 1 << 27}.values()) == SHAPE
+
+
 def test_no_tokens_is_no_launch(lib):
     assert lib.cb2_om_paged_fwd(*{**ATTEND, "n": 0, "q": None, "o": None, "scratch": None, "bytes": 0}.values()) == 0
     assert lib.cb2_paged_append(*{**APPEND, "n": 0, "q": None, "k": None, "v": None}.values()) == 0
