@@ -4,8 +4,10 @@
 // Keys are the long side of both products, so they take the M side of m16n8k16: S^T[16 keys, 8 rows] = K Q^T
 // and O^T[16 columns, 8 rows] += V^T P^T; a group of four to eight query heads fills the N side, where the
 // other orientation would leave half of the rows empty.  K comes by ldmatrix, V^T by its transposing form, and P
-// turns from accumulator into operand by one 8x8 register transpose a half.  The pace is set by memory: per 16
-// keys of d = 128 a warp issues about 90 instructions for 8 KB.
+// turns from accumulator into operand by one 8x8 register transpose a half.  A probability is split
+// into two bf16 halves, p = hi + lo up to 2^-16 of it, and V^T multiplied by both, since one half alone would lose more than the
+// rounding of o (error against 64 bits 2.1e-3 in place of 1.7e-3; 32 single tokens on up to 16384 keys: 197 us a call with
+// one half, 199 with two).  The pace is set by memory: per 16 keys of d = 128 a warp issues about 110 instructions for 8 KB.
 //
 // Warps are independent: each streams every fourth 16-key tile of the CTA's piece through its own ring of
 // asynchronous copies (two CTAs of four warps per SM keep 128 KB in flight) and keeps its own (m, l, O); they
@@ -226,7 +228,7 @@ paged_few_kernel(const PagedRows rows, const PagedPools pools, const PagedBatch 
             }
           }
       }
-      uint32_t pf[NB][2];
+      uint32_t pf[NB][2], pl[NB][2];
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
         float p[4];
@@ -236,8 +238,12 @@ paged_few_kernel(const PagedRows rows, const PagedPools pools, const PagedBatch 
           p[e] = ex2_approx(s[b][e] - ref);
           l[b][e & 1] += p[e];
         }
-        pf[b][0] = transpose8x8(pack_bf16x2(p[0], p[1]));
-        pf[b][1] = transpose8x8(pack_bf16x2(p[2], p[3]));
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t hi = pack_bf16x2(p[2 * e], p[2 * e + 1]);
+          pf[b][e] = transpose8x8(hi);
+          pl[b][e] = transpose8x8(pack_bf16x2(p[2 * e] - bf16lo_to_f32(hi), p[2 * e + 1] - bf16hi_to_f32(hi)));
+        }
       }
       {
         const int row = (lane & 7) + (lane >> 4) * 8, half = (lane >> 3) & 1;
@@ -247,7 +253,10 @@ paged_few_kernel(const PagedRows rows, const PagedPools pools, const PagedBatch 
             uint32_t a[4];
             ldsm4_t(v_tile + row * R::kRow + (((2 * ks + half) ^ (row & 7)) << 4), a);
 #pragma unroll
-            for (int b = 0; b < NB; ++b) mma16816(acc[ks][b], a, pf[b]);
+            for (int b = 0; b < NB; ++b) {
+              mma16816(acc[ks][b], a, pf[b]);
+              mma16816(acc[ks][b], a, pl[b]);
+            }
           }
         }
       }

@@ -9,6 +9,9 @@
 // block's P after every product: one exponential per score (16 a clock and SM) and the products (1024 clocks per
 // 128 x 128 scores either way) overlap.  The reference point m follows the maximum lazily (when it moved by
 // more than 2^8), so O is rarely rescaled, and only then does the softmax wait for the product before.
+// P is rounded once, to bf16, as the dense chunks' kernel of this library does (error against 64 bits 2.4e-3, of which the
+// rounding of o alone is 1.7e-3).  A second half of it (p = hi + lo, half as many products again) takes two chunks of 2048 on
+// 8192 keys from 414 to 518 us a call, chunks of 1024 with weights from 207 to 237, a mixed batch of 24 from 39 to 43.
 // Only a block that some row of the tile may not see whole is masked, per element.  Of the last block of a
 // request the value rows behind its length are zeroed in shared memory, since 0 x NaN is NaN.
 //

@@ -64,6 +64,18 @@ def test_attention_head_widths(dev, dtype, d):
     run_attend(dev, [1, 2, 1], [90, 300, 70], 2, 3, d, 8, dtype, weights=True)
 
 
+@pytest.mark.parametrize("d,group", [(64, 4), (128, 1), (40, 8), (96, 7), (128, 16)])
+@pytest.mark.parametrize("new,lens", [([1, 1, 1], [700, 3, 64]), ([2, 1], [300, 33]), ([1], [9000])], ids=["steps", "two", "long"])
+def test_few_rows_keep_their_probabilities(dev, d, group, new, lens):
+    # the product with V takes more of a probability than bf16 holds (two halves: 2^-16), and o is rounded once
+    if max(new) * group > 16:
+        new = [1] * len(new)
+    c, q, o, _ = run_attend(dev, new, lens, 2, group, d, 16, BF, seed=d)
+    want, tol, _, _ = ref.attend(q, c, new, lens, d ** -0.5, True)
+    spread, _, _, _ = ref.attend(q, {**c, "v": c["v"].abs()}, new, lens, d ** -0.5, True)
+    close(o, want, tol - spread * (ref.half_step(BF) - 2.0 ** -16), "o")
+
+
 @pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("new", [1, 40], ids=["step", "chunk"])
 def test_a_nan_that_is_seen_shows(dev, dtype, new):
