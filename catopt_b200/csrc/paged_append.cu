@@ -109,6 +109,7 @@ __device__ __forceinline__ void turn(float (&x)[8], bool norm, const float (&w)[
   if (MODE == kInterleaved) {
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
+      if (gl * 8 + i >= rot) break;          // columns behind the rotation stay what they are (0 x Inf is NaN)
       const float a = x[i], b = x[i + 1];
       x[i] = fmaf(-b, sn[i >> 1], a * cs[i >> 1]);
       x[i + 1] = fmaf(a, sn[i >> 1], b * cs[i >> 1]);

@@ -349,6 +349,26 @@ def test_append(dev, dtype, new, start, d, rot, interleaved, norm, strided):
     assert torch.equal(c["v"], want_v) and torch.equal(w, want_w)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("d,rot", [(64, 40), (40, 4), (128, 126)])
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("fill", [float("inf"), float("nan")], ids=["inf", "nan"])
+def test_append_leaves_columns_behind_the_rotation(dev, dtype, d, rot, interleaved, fill):
+    # columns that are not rotated come out as they went in, whatever stands beside them
+    from catopt_b200 import ops
+
+    c = ref.make_cache([9], 2, 16, d, dtype, dev, 17, fill=0.0)
+    q, k = (torch.randn(9, h, d, device=dev).to(dtype) for h in (3, 2))
+    for x in (q, k):
+        x[..., rot::2] = fill
+    ang = torch.rand(9, rot // 2, device=dev) * 6
+    got = ops.paged_append(q, k, k, c["k"], c["v"], c["table"], c["lens"], ref.offsets([9], dev), cos=ang.cos(), sin=ang.sin(),
+                           positions=torch.arange(9, dtype=torch.int32, device=dev), interleaved=interleaved)
+    stored = c["k"][c["table"][0, 0].long(), :, :9].transpose(0, 1)
+    for x, y in ((q, got), (k, stored)):
+        assert torch.equal(x[..., rot:].nan_to_num(7.0), y[..., rot:].nan_to_num(7.0)) and y[..., :rot].isfinite().all()
+
+
 # --------------------------------------------------------------------------- evict
 @pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("lens,budget,first,last", [
