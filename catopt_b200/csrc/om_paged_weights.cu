@@ -8,7 +8,7 @@
 // see it; a unit cut between shares leaves 128 partial sums a share, added in share order.
 //
 // A row tile is T = 64 / G whole tokens of a group (64 heads of one token when G > 64), so that one TMA box of q brings
-// it; columns past T G stay zero.  Roles: warp 0 = the key block (pages by TMA), warp 1 = MMA issue and TMEM owner,
+// it; columns past T G stay zero and count as hidden.  Roles: warp 0 = the key block (pages by TMA), warp 1 = MMA issue and TMEM owner,
 // warps 2..5 = sums, warp 6 = row tiles, their -lse and the last slot each row sees (copying the rows by 16-byte
 // asynchronous copies took 2.8 k cycles a tile and set the pace).  A ring of four stages holds row tile, -lse and S
 // together; two CTAs share an SM.  Every wait is bounded.
@@ -212,6 +212,7 @@ paged_weights_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
       const int q4 = warp & 3, key = q4 * 32 + lane;
       const uint32_t lane_base = tmem + (uint32_t(q4 * 32) << 16);
       const uint64_t scale2 = umma::f2_pack(rows.scale_log2e, rows.scale_log2e);
+      const int used = G < kRows ? cost.T * G : kRows;        // columns of a tile that are rows
       for (int p = 0; p < count; ++p) {
         const Piece* pc = &sh->pieces[p];
         const int tiles = pc->tiles, j = pc->k0 + key, base = pc->len - pc->n;
@@ -238,6 +239,13 @@ paged_weights_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
 #pragma unroll
               for (int c = 0; c < 32; ++c)
                 if (sh->last[st][cb * 32 + c] < j) sv[cb][c] = 0xff800000u;
+          }
+          // columns past T G hold rows of zeros, whose product with a key of infinities is NaN: no score either.  (They
+          // lie in the second half: 33 columns at least are used.)
+          if (used < kRows) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              if (32 + c >= used) sv[1][c] = 0xff800000u;
           }
           uint64_t s2[2] = {0ull, 0ull};
 #pragma unroll

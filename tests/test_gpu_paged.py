@@ -152,6 +152,27 @@ def test_many_heads_on_one(dev, dtype, group):
     run_attend(dev, [1, 0, 7, 40], [300, 5, 200, 150], 1 if group > 20 else 2, group, 64, 16, dtype, weights=True)
 
 
+@pytest.mark.parametrize("group", [3, 5, 7, 33, 60])
+def test_weights_beside_a_key_of_infinities(dev, group):
+    # a key that every row scores -inf gets nothing, as one that every row scores very low does
+    from catopt_b200 import ops
+
+    lens, new = [400], [100]
+    c = ref.make_cache(lens, 2, 16, 64, BF, dev, 18)
+    g = torch.Generator(device=dev).manual_seed(19)
+    q = torch.randn(100, 2 * group, 64, generator=g, device=dev).to(BF)
+    q[..., 0] = -1.0
+    page, at = c["table"][0, 70 // 16].long(), 70 % 16
+    got = []
+    for x in (float("inf"), 1e5):
+        c["k"][page, :, at, 0] = x
+        w = torch.zeros(c["k"].shape[:3], device=dev)
+        o = ops.om_paged_fwd(q, c["k"], c["v"], c["table"], c["lens"], ref.offsets(new, dev), 100, max_k=400, weights=w)
+        assert o.isfinite().all() and (w[page, :, at] == 0).all()
+        got.append((o, w))
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+
+
 def test_weights_when_the_bound_on_keys_is_far_off(dev):
     # scores of 2.3 million possible keys are not kept: the weights are computed from the keys again
     from catopt_b200 import ops
