@@ -148,6 +148,8 @@ paged_append_kernel(const AppendArgs a, const PagedBatch batch) {
   // the request of each token: every thread looks at one request, whose token range may meet this CTA's
   for (int r = tid; r < batch.R; r += kThreads) {
     const int c0 = __ldg(batch.cu + r), c1 = __ldg(batch.cu + r + 1);
+    // (offsets out of order, or behind the batch, may meet no CTA's tokens)
+    if (blockIdx.x == 0 && (c0 < 0 || c1 < c0 || c1 > batch.n_tokens)) paged_flag(batch);
     if (c1 <= t_first || c0 >= t_first + t_count) continue;
     const PagedReq q = paged_request(batch, r);
     for (int t = max(q.t0, t_first); t < min(q.t0 + q.n, t_first + t_count); ++t) {

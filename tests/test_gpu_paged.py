@@ -390,6 +390,17 @@ def test_append_leaves_columns_behind_the_rotation(dev, dtype, d, rot, interleav
         assert torch.equal(x[..., rot:].nan_to_num(7.0), y[..., rot:].nan_to_num(7.0)) and y[..., :rot].isfinite().all()
 
 
+@pytest.mark.parametrize("cu", [[0, 5, 3, 8], [0, 8, 2, 8], [3, 0, 8, 8], [0, 8, 9, 9], [0, 8, 8, -1]])
+def test_append_reports_offsets_out_of_order(dev, cu):
+    from catopt_b200 import B200Error, ops
+
+    c = ref.make_cache([40, 70, 30], 2, 16, 64, F32, dev, 6, fill=0.0)
+    k = torch.randn(8, 2, 64, device=dev)
+    ops.paged_append(None, k, k, c["k"], c["v"], c["table"], c["lens"], torch.tensor(cu, dtype=torch.int32, device=dev))
+    with pytest.raises(B200Error, match="index"):
+        ops.check_device_status(dev)
+
+
 # --------------------------------------------------------------------------- evict
 @pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("lens,budget,first,last", [
