@@ -156,7 +156,7 @@ class PagedCache:
     def evict(self, requests: list[int], budget: int, *, keep_first: int = 0, keep_last: int = 0) -> list[torch.Tensor]:
         """Cut the given requests to ``budget`` keys in every layer (``ops.paged_evict``; those that are not longer
         stay as they are).  The kept keys move to fresh pages, as many as the budget fills, and the old pages are free
-        afterwards.  Returns the kept slots per layer, ``[cut requests, Hkv, budget]``, in the order of ``requests``."""
+        afterwards: the free pages have to serve one request, those that it leaves serve the next.  Returns the kept slots per layer, ``[cut requests, Hkv, budget]``, in the order of ``requests``."""
         if self.weights is None:
             raise B200Error("PagedCache.evict: the cache does not track attention weights")
         if budget < 1 or keep_first < 0 or keep_last < 0 or keep_first + keep_last > budget:
@@ -164,11 +164,18 @@ class PagedCache:
         if len(set(requests)) != len(requests):
             raise B200Error("PagedCache.evict: a request is named twice")
         cut = [r for r in requests if self.length(r) > budget]
-        if not cut:
-            return []
         each = self._pages_for(budget)
-        if each * len(cut) > len(self._free):
-            raise B200Error(f"PagedCache.evict: {each * len(cut)} pages wanted, {len(self._free)} free")
+        if cut and each > len(self._free):
+            raise B200Error(f"PagedCache.evict: {each} pages wanted for a request, {len(self._free)} free")
+        groups = []
+        while cut:          # as many at a time as the free pages serve: each gives back no fewer than it takes
+            n = len(self._free) // each
+            groups.append(self._cut(cut[:n], budget, keep_first, keep_last))
+            cut = cut[n:]
+        return groups[0] if len(groups) == 1 else [torch.cat(x) for x in zip(*groups)]
+
+    def _cut(self, cut: list[int], budget: int, keep_first: int, keep_last: int) -> list[torch.Tensor]:
+        each = self._pages_for(budget)
         fresh = [[self._free.pop() for _ in range(each)] for _ in cut]
         width = max(len(self._pages[r]) for r in cut)
         table, lens, to = self._to_device([p for r in cut for p in self._pages[r] + [-1] * (width - len(self._pages[r]))],

@@ -139,6 +139,45 @@ def test_cache_refusals():
     assert c.length(r) == 60 and c.free_pages == 2
 
 
+def fake_evict(k, v, w, table, lens, to, budget, *, keep_first, keep_last, max_k):
+    """paged_evict on the host."""
+    import paged_reference as ref
+
+    page, kept = k.shape[2], torch.full((len(lens), k.shape[1], budget), -1, dtype=torch.int32)
+    for r, n in enumerate(lens.tolist()):
+        ids = table[r, :(n + page - 1) // page].long()
+        assert (ids >= 0).all() and not set(to[r].tolist()) & set(table.flatten().tolist())
+        for h in range(k.shape[1]):
+            j = torch.tensor(ref.keep(w[ids, h].reshape(-1), n, budget, keep_first, keep_last))
+            kept[r, h, :len(j)] = j
+            i = torch.arange(len(j))
+            for t in (k, v, w):
+                t[to[r].long()[i // page], h, i % page] = t[ids[j // page], h, j % page]
+    return kept, lens.clamp(max=budget)
+
+
+def test_cache_evicts_when_few_pages_are_free(monkeypatch):
+    # one fresh page serves requests one after the other: the pages of one that is cut are there for the next
+    from catopt_b200 import ops
+
+    monkeypatch.setattr(ops, "paged_evict", fake_evict)
+    c = make(n_layers=2)
+    a, b, d = c.open(), c.open(), c.open()
+    s = c.begin({a: 40, b: 24, d: 8})                # 9 of 10 pages
+    g = torch.Generator().manual_seed(1)
+    for t in (*c.k, *c.weights):
+        t.copy_(torch.rand(t.shape, generator=g))
+    before = [[c.k[i][s.table[r, :n // 8].long(), 0].reshape(-1, 8).clone() for r, n in ((0, 40), (1, 24))] for i in range(2)]
+    kept = c.evict([a, b, d], 8, keep_first=1, keep_last=2)
+    assert [c.length(r) for r in (a, b, d)] == [8, 8, 8] and c.free_pages == 7
+    assert [tuple(x.shape) for x in kept] == [(2, 1, 8)] * 2                       # d was not longer
+    s = c.begin({a: 0, b: 0, d: 0})
+    assert len(set(s.table[:, 0].tolist())) == 3
+    for i in range(2):
+        for r in range(2):
+            assert torch.equal(c.k[i][int(s.table[r, 0]), 0], before[i][r][kept[i][r, 0].long()])
+
+
 def test_host_calls_leave_what_is_not_in_order(lib):
     """The one-step form of a call declines whatever it does not know, without an exception: the wrapper then says why."""
     from catopt_b200 import ops
