@@ -99,6 +99,11 @@ class PagedCache:
     def _pages_for(self, n: int) -> int:
         return (n + self.page_size - 1) // self.page_size
 
+    def _fresh(self, skip: int, n: int) -> list[int]:
+        """The ``n`` free pages that are next once ``skip`` have been taken; they stay on the list."""
+        end = len(self._free) - skip
+        return self._free[end - n:end][::-1]
+
     def _to_device(self, *rows: list[int]) -> list[torch.Tensor]:
         """int32 tensors of these values on the device, in one copy that the host does not wait for."""
         flat = torch.tensor([x for r in rows for x in r], dtype=torch.int32)
@@ -119,19 +124,22 @@ class PagedCache:
         need = {r: self._pages_for(self._length[r] + n) - len(self._pages[r]) for r, n in new_tokens.items()}
         if sum(need.values()) > len(self._free):
             raise B200Error(f"PagedCache.begin: {sum(need.values())} pages wanted, {len(self._free)} free")
-        cu, positions = [0], []
+        cu, positions, pages, taken = [0], [], {}, 0
         for r, n in new_tokens.items():
-            for _ in range(need[r]):
-                self._pages[r].append(self._free.pop())
+            pages[r] = self._pages[r] + self._fresh(taken, need[r])
+            taken += need[r]
             positions.extend(range(self._position[r], self._position[r] + n))
-            self._length[r] += n
-            self._position[r] += n
             cu.append(cu[-1] + n)
         requests = tuple(new_tokens)
-        lens = [self._length[r] for r in requests]
-        width = max(1, max(len(self._pages[r]) for r in requests))
-        table = [p for r in requests for p in self._pages[r] + [-1] * (width - len(self._pages[r]))]
+        lens = [self._length[r] + n for r, n in new_tokens.items()]
+        width = max(1, max(map(len, pages.values())))
+        table = [p for x in pages.values() for p in x + [-1] * (width - len(x))]
         t, s, c, p = self._to_device(table, lens, cu, positions)
+        del self._free[len(self._free) - taken:]      # (nothing has changed before, should the copy raise)
+        self._pages.update(pages)
+        for r, n in new_tokens.items():
+            self._length[r] += n
+            self._position[r] += n
         return PagedBatch(requests, t.view(len(requests), width), s, c, p, cu[-1], max(new_tokens.values()), max(1, max(lens)))
 
     def append(self, layer: int, batch: PagedBatch, q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, *,
@@ -176,7 +184,7 @@ class PagedCache:
 
     def _cut(self, cut: list[int], budget: int, keep_first: int, keep_last: int) -> list[torch.Tensor]:
         each = self._pages_for(budget)
-        fresh = [[self._free.pop() for _ in range(each)] for _ in cut]
+        fresh = [self._fresh(i * each, each) for i in range(len(cut))]
         width = max(len(self._pages[r]) for r in cut)
         table, lens, to = self._to_device([p for r in cut for p in self._pages[r] + [-1] * (width - len(self._pages[r]))],
                                           [self._length[r] for r in cut], [p for f in fresh for p in f])
@@ -184,6 +192,7 @@ class PagedCache:
         kept = [ops.paged_evict(self.k[i], self.v[i], self.weights[i], table.view(len(cut), width), lens,
                                 to.view(len(cut), each), budget, keep_first=keep_first, keep_last=keep_last, max_k=max_k)[0]
                 for i in range(len(self.k))]
+        del self._free[len(self._free) - each * len(cut):]      # (nothing has changed before, should a call raise)
         for r, pages in zip(cut, fresh):
             self._free.extend(reversed(self._pages[r]))
             self._pages[r], self._length[r] = pages, budget

@@ -178,6 +178,36 @@ def test_cache_evicts_when_few_pages_are_free(monkeypatch):
             assert torch.equal(c.k[i][int(s.table[r, 0]), 0], before[i][r][kept[i][r, 0].long()])
 
 
+def test_cache_keeps_its_pages_when_a_call_fails(monkeypatch):
+    from catopt_b200 import B200Error, ops
+
+    c = make(n_layers=2)
+    a, b = c.open(), c.open()
+    c.begin({a: 20, b: 24})
+    calls = []
+
+    def failing(*args, **kw):
+        calls.append(0)
+        if len(calls) == 2:                          # the second layer
+            raise B200Error("no")
+        return fake_evict(*args, **kw)
+
+    def state():
+        return list(c._free), {r: list(p) for r, p in c._pages.items()}, dict(c._length), dict(c._position)
+
+    was = state()
+    monkeypatch.setattr(ops, "paged_evict", failing)
+    with pytest.raises(B200Error, match="no"):
+        c.evict([a, b], 8)
+    assert state() == was
+    monkeypatch.setattr(c, "_to_device", lambda *rows: (_ for _ in ()).throw(RuntimeError("no memory")))
+    with pytest.raises(RuntimeError, match="no memory"):
+        c.evict([a, b], 8)
+    with pytest.raises(RuntimeError, match="no memory"):
+        c.begin({a: 20, b: 1})
+    assert state() == was
+
+
 def test_host_calls_leave_what_is_not_in_order(lib):
     """The one-step form of a call declines whatever it does not know, without an exception: the wrapper then says why."""
     from catopt_b200 import ops
