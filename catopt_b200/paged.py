@@ -18,7 +18,7 @@ ordered after the reads of the last only on the same stream.
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 
 import torch
 
@@ -29,7 +29,8 @@ from ._lib import B200Error
 @dataclass(frozen=True)
 class PagedBatch:
     """The index tensors of one step: ``table [R, pages]``, ``seq_lens [R]`` (new tokens included), ``cu_q [R+1]``,
-    ``positions [n_tokens]``, all int32, and the bounds that the kernels take from the host."""
+    ``positions [n_tokens]``, all int32, and the bounds that the kernels take from the host.  Good until one of its
+    requests is closed or cut."""
     requests: tuple[int, ...]
     table: torch.Tensor
     seq_lens: torch.Tensor
@@ -38,6 +39,9 @@ class PagedBatch:
     n_tokens: int
     max_q: int
     max_k: int
+    #: the cache that made it (``None``: nobody checks), and how often each request had been given other pages by then
+    owner: object = field(default=None, repr=False)
+    hands: tuple[int, ...] = ()
 
 
 class PagedCache:
@@ -62,6 +66,8 @@ class PagedCache:
         self._pages: dict[int, list[int]] = {}
         self._length: dict[int, int] = {}
         self._position: dict[int, int] = {}
+        self._hands: dict[int, int] = {}      # times that an eviction gave the request other pages
+        self._owner = object()
         self._next = 0
 
     # ------------------------------------------------------------------ requests
@@ -69,14 +75,14 @@ class PagedCache:
         """A new, empty request."""
         r = self._next
         self._next += 1
-        self._pages[r], self._length[r], self._position[r] = [], 0, 0
+        self._pages[r], self._length[r], self._position[r], self._hands[r] = [], 0, 0, 0
         return r
 
     def close(self, request: int) -> None:
         """Give the request's pages back."""
         self._known(request)
         self._free.extend(reversed(self._pages.pop(request)))
-        del self._length[request], self._position[request]
+        del self._length[request], self._position[request], self._hands[request]
 
     def length(self, request: int) -> int:
         """Cached keys."""
@@ -140,7 +146,18 @@ class PagedCache:
         for r, n in new_tokens.items():
             self._length[r] += n
             self._position[r] += n
-        return PagedBatch(requests, t.view(len(requests), width), s, c, p, cu[-1], max(new_tokens.values()), max(1, max(lens)))
+        return PagedBatch(requests, t.view(len(requests), width), s, c, p, cu[-1], max(new_tokens.values()), max(1, max(lens)),
+                          self._owner, tuple(map(self._hands.get, requests)))
+
+    def _current(self, batch: PagedBatch) -> None:
+        """The pages of a batch made by ``begin`` are still its requests' own."""
+        if batch.owner is None:
+            return
+        if batch.owner is not self._owner:
+            raise B200Error("PagedCache: a batch of another cache")
+        if tuple(map(self._hands.get, batch.requests)) != batch.hands:
+            r = next(r for r, n in zip(batch.requests, batch.hands) if self._hands.get(r) != n)
+            raise B200Error(f"PagedCache: request {r} has been closed or cut since this batch was made")
 
     def append(self, layer: int, batch: PagedBatch, q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, *,
                q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 1e-6,
@@ -148,6 +165,7 @@ class PagedCache:
                interleaved: bool = False) -> torch.Tensor | None:
         """``ops.paged_append`` of the step's tokens into a layer, rotated at their positions if ``cos`` and ``sin``
         are given; returns the normed and rotated ``q``."""
+        self._current(batch)
         return ops.paged_append(q, k, v, self.k[layer], self.v[layer], batch.table, batch.seq_lens, batch.cu_q,
                                 q_weight=q_weight, k_weight=k_weight, eps=eps, cos=cos, sin=sin,
                                 positions=None if cos is None else batch.positions, interleaved=interleaved,
@@ -157,6 +175,7 @@ class PagedCache:
                causal: bool = True) -> torch.Tensor:
         """``ops.om_paged_fwd`` of the step's queries over a layer; the attention weight is added up if the cache
         tracks it."""
+        self._current(batch)
         return ops.om_paged_fwd(q, self.k[layer], self.v[layer], batch.table, batch.seq_lens, batch.cu_q, batch.max_q,
                                 max_k=batch.max_k, scale=scale, causal=causal,
                                 weights=self.weights[layer] if self.weights else None)
@@ -196,4 +215,5 @@ class PagedCache:
         for r, pages in zip(cut, fresh):
             self._free.extend(reversed(self._pages[r]))
             self._pages[r], self._length[r] = pages, budget
+            self._hands[r] += 1
         return kept

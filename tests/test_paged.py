@@ -208,6 +208,38 @@ def test_cache_keeps_its_pages_when_a_call_fails(monkeypatch):
     assert state() == was
 
 
+def test_cache_refuses_a_batch_whose_pages_are_gone(monkeypatch):
+    from catopt_b200 import B200Error, ops
+
+    for name in ("paged_append", "om_paged_fwd"):
+        monkeypatch.setattr(ops, name, lambda *a, **kw: "done")
+    monkeypatch.setattr(ops, "paged_evict", fake_evict)
+    c, other = make(), make()
+    a, b, d = c.open(), c.open(), c.open()
+    x = torch.zeros(1, 1, 8)
+
+    def taken(batch, cache=c):
+        return cache.append(0, batch, x, x, x), cache.attend(0, batch, x)
+
+    first = c.begin({a: 20})
+    both = c.begin({a: 1, b: 8})
+    third = c.begin({d: 3})
+    assert taken(first) == taken(both) == taken(third) == ("done", "done")          # later steps take no page away
+    assert c.evict([a, b], 30) == [] and taken(both) == ("done", "done")            # nobody was cut
+    c.evict([a], 8)
+    for call in (lambda: c.append(0, first, x, x, x), lambda: c.attend(0, both, x)):
+        with pytest.raises(B200Error, match=f"request {a}"):
+            call()
+    fourth = c.begin({b: 1, a: 1})
+    c.close(d)
+    assert taken(fourth) == ("done", "done")
+    with pytest.raises(B200Error, match=f"request {d}"):
+        taken(third)
+    other.open()
+    with pytest.raises(B200Error, match="another cache"):
+        taken(fourth, other)
+
+
 def test_host_calls_leave_what_is_not_in_order(lib):
     """The one-step form of a call declines whatever it does not know, without an exception: the wrapper then says why."""
     from catopt_b200 import ops
