@@ -264,13 +264,15 @@ extern "C" int cb2_om_paged_fwd(const void* q, long long q_token_stride, long lo
   if (dtype != CB2_BF16 && dtype != CB2_F32) return CB2_UNSUPPORTED_DTYPE;
   if (n_tokens == 0) return CB2_OK;
   if (!q || !o || !scratch) return CB2_NULL_PTR;
-  if (q == o) return CB2_BAD_SHAPE;      // rows of q are read after others of o have been written
   const int vec = dtype == CB2_BF16 ? 8 : 4;      // elements in 16 bytes
   if (!aligned16(q) || !aligned16(weights) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(o) || !aligned16(scratch) ||
       q_token_stride % vec || q_head_stride % vec || k_page_stride % vec || v_page_stride % vec)
     return CB2_BAD_ALIGN;
   const Plan p = plan(n_tokens, R, Hq, Hkv, d, max_q, max_k, weights != nullptr, dtype);
   if (scratch_bytes < p.total) return CB2_SCRATCH_TOO_SMALL;
+  // rows of q are read after others of o have been written
+  const int esz = dtype == CB2_BF16 ? 2 : 4;
+  if (paged_rows_meet(q, n_tokens, q_token_stride, Hq, q_head_stride, d, esz, o, (long long)n_tokens * Hq * d * esz)) return CB2_BAD_SHAPE;
   int page_log2 = 0;
   while ((1 << page_log2) < page_size) ++page_log2;
   const PagedBatch batch{block_table, seq_lens, cu_q, R, max_pages, n_pages, page_log2, n_tokens, max_q, max_k, dev_status};

@@ -310,6 +310,16 @@ extern "C" int cb2_paged_append(const void* q, long long q_token_stride, long lo
       k_token_stride % vec || k_head_stride % vec || v_token_stride % vec || v_head_stride % vec || k_page_stride % vec ||
       v_page_stride % vec)
     return CB2_BAD_ALIGN;
+  if (Hq) {
+    // a row of q is read before its own place in q_out is written: in place is fine, any other overlap is not
+    const int esz = dtype == CB2_BF16 ? 2 : 4;
+    const long long bytes = (long long)n_tokens * Hq * d * esz;
+    const bool in_place = q == q_out && (n_tokens == 1 || q_token_stride == (long long)Hq * d) && (Hq == 1 || q_head_stride == d);
+    if ((!in_place && paged_rows_meet(q, n_tokens, q_token_stride, Hq, q_head_stride, d, esz, q_out, bytes)) ||
+        paged_rows_meet(k, n_tokens, k_token_stride, Hkv, k_head_stride, d, esz, q_out, bytes) ||
+        paged_rows_meet(v, n_tokens, v_token_stride, Hkv, v_head_stride, d, esz, q_out, bytes))
+      return CB2_BAD_SHAPE;
+  }
   int page_log2 = 0;
   while ((1 << page_log2) < page_size) ++page_log2;
   const PagedBatch batch{block_table, seq_lens, cu_q, R, max_pages, n_pages, page_log2, n_tokens, n_tokens, max_pages * page_size, dev_status};

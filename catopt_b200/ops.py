@@ -805,7 +805,7 @@ def paged_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_pag
     rotary/2]`` with ``positions`` int32 ``[n]`` (read only then): rotation of the first ``rotary`` columns in pairs ``(i, i +
     rotary/2)``, or ``(2i, 2i+1)`` if ``interleaved``.  ``weights`` (float32 ``[n_pages, Hkv, page_size]``) is
     zeroed at the new slots.  Returns the normed and rotated ``q`` (rows behind ``cu_q[R]`` are not written); ``out`` may
-    be a contiguous ``q`` itself."""
+    be a contiguous ``q`` itself, and lies on no other operand."""
     res = _host("paged_append")(_status_words, q, k, v, k_pages, v_pages, block_table, seq_lens, cu_q, q_weight, k_weight, eps, cos, sin,
                                 positions, interleaved, weights, out)
     if res is not NotImplemented:
@@ -873,7 +873,8 @@ def om_paged_fwd(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     (all of them without ``causal``); a row that sees none gives 0.  ``max_q``, ``max_k``: bounds of the requests'
     new tokens and cached keys (``max_k`` defaults to what the table holds); the scratch grows with them.
     ``weights`` (float32 ``[n_pages, Hkv, page_size]``): the softmax probability that every cached key gets, summed
-    over rows and the heads of its group, is added to it (requests of one call must not share pages then).  ``scale`` defaults to ``1/sqrt(d)``."""
+    over rows and the heads of its group, is added to it (requests of one call must not share pages then).  ``scale`` defaults to ``1/sqrt(d)``; ``out`` is contiguous
+    and no part of it on ``q``."""
     res = _host("om_paged_fwd")(_status_words, q, k_pages, v_pages, block_table, seq_lens, cu_q, max_q, max_k, scale, causal, weights, out)
     if res is not NotImplemented:
         if res.__class__ is int:

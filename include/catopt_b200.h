@@ -432,9 +432,10 @@ int cb2_om_bias_step(const void* q, const void* k, const void* v, const float* b
  * with cos, sin: float [table_rows, rotary/2], row positions[t] (int32 [n_tokens]) for token t.
  * q: [n_tokens, Hq, d] (Hq may be 0, q NULL), k, v: [n_tokens, Hkv, d], each with its token and
  * head strides in elements, so views of a fused projection need no copy; q_out: [n_tokens, Hq,
- * d] dense; it may be q itself where q is dense, but overlap no other operand.  Norm weights have the tensors' element type.  Everything is computed
- * in fp32 and rounded once.  weights (may be NULL): set to 0 at the new slots.  No scratch.
- * Pointers 16-byte aligned, strides multiples of 16 bytes. */
+ * d] dense; it may be q itself where q is dense, but overlap no other operand (refused for q, k
+ * and v).  Norm weights have the tensors' element type.  Everything is computed in fp32 and
+ * rounded once.  weights (may be NULL): set to 0 at the new slots.  No scratch.  Pointers 16-byte
+ * aligned, strides multiples of 16 bytes. */
 int cb2_paged_append(const void* q, long long q_token_stride, long long q_head_stride, const void* k,
                      long long k_token_stride, long long k_head_stride, const void* v, long long v_token_stride,
                      long long v_head_stride, void* q_out, void* k_pages, void* v_pages, long long k_page_stride,
@@ -450,7 +451,7 @@ int cb2_paged_append(const void* q, long long q_token_stride, long long q_head_s
  * of its slots.  A row that sees no key (seq_lens[r] = 0, or less than n_r) is 0.  What the
  * slots behind seq_lens[r] hold, NaN included, has no effect.
  * q: [n_tokens, Hq, d] with token and head strides in elements (none 0); o: [n_tokens, Hq, d]
- * dense, apart from q.  max_q: no request has more new tokens; max_k: none more cached keys.
+ * dense, no part of it on q.  max_q: no request has more new tokens; max_k: none more cached keys.
  * weights (may be NULL): weights[key] += sum over the rows that see it, and the heads of its
  * group, of the softmax probability; no two requests of the call may then have a page in common
  * (without weights they may).  Results do not depend on the order in which CTAs run.

@@ -52,6 +52,24 @@ def test_append_refusals(lib, change, want):
     assert lib.cb2_paged_append(*{**APPEND, **change}.values()) == want
 
 
+FAR = 1 << 20      # operands in places of their own, 8 rows of 4 (k, v: 2) heads of 64 bf16 each: 4096 (2048) bytes
+
+
+@pytest.mark.parametrize("out", [FAR - 4080, FAR - 16, FAR + 16, FAR + 4080])
+def test_attention_output_on_the_queries(lib, out):
+    assert lib.cb2_om_paged_fwd(*{**ATTEND, "q": FAR, "o": out}.values()) == SHAPE
+    # heads first in memory: rows of 512 bytes, 4 heads of 1024
+    assert lib.cb2_om_paged_fwd(*{**ATTEND, "q": FAR, "qt": 64, "qh": 512, "o": out}.values()) == SHAPE
+
+
+@pytest.mark.parametrize("change", [dict(out=FAR - 4080), dict(out=FAR + 16), dict(out=FAR + 4080),        # part of q
+                                    dict(out=FAR, qt=512), dict(out=FAR, qt=64, qh=512),                    # q itself, not dense
+                                    dict(out=2 * FAR - 4080), dict(out=2 * FAR + 2032), dict(out=3 * FAR - 16), dict(out=3 * FAR)], ids=str)
+def test_append_output_on_other_operands(lib, change):
+    call = {**APPEND, "q": FAR, "k": 2 * FAR, "v": 3 * FAR, "kp": 5 * FAR, "vp": 6 * FAR, **change}
+    assert lib.cb2_paged_append(*call.values()) == SHAPE
+
+
 @pytest.mark.parametrize("change,want", [
     (dict(w=None), NULL), (dict(kept=None), NULL), (dict(budget=0), SHAPE), (dict(budget=17), SHAPE), (dict(first=-1), SHAPE),
     (dict(first=5, last=4), SHAPE), (dict(max_k=40), SHAPE), (dict(R=65536), SHAPE), (dict(page=0), SHAPE), (dict(dtype=5), DTYPE),
@@ -259,14 +277,22 @@ INT_MIN, INT_MAX = -(1 << 31), (1 << 31) - 1
 
 
 @pytest.fixture(scope="module")
-def clamp(tmp_path_factory):
-    """The kernels' clamp of a request, compiled for the host: ``f(c0, c1, len, n_tokens, max_q, max_k)``."""
+def host_lib(tmp_path_factory):
     d = tmp_path_factory.mktemp("clamp")
     (d / "clamp.cpp").write_text('#include "paged_clamp.cuh"\nextern "C" int clamp(int a, int b, int l, int n, int q, int k, int* out) {\n'
                                  "  cb2::PagedReq r;\n  const bool ok = cb2::paged_clamp(a, b, l, n, q, k, &r);\n"
-                                 "  out[0] = r.t0, out[1] = r.n, out[2] = r.len;\n  return ok;\n}\n")
+                                 "  out[0] = r.t0, out[1] = r.n, out[2] = r.len;\n  return ok;\n}\n"
+                                 'extern "C" int meet(long long at, long long n, long long token, long long heads, long long head, int d, int size,\n'
+                                 "                    long long to, long long bytes) {\n"
+                                 "  return cb2::paged_rows_meet((void*)at, n, token, heads, head, d, size, (void*)to, bytes);\n}\n")
     subprocess.check_call(["g++", "-O2", "-fwrapv", "-shared", "-fPIC", f"-I{CSRC}", str(d / "clamp.cpp"), "-o", str(d / "clamp.so")])
-    f = C.CDLL(str(d / "clamp.so")).clamp
+    return C.CDLL(str(d / "clamp.so"))
+
+
+@pytest.fixture(scope="module")
+def clamp(host_lib):
+    """The kernels' clamp of a request, compiled for the host: ``f(c0, c1, len, n_tokens, max_q, max_k)``."""
+    f = host_lib.clamp
 
     def call(*a):
         out = (C.c_int * 3)()
@@ -290,6 +316,21 @@ def test_no_index_leads_out_of_bounds(clamp):
         for max_k in (1, 8, 1 << 30):
             ok, _, _, got = clamp(0, 0, length, 8, 8, max_k)
             assert got == min(max(length, 0), max_k) and ok == (got == length)
+
+
+def test_where_rows_meet(host_lib):
+    """Rows [n, heads, d] with strides against a run of bytes: exact along the longer stride, the rows' whole extent
+    along the other."""
+    d, size = 8, 2
+    for n, token, heads, head in ((1, 0, 1, 0), (3, 0, 1, 0), (3, 0, 2, 0), (2, 0, 3, 24), (3, 40, 2, 8), (3, 8, 2, 40), (4, 8, 1, 0), (1, 8, 3, 24), (2, 16, 4, 8)):
+        outer, inner = ((n, token), (heads, head)) if n == 1 or heads == 1 or token >= head else ((heads, head), (n, token))
+        row = ((inner[0] - 1) * inner[1] + d) * size
+        used = {a for i in range(outer[0]) for a in range(i * outer[1] * size, i * outer[1] * size + row)}
+        for to in range(-70, max(used) + 20):
+            for count in (1, 16, 70):
+                got = host_lib.meet(C.c_longlong(FAR), *(C.c_longlong(x) for x in (n, token, heads, head)), d, size, C.c_longlong(FAR + to),
+                                    C.c_longlong(count))
+                assert got == (not used.isdisjoint(range(to, to + count))), (n, token, heads, head, to, count)
 
 
 # --------------------------------------------------------------------------- kernels launched while the one before runs
