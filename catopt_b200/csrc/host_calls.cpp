@@ -26,7 +26,8 @@ struct NotTaken {};
 const Tensor* tensor(PyObject* o, int dev) {
   if (!THPVariable_CheckExact(o)) throw NotTaken{};
   const Tensor* t = &THPVariable_Unpack(o);
-  if (!t->is_cuda() || t->get_device() != dev || t->layout() != at::kStrided || (t->requires_grad() && c10::GradMode::is_enabled()))
+  if (!t->is_cuda() || t->get_device() != dev || t->layout() != at::kStrided || (t->requires_grad() && c10::GradMode::is_enabled()) ||
+      t->_fw_grad(0).defined())
     throw NotTaken{};
   return t;
 }

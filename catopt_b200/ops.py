@@ -13,6 +13,7 @@ import ctypes as C
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import B200Error, check, dtype_code, require_cuda, require_device, stream_ptr
@@ -728,10 +729,13 @@ def _raw_stream(dev: int) -> int:
 
 
 def _no_grad_asked(what: str, *tensors: torch.Tensor | None) -> None:
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise B200Error(f"{what} serves a cache and has no gradient: call it under torch.no_grad()")
+    """No operand asks for a gradient, backward (under grad mode) or forward (a tangent of an open dual level)."""
+    grad = torch.is_grad_enabled()
+    for t in tensors:
+        if t is not None and grad and t.requires_grad:
+            raise B200Error(f"{what} serves a cache and has no gradient: call it under torch.no_grad()")
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise B200Error(f"{what} serves a cache and has no gradient, in forward mode either: call it with primals")
 
 
 def _pools(what: str, dev: int, k_pages: torch.Tensor, v_pages: torch.Tensor) -> tuple[int, int, int, int, int, int]:
@@ -836,7 +840,7 @@ def paged_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_pag
         cos_ptr = _dense(what, dev, "cos", cos, torch.float32, (rows, half))
         sin_ptr = _dense(what, dev, "sin", sin, torch.float32, (rows, half))
         pos_ptr = _dense(what, dev, "positions", positions, torch.int32, (n,))
-    _no_grad_asked(what, q, k, v, k_pages, v_pages, q_weight, k_weight)
+    _no_grad_asked(what, q, k, v, k_pages, v_pages, q_weight, k_weight, cos, sin, weights, out)
     res, hq, q_args = None, 0, (None, 0, 0)
     if q is not None:
         _here(what, dev, q)
@@ -889,7 +893,7 @@ def om_paged_fwd(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     if q.dim() != 3 or q.shape[2] != d or dt != k_pages.dtype or q.shape[1] == 0 or q.shape[1] % hkv:
         raise B200Error(f"{what}: q is [n_tokens, Hq, {d}] of the pools' dtype, Hq a multiple of {hkv}")
     w_ptr = None if weights is None else _dense(what, dev, "weights", weights, torch.float32, (n_pages, hkv, ps))
-    _no_grad_asked(what, q, k_pages, v_pages)
+    _no_grad_asked(what, q, k_pages, v_pages, weights, out)
     res = _dense_out(what, dev, out, q)
     q, *q_args = _token_rows(q)
     n, hq, _ = q.shape

@@ -551,6 +551,43 @@ def test_gradients_are_refused(dev):
         ops.paged_append(q, k, k, c["k"], c["v"], c["table"], c["lens"], cu)
 
 
+def test_tangents_are_refused(dev):
+    import torch.autograd.forward_ad as fwd
+    from catopt_b200 import B200Error, ops
+
+    c = ref.make_cache([20], 1, 16, 64, F32, dev, 10)
+    cu = ref.offsets([1], dev)
+    q, k = torch.randn(1, 2, 64, device=dev), torch.randn(1, 1, 64, device=dev)
+    with fwd.dual_level():
+        dual = [fwd.make_dual(x, torch.ones_like(x)) for x in (q, k)]
+        for call in (lambda: ops.om_paged_fwd(dual[0], c["k"], c["v"], c["table"], c["lens"], cu, 1),
+                     lambda: ops.paged_append(q, dual[1], k, c["k"], c["v"], c["table"], c["lens"], cu),
+                     lambda: ops.paged_append(dual[0].mT.contiguous().mT, k, k, c["k"], c["v"], c["table"], c["lens"], cu)):
+            with pytest.raises(B200Error, match="no gradient"):
+                call()
+        ops.om_paged_fwd(q, c["k"], c["v"], c["table"], c["lens"], cu, 1)
+
+
+def test_tables_that_ask_for_a_gradient_are_refused(dev):
+    from catopt_b200 import B200Error, ops
+
+    c = ref.make_cache([20], 1, 16, 64, F32, dev, 10)
+    cu = ref.offsets([1], dev)
+    k = torch.randn(1, 1, 64, device=dev)
+    cos, sin = (torch.randn(4, 32, device=dev) for _ in range(2))
+    pos = torch.zeros(1, dtype=torch.int32, device=dev)
+    w = torch.zeros(c["k"].shape[:3], device=dev)
+    q = torch.randn(1, 2, 64, device=dev)
+    grad = lambda x: x.clone().requires_grad_()
+    for call in (lambda: ops.paged_append(None, k, k, c["k"], c["v"], c["table"], c["lens"], cu, cos=grad(cos), sin=sin, positions=pos),
+                 lambda: ops.paged_append(None, k, k, c["k"], c["v"], c["table"], c["lens"], cu, weights=grad(w)),
+                 lambda: ops.paged_append(q, k, k, c["k"], c["v"], c["table"], c["lens"], cu, out=grad(q)),
+                 lambda: ops.om_paged_fwd(q, c["k"], c["v"], c["table"], c["lens"], cu, 1, weights=grad(w)),
+                 lambda: ops.om_paged_fwd(q, c["k"], c["v"], c["table"], c["lens"], cu, 1, out=grad(q))):
+        with pytest.raises(B200Error, match="no gradient"):
+            call()
+
+
 def test_wrong_arguments_are_refused(dev):
     from catopt_b200 import B200Error, ops
 
