@@ -83,8 +83,9 @@ Pools pools(PyObject* ko, PyObject* vo, int dev) {
   p.n = p.k->size(0), p.hkv = p.k->size(1), p.ps = p.k->size(2), p.d = p.k->size(3);
   need(p.n <= INT_MAX && p.hkv <= INT_MAX && p.ps <= 1024 && p.d <= 128);
   for (const Tensor* t : {p.k, p.v}) {
-    need(t->stride(3) == 1 && t->stride(2) == p.d && t->stride(1) == p.ps * p.d && t->stride(0) >= p.hkv * p.ps * p.d);
-    (t == p.k ? p.ks : p.vs) = t->stride(0);
+    const long long page = p.hkv * p.ps * p.d, step = p.n > 1 ? t->stride(0) : page;      // of one page, the stride says nothing
+    need(t->stride(3) == 1 && t->stride(2) == p.d && t->stride(1) == p.ps * p.d && step >= page);
+    (t == p.k ? p.ks : p.vs) = step;
   }
   if (p.k == p.v) p.vs = p.ks;
   return p;

@@ -588,6 +588,22 @@ def test_tables_that_ask_for_a_gradient_are_refused(dev):
             call()
 
 
+def test_a_pool_of_one_page(dev):
+    # the distance to a second page that is not there has no meaning
+    from catopt_b200 import ops
+
+    wide = torch.zeros(2 * 16 * 64 + 3, dtype=BF, device=dev)
+    k, v = (wide.new_zeros(wide.shape).as_strided((1, 2, 16, 64), (x, 16 * 64, 64, 1)) for x in (2 * 16 * 64 + 3, 2 * 16 * 64 + 1))
+    table = torch.zeros(1, 1, dtype=torch.int32, device=dev)
+    lens = torch.tensor([10], dtype=torch.int32, device=dev)
+    cu = ref.offsets([10], dev)
+    x = torch.randn(10, 2, 64, device=dev).to(BF)
+    w = torch.zeros(1, 2, 16, device=dev)
+    ops.paged_append(None, x, x, k, v, table, lens, cu, weights=w)
+    o = ops.om_paged_fwd(x, k, v, table, lens, cu, 10, weights=w)
+    assert torch.equal(k[0, :, :10].transpose(0, 1), x) and torch.equal(o[0], x[0])
+
+
 def test_wrong_arguments_are_refused(dev):
     from catopt_b200 import B200Error, ops
 
