@@ -100,14 +100,16 @@ def build(force: bool = False, verbose: bool = False) -> Path:
 
 
 def _build_host(force: bool) -> None:
-    """``_host.so``: the Python module of ``host_calls.cpp``, against torch's headers and the library beside it."""
-    src = CSRC / "host_calls.cpp"
-    if not force and not _stale(HOST, src):
-        return
+    """``_host.so``: the Python module of ``host_calls.cpp``, against torch's headers and the library beside it.  A file
+    beside the objects names the Python and torch that it was built for."""
     import sysconfig
 
     import torch
 
+    src, key = CSRC / "host_calls.cpp", HOST.parent / "build" / (HOST.name + ".for")
+    want = f"{sys.implementation.cache_tag} torch {torch.__version__}"
+    if not force and not _stale(HOST, src) and key.exists() and key.read_text() == want:
+        return
     root = Path(torch.__file__).resolve().parent
     cuda = Path(_nvcc()).resolve().parent.parent if Path(_nvcc()).exists() else Path("/usr/local/cuda")
     include = [root / "include", root / "include/torch/csrc/api/include", sysconfig.get_paths()["include"], cuda / "include"]
@@ -116,6 +118,8 @@ def _build_host(force: bool) -> None:
            f"-L{HERE}", "-l:libcatopt_b200.so", "-Wl,-rpath,$ORIGIN", f"-L{root / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu",
            "-lc10", "-lc10_cuda"]
     subprocess.check_call(cmd)
+    key.parent.mkdir(exist_ok=True)
+    key.write_text(want)
 
 
 if __name__ == "__main__":

@@ -689,8 +689,8 @@ def _host(name: str):
     _lib.load()
     try:
         from . import _host as module
-    except ModuleNotFoundError as e:
-        raise B200Error("_host.so is not built (python -m catopt_b200.build)") from e
+    except ImportError as e:      # missing, or built for another Python or torch
+        raise B200Error(f"_host.so does not load, build it with `python -m catopt_b200.build` ({e})") from e
     return getattr(module, name)
 
 

@@ -271,6 +271,45 @@ def test_host_calls_leave_what_is_not_in_order(lib):
     assert ops._host("paged_evict")({}, t, t, t, i, i[0], i, 1, 0, 0, 1 << 80) is NotImplemented
 
 
+def test_host_module_follows_torch_and_python(tmp_path, monkeypatch):
+    from catopt_b200 import build
+
+    calls = []
+
+    def compile_(cmd):
+        calls.append(cmd)
+        build.HOST.touch()
+
+    monkeypatch.setattr(build, "HOST", tmp_path / "_host.so")
+    monkeypatch.setattr(build.subprocess, "check_call", compile_)
+    for version, tag, want in ((torch.__version__, "cpython-312", 1), (torch.__version__, "cpython-312", 1), ("9.9", "cpython-312", 2),
+                               ("9.9", "cpython-399", 3), ("9.9", "cpython-399", 3)):
+        monkeypatch.setattr(torch, "__version__", version)
+        monkeypatch.setattr(build.sys.implementation, "cache_tag", tag)
+        build._build_host(False)
+        assert len(calls) == want
+    assert build.HOST.exists()
+
+
+def test_host_module_that_does_not_load(lib, monkeypatch):
+    import sys
+
+    import catopt_b200
+    from catopt_b200 import B200Error, ops
+
+    class Refuses:
+        @staticmethod
+        def find_spec(name, path=None, target=None):
+            if name == "catopt_b200._host":
+                raise ImportError("undefined symbol")
+
+    monkeypatch.delattr(catopt_b200, "_host", raising=False)
+    monkeypatch.delitem(sys.modules, "catopt_b200._host", raising=False)
+    monkeypatch.setattr(sys, "meta_path", [Refuses, *sys.meta_path])
+    with pytest.raises(B200Error, match="catopt_b200.build"):
+        ops._host.__wrapped__("paged_append")
+
+
 # --------------------------------------------------------------------------- index tensors of any content
 CSRC = Path(__file__).resolve().parent.parent / "catopt_b200" / "csrc"
 INT_MIN, INT_MAX = -(1 << 31), (1 << 31) - 1
