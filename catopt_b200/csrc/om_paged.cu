@@ -128,6 +128,7 @@ paged_combine_tiles_kernel(const PagedScratch scratch, __nv_bfloat16* __restrict
     if (col < d) *reinterpret_cast<uint4*>(o + sh_at[rr] * d + col) = *reinterpret_cast<const uint4*>(&sh[rr][col]);
 }
 
+constexpr float kLog2e = 1.4426950408889634f;
 size_t up16(size_t n) { return (n + 15) & ~size_t(15); }
 
 // Which kernels a call takes.  Requests of at most `few` packed rows are bound by reading their keys: a batch of
@@ -257,7 +258,7 @@ extern "C" int cb2_om_paged_fwd(const void* q, long long q_token_stride, long lo
   if (!k_pages || !v_pages || !block_table || !seq_lens || !cu_q) return CB2_NULL_PTR;
   if (!sizes_ok(n_tokens, R, Hq, Hkv, d, max_q, max_k)) return CB2_BAD_SHAPE;
   if (page_size < 8 || page_size > 1024 || (page_size & (page_size - 1)) || n_pages < 1 || max_pages < 1) return CB2_BAD_SHAPE;
-  if (int64_t(max_pages) * page_size < max_k || !(scale > 0.f) || scale > 3e38f) return CB2_BAD_SHAPE;
+  if (int64_t(max_pages) * page_size < max_k || !(scale > 0.f) || !(scale * kLog2e < INFINITY)) return CB2_BAD_SHAPE;
   const long long page = (long long)Hkv * page_size * d;
   if (k_page_stride < page || v_page_stride < page || q_token_stride < 0 || q_head_stride < 0) return CB2_BAD_SHAPE;
   if ((n_tokens > 1 && q_token_stride == 0) || (Hq > 1 && q_head_stride == 0)) return CB2_BAD_SHAPE;
@@ -277,7 +278,7 @@ extern "C" int cb2_om_paged_fwd(const void* q, long long q_token_stride, long lo
   while ((1 << page_log2) < page_size) ++page_log2;
   const PagedBatch batch{block_table, seq_lens, cu_q, R, max_pages, n_pages, page_log2, n_tokens, max_q, max_k, dev_status};
   const PagedPools pools{k_pages, v_pages, k_page_stride, v_page_stride, Hkv, d};
-  const PagedRows rows{q, q_token_stride, q_head_stride, Hq / Hkv, Hkv, scale * 1.4426950408889634f};
+  const PagedRows rows{q, q_token_stride, q_head_stride, Hq / Hkv, Hkv, scale * kLog2e};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   char* ws = static_cast<char*>(scratch);
   if (dtype == CB2_BF16) return run_bf16(rows, pools, batch, causal != 0, static_cast<__nv_bfloat16*>(o), weights, ws, p, st);

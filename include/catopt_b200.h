@@ -457,7 +457,8 @@ int cb2_paged_append(const void* q, long long q_token_stride, long long q_head_s
  * (without weights they may).  Results do not depend on the order in which CTAs run.
  * Products of bf16 tensors accumulate in fp32; for the product with v a probability keeps 2^-16
  * of itself where max_q * Hq / Hkv <= 16 and is rounded to bf16 in other batches.  Sums, maxima
- * and accumulators are fp32 throughout.  scale > 0, (n_tokens + max_k + 256) * Hq / Hkv < 2^30.
+ * and accumulators are fp32 throughout.  scale > 0 and scale / ln 2 finite, (n_tokens + max_k +
+ * 256) * Hq / Hkv < 2^30.
  * scratch: cb2_om_paged_scratch_bytes() bytes, 16-byte aligned. */
 size_t cb2_om_paged_scratch_bytes(int n_tokens, int R, int Hq, int Hkv, int d, int max_q, int max_k, int weights,
                                   int dtype);

@@ -52,6 +52,12 @@ def test_append_refusals(lib, change, want):
     assert lib.cb2_paged_append(*{**APPEND, **change}.values()) == want
 
 
+@pytest.mark.parametrize("scale", [2.4e38, 3e38, 3.4e38])
+def test_scale_in_base_two(lib, scale):
+    # scale / ln 2 is what the kernels multiply by: it has to be finite
+    assert lib.cb2_om_paged_fwd(*{**ATTEND, "scale": scale}.values()) == SHAPE
+
+
 FAR = 1 << 20      # operands in places of their own, 8 rows of 4 (k, v: 2) heads of 64 bf16 each: 4096 (2048) bytes
 
 
