@@ -190,6 +190,52 @@ def test_weights_when_the_bound_on_keys_is_far_off(dev):
     close(w, ww, wtol, "weights")
 
 
+def test_fp32_weights_when_the_bound_on_keys_is_far_off(dev):
+    # the same in fp32, where the scores' buffer is as large: few rows from the keys again
+    from catopt_b200 import ops
+
+    lens, new = [700, 5, 0], [1, 2, 0]
+    c = ref.make_cache(lens, 2, 256, 64, F32, dev, 8)
+    wide = torch.full((3, 9000), -1, dtype=torch.int32, device=dev)
+    wide[:, :c["table"].shape[1]] = c["table"]
+    q = torch.randn(3, 8, 64, device=dev)
+    w = torch.zeros(c["k"].shape[:3], device=dev)
+    o = ops.om_paged_fwd(q, c["k"], c["v"], wide, c["lens"], ref.offsets(new, dev), 2, weights=w)
+    ops.check_device_status(dev)
+    want, tol, ww, wtol = ref.attend(q, c, new, lens, 0.125, True)
+    close(o, want, tol, "o")
+    close(w, ww, wtol, "weights")
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+def test_chunks_of_many_requests(dev, dtype):
+    # more requests than a CTA has threads: the search for a share, and the weights' loop over requests, take several rounds
+    new = [(5 * i) % 23 if i % 7 else 0 for i in range(600)]
+    lens = [n + (11 * i) % 40 if n else 0 for i, n in enumerate(new)]
+    assert max(new) * 2 > 16
+    run_attend(dev, new, lens, 1, 2, 32, 8, dtype, weights=True)
+
+
+def test_append_of_many_requests(dev):
+    # more requests than threads of a CTA
+    from catopt_b200 import ops
+
+    new = [i % 3 for i in range(700)]
+    lens = [n + i % 20 if n else 0 for i, n in enumerate(new)]
+    c = ref.make_cache(lens, 2, 8, 16, F32, dev, 23, fill=0.0)
+    k, v = (torch.randn(sum(new), 2, 16, device=dev) for _ in range(2))
+    want = [c["k"].clone(), c["v"].clone()]
+    t = 0
+    for r, n in enumerate(new):
+        for j in range(lens[r] - n, lens[r]):
+            p = int(c["table"][r, j // 8])
+            want[0][p, :, j % 8], want[1][p, :, j % 8] = k[t], v[t]
+            t += 1
+    ops.paged_append(None, k, v, c["k"], c["v"], c["table"], c["lens"], ref.offsets(new, dev))
+    ops.check_device_status(dev)
+    assert torch.equal(c["k"], want[0]) and torch.equal(c["v"], want[1])
+
+
 def test_large_scores_and_ties(dev):
     # a few keys dominate; the running maximum moves late, then by a lot
     from catopt_b200 import ops
@@ -438,7 +484,65 @@ def test_evict(dev, dtype, lens, budget, first, last, kv, d, page):
         assert torch.equal(got.view(bits[got.element_size()]), exp.view(bits[exp.element_size()]))
 
 
+@pytest.mark.parametrize("budget", [1000, 49200, 52000])
+def test_evict_from_more_keys_than_shared_memory_holds(dev, budget):
+    # 49152 keys are held, the others read again in every pass; many ties, kept and dropped ones on both sides
+    from catopt_b200 import ops
+
+    n, d, page, first, last = 53000, 8, 64, 3, 40
+    need = (budget + page - 1) // page
+    c = ref.make_cache([n], 1, page, d, F32, dev, 31, fill=0.0, spare=need)
+    g = torch.Generator(device=dev).manual_seed(budget)
+    w = torch.randint(0, 50, c["k"].shape[:3], generator=g, device=dev).float() / 8
+    to = torch.tensor([c["free"]], dtype=torch.int32, device=dev)
+    ids = c["table"][0, :(n + page - 1) // page].long()
+    want = ref.keep(w[ids, 0].reshape(-1).cpu(), n, budget, first, last)
+    kept, new_lens = ops.paged_evict(c["k"], c["v"], w, c["table"], c["lens"], to, budget, keep_first=first, keep_last=last)
+    ops.check_device_status(dev)
+    assert kept[0, 0].tolist() == want and new_lens.tolist() == [budget]
+    assert budget == 1000 or 49152 < want[-last - 1]          # (the 960 lowest of the heaviest keys lie in front)
+    for pool in (c["k"], c["v"], w.unsqueeze(-1)):
+        rows = pool[ids, 0].reshape(-1, pool.shape[-1])[torch.tensor(want, device=dev)]
+        assert torch.equal(pool[to[0].long(), 0].reshape(-1, pool.shape[-1])[:budget], rows)
+
+
 # --------------------------------------------------------------------------- together
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("steps", [[40], [1] * 12, [200, 1, 30, 1]], ids=["chunk", "tokens", "both"])
+def test_eviction_by_the_weights_that_attention_leaves(dev, dtype, steps):
+    """Against 64-bit sums over the keys that the cache holds: what is kept is not lighter than what is dropped, but by
+    the error bounds of two sums."""
+    from catopt_b200.paged import PagedCache
+
+    kv, group, d, budget, first, last = 2, 3, 64, 24, 2, 4
+    g = torch.Generator(device=dev).manual_seed(5)
+    cache = PagedCache(1, 40, 16, kv, d, dtype=dtype, device=dev, track_weights=True)
+    r, other = cache.open(), cache.open()
+    total, bound = (torch.zeros(40, kv, 16, dtype=torch.float64, device=dev) for _ in range(2))
+    for n in [30, *steps]:
+        batch = cache.begin({other: 1, r: n})
+        x = torch.randn(n + 1, kv * (group + 2), d, generator=g, device=dev).to(dtype)
+        cache.append(0, batch, None, x[:, -2 * kv:-kv], x[:, -kv:])
+        q = x[:, :kv * group]
+        cache.attend(0, batch, q)
+        held = {"k": cache.k[0], "v": cache.v[0], "table": batch.table, "page": 16}
+        _, _, w, tol = ref.attend(q, held, [1, n], batch.seq_lens.tolist(), d ** -0.5, True)
+        total += w
+        bound += tol + 2 * ref.U32 * total          # one more addition
+    length = cache.length(r)
+    assert budget < length
+    ids = batch.table[1, :(length + 15) // 16].long()
+    sums, bounds = (t[ids].transpose(0, 1).reshape(kv, -1)[:, :length] for t in (total, bound))
+    close(cache.weights[0][ids].transpose(0, 1).reshape(kv, -1)[:, :length], sums, bounds, "weights")
+    kept = cache.evict([r], budget, keep_first=first, keep_last=last)[0][0].long()
+    for h in range(kv):
+        assert kept[h].tolist() == sorted(set(kept[h].tolist()))
+        dropped = torch.ones(length, dtype=torch.bool, device=dev)
+        dropped[kept[h]] = False
+        assert not dropped[:first].any() and not dropped[length - last:].any()
+        assert (sums + bounds)[h][kept[h, first:-last]].min() >= (sums - bounds)[h][dropped].max()
+
+
 @pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
 def test_decode_loop(dev, dtype):
     """Prompts in chunks, single tokens, an eviction, more tokens, a request that ends and one that begins: every output
