@@ -137,7 +137,10 @@ size_t up16(size_t n) { return (n + 15) & ~size_t(15); }
 // the two launches more of the streaming kernel never paid (31 single tokens on up to 16384 keys beside a chunk of 64:
 // 237 us with one kernel, 255 with both; 21 on up to 2048 beside three chunks: 45 and 62).  In fp32 a row that is not
 // there costs as much as one that is, so there the few rows of a mixed batch have the narrow tiles, unless the batch is
-// sure to be small (15 single tokens on up to 4096 keys: 351 us with both, 466 with one; 12 on 512: 75 and 71).
+// sure to be small.  Measured with a chunk of 64 beside 1, 3, 7, 15 or 31 single tokens on up to 128, 512, 2048 or 8192
+// keys, 32 heads on 8 (d 128), 8 on 2 and 4 on 4 (d 64): with up to 4 blocks an SM one kernel is the faster, by up to 21 us
+// (but for one case, 66 us and 64 with both); from 14 on both are, or are within 3 % (16 blocks an SM: 148 us with one, 112 with
+// both; 223: 1706 and 1076); around 8 it goes either way (95 and 79; 43 and 51).
 struct Plan {
   int few;                     // 0: no streaming kernel
   bool chunks;

@@ -13,8 +13,8 @@
 // asynchronous copies (two CTAs of four warps per SM keep 128 KB in flight) and keeps its own (m, l, O); they
 // meet once per piece, in shared memory.  m follows the maximum lazily (by 2^8), decided by one vote per tile.
 //
-// Measured: 32 single tokens on 2048 .. 16384 keys, 32 heads on 8, d 128: 191 us, 6.5 TB/s, all of the copy rate.  One
-// stream of 65536 keys: 48 us, 5.6 TB/s; the rest is its CTAs' start and the join of 37 carriers a head.
+// Measured: 32 single tokens on 2048 .. 16384 keys, 32 heads on 8, d 128: 199 us, 6.2 TB/s, 95 % of the copy rate.  One
+// stream of 65536 keys: 49 us, 5.5 TB/s; the rest is its CTAs' start and the join of 37 carriers a head.
 #include "om_paged.cuh"
 
 namespace cb2 {

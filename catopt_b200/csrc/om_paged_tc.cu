@@ -9,7 +9,7 @@
 // block's P after every product: one exponential per score (16 a clock and SM) and the products (1024 clocks per
 // 128 x 128 scores either way) overlap.  The reference point m follows the maximum lazily (when it moved by
 // more than 2^8), so O is rarely rescaled, and only then does the softmax wait for the product before.
-// P is rounded once, to bf16, as the dense chunks' kernel of this library does (error against 64 bits 2.4e-3, of which the
+// P is rounded once, to bf16, as the dense chunks' kernel of this library does (error against 64 bits 2.3e-3, of which the
 // rounding of o alone is 1.7e-3).  A second half of it (p = hi + lo, half as many products again) takes two chunks of 2048 on
 // 8192 keys from 414 to 518 us a call, chunks of 1024 with weights from 207 to 237, a mixed batch of 24 from 39 to 43.
 // Only a block that some row of the tile may not see whole is masked, per element.  Of the last block of a
@@ -22,11 +22,11 @@
 // pieces of a share are listed in shared memory in batches, so that the softmax threads spend no registers on
 // the walk.  Every wait is bounded.
 //
-// Measured: two chunks of 2048 tokens on 8192 keys in all, 32 heads on 8, d 128: 372 us with the join, 994 TFLOP/s; a
-// piece costs about four blocks' time to start and end, which the line counts.  What bounds a long piece is shared
-// memory: a 64-column product reads Q again for every 64 keys (48 KB a block), P V reads 16 KB, the loads write 32 KB;
-// two CTAs move 192 KB in about 1680 clocks, 115 of 128 bytes a clock.  Tried and slower: 128-key blocks with one S
-// buffer (487 us), two row tiles that share key and value blocks in one CTA of an SM (595 us), part of the
+// Measured: two chunks of 2048 tokens on 8192 keys in all, 32 heads on 8, d 128, with the join, at 1965 MHz: 352..367 us
+// replayed in a graph (1.0 PFLOP/s), 414..420 us a call when the inputs change from call to call; a piece costs about four
+// blocks' time to start and end, which the line counts.  What bounds a long piece is shared memory: a 64-column product reads
+// Q again for every 64 keys (48 KB a block), P V reads 16 KB, the loads write 32 KB; two CTAs move 192 KB in about 1680
+// clocks of a long piece, 115 of 128 bytes a clock.  Tried and slower: 128-key blocks with one S buffer (487 us), two row tiles that share key and value blocks in one CTA of an SM (595 us), part of the
 // exponentials as polynomials on the FMA pipes (+7 %), eight softmax warps (+7 %).
 #include "om_paged.cuh"
 #include "umma.cuh"

@@ -11,8 +11,8 @@
 // apart for pairs (i, i + d/2); only a rotation of part of the columns in halves exchanges through shared
 // memory.  A lane's columns are the same for every head of a token, so its angles and norm weights are loaded once.
 //
-// Measured: prompts of 6868 tokens, 32 + 8 + 8 heads of 128, norm and rotation: 40 us, 4.3 TB/s (instruction issue is busy
-// half of the time, the rest is the latency of a CTA's chain of look-ups, loads and stores); 64 tokens: 3.9 us.
+// Measured: prompts of 6868 tokens, 32 + 8 + 8 heads of 128, norm and rotation: 40..42 us, 4.1..4.3 TB/s (issue is busy 47 %
+// of the time at 22 warps an SM: the rest is the latency of a CTA's chain of look-ups, loads and stores); 64 tokens: 4 us.
 #include "om_paged.cuh"
 
 namespace cb2 {

@@ -874,7 +874,8 @@ def om_paged_fwd(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     ``q [n, Hq, d]`` (any strides), request r's rows ``cu_q[r]:cu_q[r+1]``; its ``seq_lens[r]`` cached keys, the
     new tokens' included, lie in pages ``block_table[r]`` of the pools ``[n_pages, Hkv, page_size, d]``; query
     head h reads kv head ``h // (Hq // Hkv)``.  Row i of n_r sees the slots up to ``seq_lens[r] - n_r + i``
-    (all of them without ``causal``); a row that sees none gives 0.  ``max_q``, ``max_k``: bounds of the requests'
+    (all of them without ``causal``); a row that sees none gives 0.  An Inf or NaN in ``v`` of a
+    later new token of the same request may reach a row that does not see it.  ``max_q``, ``max_k``: bounds of the requests'
     new tokens and cached keys (``max_k`` defaults to what the table holds); the scratch grows with them.
     ``weights`` (float32 ``[n_pages, Hkv, page_size]``): the softmax probability that every cached key gets, summed
     over rows and the heads of its group, is added to it (requests of one call must not share pages then).  ``scale`` defaults to ``1/sqrt(d)``; ``out`` is contiguous

@@ -449,7 +449,8 @@ int cb2_paged_append(const void* q, long long q_token_stride, long long q_head_s
  *     o[t, head] = sum_j softmax_j(scale q.k_j) v_j,   kv head = head / (Hq / Hkv),
  * over the slots j <= seq_lens[r] - n_r + i that row i of request r sees (causal != 0), or all
  * of its slots.  A row that sees no key (seq_lens[r] = 0, or less than n_r) is 0.  What the
- * slots behind seq_lens[r] hold, NaN included, has no effect.
+ * slots behind seq_lens[r] hold, NaN included, has no effect; an Inf or NaN in v of a later new
+ * token of the same request may reach a row that does not see it (0 x Inf).
  * q: [n_tokens, Hq, d] with token and head strides in elements (none 0); o: [n_tokens, Hq, d]
  * dense, no part of it on q.  max_q: no request has more new tokens; max_k: none more cached keys.
  * weights (may be NULL): weights[key] += sum over the rows that see it, and the heads of its
@@ -473,7 +474,7 @@ int cb2_om_paged_fwd(const void* q, long long q_token_stride, long long q_head_s
  * between (ties to the lowest slot; NaN counts as the smallest), `budget` in all, in slot order;
  * a shorter request keeps all.  Kept keys, values and weights are copied to the pages
  * new_table[r][..] (int32 [R, new_pages]) of the same pools; none of them may be among the pages of
- * a request of this call.  The old pages stay as they are, so requests may share them.
+ * a request of this call, and none is named twice.  The old pages stay as they are, so requests may share them.
  * kept: int32 [R, Hkv, budget], the old slot of every new one, -1 behind the last; new_lens: int32
  * [R] = min(seq_lens, budget).  max_k: no request has more cached keys.  budget <= 2^30.  No
  * scratch. */
