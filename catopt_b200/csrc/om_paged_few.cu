@@ -4,10 +4,12 @@
 // Keys are the long side of both products, so they take the M side of m16n8k16: S^T[16 keys, 8 rows] = K Q^T
 // and O^T[16 columns, 8 rows] += V^T P^T; a group of four to eight query heads fills the N side, where the
 // other orientation would leave half of the rows empty.  K comes by ldmatrix, V^T by its transposing form, and P
-// turns from accumulator into operand by one 8x8 register transpose a half.  A probability is split
-// into two bf16 halves, p = hi + lo up to 2^-16 of it, and V^T multiplied by both, since one half alone would lose more than the
-// rounding of o (error against 64 bits 2.1e-3 in place of 1.7e-3; 32 single tokens on up to 16384 keys: 197 us a call with
-// one half, 199 with two).  The pace is set by memory: per 16 keys of d = 128 a warp issues about 110 instructions for 8 KB.
+// turns from accumulator into operand by one 8x8 register transpose a half.  A probability is split into two
+// bf16 halves, p = hi + lo up to 2^-16 of it, and V^T multiplied by both, since one half alone would lose more than the
+// rounding of o (error against 64 bits 2.1e-3 in place of 1.7e-3; 32 single tokens on up to 16384 keys: 197 us a call
+// with one half, 199 with two).  hi is p cut off, and lo at least 2^-24 of p, so that neither half of a positive p is
+// zero or negative: an infinite value that a row sees comes out as it is.  The pace is set by memory: per 16 keys of
+// d = 128 a warp issues about 115 instructions for 8 KB.
 //
 // Warps are independent: each streams every fourth 16-key tile of the CTA's piece through its own ring of
 // asynchronous copies (two CTAs of four warps per SM keep 128 KB in flight) and keeps its own (m, l, O); they
@@ -84,7 +86,7 @@ paged_few_kernel(const PagedRows rows, const PagedPools pools, const PagedBatch 
   constexpr int kChunks = KS * 2, kRowsPerCopy = 32 / kChunks, kCopies = kTileKeys / kRowsPerCopy;
   const int cp_chunk = lane % kChunks, cp_row = lane / kChunks;
   const bool cp_col = cp_chunk * 8 < d;
-  constexpr float kLazy = 8.f;
+  constexpr float kLazy = 8.f, kLeast = 0x1p-24f;
 
   for (PagedWalk<Cost> w(batch, cost, share); w.valid(); w.next()) {
     w.clip();
@@ -240,9 +242,10 @@ paged_few_kernel(const PagedRows rows, const PagedPools pools, const PagedBatch 
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const uint32_t hi = pack_bf16x2(p[2 * e], p[2 * e + 1]);
+          const float p0 = p[2 * e], p1 = p[2 * e + 1];
+          const uint32_t hi = __byte_perm(__float_as_uint(p0), __float_as_uint(p1), 0x7632);
           pf[b][e] = transpose8x8(hi);
-          pl[b][e] = transpose8x8(pack_bf16x2(p[2 * e] - bf16lo_to_f32(hi), p[2 * e + 1] - bf16hi_to_f32(hi)));
+          pl[b][e] = transpose8x8(pack_bf16x2(fmaxf(p0 - bf16lo_to_f32(hi), p0 * kLeast), fmaxf(p1 - bf16hi_to_f32(hi), p1 * kLeast)));
         }
       }
       {

@@ -90,6 +90,25 @@ def test_a_nan_that_is_seen_shows(dev, dtype, new):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("new,group", [(1, 1), (1, 4), (2, 8), (40, 4)])
+@pytest.mark.parametrize("length", [90, 500, 6000])
+def test_an_infinite_value_that_is_seen_shows(dev, dtype, new, group, length):
+    # every probability is above zero, so the sum is infinite where a value is, with its sign, and finite elsewhere
+    from catopt_b200 import ops
+
+    c = ref.make_cache([length], 2, 16, 64, dtype, dev, 14)
+    g = torch.Generator(device=dev).manual_seed(15)
+    for slot, col, x in ((0, 3, float("inf")), (37, 4, -float("inf")), (length - new, 5, float("inf")), (length - new - 1, 6, -float("inf"))):
+        c["v"][c["table"][0, slot // 16].long(), :, slot % 16, col] = x
+    q = torch.randn(new, 2 * group, 64, generator=g, device=dev).to(dtype)
+    q[0, 0] = 0          # probabilities that are the same, and powers of two where the length is one
+    o = ops.om_paged_fwd(q, c["k"], c["v"], c["table"], c["lens"], ref.offsets([new], dev), new, max_k=length)
+    assert (o[..., [3, 5]] == float("inf")).all() and (o[..., [4, 6]] == -float("inf")).all()
+    rest = [i for i in range(64) if i not in (3, 4, 5, 6)]
+    assert o[..., rest].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("new,lens", [([1, 1], [200, 130]), ([50, 20], [200, 130])], ids=["step", "chunk"])
 def test_requests_that_share_pages(dev, dtype, new, lens):
     # the second request's first pages are the first one's: reading them twice is fine
