@@ -878,8 +878,8 @@ def om_paged_fwd(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     later new token of the same request may reach a row that does not see it.  ``max_q``, ``max_k``: bounds of the requests'
     new tokens and cached keys (``max_k`` defaults to what the table holds); the scratch grows with them.
     ``weights`` (float32 ``[n_pages, Hkv, page_size]``): the softmax probability that every cached key gets, summed
-    over rows and the heads of its group, is added to it (requests of one call must not share pages then).  ``scale`` defaults to ``1/sqrt(d)``; ``out`` is contiguous
-    and no part of it on ``q``."""
+    over rows and the heads of its group, is added to it (requests of one call must not share pages then).  ``scale``
+    defaults to ``1/sqrt(d)``; ``out`` is contiguous and no part of it on ``q``."""
     res = _host("om_paged_fwd")(_status_words, q, k_pages, v_pages, block_table, seq_lens, cu_q, max_q, max_k, scale, causal, weights, out)
     if res is not NotImplemented:
         if res.__class__ is int:

@@ -183,7 +183,8 @@ class PagedCache:
     def evict(self, requests: list[int], budget: int, *, keep_first: int = 0, keep_last: int = 0) -> list[torch.Tensor]:
         """Cut the given requests to ``budget`` keys in every layer (``ops.paged_evict``; those that are not longer
         stay as they are).  The kept keys move to fresh pages, as many as the budget fills, and the old pages are free
-        afterwards: the free pages have to serve one request, those that it leaves serve the next.  Returns the kept slots per layer, ``[cut requests, Hkv, budget]``, in the order of ``requests``."""
+        afterwards: the free pages have to serve one request, those that it leaves serve the next.  Returns the kept slots
+        per layer, ``[cut requests, Hkv, budget]``, in the order of ``requests``."""
         if self.weights is None:
             raise B200Error("PagedCache.evict: the cache does not track attention weights")
         if budget < 1 or keep_first < 0 or keep_last < 0 or keep_first + keep_last > budget:
